@@ -201,6 +201,73 @@ int tv_search_dev_noalloc(tv_index *ix, const float *d_queries, size_t nq, size_
                           float *d_out_scores, int64_t *d_out_indices, size_t *out_k_eff);
 size_t tv_noalloc_scratch_bytes(void);
 
+/* ---- operators beside the search ------------------------------------------
+ *
+ * Rows in 8 bits, their products, re-scoring of what a search returned, and
+ * drawing a slot from scores.  No counterpart in the reference.  They hold no
+ * state and take no index: every pointer but `stream` is a device pointer of
+ * `device`, and the call puts its kernels on `stream` (a hipStream_t of that
+ * device; NULL: its default stream) and returns without waiting.  Inputs must
+ * be complete in that stream's order and stay untouched until the kernels have
+ * run.  Nothing is allocated: a call may be recorded into a graph, which holds
+ * the buffers and the workspace it was recorded with.  Calls that may run at
+ * the same time need workspaces of their own; a workspace needs no clearing and
+ * holds nothing from one call to the next.  Any thread may call; the caller's
+ * current device stays what it was.  Strides count elements from one row to the
+ * next, elements of a row lie next to each other.  Results overlap no input.
+ * Arguments are checked before anything is launched (TV_ERR_BAD_ARGUMENT,
+ * tv_last_error() says which); what lies in device memory is not.  Calls of
+ * no rows do nothing. */
+
+/* Types of values, and of the scales of 8-bit rows. */
+typedef enum { TV_F32 = 0, TV_F16 = 1, TV_BF16 = 2 } tv_value_type;
+typedef enum {
+    TV_SCALE_E8M0 = 0, /* a byte e: 2^(e - 127); 255 is NaN */
+    TV_SCALE_F32 = 1   /* a float */
+} tv_scale_type;
+
+/* 8-bit rows hold e4m3 codes (1 sign, 4 exponent and 3 mantissa bits, no infinity, largest value 448) of
+ * dim coordinates, 1 to 16384, and a scale for every block of 128 coordinates (the last may be shorter) of
+ * `group` rows: 1, or 128 (the last tile may hold fewer).  A coordinate is code * scale.  Scale of row r and
+ * coordinate c: scales[(r / group) * scale_stride + c / 128]. */
+
+/* Makes 8-bit rows of values.  With `amax` the largest finite magnitude of a block, its scale is
+ * max(amax / 448, 2^-126) as a float, or the smallest power of two 2^e, e >= -126, with amax <= 448 * 2^e;
+ * codes are x / scale rounded to the nearest, ties to even.  Infinities and NaN become NaN codes and leave
+ * their block's scale to the others. */
+int tv_fp8_quantize_dev(int device, void *stream, const void *d_x, int x_type, size_t x_stride, size_t rows, size_t dim,
+                        int scale_type, int group, uint8_t *d_codes, size_t code_stride, void *d_scales, size_t scale_stride);
+/* out[i][j] = the inner product of row i of a (m rows, a scale of each row) with row j of b (n rows, scales of
+ * `group` rows): sums of products of codes within a block times both scales, blocks added in 32 bits, rounded
+ * once to out_type.  Rows that start at multiples of 16 bytes (codes and stride) are read fastest. */
+int tv_fp8_matmul_dev(int device, void *stream, const uint8_t *d_a, size_t a_stride, const void *d_a_scales, size_t a_scale_stride, size_t m,
+                      const uint8_t *d_b, size_t b_stride, const void *d_b_scales, size_t b_scale_stride, size_t n, int group,
+                      size_t dim, int scale_type, void *d_out, int out_type, size_t out_stride);
+/* Scores the m slots of each query (m <= 16384) against their 8-bit rows and writes the k <= m best, sorted
+ * (score desc, slot asc), as the search does: nq * k scores and slots.  Products and sums are taken in 64 bits,
+ * a score is rounded once.  A slot below 0 or not below n counts as absent, the same slot twice as two
+ * candidates; a query with fewer than k present ends in scores of -infinity at slot -1.  NaN scores come last.
+ * Scales that are NaN or infinite make their rows' scores so. */
+int tv_fp8_rescore_dev(int device, void *stream, const void *d_queries, int q_type, size_t q_stride, size_t nq,
+                       const uint8_t *d_rows, size_t row_stride, const void *d_scales, size_t scale_stride, size_t n, int group, size_t dim, int scale_type,
+                       const int64_t *d_slots, size_t slot_stride, size_t m, size_t k, float *d_out_scores, int64_t *d_out_slots,
+                       void *d_workspace, size_t workspace_bytes);
+size_t tv_fp8_rescore_workspace(size_t nq, size_t m);
+/* Draws one slot from each row of n scores.  Allowed are the slots whose mask bit is set (d_mask_words NULL: all;
+ * 64 slots a word, as tv_pack_mask makes them; mask_stride 0: one mask for all rows) and whose score is neither NaN nor
+ * -infinity.  With slots ranked by score, ties to the lower slot, and w = exp((score - best) / temperature):
+ * top_k > 0 keeps the first top_k; of those, top_p < 1 keeps a slot while the ones before it hold less than
+ * top_p of their mass; of those, min_p > 0 keeps w >= min(min_p, 1); the best one always stays.  Drawn is the first
+ * slot, in order of slots, at which the running sum of the kept w exceeds u times their sum, 0 <= u < 1.  A temperature
+ * that is not above 0 draws the best.  out_probs: w over the sum of the kept ones.  A row that allows nothing: slot -1,
+ * probability 0.  Weights are taken in 64 bits and held as multiples of 2^-(63 - ceil(log2 n)); sums of them are exact,
+ * so that a draw never depends on the order of additions.  d_u holds a value a row; each of the four parameters does
+ * too, or is NULL: temperature 1, no limit. */
+int tv_sample_dev(int device, void *stream, const void *d_scores, int score_type, size_t score_stride, size_t rows, size_t n,
+                  const uint64_t *d_mask_words, size_t mask_stride, const float *d_u, const float *d_temperature, const int32_t *d_top_k,
+                  const float *d_top_p, const float *d_min_p, int64_t *d_out_slots, float *d_out_probs, void *d_workspace, size_t workspace_bytes);
+size_t tv_sample_workspace(size_t rows, size_t n);
+
 /* ---- host-only derivations (no GPU touched) ------------------------------- */
 
 /* The tables tv_index_create derives: Rotation::new (rotation.rs:141-187;

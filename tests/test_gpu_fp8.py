@@ -1,0 +1,379 @@
+"""8-bit rows -- made, multiplied, re-scored -- against plain 64-bit forms of the same definitions, at the sizes, strides and
+values where a tile, a block or a load ends."""
+import itertools
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+@pytest.fixture(scope="module")
+def fp8():
+    from turbovec_amd import fp8
+    return fp8
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def wild(rows, dim, seed):
+    """Values whose magnitudes differ by orders from block to block and within."""
+    g = gen(seed)
+    x = torch.randn(rows, dim, generator=g, device="cuda") * torch.exp(2 * torch.randn(rows, dim, generator=g, device="cuda"))
+    return x * torch.exp2(torch.randint(-20, 20, (rows, 1), generator=g, device="cuda").float())
+
+
+def spread(scales, group, rows, dim):
+    return scales.double().repeat_interleave(group, 0)[:rows].repeat_interleave(128, 1)[:, :dim]
+
+
+def values(r):
+    return r.codes.double() * spread(r.scales, r.group, *r.codes.shape)
+
+
+# ---- quantize -------------------------------------------------------------------------------------
+
+def check_rows(fp8, x, scale, group):
+    r = fp8.quantize(x, scale=scale, group=group)
+    rows, dim = x.shape
+    x = x.double()
+    fine = torch.isfinite(x)
+    padded = torch.nn.functional.pad(torch.where(fine, x.abs(), 0.0), (0, -dim % 128, 0, -rows % group))
+    most = padded.view(-1, group, padded.shape[1] // 128, 128).amax((1, 3))
+    if scale == "f32":
+        # the rounded quotient: 53 bits are more than 2 * 24 + 2, so that rounding to them first changes nothing (a tensor
+        # divided by a number would be multiplied by its reciprocal)
+        want = torch.clamp((most / torch.full_like(most, 448.0)).float(), min=2.0 ** -126)
+        assert torch.equal(r.scales, want)
+    else:
+        s = r.scales.double()
+        assert r.scales.dtype == torch.float8_e8m0fnu
+        assert bool((most <= 448 * s).all())                           # it fits
+        assert bool(((most > 224 * s) | (s == 2.0 ** -126)).all())     # and would not with half of it
+    q = x / spread(r.scales, group, rows, dim)
+    c = r.codes.double()
+    assert torch.equal(torch.isnan(c), ~fine)
+    # the nearest code: half a step of 3 mantissa bits, 2^-10 below 2^-6; the quotient was rounded to 32 bits first
+    half = torch.clamp(torch.exp2(torch.floor(torch.log2(q.abs().clamp(min=2.0 ** -40)))) * 2.0 ** -4, min=2.0 ** -10)
+    off = torch.where(fine, (c - q).abs(), 0.0)
+    assert bool((off <= torch.where(fine, half + q.abs() * 2.0 ** -23, 0.0)).all())
+    return r
+
+
+@pytest.mark.parametrize("rows,dim", [(1, 1), (3, 7), (5, 127), (4, 128), (4, 129), (130, 200), (257, 1000), (64, 1536), (128, 128), (300, 385)])
+@pytest.mark.parametrize("scale,group", [("e8m0", 1), ("f32", 1), ("e8m0", 128), ("f32", 128)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize(fp8, rows, dim, scale, group, dtype):
+    x = wild(rows, dim, 1)
+    check_rows(fp8, (x / x.abs().max() * 1000).to(dtype), scale, group)
+
+
+@pytest.mark.parametrize("scale", ["e8m0", "f32"])
+@pytest.mark.parametrize("group", [1, 128])
+def test_quantize_special_values(fp8, scale, group):
+    """Blocks of zeros, of nothing finite, of denormals, of the largest values; maxima at the border between two powers."""
+    x = torch.randn(260, 512, generator=gen(2), device="cuda")
+    x[0] = 0
+    x[1, :128] = float("nan")
+    x[1, 200] = float("inf")
+    x[1, 201] = -float("inf")
+    x[2] *= 1e-40
+    x[3] = 3.4e38
+    x[4, :128] = 448.0
+    x[4, 128:256] = 448.00003
+    x[4, 256:384] = 3.5
+    x[4, 384:] = 2.0 ** -126 * 448
+    x[5] = 2.0 ** -149
+    x[6] = -0.0
+    if group == 128:
+        x = x.repeat_interleave(128, 0)[:128 * 7 + 3]
+    r = check_rows(fp8, x, scale, group)
+    assert bool((r.codes[0].float() == 0).all()) and bool((r.scales[0].double() == 2.0 ** -126).all())
+
+
+def test_quantize_ties_go_to_even(fp8):
+    x = torch.tensor([448.0] + [v for v in (1.0625, 1.1875, 1.3125, 17.0, 19.0, 2.0 ** -10, 3 * 2.0 ** -10)] + [0.0] * 120, device="cuda")[None]
+    c = fp8.quantize(x, scale="f32").codes.float()[0, 1:8].tolist()
+    assert c == [1.0, 1.25, 1.25, 16.0, 20.0, 0.0, 2.0 ** -8]
+
+
+@pytest.mark.parametrize("scale,group", itertools.product(["e8m0", "f32"], [1, 128]))
+def test_quantize_strided_and_beside_others(fp8, scale, group):
+    """Rows inside a wider buffer, starting off every alignment, into codes and scales inside wider ones: nothing else changes."""
+    from turbovec_amd import _lib as T
+    base = wild(140, 700, 3)
+    for off, dim in ((0, 256), (1, 256), (3, 255), (128, 300)):
+        x = base[:, off:off + dim]
+        want = fp8.quantize(x.contiguous(), scale=scale, group=group)
+        got = fp8.quantize(x, scale=scale, group=group)
+        assert torch.equal(got.codes.view(torch.uint8), want.codes.view(torch.uint8)) and torch.equal(got.scales.view(torch.uint8), want.scales.view(torch.uint8))
+        codes = torch.full((142, 512), 0x55, dtype=torch.uint8, device="cuda")
+        blocks, size = -(-dim // 128), 1 if scale == "e8m0" else 4
+        scales = torch.full((-(-140 // group) + 2, blocks + 3, size), 0x55, dtype=torch.uint8, device="cuda")
+        T.check(T.lib().tv_fp8_quantize_dev(0, torch.cuda.current_stream().cuda_stream, x.data_ptr(), T.F32, x.stride(0), 140, dim, T.SCALE_E8M0 if scale == "e8m0" else T.SCALE_F32, group,
+                                            codes[1:].data_ptr() + off, 512, scales[1:].data_ptr(), blocks + 3))
+        assert torch.equal(codes[1:141, off:off + dim], want.codes.view(torch.uint8))
+        assert torch.equal(scales[1:-1, :blocks].reshape(-(-140 // group), -1), want.scales.view(torch.uint8).reshape(-(-140 // group), -1))
+        codes[1:141, off:off + dim] = 0x55
+        scales[1:-1, :blocks] = 0x55
+        assert bool((codes == 0x55).all()) and bool((scales == 0x55).all())
+
+
+# ---- matmul ---------------------------------------------------------------------------------------
+
+def stored(fp8, x, scale, group, pad=None, offset=0):
+    """8-bit rows of x inside a buffer of NaN codes: rows at a stride of `pad`, `offset` bytes in."""
+    r = fp8.quantize(x, scale=scale, group=group)
+    if pad is None:
+        return r
+    rows, dim = x.shape
+    buffer = torch.full((rows * pad + offset + 64,), 0x7f, dtype=torch.uint8, device="cuda")
+    codes = torch.as_strided(buffer, (rows, dim), (pad, 1), offset)
+    codes.copy_(r.codes.view(torch.uint8))
+    return fp8.Fp8Rows(codes.view(torch.float8_e4m3fn), r.scales, group)
+
+
+def check_product(a, b, got):
+    x, y = values(a), values(b)
+    want = x @ y.t()
+    dim = x.shape[1]
+    # sums in 32 bits: one rounding or truncation (2^-23) for each of dim products and additions, three more a block for its
+    # scales; then half a step of the result's type, and for float16 half its smallest step
+    bound = (2 * dim + 3 * (-(-dim // 128))) * 2.0 ** -23 * (x.abs() @ y.abs().t()) + 2.0 ** -126
+    step = torch.finfo(got.dtype).eps / 2
+    bound = bound + (want.abs() + bound) * step + torch.finfo(got.dtype).smallest_normal * torch.finfo(got.dtype).eps
+    over = want.abs() > torch.finfo(got.dtype).max
+    off = (got.double() - want).abs()
+    assert bool(((off <= bound) | over).all()), float((off / bound).max())
+
+
+@pytest.mark.parametrize("scale,group", [("e8m0", 1), ("f32", 1), ("e8m0", 128), ("f32", 128)])
+@pytest.mark.parametrize("dim", [1, 8, 16, 100, 127, 128, 129, 200, 256, 384, 520, 1000, 1536])
+def test_matmul(fp8, scale, group, dim):
+    for i, (m, n) in enumerate([(1, 1), (1, 300), (3, 65), (16, 128), (17, 257), (33, 15), (65, 130), (128, 64), (130, 127), (257, 300), (300, 1)]):
+        a = fp8.quantize(torch.randn(m, dim, generator=gen(i), device="cuda"), scale=scale)
+        b = fp8.quantize(torch.randn(n, dim, generator=gen(100 + i), device="cuda") * torch.exp2(torch.arange(n, device="cuda") % 7 - 3.0)[:, None], scale=scale, group=group)
+        check_product(a, b, fp8.matmul(a, b, dtype=DTYPES[i % 3]))
+
+
+@pytest.mark.parametrize("scale,group", [("e8m0", 1), ("f32", 128)])
+@pytest.mark.parametrize("m,n,dim", [(1, 5000, 4096), (256, 1000, 2048), (512, 777, 1111), (1024, 1024, 640), (1000, 3000, 128), (2049, 515, 384)])
+def test_matmul_larger(fp8, scale, group, m, n, dim):
+    a = fp8.quantize(torch.randn(m, dim, generator=gen(7), device="cuda"), scale=scale)
+    b = fp8.quantize(torch.randn(n, dim, generator=gen(8), device="cuda"), scale=scale, group=group)
+    for dtype in DTYPES:
+        check_product(a, b, fp8.matmul(a, b, dtype=dtype))
+
+
+@pytest.mark.parametrize("scale,group", [("e8m0", 1), ("f32", 1), ("f32", 128)])
+@pytest.mark.parametrize("dim,pad,offset", [(256, 272, 0), (256, 256, 4), (256, 257, 0), (200, 208, 0), (200, 201, 3), (1000, 1008, 0), (129, 130, 1), (100, 4096, 16)])
+@pytest.mark.parametrize("m,n", [(2, 70), (70, 300), (300, 290)])
+def test_matmul_strided(fp8, scale, group, dim, pad, offset, m, n):
+    """Codes at odd places and strides with NaN codes between the rows, results inside a wider buffer: nothing else changes."""
+    a = stored(fp8, torch.randn(m, dim, generator=gen(9), device="cuda"), scale, 1, pad, offset)
+    b = stored(fp8, torch.randn(n, dim, generator=gen(10), device="cuda"), scale, group, pad, offset)
+    for dtype in DTYPES:
+        buffer = torch.full((m + 2, n + 5), -7.0, dtype=dtype, device="cuda")
+        out = buffer[1:-1, 3:-2]
+        assert fp8.matmul(a, b, out=out) is out
+        check_product(a, b, out)
+        out.fill_(-7.0)
+        assert bool((buffer == -7.0).all())
+
+
+def test_matmul_shared_and_strided_scales(fp8):
+    """Scales inside a wider buffer, and one row of a seen many times (stride 0)."""
+    x, y = torch.randn(1, 300, generator=gen(11), device="cuda"), torch.randn(200, 300, generator=gen(12), device="cuda")
+    for scale, group in (("e8m0", 1), ("f32", 128), ("e8m0", 128)):
+        a, b = fp8.quantize(x, scale=scale), fp8.quantize(y, scale=scale, group=group)
+        wide = torch.zeros(b.scales.shape[0], 9, dtype=torch.uint8 if scale == "e8m0" else torch.float32, device="cuda")
+        wide[:, 2:5] = b.scales.view(wide.dtype)
+        b2 = fp8.Fp8Rows(b.codes, wide.view(b.scales.dtype)[:, 2:5], group)
+        a2 = fp8.Fp8Rows(a.codes.expand(40, -1), a.scales.view(wide.dtype).expand(40, -1).view(a.scales.dtype), 1)
+        one, many = fp8.matmul(a, b), fp8.matmul(a2, b2)
+        check_product(a2, b2, many)
+        check_product(a, b, one)
+
+
+@pytest.mark.parametrize("m", [1, 20, 300])
+@pytest.mark.parametrize("scale", ["e8m0", "f32"])
+def test_matmul_nan_stays_in_its_row(fp8, scale, m):
+    x, y = torch.randn(m, 300, generator=gen(13), device="cuda"), torch.randn(280, 300, generator=gen(14), device="cuda")
+    x[m // 2, 290] = float("nan")
+    y[40, 5] = float("inf")
+    a, b = fp8.quantize(x, scale=scale), fp8.quantize(y, scale=scale)
+    got = torch.isnan(fp8.matmul(a, b))
+    want = torch.zeros_like(got)
+    want[m // 2] = True
+    want[:, 40] = True
+    assert torch.equal(got, want)
+
+
+def test_matmul_zero_scales_and_extremes(fp8):
+    """Rows of zeros, the smallest and the largest scales: products that leave 32 bits at either end."""
+    x = torch.zeros(5, 256, device="cuda")
+    x[1] = 1e-38
+    x[2] = 1e30
+    x[3] = 1e8
+    x[4, 0] = 1.0
+    for scale in ("e8m0", "f32"):
+        r = fp8.quantize(x, scale=scale)
+        got = fp8.matmul(r, r)
+        assert bool((got[0] == 0).all()) and bool((got[:, 0] == 0).all())
+        assert torch.isinf(got[2, 2]) and float(got[1, 1]) == 0.0
+        check_product(r, r, torch.where(torch.isinf(got), 3.0e38, got))
+
+
+# ---- rescore --------------------------------------------------------------------------------------
+
+def plain_rescore(queries, rows, slots, k):
+    v, n = values(rows).cpu().numpy(), len(rows)
+    q, slots = queries.double().cpu().numpy(), slots.cpu().numpy()
+    out_s, out_i = np.full((len(q), k), -np.inf, np.float32), np.full((len(q), k), -1, np.int64)
+    for r in range(len(q)):
+        there = slots[r][(slots[r] >= 0) & (slots[r] < n)]
+        s = (v[there] @ q[r]).astype(np.float32)
+        order = np.lexsort((there, -s))[:k]
+        out_s[r, :len(order)], out_i[r, :len(order)] = s[order], there[order]
+    return out_s, out_i
+
+
+def check_best(fp8, queries, rows, slots, k):
+    s, i = fp8.rescore(queries, rows, slots, k)
+    ws, wi = plain_rescore(queries, rows, slots, k)
+    assert np.array_equal(i.cpu().numpy(), wi)
+    s = s.cpu().numpy()
+    fine = np.isfinite(ws)
+    assert np.array_equal(s[~fine], ws[~fine])
+    # sums in 64 bits, then one rounding to 32: the same value, or its neighbour where the sums fall on either side of a border
+    assert bool((np.abs(s[fine] - ws[fine]) <= np.spacing(np.abs(ws[fine]))).all())
+
+
+@pytest.mark.parametrize("scale,group", [("e8m0", 1), ("f32", 1), ("e8m0", 128), ("f32", 128)])
+@pytest.mark.parametrize("dim", [1, 8, 100, 128, 200, 512, 1000, 1536])
+def test_rescore(fp8, scale, group, dim):
+    n = 500
+    rows = fp8.quantize(torch.randn(n, dim, generator=gen(20), device="cuda"), scale=scale, group=group)
+    for j, (nq, m, k) in enumerate([(1, 1, 1), (1, 100, 10), (3, 17, 17), (40, 33, 5), (7, 500, 100)]):
+        q = torch.randn(nq, dim, generator=gen(21 + j), device="cuda").to(DTYPES[j % 3])
+        slots = torch.randint(0, n, (nq, m), generator=gen(31 + j), device="cuda")
+        check_best(fp8, q, rows, slots, k)
+
+
+@pytest.mark.parametrize("m,k", [(1000, 1), (1025, 1025), (5000, 30), (16384, 100)])
+def test_rescore_many_candidates(fp8, m, k):
+    rows = fp8.quantize(torch.randn(20000, 64, generator=gen(40), device="cuda"))
+    q = torch.randn(2, 64, generator=gen(41), device="cuda")
+    check_best(fp8, q, rows, torch.randint(0, 20000, (2, m), generator=gen(42), device="cuda"), k)
+
+
+@pytest.mark.parametrize("dim,pad,offset", [(256, 257, 0), (200, 201, 3), (16384, 16384, 0), (10000, 10000, 0)])
+def test_rescore_odd_places_and_long_rows(fp8, dim, pad, offset):
+    rows = stored(fp8, torch.randn(50, dim, generator=gen(43), device="cuda"), "e8m0", 1, pad, offset)
+    base = torch.randn(4, dim + 5, generator=gen(44), device="cuda")
+    slots = torch.randint(0, 50, (4, 60), generator=gen(45), device="cuda")
+    check_best(fp8, base[:, 3:3 + dim], rows, slots[:, 7:40], 9)
+
+
+def test_rescore_absent_and_repeated(fp8):
+    """Slots outside the rows, the same slot twice, rows of equal scores, queries with fewer candidates than k, and with none."""
+    x = torch.randn(64, 128, generator=gen(46), device="cuda")
+    x[10:20] = x[10]
+    rows = fp8.quantize(x)
+    slots = torch.randint(0, 64, (5, 30), generator=gen(47), device="cuda")
+    slots[0, :5] = torch.tensor([-1, 64, 2 ** 40, -2 ** 62, 63], device="cuda")
+    slots[1] = -1
+    slots[2, :10] = torch.arange(19, 9, -1, device="cuda")
+    slots[3] = 7
+    slots[4, 3:] = 1 << 31
+    check_best(fp8, torch.randn(5, 128, generator=gen(48), device="cuda"), rows, slots, 30)
+    check_best(fp8, torch.zeros(5, 128, device="cuda"), rows, slots, 12)
+    empty = fp8.Fp8Rows(rows.codes[:0], rows.scales[:0])
+    s, i = fp8.rescore(torch.randn(5, 128, device="cuda"), empty, slots, 3)
+    assert bool(torch.isinf(s).all()) and bool((i == -1).all())
+
+
+def test_rescore_nan_comes_last(fp8):
+    x = torch.randn(20, 130, generator=gen(49), device="cuda")
+    x[3, 129] = float("nan")
+    rows = fp8.quantize(x)
+    slots = torch.arange(20, device="cuda")[None]
+    s, i = fp8.rescore(torch.randn(1, 130, generator=gen(50), device="cuda"), rows, slots, 20)
+    assert int(i[0, 19]) == 3 and bool(torch.isnan(s[0, 19])) and not bool(torch.isnan(s[0, :19]).any())
+
+
+# ---- how calls run ----------------------------------------------------------------------------------
+
+def test_on_another_stream_and_in_a_graph(fp8):
+    """Each call on a stream of the caller's, and recorded: every replay gives what a call gives, with other inputs in the same
+    buffers, other work between them and two graphs taken in turn."""
+    q = torch.randn(70, 512, generator=gen(60), device="cuda")
+    rows = fp8.quantize(torch.randn(1000, 512, generator=gen(61), device="cuda"))
+    slots = torch.randint(0, 1000, (70, 40), generator=gen(62), device="cuda")
+
+    def everything(n):
+        a = fp8.quantize(q[:n])
+        return (a.codes.view(torch.uint8), a.scales.view(torch.uint8), fp8.matmul(a, rows)) + fp8.rescore(q[:n], rows, slots[:n], 8)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    want = everything(70)
+    with torch.cuda.stream(side):
+        got = everything(70)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(x, y) for x, y in zip(want, got))
+    graphs = []
+    for n in (70, 3):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = everything(n)
+        graphs.append((n, graph, held))
+    for turn in range(3):
+        q.copy_(torch.randn(70, 512, generator=gen(70 + turn), device="cuda"))
+        for n, graph, held in graphs:
+            graph.replay()
+            torch.randn(100_000, device="cuda").sum().item()
+            assert all(torch.equal(x, y) for x, y in zip(everything(n), held))
+
+
+def test_search_then_rescore_then_product(fp8):
+    """As a service would: 2-bit codes find candidates, 8-bit rows put them in order; the product over all rows agrees."""
+    from turbovec_amd import _lib as T
+    n, dim, nq, m, k = 20000, 256, 9, 100, 10
+    x = torch.nn.functional.normalize(torch.randn(n, dim, generator=gen(80), device="cuda"))
+    q = torch.nn.functional.normalize(x[:nq] + 0.02 * torch.randn(nq, dim, generator=gen(81), device="cuda"))
+    ix = T.NativeIndex(dim, 2)
+    torch.cuda.synchronize()
+    ix.add_dev(x.data_ptr(), n)
+    scores, slots = torch.empty(nq, m, device="cuda"), torch.empty(nq, m, dtype=torch.int64, device="cuda")
+    assert ix.search_dev(q.data_ptr(), nq, m, scores.data_ptr(), slots.data_ptr()) == m
+    rows = fp8.quantize(x)
+    s, best = fp8.rescore(q, rows, slots, k)
+    check_best(fp8, q, rows, slots, k)
+    assert bool((best[:, 0] == torch.arange(nq, device="cuda")).all())
+    a = fp8.quantize(q)
+    full = fp8.matmul(a, rows)
+    check_product(a, rows, full)
+    assert bool((full.argmax(1) == torch.arange(nq, device="cuda")).all())
+    ix.close()
+
+
+def test_a_buffer_past_four_gigabytes(fp8):
+    """Rows and results whose offsets pass 32 bits."""
+    n, dim = 33_000, 16384 * 8
+    buffer = torch.zeros(n, dim, dtype=torch.uint8, device="cuda")          # 4.3 GB; rows are 256 of each 131072 codes
+    x = torch.randn(n, 256, generator=gen(90), device="cuda")
+    r = fp8.quantize(x)
+    buffer[:, :256] = r.codes.view(torch.uint8)
+    far = fp8.Fp8Rows(buffer.view(torch.float8_e4m3fn)[:, :256], r.scales)
+    for m in (2, 100):
+        a = fp8.quantize(torch.randn(m, 256, generator=gen(91), device="cuda"))
+        assert torch.equal(fp8.matmul(a, far), fp8.matmul(a, r))
+    slots = torch.randint(32_000, n, (3, 50), generator=gen(92), device="cuda")
+    for x, y in zip(fp8.rescore(x[:3], far, slots, 9), fp8.rescore(x[:3], r, slots, 9)):
+        assert torch.equal(x, y)

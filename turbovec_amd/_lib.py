@@ -23,6 +23,9 @@ ERR_INDEX_OUT_OF_RANGE = 9
 
 SCORE_AUTO, SCORE_L_SCALAR, SCORE_L_CLASSIC, SCORE_L_U32, SCORE_P = 0, 1, 2, 3, 4
 
+F32, F16, BF16 = 0, 1, 2                       # tv_value_type
+SCALE_E8M0, SCALE_F32 = 0, 1                   # tv_scale_type
+
 # every symbol include/turbovec_hip.h declares
 EXPORTS = [
     "tv_status_string", "tv_last_error", "tv_index_create", "tv_index_destroy", "tv_index_set_tables",
@@ -35,6 +38,7 @@ EXPORTS = [
     "tv_index_to_bytes", "tv_index_from_bytes", "tv_search_dev_noalloc", "tv_noalloc_scratch_bytes",
     "tv_debug_exact_redos", "tv_debug_sampling_plan", "tv_debug_merged_calls", "tv_debug_level_repeats", "tv_debug_workspace_bytes",
     "tv_debug_gathered_searches",
+    "tv_fp8_quantize_dev", "tv_fp8_matmul_dev", "tv_fp8_rescore_dev", "tv_fp8_rescore_workspace", "tv_sample_dev", "tv_sample_workspace",
 ]
 
 _lib = None
@@ -112,6 +116,14 @@ def lib():
     L.tv_debug_mfma_probe.argtypes = [vp, i32, i32, C.POINTER(C.c_float), C.POINTER(C.c_double)]
     L.tv_host_rotation_tables.argtypes = [i32, vp, vp, C.POINTER(i32), C.POINTER(C.c_float)]
     L.tv_host_codebook.argtypes = [i32, i32, vp, vp]
+    L.tv_fp8_quantize_dev.argtypes = [i32, vp, vp, i32, sz, sz, sz, i32, i32, vp, sz, vp, sz]
+    L.tv_fp8_matmul_dev.argtypes = [i32, vp, vp, sz, vp, sz, sz, vp, sz, vp, sz, sz, i32, sz, i32, vp, i32, sz]
+    L.tv_fp8_rescore_dev.argtypes = [i32, vp, vp, i32, sz, sz, vp, sz, vp, sz, sz, i32, sz, i32, vp, sz, sz, sz, vp, vp, vp, sz]
+    L.tv_fp8_rescore_workspace.restype = sz
+    L.tv_fp8_rescore_workspace.argtypes = [sz, sz]
+    L.tv_sample_dev.argtypes = [i32, vp, vp, i32, sz, sz, sz, vp, sz, vp, vp, vp, vp, vp, vp, vp, vp, sz]
+    L.tv_sample_workspace.restype = sz
+    L.tv_sample_workspace.argtypes = [sz, sz]
     _lib = L
     return L
 

@@ -17,6 +17,7 @@
 #include <vector>
 
 #include "tv_internal.h"
+#include "tv_ops.h"
 #include "tv_snapshot.h"
 
 namespace {
@@ -2185,6 +2186,23 @@ int search_merged(tv_index *ix, tv_request &r) {
 }
 
 }  // namespace
+
+namespace tv {
+int op_refused(const char *why) {
+    try {
+        g_last_error = why;
+    } catch (const std::exception &) {     // no memory for the text
+    }
+    return TV_ERR_BAD_ARGUMENT;
+}
+int op_failed(hipError_t e, const char *what) {
+    try {
+        return fail_hip(e, what);
+    } catch (const std::exception &) {
+        return TV_ERR_HIP;
+    }
+}
+}  // namespace tv
 
 extern "C" {
 
