@@ -144,7 +144,11 @@ def check_product(a, b, got):
     dim = x.shape[1]
     # sums in 32 bits: one rounding or truncation (2^-23) for each of dim products and additions, three more a block for its
     # scales; then half a step of the result's type, and for float16 half its smallest step
-    bound = (2 * dim + 3 * (-(-dim // 128))) * 2.0 ** -23 * (x.abs() @ y.abs().t()) + 2.0 ** -126
+    sums = x.abs() @ y.abs().t()
+    bound = (2 * dim + 3 * (-(-dim // 128))) * 2.0 ** -23 * sums + 2.0 ** -126
+    if got.dtype != torch.float32:
+        # the 8-bit matrix instructions add products in groups of eight, each cut off at 2^-13 of the largest: seven may lose that much
+        bound = bound + 7 * 2.0 ** -13 * sums
     step = torch.finfo(got.dtype).eps / 2
     bound = bound + (want.abs() + bound) * step + torch.finfo(got.dtype).smallest_normal * torch.finfo(got.dtype).eps
     over = want.abs() > torch.finfo(got.dtype).max
@@ -212,6 +216,26 @@ def test_matmul_nan_stays_in_its_row(fp8, scale, m):
     want[m // 2] = True
     want[:, 40] = True
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m", [1, 200])
+def test_matmul_every_scale_byte(fp8, dtype, m):
+    """Products of each e8m0 scale, the smallest and NaN among them, with one that brings it near 1."""
+    scale = torch.arange(256, device="cuda", dtype=torch.uint8)
+    codes = torch.randint(0, 256, (256, 128), generator=gen(15), device="cuda").to(torch.uint8)
+    codes[(codes & 0x78) < 0x30] = 0x38                    # magnitudes of 1/2 and more: normal numbers whatever the scale
+    codes[(codes & 0x7f) == 0x7f] = 0x3c
+    b = fp8.Fp8Rows(codes.view(torch.float8_e4m3fn), scale[:, None].view(torch.float8_e8m0fnu))
+    for e in (0, 1, 60, 127, 200, 254):
+        a = fp8.Fp8Rows(codes[:1].expand(m, -1).contiguous().view(torch.float8_e4m3fn), torch.full((m, 1), e, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu))
+        got = fp8.matmul(a, b, dtype=dtype)
+        assert bool(torch.isnan(got[:, 255]).all())
+        near = (scale.long() + e - 254 > -90) & (scale.long() + e - 254 < 90) & (scale.long() > 1) & (scale.long() < 240) & (torch.tensor(1 < e < 240, device="cuda"))
+        if dtype == torch.float16:
+            near &= (scale.long() + e - 254 > -20) & (scale.long() + e - 254 < -10)
+        if bool(near.any()):
+            check_product(a, fp8.Fp8Rows(b.codes[near], b.scales.view(torch.uint8)[near].view(torch.float8_e8m0fnu)), got[:, near])
 
 
 def test_matmul_zero_scales_and_extremes(fp8):

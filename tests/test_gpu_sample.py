@@ -20,7 +20,9 @@ def gen(seed):
 
 
 def plain_row(s, u, t, k, p, m, allowed):
-    """(slot, probability) of one row; s float64."""
+    """(slot, probability) of one row; s float64.  Weights are multiples of 2^-(63 - ceil(log2 n)): one below half of that is
+    never drawn, not even by u = 0."""
+    unit = 2.0 ** -(63 - max(1, int(len(s) - 1).bit_length()))
     s = np.where(allowed & ~np.isnan(s), s, -np.inf)
     if np.all(s == -np.inf):
         return -1, 0.0
@@ -34,14 +36,14 @@ def plain_row(s, u, t, k, p, m, allowed):
     if k > 0:
         order = order[:k]
     if p < 1:
-        mass = np.cumsum(w[order])
+        mass = np.cumsum(np.rint(w[order] / unit) * unit)
         stays = np.concatenate(([0.0], mass[:-1])) < p * mass[-1]
         stays[0] = True
         order = order[stays]
     if m > 0:
         order = order[w[order] >= min(m, 1.0)]
     kept = np.sort(order)
-    mass = np.cumsum(w[kept])
+    mass = np.cumsum(np.rint(w[kept] / unit) * unit)
     want = u * mass[-1]
     at = min(int(np.searchsorted(mass, want, side="right")), len(kept) - 1)
     return int(kept[at]), w[kept[at]] / mass[-1]
