@@ -247,6 +247,28 @@ __device__ __forceinline__ void store_out(void *out, size_t at, float v, int typ
     else static_cast<bf16 *>(out)[at] = bf16(v);
 }
 
+// Four results next to each other, those of them past `end` left out.
+__device__ __forceinline__ void store_out4(void *out, size_t row, uint32_t n, uint32_t end, v4f v, int type) {
+    typedef f16 v4h __attribute__((ext_vector_type(4)));
+    typedef bf16 v4b __attribute__((ext_vector_type(4)));
+    const size_t at = row + n;
+    if (n + 4u <= end) {
+        if (type == kF32) {
+            float *const to = static_cast<float *>(out) + at;
+            if ((reinterpret_cast<uintptr_t>(to) & 15) == 0) { *reinterpret_cast<v4f *>(to) = v; return; }
+        } else if (type == kF16) {
+            f16 *const to = static_cast<f16 *>(out) + at;
+            if ((reinterpret_cast<uintptr_t>(to) & 7) == 0) { *reinterpret_cast<v4h *>(to) = __builtin_convertvector(v, v4h); return; }
+        } else {
+            bf16 *const to = static_cast<bf16 *>(out) + at;
+            if ((reinterpret_cast<uintptr_t>(to) & 7) == 0) { *reinterpret_cast<v4b *>(to) = __builtin_convertvector(v, v4b); return; }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        if (n + r < end) store_out(out, at + r, v[r], type);
+}
+
 // Few rows of a: a wave to 16 rows of b, which it reads once, straight from memory, against all rows of a (MT tiles of 16).
 // Four blocks' loads are on their way at a time.
 constexpr int kDirectThreads = 256;
@@ -315,13 +337,187 @@ static hipError_t direct(const MatmulArgs &a, hipStream_t s) {
     const dim3 grid((a.b.rows + 63) / 64, tiles < 65535u ? tiles : 65535u);
     return launch(k_fp8_direct<EXACT, E8, MT>, grid, kDirectThreads, 0, s, a);
 }
-template <bool EXACT, bool E8>
+// Many rows of a: a workgroup to a tile of TM rows of a and TN of b, WM x WN waves.  A block's codes of both go to LDS, as they are,
+// while the block before is multiplied; a wave reads each operand once and keeps its part of the tile in registers.
+//
+// A row's block is 128 bytes in LDS, its eight runs of 16 swapped about by the row's number: eight neighbouring lanes, which read
+// the same run of eight rows, find it in different banks.  Loads that go past the registers write lane l at 16 l, so each lane asks for the
+// run that belongs there.
+enum { kScaleBytes = 0, kScaleRows = 1, kScaleTiles = 2 };      // e8m0; floats of each row of b; floats of 128 rows of b
+
+__device__ __forceinline__ void load16_to_lds(uint32_t lds, const uint8_t *base, uint32_t offset) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+template <int TM, int TN> constexpr size_t tile_lds() { return 2 * size_t(TM + TN) * (kScaleBlock + 4); }
+
+template <bool EXACT, int SC, int TM, int TN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_fp8_tile(MatmulArgs p, uint32_t m_tiles, uint32_t n_tiles, bool by_n, bool direct16) {
+    extern __shared__ uint8_t smem[];
+    constexpr int kWaves = WM * WN, kRows = TM + TN, kGroups = kRows / 8 / kWaves, MT = TM / WM / 16, NT = TN / WN / 16;
+    constexpr uint32_t kBuffer = kRows * kScaleBlock;
+    static_assert(kRows <= 64 * kWaves && kRows % (8 * kWaves) == 0, "a thread to a row's scale, whole groups of eight rows to a wave");
+    // Tiles of one strip follow each other on one XCD (workgroups go to the eight in turn), so that they find it in that one's L2.
+    uint32_t tm, tn;
+    {
+        const uint32_t xcd = blockIdx.x & 7u, i = blockIdx.x >> 3;
+        if (by_n) { tn = i / m_tiles * 8u + xcd; tm = i % m_tiles; }
+        else { tm = i / n_tiles * 8u + xcd; tn = i % n_tiles; }
+        if (tm >= m_tiles || tn >= n_tiles) return;
+    }
+    const uint32_t m0 = tm * TM, n0 = tn * TN;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)), col = lane & 15, g = lane >> 4;
+    const uint32_t blocks = (p.dim + kScaleBlock - 1) / kScaleBlock;
+    const uint32_t lds0 = uint32_t(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) uint8_t *)smem));
+    float *const scales = reinterpret_cast<float *>(smem + 2 * kBuffer);
+
+    // Of the rows of a and, after them, of b, wave w loads groups w, w + kWaves, ...: lane l row l / 8 of the group, run (l % 8) ^ (l / 8).
+    // (Rows past the end are the last one: their results are not stored.)
+    const uint8_t *const a0 = p.a.codes + size_t(m0) * p.a.stride, *const b0 = p.b.codes + size_t(n0) * p.b.stride;
+    const uint32_t run16 = uint32_t((lane & 7) ^ (lane >> 3)) * 16u;
+    uint32_t offset[kGroups];
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+        const uint32_t row = uint32_t((i * kWaves + wave) * 8 + (lane >> 3));
+        const bool of_a = row < uint32_t(TM);
+        const uint32_t r = of_a ? min(row, p.a.rows - 1 - m0) : min(row - TM, p.b.rows - 1 - n0);
+        offset[i] = r * uint32_t(of_a ? p.a.stride : p.b.stride) + run16;
+    }
+    auto stage = [&](uint32_t k, uint32_t buffer) {
+        if (direct16 && (k + 1) * kScaleBlock <= p.dim) {
+#pragma unroll
+            for (int i = 0; i < kGroups; ++i) {
+                const uint32_t group = uint32_t(i * kWaves + wave);
+                load16_to_lds(lds0 + buffer * kBuffer + group * 1024u, (group * 8 < TM ? a0 : b0) + size_t(k) * kScaleBlock, offset[i]);
+            }
+            return;
+        }
+#pragma unroll 1
+        for (int i = 0; i < kGroups; ++i) {
+            const uint32_t group = uint32_t(i * kWaves + wave), row = group * 8 + uint32_t(lane >> 3);
+            const uint8_t *at = row < uint32_t(TM) ? a0 + size_t(min(row, p.a.rows - 1 - m0)) * p.a.stride : b0 + size_t(min(row - TM, p.b.rows - 1 - n0)) * p.b.stride;
+            *reinterpret_cast<v4i *>(smem + buffer * kBuffer + group * 1024u + lane * 16) = codes16(at, k * kScaleBlock + run16, p.dim);
+        }
+    };
+    // A thread to a row's scale.
+    const uint32_t t = threadIdx.x;
+    const bool scale_a = t < uint32_t(TM), has_scale = t < uint32_t(kRows);
+    const size_t scale_at = scale_a ? size_t(min(m0 + t, p.a.rows - 1)) * p.a.scale_stride
+                                    : size_t(min(n0 + min(t, uint32_t(kRows - 1)) - TM, p.b.rows - 1) >> p.b.group_shift) * p.b.scale_stride;
+    const void *const scale_of_row = scale_a ? p.a.scales : p.b.scales;
+    auto load_scale = [&](uint32_t k) -> uint32_t {
+        if (!has_scale) return 0;
+        if (SC == kScaleBytes) return static_cast<const uint8_t *>(scale_of_row)[scale_at + k];
+        return static_cast<const uint32_t *>(scale_of_row)[scale_at + k];
+    };
+    auto put_scale = [&](uint32_t x, uint32_t buffer) {
+        if (has_scale) scales[buffer * kRows + t] = EXACT && SC == kScaleBytes ? e8_value(x) : __uint_as_float(x);
+    };
+
+    const int wm = wave % WM * (TM / WM), wn = wave / WM * (TN / WN);
+    v4f acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = v4f{0, 0, 0, 0};
+    // (rows of a tile of 16 start at a multiple of 8, so a lane's place within them decides the swap)
+    const uint32_t lo = uint32_t(col) * kScaleBlock + uint32_t(g ^ (col & 7)) * 16u, hi = uint32_t(col) * kScaleBlock + uint32_t((g + 4) ^ (col & 7)) * 16u;
+
+    stage(0, 0);
+    put_scale(load_scale(0), 0);
+    for (uint32_t k = 0; k < blocks; ++k) {
+        const uint32_t buffer = k & 1u;
+        wait_loads();
+        __syncthreads();
+        uint32_t next_scale = 0;
+        if (k + 1 < blocks) {
+            next_scale = load_scale(k + 1);
+            stage(k + 1, buffer ^ 1u);
+        }
+        const uint8_t *const ca = smem + buffer * kBuffer + wm * kScaleBlock, *const cb = smem + buffer * kBuffer + (TM + wn) * kScaleBlock;
+        const float *const sa = scales + buffer * kRows + wm, *const sb = scales + buffer * kRows + TM + wn;
+        Operand<EXACT> y[NT];
+        int ys[NT];
+        v4f yf[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            float s = 1.0f;
+            ys[j] = kUnitScale;
+            if (SC == kScaleBytes) { s = sb[j * 16 + col]; ys[j] = __float_as_int(s); }
+            if (SC == kScaleRows) yf[j] = *reinterpret_cast<const v4f *>(sb + j * 16 + 4 * g);
+            y[j].set(*reinterpret_cast<const v4i *>(cb + j * 16 * kScaleBlock + lo), *reinterpret_cast<const v4i *>(cb + j * 16 * kScaleBlock + hi), s);
+        }
+        // (the next 16 rows' codes are requested before the products of these, and no sooner: the tile fills the registers)
+        v4i xlo = *reinterpret_cast<const v4i *>(ca + lo), xhi = *reinterpret_cast<const v4i *>(ca + hi);
+        float xs = sa[col];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const float s = xs;
+            Operand<EXACT> x;
+            x.set(xlo, xhi, SC == kScaleBytes ? s : 1.0f);
+            if (i + 1 < MT) {
+                xlo = *reinterpret_cast<const v4i *>(ca + (i + 1) * 16 * kScaleBlock + lo);
+                xhi = *reinterpret_cast<const v4i *>(ca + (i + 1) * 16 * kScaleBlock + hi);
+                xs = sa[(i + 1) * 16 + col];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (SC == kScaleBytes) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = block_product(y[j], x, acc[i][j], ys[j], __float_as_int(s));
+            } else {
+                const float tile = SC == kScaleTiles ? s * sb[0] : 0.0f;      // (a wave's rows of b lie in one group)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const v4f part = block_product(y[j], x, v4f{0, 0, 0, 0}, kUnitScale, kUnitScale);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(part[r], SC == kScaleTiles ? tile : s * yf[j][r], acc[i][j][r]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (k + 1 < blocks) put_scale(next_scale, buffer ^ 1u);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const uint32_t m = m0 + uint32_t(wm + i * 16 + col);
+        if (m >= p.a.rows) continue;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) store_out4(p.out, size_t(m) * p.out_stride, n0 + uint32_t(wn + j * 16 + 4 * g), p.b.rows, acc[i][j], p.out_type);
+    }
+}
+
+template <bool EXACT, int SC, int TM, int TN, int WM, int WN>
+static hipError_t tile(const MatmulArgs &a, hipStream_t s) {
+    static_assert(SC != kScaleTiles || (kScaleBlock % (TN / WN) == 0 && TN % (TN / WN) == 0), "a wave's rows of b lie in one group");
+    const uint32_t mt = (a.a.rows + TM - 1) / TM, nt = (a.b.rows + TN - 1) / TN;
+    const bool by_n = nt >= mt;
+    const uint64_t grid = by_n ? (uint64_t(nt) + 7) / 8 * 8 * mt : (uint64_t(mt) + 7) / 8 * 8 * nt;
+    // 16 bytes at a time past the registers: rows at multiples of 16 bytes, and a tile's offsets in 32 bits
+    const bool direct16 = ((uintptr_t(a.a.codes) | uintptr_t(a.b.codes) | a.a.stride | a.b.stride) & 15) == 0 && a.a.stride < (1u << 23) && a.b.stride < (1u << 23);
+    const auto kernel = k_fp8_tile<EXACT, SC, TM, TN, WM, WN>;
+    if (const hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), tile_lds<TM, TN>()); e != hipSuccess) return e;
+    return launch(kernel, uint32_t(grid), 64 * WM * WN, tile_lds<TM, TN>(), s, a, mt, nt, by_n, direct16);
+}
+
+template <bool EXACT, int SC>
 static hipError_t matmul(const MatmulArgs &a, hipStream_t s) {
-    return a.a.rows <= 16 ? direct<EXACT, E8, 1>(a, s) : direct<EXACT, E8, 4>(a, s);
+    if (a.a.rows <= 16) return direct<EXACT, SC == kScaleBytes, 1>(a, s);
+    if (a.a.rows <= 64) return direct<EXACT, SC == kScaleBytes, 4>(a, s);
+    const uint64_t large = uint64_t((a.a.rows + 255) / 256) * ((a.b.rows + 255) / 256), middle = uint64_t((a.a.rows + 127) / 128) * ((a.b.rows + 127) / 128);
+    if constexpr (!EXACT || SC == kScaleBytes) {
+        if (large >= 200) return tile<EXACT, SC, 256, 256, 2, 4>(a, s);
+    }
+    if (middle >= 200) return tile<EXACT, SC, 128, 128, 2, 2>(a, s);
+    return tile<EXACT, SC, 64, 64, 2, 2>(a, s);
+}
+template <bool EXACT>
+static hipError_t matmul_as(const MatmulArgs &a, int scale_type, hipStream_t s) {
+    if (scale_type == kScaleE8M0) return matmul<EXACT, kScaleBytes>(a, s);
+    return a.b.group_shift == 0 ? matmul<EXACT, kScaleRows>(a, s) : matmul<EXACT, kScaleTiles>(a, s);
 }
 hipError_t launch_fp8_matmul(const MatmulArgs &a, int scale_type, hipStream_t s) {
-    if (a.out_type == kF32) return scale_type == kScaleE8M0 ? matmul<true, true>(a, s) : matmul<true, false>(a, s);
-    return scale_type == kScaleE8M0 ? matmul<false, true>(a, s) : matmul<false, false>(a, s);
+    return a.out_type == kF32 ? matmul_as<true>(a, scale_type, s) : matmul_as<false>(a, scale_type, s);
 }
 
 }  // namespace tv
