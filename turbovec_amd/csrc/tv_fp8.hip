@@ -198,15 +198,13 @@ __device__ __forceinline__ v4i codes16(const uint8_t *row, uint32_t k, uint32_t 
         __builtin_memcpy(&v, row + k, 16);
         return v;
     }
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        uint32_t x = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (k + w * 4 + i < dim) x |= uint32_t(row[k + w * 4 + i]) << (8 * i);
-        v[w] = int(x);
+    uint64_t lo = 0, hi = 0;
+#pragma unroll 1
+    for (uint32_t i = k < dim ? dim - k : 0u; i-- > 0;) {
+        hi = hi << 8 | lo >> 56;
+        lo = lo << 8 | row[k + i];
     }
-    return v;
+    return v4i{int(uint32_t(lo)), int(uint32_t(lo >> 32)), int(uint32_t(hi)), int(uint32_t(hi >> 32))};
 }
 
 // An operand of a block: 32 codes of a lane, as they are or as bfloat16 times a power of two.
@@ -245,28 +243,6 @@ __device__ __forceinline__ void store_out(void *out, size_t at, float v, int typ
     if (type == kF32) static_cast<float *>(out)[at] = v;
     else if (type == kF16) static_cast<f16 *>(out)[at] = f16(v);
     else static_cast<bf16 *>(out)[at] = bf16(v);
-}
-
-// Four results next to each other, those of them past `end` left out.
-__device__ __forceinline__ void store_out4(void *out, size_t row, uint32_t n, uint32_t end, v4f v, int type) {
-    typedef f16 v4h __attribute__((ext_vector_type(4)));
-    typedef bf16 v4b __attribute__((ext_vector_type(4)));
-    const size_t at = row + n;
-    if (n + 4u <= end) {
-        if (type == kF32) {
-            float *const to = static_cast<float *>(out) + at;
-            if ((reinterpret_cast<uintptr_t>(to) & 15) == 0) { *reinterpret_cast<v4f *>(to) = v; return; }
-        } else if (type == kF16) {
-            f16 *const to = static_cast<f16 *>(out) + at;
-            if ((reinterpret_cast<uintptr_t>(to) & 7) == 0) { *reinterpret_cast<v4h *>(to) = __builtin_convertvector(v, v4h); return; }
-        } else {
-            bf16 *const to = static_cast<bf16 *>(out) + at;
-            if ((reinterpret_cast<uintptr_t>(to) & 7) == 0) { *reinterpret_cast<v4b *>(to) = __builtin_convertvector(v, v4b); return; }
-        }
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-        if (n + r < end) store_out(out, at + r, v[r], type);
 }
 
 // Few rows of a: a wave to 16 rows of b, which it reads once, straight from memory, against all rows of a (MT tiles of 16).
@@ -350,13 +326,48 @@ __device__ __forceinline__ void load16_to_lds(uint32_t lds, const uint8_t *base,
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-template <int TM, int TN> constexpr size_t tile_lds() { return 2 * size_t(TM + TN) * (kScaleBlock + 4); }
+template <int TM, int TN, int WM, int WN> constexpr size_t tile_lds() { return 2 * (size_t(TM + TN) * kScaleBlock + 64 * WM * WN * 4); }
+
+// A strip of 16 rows and COLS columns in LDS, with 16 bytes between rows so that lanes of neighbouring rows write to different banks.
+template <typename T, int COLS> constexpr int kStripBytes = 16 * (COLS * int(sizeof(T)) + 16);
+
+// A wave's results, whose lane l holds columns 4 * (l / 16) .. + 3 of row l % 16 of each tile, to rows from m on and columns from n on.
+// wide: rows of the result start at multiples of 16 bytes.
+template <typename T, int COLS, int MT, int NT>
+__device__ __forceinline__ void store_strips(const MatmulArgs &p, const v4f (&acc)[MT][NT], uint8_t *strip, uint32_t m, uint32_t n, bool wide, int lane) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    constexpr int kEach = 16 / int(sizeof(T)), kLanes = COLS / kEach, kRowsAtOnce = 64 / kLanes, kRow = COLS * int(sizeof(T)) + 16;
+    const int col = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) *reinterpret_cast<T4 *>(strip + col * kRow + (j * 16 + 4 * g) * int(sizeof(T))) = __builtin_convertvector(acc[i][j], T4);
+#pragma unroll
+        for (int r = 0; r < 16; r += kRowsAtOnce) {
+            const int row = r + lane / kLanes, at = lane % kLanes * kEach;
+            const v4i x = *reinterpret_cast<const v4i *>(strip + row * kRow + at * int(sizeof(T)));
+            const uint32_t om = m + uint32_t(i * 16 + row), on = n + uint32_t(at);
+            if (om >= p.a.rows || on >= p.b.rows) continue;
+            T *const to = static_cast<T *>(p.out) + size_t(om) * p.out_stride + on;
+            if (wide && on + kEach <= p.b.rows) {
+                *reinterpret_cast<v4i *>(to) = x;
+            } else {
+                T e[kEach];
+                __builtin_memcpy(e, &x, 16);
+#pragma unroll
+                for (int l = 0; l < kEach; ++l)
+                    if (on + l < p.b.rows) to[l] = e[l];
+            }
+        }
+    }
+}
 
 template <bool EXACT, int SC, int TM, int TN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, 2) void k_fp8_tile(MatmulArgs p, uint32_t m_tiles, uint32_t n_tiles, bool by_n, bool direct16) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_fp8_tile(MatmulArgs p, uint32_t m_tiles, uint32_t n_tiles, bool by_n, bool direct16, bool wide) {
     extern __shared__ uint8_t smem[];
-    constexpr int kWaves = WM * WN, kRows = TM + TN, kGroups = kRows / 8 / kWaves, MT = TM / WM / 16, NT = TN / WN / 16;
-    constexpr uint32_t kBuffer = kRows * kScaleBlock;
+    constexpr int kWaves = WM * WN, kRows = TM + TN, kGroups = kRows / 8 / kWaves, MT = TM / WM / 16, NT = TN / WN / 16, kEach = (kGroups + MT - 1) / MT;
+    constexpr uint32_t kBuffer = kRows * kScaleBlock, kScales = 64 * kWaves;
+    static_assert(kWaves * kStripBytes<float, TN / WN> <= int(2 * kBuffer), "strips of all waves at once");
     static_assert(kRows <= 64 * kWaves && kRows % (8 * kWaves) == 0, "a thread to a row's scale, whole groups of eight rows to a wave");
     // Tiles of one strip follow each other on one XCD (workgroups go to the eight in turn), so that they find it in that one's L2.
     uint32_t tm, tn;
@@ -384,15 +395,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_fp8_tile(MatmulArgs p, uint
         const uint32_t r = of_a ? min(row, p.a.rows - 1 - m0) : min(row - TM, p.b.rows - 1 - n0);
         offset[i] = r * uint32_t(of_a ? p.a.stride : p.b.stride) + run16;
     }
-    auto stage = [&](uint32_t k, uint32_t buffer) {
-        if (direct16 && (k + 1) * kScaleBlock <= p.dim) {
-#pragma unroll
-            for (int i = 0; i < kGroups; ++i) {
-                const uint32_t group = uint32_t(i * kWaves + wave);
-                load16_to_lds(lds0 + buffer * kBuffer + group * 1024u, (group * 8 < TM ? a0 : b0) + size_t(k) * kScaleBlock, offset[i]);
-            }
-            return;
-        }
+    const uint32_t whole = direct16 ? p.dim / kScaleBlock : 0u;      // blocks that go to LDS past the registers: the first ones
+    auto load_group = [&](uint32_t k, uint32_t buffer, int i) {
+        const uint32_t group = uint32_t(i * kWaves + wave);
+        load16_to_lds(lds0 + buffer * kBuffer + group * 1024u, (group * 8 < TM ? a0 : b0) + size_t(k) * kScaleBlock, offset[i]);
+    };
+    auto copy_groups = [&](uint32_t k, uint32_t buffer) {
 #pragma unroll 1
         for (int i = 0; i < kGroups; ++i) {
             const uint32_t group = uint32_t(i * kWaves + wave), row = group * 8 + uint32_t(lane >> 3);
@@ -400,19 +408,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_fp8_tile(MatmulArgs p, uint
             *reinterpret_cast<v4i *>(smem + buffer * kBuffer + group * 1024u + lane * 16) = codes16(at, k * kScaleBlock + run16, p.dim);
         }
     };
-    // A thread to a row's scale.
+    // A thread to a row's scale; threads beyond the rows load the last one's and put it where nobody looks.
     const uint32_t t = threadIdx.x;
-    const bool scale_a = t < uint32_t(TM), has_scale = t < uint32_t(kRows);
+    const bool scale_a = t < uint32_t(TM);
     const size_t scale_at = scale_a ? size_t(min(m0 + t, p.a.rows - 1)) * p.a.scale_stride
                                     : size_t(min(n0 + min(t, uint32_t(kRows - 1)) - TM, p.b.rows - 1) >> p.b.group_shift) * p.b.scale_stride;
     const void *const scale_of_row = scale_a ? p.a.scales : p.b.scales;
     auto load_scale = [&](uint32_t k) -> uint32_t {
-        if (!has_scale) return 0;
         if (SC == kScaleBytes) return static_cast<const uint8_t *>(scale_of_row)[scale_at + k];
         return static_cast<const uint32_t *>(scale_of_row)[scale_at + k];
     };
     auto put_scale = [&](uint32_t x, uint32_t buffer) {
-        if (has_scale) scales[buffer * kRows + t] = EXACT && SC == kScaleBytes ? e8_value(x) : __uint_as_float(x);
+        scales[buffer * kScales + t] = EXACT && SC == kScaleBytes ? e8_value(x) : __uint_as_float(x);
     };
 
     const int wm = wave % WM * (TM / WM), wn = wave / WM * (TN / WN);
@@ -424,19 +431,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_fp8_tile(MatmulArgs p, uint
     // (rows of a tile of 16 start at a multiple of 8, so a lane's place within them decides the swap)
     const uint32_t lo = uint32_t(col) * kScaleBlock + uint32_t(g ^ (col & 7)) * 16u, hi = uint32_t(col) * kScaleBlock + uint32_t((g + 4) ^ (col & 7)) * 16u;
 
-    stage(0, 0);
-    put_scale(load_scale(0), 0);
-    for (uint32_t k = 0; k < blocks; ++k) {
-        const uint32_t buffer = k & 1u;
-        wait_loads();
-        __syncthreads();
-        uint32_t next_scale = 0;
-        if (k + 1 < blocks) {
-            next_scale = load_scale(k + 1);
-            stage(k + 1, buffer ^ 1u);
-        }
+    // (Straight-line code, with loads of the next block or without: across a branch the compiler moves products behind the
+    // wait for those loads.)
+    auto multiply = [&](uint32_t k, uint32_t buffer, auto loads) {
         const uint8_t *const ca = smem + buffer * kBuffer + wm * kScaleBlock, *const cb = smem + buffer * kBuffer + (TM + wn) * kScaleBlock;
-        const float *const sa = scales + buffer * kRows + wm, *const sb = scales + buffer * kRows + TM + wn;
+        const float *const sa = scales + buffer * kScales + wm, *const sb = scales + buffer * kScales + TM + wn;
         Operand<EXACT> y[NT];
         int ys[NT];
         v4f yf[NT];
@@ -461,6 +460,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_fp8_tile(MatmulArgs p, uint
                 xhi = *reinterpret_cast<const v4i *>(ca + (i + 1) * 16 * kScaleBlock + hi);
                 xs = sa[(i + 1) * 16 + col];
             }
+            // the next block's loads one by one, between products: all at once they hold up the wave until the last is accepted
+            if constexpr (decltype(loads)::value) {
+#pragma unroll
+                for (int l = i * kEach; l < (i + 1) * kEach && l < kGroups; ++l) load_group(k + 1, buffer ^ 1u, l);
+            }
             __builtin_amdgcn_sched_barrier(0);
             if (SC == kScaleBytes) {
 #pragma unroll
@@ -476,15 +480,35 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_fp8_tile(MatmulArgs p, uint
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-        if (k + 1 < blocks) put_scale(next_scale, buffer ^ 1u);
-    }
+    };
+    if (whole != 0) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const uint32_t m = m0 + uint32_t(wm + i * 16 + col);
-        if (m >= p.a.rows) continue;
-#pragma unroll
-        for (int j = 0; j < NT; ++j) store_out4(p.out, size_t(m) * p.out_stride, n0 + uint32_t(wn + j * 16 + 4 * g), p.b.rows, acc[i][j], p.out_type);
+        for (int i = 0; i < kGroups; ++i) load_group(0, 0, i);
+        put_scale(load_scale(0), 0);
     }
+    uint32_t k = 0;
+    for (; k + 1 < whole; ++k) {
+        wait_loads();
+        __syncthreads();
+        const uint32_t next_scale = load_scale(k + 1);
+        multiply(k, k & 1u, IntC<1>{});
+        put_scale(next_scale, (k & 1u) ^ 1u);
+    }
+    for (; k < blocks; ++k) {      // the last whole block, and one that ends early; all of them where rows start anywhere
+        if (k >= whole) {
+            __syncthreads();
+            copy_groups(k, k & 1u);
+            put_scale(load_scale(k), k & 1u);
+        }
+        wait_loads();
+        __syncthreads();
+        multiply(k, k & 1u, IntC<0>{});
+    }
+    // Sixteen rows of a wave's results at a time go through LDS, so that they leave in runs of whole cache lines.
+    __syncthreads();
+    if (EXACT) store_strips<float, TN / WN, MT, NT>(p, acc, smem + wave * kStripBytes<float, TN / WN>, m0 + wm, n0 + wn, wide, lane);
+    else if (p.out_type == kF16) store_strips<f16, TN / WN, MT, NT>(p, acc, smem + wave * kStripBytes<f16, TN / WN>, m0 + wm, n0 + wn, wide, lane);
+    else store_strips<bf16, TN / WN, MT, NT>(p, acc, smem + wave * kStripBytes<bf16, TN / WN>, m0 + wm, n0 + wn, wide, lane);
 }
 
 template <bool EXACT, int SC, int TM, int TN, int WM, int WN>
@@ -495,9 +519,11 @@ static hipError_t tile(const MatmulArgs &a, hipStream_t s) {
     const uint64_t grid = by_n ? (uint64_t(nt) + 7) / 8 * 8 * mt : (uint64_t(mt) + 7) / 8 * 8 * nt;
     // 16 bytes at a time past the registers: rows at multiples of 16 bytes, and a tile's offsets in 32 bits
     const bool direct16 = ((uintptr_t(a.a.codes) | uintptr_t(a.b.codes) | a.a.stride | a.b.stride) & 15) == 0 && a.a.stride < (1u << 23) && a.b.stride < (1u << 23);
+    const size_t size = EXACT ? 4 : 2;
+    const bool wide = ((uintptr_t(a.out) | a.out_stride * size) & 15) == 0;
     const auto kernel = k_fp8_tile<EXACT, SC, TM, TN, WM, WN>;
-    if (const hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), tile_lds<TM, TN>()); e != hipSuccess) return e;
-    return launch(kernel, uint32_t(grid), 64 * WM * WN, tile_lds<TM, TN>(), s, a, mt, nt, by_n, direct16);
+    if (const hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), tile_lds<TM, TN, WM, WN>()); e != hipSuccess) return e;
+    return launch(kernel, uint32_t(grid), 64 * WM * WN, tile_lds<TM, TN, WM, WN>(), s, a, mt, nt, by_n, direct16, wide);
 }
 
 template <bool EXACT, int SC>
