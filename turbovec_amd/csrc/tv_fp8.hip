@@ -245,73 +245,158 @@ __device__ __forceinline__ void store_out(void *out, size_t at, float v, int typ
     else static_cast<bf16 *>(out)[at] = bf16(v);
 }
 
-// Few rows of a: a wave to 16 rows of b, which it reads once, straight from memory, against all rows of a (MT tiles of 16).
-// Four blocks' loads are on their way at a time.
-constexpr int kDirectThreads = 256;
-template <bool EXACT, bool E8, int MT>
-__global__ __launch_bounds__(kDirectThreads) void k_fp8_direct(MatmulArgs p) {
-    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-    const uint32_t n0 = (blockIdx.x * (kDirectThreads / 64) + (threadIdx.x >> 6)) * 16u;
-    if (n0 >= p.b.rows) return;
-    const uint32_t blocks = (p.dim + kScaleBlock - 1) / kScaleBlock;
-    // (rows past the end are the last one: their results are not stored)
-    const uint32_t br = min(n0 + uint32_t(col), p.b.rows - 1);
-    const uint8_t *b = p.b.codes + size_t(br) * p.b.stride;
-    const size_t bs_at = size_t(br >> p.b.group_shift) * p.b.scale_stride;
-    for (uint32_t m0 = blockIdx.y * (16u * MT); m0 < p.a.rows; m0 += gridDim.y * (16u * MT)) {
-        const uint8_t *a[MT];
-        uint32_t ar[MT];
-        v4f acc[MT];
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            ar[t] = min(m0 + uint32_t(t * 16 + col), p.a.rows - 1);
-            a[t] = p.a.codes + size_t(ar[t]) * p.a.stride;
-            acc[t] = v4f{0, 0, 0, 0};
-        }
-        for (uint32_t k = 0; k < blocks; ++k) {
-            const uint32_t lo = k * kScaleBlock + g * 16, hi = lo + 64;
-            Operand<EXACT> bv, av;
-            const v4i b0 = codes16(b, lo, p.dim), b1 = codes16(b, hi, p.dim);
-            if (E8) {
-                const int bs = static_cast<const uint8_t *>(p.b.scales)[bs_at + k];
-                bv.set(b0, b1, e8_value(bs));
-#pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    const int as = static_cast<const uint8_t *>(p.a.scales)[size_t(ar[t]) * p.a.scale_stride + k];
-                    av.set(codes16(a[t], lo, p.dim), codes16(a[t], hi, p.dim), e8_value(as));
-                    acc[t] = block_product(av, bv, acc[t], as, bs);
-                }
+// Up to sixteen rows of a: bound by reading b once.  A wave streams 16 rows of b from memory into registers, four blocks while the four
+// before are multiplied, and goes on to its next 16 rows without a pause; a lies in LDS.  Where there are few rows of b (SPLIT), the four
+// waves of a workgroup share 16 rows, each taking every fourth step, and their sums are added in the waves' order.
+constexpr int kDirectThreads = 256, kDirectWaves = kDirectThreads / 64, kDirectBlocks = 4;
+constexpr size_t kDirectLds = 64 << 10;      // of a's rows, at most
+
+// Scales of kDirectBlocks blocks from k on, of `blocks` in the row; those past the end are whatever.
+typedef int v4i_any __attribute__((ext_vector_type(4), aligned(1)));
+struct Scales4 {
+    uint32_t v[4];
+    template <bool E8>
+    __device__ __forceinline__ void load(const void *scales, size_t row, uint32_t k, uint32_t blocks) {
+        static_assert(kDirectBlocks == 4, "a word of bytes");
+        if (E8) {
+            const uint8_t *const s = static_cast<const uint8_t *>(scales) + row;
+            if (k + 4u <= blocks) {
+                __builtin_memcpy(&v[0], s + k, 4);
             } else {
-                const float bs = static_cast<const float *>(p.b.scales)[bs_at + k];
-                bv.set(b0, b1, 1.0f);
-#pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    av.set(codes16(a[t], lo, p.dim), codes16(a[t], hi, p.dim), 1.0f);
-                    const v4f part = block_product(av, bv, v4f{0, 0, 0, 0}, kUnitScale, kUnitScale);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const uint32_t m = min(m0 + uint32_t(t * 16 + 4 * g + r), p.a.rows - 1);
-                        acc[t][r] = fmaf(part[r], bs * static_cast<const float *>(p.a.scales)[size_t(m) * p.a.scale_stride + k], acc[t][r]);
-                    }
-                }
+                v[0] = 0;
+                for (uint32_t i = 0; k + i < blocks; ++i) v[0] |= uint32_t(s[k + i]) << (8 * i);
             }
-        }
+        } else {
+            const uint32_t *const s = static_cast<const uint32_t *>(scales) + row;
+            if (k + 4u <= blocks) __builtin_memcpy(v, s + k, 16);
+            else
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const uint32_t m = m0 + uint32_t(t * 16 + 4 * g + r);
-                if (m < p.a.rows && n0 + col < p.b.rows) store_out(p.out, size_t(m) * p.out_stride + n0 + col, acc[t][r], p.out_type);
-            }
+                for (int i = 0; i < 4; ++i) v[i] = s[min(k + i, blocks - 1)];
         }
+    }
+    template <bool E8>
+    __device__ __forceinline__ uint32_t at(int i) const { return E8 ? (v[0] >> (8 * i)) & 255u : v[i]; }
+};
+
+__host__ __device__ inline uint32_t direct_row(uint32_t dim) { return (dim + 127u) / 128u * 128u + 16u; }     // (rows of a a few banks apart)
+inline size_t direct_lds(uint32_t rows, uint32_t dim) { return size_t(rows) * direct_row(dim) + (dim + 127) / 128 * 64 + kDirectWaves * 64 * 16; }
+
+template <bool EXACT, bool E8, bool SPLIT>
+__global__ __launch_bounds__(kDirectThreads, SPLIT ? 2 : E8 || !EXACT ? 4 : 3) void k_fp8_direct(MatmulArgs p) {
+    extern __shared__ uint8_t smem[];
+    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
+    const uint32_t blocks = (p.dim + kScaleBlock - 1) / kScaleBlock, whole = p.dim / kScaleBlock, row_bytes = direct_row(p.dim), m = p.a.rows;
+    uint32_t *const a_scales = reinterpret_cast<uint32_t *>(smem + m * row_bytes);       // [block][16]
+    v4f *const sums = reinterpret_cast<v4f *>(a_scales + blocks * 16);                   // SPLIT: [wave][lane]
+    for (uint32_t i = threadIdx.x; i < m * blocks * 8u; i += kDirectThreads) {
+        const uint32_t r = i / (blocks * 8u), c = i % (blocks * 8u) * 16u;
+        *reinterpret_cast<v4i *>(smem + r * row_bytes + c) = codes16(p.a.codes + size_t(r) * p.a.stride, c, p.dim);
+    }
+    for (uint32_t i = threadIdx.x; i < blocks * 16u; i += kDirectThreads) {
+        const size_t at = size_t(min(i & 15u, m - 1)) * p.a.scale_stride + (i >> 4);
+        a_scales[i] = E8 ? static_cast<const uint8_t *>(p.a.scales)[at] : static_cast<const uint32_t *>(p.a.scales)[at];
+    }
+    __syncthreads();
+    // (rows past the end are the last one: their results are not stored)
+    const uint8_t *const a = smem + min(uint32_t(col), m - 1) * row_bytes + g * 16;
+
+    const uint32_t tiles = (p.b.rows + 15) / 16, steps = (whole + kDirectBlocks - 1) / kDirectBlocks;
+    const uint32_t tile_stride = SPLIT ? gridDim.x : gridDim.x * kDirectWaves, step_stride = SPLIT ? kDirectWaves : 1, first_step = SPLIT ? wave : 0;
+    struct Place {
+        uint32_t tile, step;
+        const uint8_t *codes;
+        size_t scales;
+    };
+    auto go_to = [&](Place &at, uint32_t tile) {
+        const uint32_t row = min(tile * 16u + uint32_t(col), p.b.rows - 1);
+        at = Place{tile, first_step, p.b.codes + size_t(row) * p.b.stride + g * 16, size_t(row >> p.b.group_shift) * p.b.scale_stride};
+    };
+    struct Step {
+        v4i codes[kDirectBlocks][2];
+        Scales4 scales;
+    };
+    auto load = [&](Step &s, const Place &at) {
+        if (at.tile >= tiles || at.step >= steps) return;
+#pragma unroll
+        for (int i = 0; i < kDirectBlocks; ++i) {
+            const uint8_t *const from = at.codes + min(at.step * kDirectBlocks + i, whole - 1) * kScaleBlock;
+            s.codes[i][0] = *reinterpret_cast<const v4i_any *>(from);
+            s.codes[i][1] = *reinterpret_cast<const v4i_any *>(from + 64);
+        }
+        s.scales.template load<E8>(p.b.scales, at.scales, at.step * kDirectBlocks, blocks);
+    };
+    v4f acc = v4f{0, 0, 0, 0};
+    auto block = [&](uint32_t k, const v4i &b0, const v4i &b1, uint32_t bs) {
+        const uint8_t *const from = a + k * kScaleBlock;
+        const v4i a0 = *reinterpret_cast<const v4i *>(from), a1 = *reinterpret_cast<const v4i *>(from + 64);
+        Operand<EXACT> x, y;
+        if (E8) {
+            const uint32_t as = a_scales[k * 16 + col];
+            x.set(a0, a1, EXACT ? e8_value(as) : 1.0f);
+            y.set(b0, b1, EXACT ? e8_value(bs) : 1.0f);
+            acc = block_product(x, y, acc, int(as), int(bs));
+        } else {
+            x.set(a0, a1, 1.0f);
+            y.set(b0, b1, 1.0f);
+            const v4f part = block_product(x, y, v4f{0, 0, 0, 0}, kUnitScale, kUnitScale);
+            const v4f as = *reinterpret_cast<const v4f *>(a_scales + k * 16 + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[r] = fmaf(part[r], __uint_as_float(bs) * as[r], acc[r]);
+        }
+    };
+    auto multiply = [&](const Step &s, const Place &at) {
+#pragma unroll
+        for (int i = 0; i < kDirectBlocks; ++i) {
+            const uint32_t k = at.step * kDirectBlocks + i;
+            if (k < whole) block(k, s.codes[i][0], s.codes[i][1], s.scales.template at<E8>(i));
+        }
+    };
+    auto finish = [&](const Place &at) {
+        if (whole < blocks && (!SPLIT || wave == 0)) {         // a last block that ends early
+            const v4i b0 = codes16(at.codes - g * 16, whole * kScaleBlock + g * 16, p.dim), b1 = codes16(at.codes - g * 16, whole * kScaleBlock + 64 + g * 16, p.dim);
+            block(whole, b0, b1, E8 ? static_cast<const uint8_t *>(p.b.scales)[at.scales + whole] : static_cast<const uint32_t *>(p.b.scales)[at.scales + whole]);
+        }
+        if (SPLIT) {
+            sums[threadIdx.x] = acc;
+            __syncthreads();
+            if (wave != 0) return;
+#pragma unroll
+            for (int w = 1; w < kDirectWaves; ++w) acc += sums[w * 64 + lane];
+        }
+        const uint32_t n = at.tile * 16u + uint32_t(col);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (uint32_t(4 * g + r) < m && n < p.b.rows) store_out(p.out, size_t(4 * g + r) * p.out_stride + n, acc[r], p.out_type);
+        acc = v4f{0, 0, 0, 0};
+    };
+    Place here, next;
+    Step even, odd;
+    go_to(here, SPLIT ? blockIdx.x : blockIdx.x * kDirectWaves + wave);
+    load(even, here);
+    auto turn = [&](const Step &now, Step &then) {
+        next = here;
+        next.step += step_stride;
+        if (next.step >= steps) go_to(next, SPLIT ? tiles : here.tile + tile_stride);
+        load(then, next);
+        multiply(now, here);
+        if (next.tile != here.tile) finish(here);
+        here = next;
+    };
+    while (here.tile < tiles) {
+        turn(even, odd);
+        if (here.tile >= tiles) break;
+        turn(odd, even);
     }
 }
 
-template <bool EXACT, bool E8, int MT>
+template <bool EXACT, bool E8, bool SPLIT>
 static hipError_t direct(const MatmulArgs &a, hipStream_t s) {
-    const uint32_t tiles = (a.a.rows + 16 * MT - 1) / (16 * MT);
-    const dim3 grid((a.b.rows + 63) / 64, tiles < 65535u ? tiles : 65535u);
-    return launch(k_fp8_direct<EXACT, E8, MT>, grid, kDirectThreads, 0, s, a);
+    const uint32_t tiles = (a.b.rows + 15) / 16, most = SPLIT ? tiles : 256 * (E8 || !EXACT ? 4 : 3);      // (as many as there are at a time)
+    const uint32_t grid = SPLIT ? tiles : (tiles + kDirectWaves - 1) / kDirectWaves;
+    const size_t lds = direct_lds(a.a.rows, a.dim);
+    const auto kernel = k_fp8_direct<EXACT, E8, SPLIT>;
+    if (const hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), lds); e != hipSuccess) return e;
+    return launch(kernel, grid < most ? grid : most, kDirectThreads, lds, s, a);
 }
 // Many rows of a: a workgroup to a tile of TM rows of a and TN of b, WM x WN waves.  A block's codes of both go to LDS, as they are,
 // while the block before is multiplied; a wave reads each operand once and keeps its part of the tile in registers.
@@ -528,14 +613,20 @@ static hipError_t tile(const MatmulArgs &a, hipStream_t s) {
 
 template <bool EXACT, int SC>
 static hipError_t matmul(const MatmulArgs &a, hipStream_t s) {
-    if (a.a.rows <= 16) return direct<EXACT, SC == kScaleBytes, 1>(a, s);
-    if (a.a.rows <= 64) return direct<EXACT, SC == kScaleBytes, 4>(a, s);
-    const uint64_t large = uint64_t((a.a.rows + 255) / 256) * ((a.b.rows + 255) / 256), middle = uint64_t((a.a.rows + 127) / 128) * ((a.b.rows + 127) / 128);
-    if constexpr (!EXACT || SC == kScaleBytes) {
-        if (large >= 200) return tile<EXACT, SC, 256, 256, 2, 4>(a, s);
+    if (a.a.rows <= 16 && size_t(a.a.rows) * direct_row(a.dim) <= kDirectLds) {
+        // (sixteen rows to a wave leave waves without any)
+        return a.b.rows < 256 * 4 * 16 ? direct<EXACT, SC == kScaleBytes, true>(a, s) : direct<EXACT, SC == kScaleBytes, false>(a, s);
     }
-    if (middle >= 200) return tile<EXACT, SC, 128, 128, 2, 2>(a, s);
-    return tile<EXACT, SC, 64, 64, 2, 2>(a, s);
+    // A CU's time: the tiles it gets times what one takes.
+    auto time = [&](uint32_t tm, uint32_t tn, double rate) {
+        const uint64_t tiles = uint64_t((a.a.rows + tm - 1) / tm) * ((a.b.rows + tn - 1) / tn);
+        return double((tiles + 255) / 256) * tm * tn / rate;
+    };
+    const double l = time(256, 256, 1.0), m = time(128, 128, 0.75), sm = time(64, 64, 0.55);
+    if constexpr (!EXACT || SC == kScaleBytes) {
+        if (l <= m && l <= sm) return tile<EXACT, SC, 256, 256, 2, 4>(a, s);
+    }
+    return m <= sm ? tile<EXACT, SC, 128, 128, 2, 2>(a, s) : tile<EXACT, SC, 64, 64, 2, 2>(a, s);
 }
 template <bool EXACT>
 static hipError_t matmul_as(const MatmulArgs &a, int scale_type, hipStream_t s) {
