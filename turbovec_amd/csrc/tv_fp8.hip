@@ -191,20 +191,31 @@ constexpr int kUnitScale = 0x7f;             // 2^0
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef __bf16 v2b __attribute__((ext_vector_type(2)));
 
-// 16 codes of a row from k on, those past `dim` zero, without touching what lies behind the row.
-__device__ __forceinline__ v4i codes16(const uint8_t *row, uint32_t k, uint32_t dim) {
-    v4i v;
-    if (k + 16u <= dim) {
-        __builtin_memcpy(&v, row + k, 16);
-        return v;
-    }
-    uint64_t lo = 0, hi = 0;
-#pragma unroll 1
-    for (uint32_t i = k < dim ? dim - k : 0u; i-- > 0;) {
-        hi = hi << 8 | lo >> 56;
-        lo = lo << 8 | row[k + i];
-    }
+typedef int v4i_any __attribute__((ext_vector_type(4), aligned(1)));
+
+// 16 bytes moved down by so many, zeros from above; 16 and more leave nothing.
+__device__ __forceinline__ v4i bytes_down(v4i v, uint32_t bytes) {
+    uint64_t lo = uint64_t(uint32_t(v[0])) | uint64_t(uint32_t(v[1])) << 32, hi = uint64_t(uint32_t(v[2])) | uint64_t(uint32_t(v[3])) << 32;
+    if (bytes & 8u) { lo = hi; hi = 0; }
+    const uint32_t bits = (bytes & 7u) * 8u;
+    lo = lo >> bits | (hi << 1) << (63u - bits);
+    hi >>= bits;
+    if (bytes >= 16u) lo = hi = 0;
     return v4i{int(uint32_t(lo)), int(uint32_t(lo >> 32)), int(uint32_t(hi)), int(uint32_t(hi >> 32))};
+}
+// 16 codes of a row from k on, those past `dim` zero, without touching what lies behind the row: a run that the row ends in is
+// the end of the row's last 16 codes.
+__device__ __forceinline__ v4i codes16(const uint8_t *row, uint32_t k, uint32_t dim) {
+    if (dim >= 16u) {
+        const uint32_t at = min(k, dim - 16u);
+        return bytes_down(*reinterpret_cast<const v4i_any *>(row + at), k - at);
+    }
+    v4i v{0, 0, 0, 0};
+    for (uint32_t i = 0; k + i < dim; ++i) {
+        const v4i x = bytes_down(v4i{0, 0, 0, int(uint32_t(row[k + i]) << 24)}, 15u - i);
+        v |= x;
+    }
+    return v;
 }
 
 // An operand of a block: 32 codes of a lane, as they are or as bfloat16 times a power of two.
@@ -249,10 +260,10 @@ __device__ __forceinline__ void store_out(void *out, size_t at, float v, int typ
 // before are multiplied, and goes on to its next 16 rows without a pause; a lies in LDS.  Where there are few rows of b (SPLIT), the four
 // waves of a workgroup share 16 rows, each taking every fourth step, and their sums are added in the waves' order.
 constexpr int kDirectThreads = 256, kDirectWaves = kDirectThreads / 64, kDirectBlocks = 4;
+constexpr uint32_t kDirectGroups = 4;         // workgroups of a compute unit at a time
 constexpr size_t kDirectLds = 64 << 10;      // of a's rows, at most
 
 // Scales of kDirectBlocks blocks from k on, of `blocks` in the row; those past the end are whatever.
-typedef int v4i_any __attribute__((ext_vector_type(4), aligned(1)));
 struct Scales4 {
     uint32_t v[4];
     template <bool E8>
@@ -282,7 +293,7 @@ __host__ __device__ inline uint32_t direct_row(uint32_t dim) { return (dim + 127
 inline size_t direct_lds(uint32_t rows, uint32_t dim) { return size_t(rows) * direct_row(dim) + (dim + 127) / 128 * 64 + kDirectWaves * 64 * 16; }
 
 template <bool EXACT, bool E8, bool SPLIT>
-__global__ __launch_bounds__(kDirectThreads, SPLIT ? 2 : E8 || !EXACT ? 4 : 3) void k_fp8_direct(MatmulArgs p) {
+__global__ __launch_bounds__(kDirectThreads, kDirectGroups) void k_fp8_direct(MatmulArgs p) {
     extern __shared__ uint8_t smem[];
     const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
     const uint32_t blocks = (p.dim + kScaleBlock - 1) / kScaleBlock, whole = p.dim / kScaleBlock, row_bytes = direct_row(p.dim), m = p.a.rows;
@@ -300,7 +311,7 @@ __global__ __launch_bounds__(kDirectThreads, SPLIT ? 2 : E8 || !EXACT ? 4 : 3) v
     // (rows past the end are the last one: their results are not stored)
     const uint8_t *const a = smem + min(uint32_t(col), m - 1) * row_bytes + g * 16;
 
-    const uint32_t tiles = (p.b.rows + 15) / 16, steps = (whole + kDirectBlocks - 1) / kDirectBlocks;
+    const uint32_t tiles = (p.b.rows + 15) / 16, steps = (blocks + kDirectBlocks - 1) / kDirectBlocks;
     const uint32_t tile_stride = SPLIT ? gridDim.x : gridDim.x * kDirectWaves, step_stride = SPLIT ? kDirectWaves : 1, first_step = SPLIT ? wave : 0;
     struct Place {
         uint32_t tile, step;
@@ -309,7 +320,7 @@ __global__ __launch_bounds__(kDirectThreads, SPLIT ? 2 : E8 || !EXACT ? 4 : 3) v
     };
     auto go_to = [&](Place &at, uint32_t tile) {
         const uint32_t row = min(tile * 16u + uint32_t(col), p.b.rows - 1);
-        at = Place{tile, first_step, p.b.codes + size_t(row) * p.b.stride + g * 16, size_t(row >> p.b.group_shift) * p.b.scale_stride};
+        at = Place{tile, first_step, p.b.codes + size_t(row) * p.b.stride, size_t(row >> p.b.group_shift) * p.b.scale_stride};
     };
     struct Step {
         v4i codes[kDirectBlocks][2];
@@ -319,9 +330,9 @@ __global__ __launch_bounds__(kDirectThreads, SPLIT ? 2 : E8 || !EXACT ? 4 : 3) v
         if (at.tile >= tiles || at.step >= steps) return;
 #pragma unroll
         for (int i = 0; i < kDirectBlocks; ++i) {
-            const uint8_t *const from = at.codes + min(at.step * kDirectBlocks + i, whole - 1) * kScaleBlock;
-            s.codes[i][0] = *reinterpret_cast<const v4i_any *>(from);
-            s.codes[i][1] = *reinterpret_cast<const v4i_any *>(from + 64);
+            const uint32_t k = (at.step * kDirectBlocks + i) * kScaleBlock + g * 16;
+            s.codes[i][0] = *reinterpret_cast<const v4i_any *>(at.codes + min(k, p.dim - 16));
+            s.codes[i][1] = *reinterpret_cast<const v4i_any *>(at.codes + min(k + 64, p.dim - 16));
         }
         s.scales.template load<E8>(p.b.scales, at.scales, at.step * kDirectBlocks, blocks);
     };
@@ -347,15 +358,13 @@ __global__ __launch_bounds__(kDirectThreads, SPLIT ? 2 : E8 || !EXACT ? 4 : 3) v
     auto multiply = [&](const Step &s, const Place &at) {
 #pragma unroll
         for (int i = 0; i < kDirectBlocks; ++i) {
-            const uint32_t k = at.step * kDirectBlocks + i;
+            const uint32_t k = at.step * kDirectBlocks + i, from = k * kScaleBlock + g * 16;
             if (k < whole) block(k, s.codes[i][0], s.codes[i][1], s.scales.template at<E8>(i));
+            else if (k < blocks)               // (the last block ends early: what was loaded are the row's last 16 codes)
+                block(k, bytes_down(s.codes[i][0], from - min(from, p.dim - 16)), bytes_down(s.codes[i][1], from + 64 - min(from + 64, p.dim - 16)), s.scales.template at<E8>(i));
         }
     };
     auto finish = [&](const Place &at) {
-        if (whole < blocks && (!SPLIT || wave == 0)) {         // a last block that ends early
-            const v4i b0 = codes16(at.codes - g * 16, whole * kScaleBlock + g * 16, p.dim), b1 = codes16(at.codes - g * 16, whole * kScaleBlock + 64 + g * 16, p.dim);
-            block(whole, b0, b1, E8 ? static_cast<const uint8_t *>(p.b.scales)[at.scales + whole] : static_cast<const uint32_t *>(p.b.scales)[at.scales + whole]);
-        }
         if (SPLIT) {
             sums[threadIdx.x] = acc;
             __syncthreads();
@@ -391,7 +400,7 @@ __global__ __launch_bounds__(kDirectThreads, SPLIT ? 2 : E8 || !EXACT ? 4 : 3) v
 
 template <bool EXACT, bool E8, bool SPLIT>
 static hipError_t direct(const MatmulArgs &a, hipStream_t s) {
-    const uint32_t tiles = (a.b.rows + 15) / 16, most = SPLIT ? tiles : 256 * (E8 || !EXACT ? 4 : 3);      // (as many as there are at a time)
+    const uint32_t tiles = (a.b.rows + 15) / 16, most = SPLIT ? tiles : 256 * kDirectGroups;
     const uint32_t grid = SPLIT ? tiles : (tiles + kDirectWaves - 1) / kDirectWaves;
     const size_t lds = direct_lds(a.a.rows, a.dim);
     const auto kernel = k_fp8_direct<EXACT, E8, SPLIT>;
@@ -613,7 +622,7 @@ static hipError_t tile(const MatmulArgs &a, hipStream_t s) {
 
 template <bool EXACT, int SC>
 static hipError_t matmul(const MatmulArgs &a, hipStream_t s) {
-    if (a.a.rows <= 16 && size_t(a.a.rows) * direct_row(a.dim) <= kDirectLds) {
+    if (a.a.rows <= 16 && a.dim >= 16 && size_t(a.a.rows) * direct_row(a.dim) <= kDirectLds) {
         // (sixteen rows to a wave leave waves without any)
         return a.b.rows < 256 * 4 * 16 ? direct<EXACT, SC == kScaleBytes, true>(a, s) : direct<EXACT, SC == kScaleBytes, false>(a, s);
     }
