@@ -16,7 +16,8 @@ namespace tv {
 constexpr int kSampleThreads = 1024, kSampleWaves = kSampleThreads / 64;
 constexpr uint32_t kNoKey = 0x007fffffu;     // -infinity's; what is not allowed has it too
 constexpr uint32_t kBins = 1024;             // a bin to a thread
-constexpr uint32_t kListed = 4096, kListedEach = kListed / kSampleThreads;     // slots that are gathered and sorted, at most
+constexpr uint32_t kListed = 4000, kListedEach = 4;     // slots that are gathered, at most: four to a thread, and two workgroups' LDS to a compute unit
+constexpr uint32_t kSorted = 512;            // of which so many are sorted
 
 // The scores' order as unsigned numbers; -0 counts as +0, NaN as -infinity.
 __device__ __forceinline__ uint32_t score_key(float s) {
@@ -135,10 +136,21 @@ struct SampleRow {
     }
 };
 
-__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
-    return v;
+// v plus what lane moves of both halves bring (0 where they bring nothing).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t plus_moved(uint64_t v) {
+    const uint32_t lo = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(v)), CTRL, ROWS, 0xf, false));
+    const uint32_t hi = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(v >> 32)), CTRL, ROWS, 0xf, false));
+    return v + (uint64_t(hi) << 32 | lo);
+}
+// The sum over the lanes up to this one (all 64 active): within rows of 16, then the row ends handed on.
+__device__ __forceinline__ uint64_t wave_upto(uint64_t v) {
+    v = plus_moved<0x111, 0xf>(v);      // row_shr 1, 2, 4, 8
+    v = plus_moved<0x112, 0xf>(v);
+    v = plus_moved<0x114, 0xf>(v);
+    v = plus_moved<0x118, 0xf>(v);
+    v = plus_moved<0x142, 0xa>(v);      // row_bcast 15 into rows 1 and 3
+    return plus_moved<0x143, 0xc>(v);   // row_bcast 31 into rows 2 and 3
 }
 
 // Scores crowd into some fifty bins: four copies of each keep the lanes of a wave from waiting for each other (ten million
@@ -149,68 +161,46 @@ struct SampleShared {
     uint32_t part32[kSampleWaves], listed, picked, found_count, last;
     uint32_t count[kBins * kCopies];
     uint64_t mass[kBins * kCopies];
-    uint64_t list[kListed], held[kListed];       // (last: kernels that list nothing leave them out)
+    uint64_t list[kListed];       // (last: kernels that list nothing leave it out)
 };
 
 __device__ uint64_t block_sum(uint64_t v, SampleShared &sh) {
-    v = wave_sum64(v);
+    v = wave_upto(v);
     __syncthreads();
-    if ((threadIdx.x & 63u) == 0u) sh.part[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63u) == 63u) sh.part[threadIdx.x >> 6] = v;
     __syncthreads();
     uint64_t all = 0;
+#pragma unroll
     for (int w = 0; w < kSampleWaves; ++w) all += sh.part[w];
     return all;
 }
 // The sum over the threads before this one; `all` the sum over all of them.
 __device__ uint64_t block_before(uint64_t v, SampleShared &sh, uint64_t &all) {
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    uint64_t upto = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t o = __shfl_up(upto, d);
-        if (int(lane) >= d) upto += o;
-    }
+    const uint32_t wave = threadIdx.x >> 6;
+    const uint64_t upto = wave_upto(v);
     __syncthreads();
-    if (lane == 63u) sh.part[wave] = upto;
+    if ((threadIdx.x & 63u) == 63u) sh.part[wave] = upto;
     __syncthreads();
     uint64_t before = upto - v;
     all = 0;
+#pragma unroll
     for (uint32_t w = 0; w < uint32_t(kSampleWaves); ++w) {
-        if (w < wave) before += sh.part[w];
-        all += sh.part[w];
+        const uint64_t x = sh.part[w];
+        before += w < wave ? x : 0;
+        all += x;
     }
     return before;
 }
 
-// Sorts `size` (a power of two) different words, or zeros, falling.  Up to 512 of them by counting those above each: a few reads instead of
-// the 45 steps of a bitonic sort, each with a wait for the whole workgroup.
+// Sorts up to kSorted different words, none of them 0, falling, by counting those above each.
 __device__ void sort_falling(uint64_t *x, uint32_t size) {
     __syncthreads();
-    if (size <= 512u) {
-        const uint64_t mine = threadIdx.x < size ? x[threadIdx.x] : 0;
-        uint32_t above = 0;
-        if (mine != 0)
-            for (uint32_t i = 0; i < size; i += 2) {
-                const ulong2 v = *reinterpret_cast<const ulong2 *>(x + i);
-                above += uint32_t(v.x > mine) + uint32_t(v.y > mine);
-            }
-        __syncthreads();
-        if (threadIdx.x < size) x[threadIdx.x] = 0;
-        __syncthreads();
-        if (mine != 0) x[above] = mine;
-        __syncthreads();
-        return;
-    }
-    for (uint32_t run = 2; run <= size; run <<= 1) {
-        for (uint32_t step = run >> 1; step > 0; step >>= 1) {
-            __syncthreads();
-            for (uint32_t i = threadIdx.x; i < size / 2; i += kSampleThreads) {
-                const uint32_t lo = 2 * i - (i & (step - 1)), hi = lo + step;
-                const uint64_t a = x[lo], b = x[hi];
-                if ((a < b) == ((lo & run) == 0)) { x[lo] = b; x[hi] = a; }
-            }
-        }
-    }
+    const uint64_t mine = threadIdx.x < size ? x[threadIdx.x] : 0;
+    uint32_t above = 0;
+    if (mine != 0)
+        for (uint32_t i = 0; i < size; ++i) above += uint32_t(x[i] > mine);
+    __syncthreads();
+    if (mine != 0) x[above] = mine;
     __syncthreads();
 }
 
@@ -223,9 +213,9 @@ __device__ uint32_t locate_in(const SampleRow<T> &row, SampleShared &sh, uint32_
         const uint32_t from = min(len, wave * seg), to = min(len, from + seg);
         uint64_t sum = 0;
         row.each(lo + from, lo + to, lane, 64u, [&](uint32_t i, uint32_t k) { if (k != kNoKey) sum += f(i, k); });
-        sum = wave_sum64(sum);
+        sum = wave_upto(sum);
         __syncthreads();
-        if (lane == 0) sh.part[wave] = sum;
+        if (lane == 63u) sh.part[wave] = sum;
         __syncthreads();
         uint32_t w = 0;
         uint64_t upto = sh.part[0], before = 0;
@@ -262,9 +252,8 @@ struct Range {
     uint64_t count_before, mass_before;
 };
 
-// One histogram: of the slots lo .. hi - 1 whose keys lie in r, the bins by bin_of.
-template <bool MASS, typename T, typename B>
-__device__ void fill_bins(const SampleRow<T> &row, SampleShared &sh, const Range &r, uint32_t lo, uint32_t hi, B &&bin_of) {
+template <bool MASS>
+__device__ void clear_bins(SampleShared &sh) {
     __syncthreads();
 #pragma unroll
     for (uint32_t c = 0; c < kCopies; ++c) {
@@ -272,6 +261,11 @@ __device__ void fill_bins(const SampleRow<T> &row, SampleShared &sh, const Range
         if (MASS) sh.mass[c * kBins + threadIdx.x] = 0;
     }
     __syncthreads();
+}
+// One histogram: of the slots lo .. hi - 1 whose keys lie in r, the bins by bin_of.
+template <bool MASS, typename T, typename B>
+__device__ void fill_bins(const SampleRow<T> &row, SampleShared &sh, const Range &r, uint32_t lo, uint32_t hi, B &&bin_of) {
+    clear_bins<MASS>(sh);
     const uint32_t copy = threadIdx.x % kCopies;
     row.each(lo, hi, threadIdx.x, kSampleThreads, [&](uint32_t, uint32_t k) {
         if (k < r.lo || k > r.hi) return;
@@ -339,57 +333,51 @@ __device__ uint32_t list_slots(const SampleRow<T> &row, SampleShared &sh, uint32
     __syncthreads();
     return min(sh.listed, kListed);
 }
-// In the order of their keys, ties to the lower slot.
-__device__ void sort_list(SampleShared &sh, uint32_t listed) {
-    uint32_t size = 2;
-    while (size < listed) size <<= 1;
-    for (uint32_t i = listed + threadIdx.x; i < size; i += kSampleThreads) sh.list[i] = 0;
-    sort_falling(sh.list, size);
+// A thread's slots of the list.
+struct Listed {
+    uint32_t key[kListedEach], place[kListedEach];      // place: the complement of the slot, which falls as the slot rises
+    uint64_t mass[kListedEach];
+    bool in[kListedEach];
+    template <bool MASS, typename T>
+    __device__ __forceinline__ void take(const SampleRow<T> &row, const SampleShared &sh, uint32_t listed) {
+#pragma unroll
+        for (uint32_t j = 0; j < kListedEach; ++j) {
+            const uint32_t e = j * kSampleThreads + threadIdx.x;
+            in[j] = e < listed;
+            const uint64_t x = in[j] ? sh.list[e] : 0;
+            key[j] = uint32_t(x >> 32);
+            place[j] = uint32_t(x);
+            mass[j] = MASS && in[j] ? row.units(key[j]) : 0;
+        }
+    }
+};
+// Narrows r to one value v: the last, in falling order, that has slots that are in and that reaches(count before, mass before) says yes to.
+template <bool MASS, typename F>
+__device__ void narrow_listed(SampleShared &sh, const Listed &l, const uint32_t (&v)[kListedEach], Range &r, F &&reaches) {
+    do {      // (once at least: r's count may not be known yet)
+        const uint32_t shift = narrow_shift(r), copy = threadIdx.x % kCopies;
+        clear_bins<MASS>(sh);
+#pragma unroll
+        for (uint32_t j = 0; j < kListedEach; ++j) {
+            if (!l.in[j] || v[j] < r.lo || v[j] > r.hi) continue;
+            const uint32_t at = ((r.hi - v[j]) >> shift) * kCopies + copy;
+            atomicAdd(&sh.count[at], 1u);
+            if (MASS) atomicAdd(reinterpret_cast<unsigned long long *>(&sh.mass[at]), (unsigned long long)l.mass[j]);
+        }
+        __syncthreads();
+        uint32_t count;
+        uint64_t mass, total;
+        own_bin<MASS>(sh, count, mass);
+        narrow_to(r, pick_bin<MASS>(sh, r, count, mass, reaches, total), shift);
+    } while (r.lo < r.hi);
 }
-template <typename T>
-__device__ uint32_t gather(const SampleRow<T> &row, SampleShared &sh, uint32_t lo, uint32_t hi) {
-    const uint32_t listed = list_slots(row, sh, 0, row.n, lo, hi);
-    sort_list(sh, listed);
-    return listed;
-}
-
-// The same among all slots of r, sorted in the list.
-template <bool MASS, typename T, typename F>
-__device__ void narrow_in_list(const SampleRow<T> &row, SampleShared &sh, uint32_t listed, Range &r, F &&reaches) {
-    // every slot of the list by itself: the last one that is reached has the key
-    uint64_t mass[kListedEach], sum = 0, all = 0;
+// The slot up to which `ties` of those that are in and have this key lie.
+__device__ uint32_t last_tie(SampleShared &sh, Listed l, uint32_t key, uint32_t ties) {
 #pragma unroll
-    for (uint32_t j = 0; j < kListedEach; ++j) {
-        const uint32_t e = threadIdx.x * kListedEach + j;
-        mass[j] = MASS && e < listed ? row.units(uint32_t(sh.list[e] >> 32)) : 0;
-        sum += mass[j];
-    }
-    uint64_t before = r.mass_before + (MASS ? block_before(sum, sh, all) : 0);
-    if (threadIdx.x == 0) sh.picked = 0;
-    __syncthreads();
-#pragma unroll
-    for (uint32_t j = 0; j < kListedEach; ++j) {
-        const uint32_t e = threadIdx.x * kListedEach + j;
-        if (e < listed && (e == 0 || reaches(r.count_before + e, before))) atomicMax(&sh.picked, e);
-        before += mass[j];
-    }
-    __syncthreads();
-    const uint32_t key = uint32_t(sh.list[sh.picked] >> 32);
-    // the slots above it, and those that have it
-    uint64_t above = 0, equal = 0, heavier = 0;
-#pragma unroll
-    for (uint32_t j = 0; j < kListedEach; ++j) {
-        const uint32_t e = threadIdx.x * kListedEach + j;
-        if (e >= listed) continue;
-        const uint32_t k = uint32_t(sh.list[e] >> 32);
-        above += k > key;
-        equal += k == key;
-        heavier += k > key ? mass[j] : 0;
-    }
-    r.count_before += block_sum(above, sh);
-    r.mass_before += MASS ? block_sum(heavier, sh) : 0;
-    r.count = uint32_t(block_sum(equal, sh));
-    r.lo = r.hi = key;
+    for (uint32_t j = 0; j < kListedEach; ++j) l.in[j] &= l.key[j] == key;
+    Range r{0u, ~0u, 0, 0, 0};
+    narrow_listed<false>(sh, l, l.place, r, [&](uint64_t c, uint64_t) { return c < uint64_t(ties); });
+    return ~r.lo;
 }
 
 // Narrows r to one key: the last, in falling order, that has slots and that reaches(count before, mass before) says yes to.
@@ -402,7 +390,9 @@ __device__ void narrow(const SampleRow<T> &row, SampleShared &sh, Range &r, F &&
         narrow_to(r, b, shift);
     }
     if (r.lo == r.hi) return;
-    narrow_in_list<MASS>(row, sh, gather(row, sh, r.lo, r.hi), r, reaches);
+    Listed l;
+    l.take<MASS>(row, sh, list_slots(row, sh, 0, row.n, r.lo, r.hi));
+    narrow_listed<MASS>(sh, l, l.key, r, reaches);
 }
 
 __device__ __forceinline__ uint64_t drawn_mass(float u, uint64_t sum) {
@@ -410,58 +400,85 @@ __device__ __forceinline__ uint64_t drawn_mass(float u, uint64_t sum) {
     return want >= double(sum) ? sum - 1 : want > 0.0 ? uint64_t(want) : uint64_t(0);
 }
 
-// Draws from the slots of sh.list, in the order of their rank, `listed` of them: the first top_k, those of them that less than `limit` of
-// mass lies before, those of at least min_key.  top_p: the share that limit is of the mass of the first top_k, where it is one of the list's.
+// Draws from the slots of sh.list: of the first top_k in the order of their rank (0: all), those that less than a limit of mass lies before
+// (limit_p), and of those the ones of at least min_key.  The limit is top_p of the mass of the first top_k, or given.
+struct ListLimits {
+    uint32_t top_k, min_key;
+    bool limit_p;
+    double top_p, limit;
+    float u;
+};
+
+// Few slots: sorted by rank, then, what stays of them, by slot.
 template <typename T>
-__device__ void draw_from_list(const SampleRow<T> &row, SampleShared &sh, uint32_t listed, bool limit_p, bool share, double top_p, double limit, uint32_t min_key,
-                               float u, int64_t &slot, float &prob) {
-    uint64_t mass[kListedEach], sum = 0, all;
+__device__ void draw_sorted(const SampleRow<T> &row, SampleShared &sh, uint32_t listed, ListLimits lim, int64_t &slot, float &prob) {
+    const uint32_t t = threadIdx.x;
+    sort_falling(sh.list, listed);
+    if (lim.top_k != 0) listed = min(listed, lim.top_k);
+    const uint64_t x = t < listed ? sh.list[t] : 0;
+    const uint32_t key = uint32_t(x >> 32);
+    const uint64_t mass = x != 0 ? row.units(key) : 0;
+    uint64_t all, total;
+    const uint64_t before = block_before(mass, sh, all);
+    if (lim.top_k != 0) lim.limit = lim.top_p * double(all);
+    const bool stays = x != 0 && (t == 0 || ((!lim.limit_p || double(before) < lim.limit) && key >= lim.min_key));
+    // (what stays is a prefix: min-p and top-p both leave one)
+    block_before(stays, sh, all);
+    const uint32_t kept = uint32_t(all);
+    if (stays) sh.list[t] = uint64_t(uint32_t(x)) << 32 | key;
+    sort_falling(sh.list, kept);
+    const uint64_t y = t < kept ? sh.list[t] : 0;
+    const uint64_t own = y != 0 ? row.units(uint32_t(y)) : 0, upto = block_before(own, sh, total), want = drawn_mass(lim.u, total);
+    if (t == 0) sh.picked = 0;
+    __syncthreads();
+    if (upto <= want && upto + own > want) sh.picked = t;
+    __syncthreads();
+    const uint64_t z = sh.list[sh.picked];
+    slot = int64_t(~uint32_t(z >> 32));
+    prob = float(ldexp(row.weight(uint32_t(z)), row.shift) / double(total));
+}
+
+template <typename T>
+__device__ void draw_from_list(const SampleRow<T> &row, SampleShared &sh, uint32_t listed, ListLimits lim, int64_t &slot, float &prob) {
+    if (listed <= kSorted) return draw_sorted(row, sh, listed, lim, slot, prob);
+    Listed l;
+    l.take<true>(row, sh, listed);
+    uint64_t sum;
+    const auto mass_in = [&] {
+        sum = 0;
 #pragma unroll
-    for (uint32_t j = 0; j < kListedEach; ++j) {
-        const uint32_t e = threadIdx.x * kListedEach + j;
-        mass[j] = e < listed ? row.units(uint32_t(sh.list[e] >> 32)) : 0;
-        sum += mass[j];
-    }
-    uint64_t before = block_before(sum, sh, all);
-    if (share) limit = top_p * double(all);
-    sum = 0;
-    uint32_t size = 2;
-    while (size < listed) size <<= 1;
-    for (uint32_t e = listed + threadIdx.x; e < size; e += kSampleThreads) sh.held[e] = 0;
+        for (uint32_t j = 0; j < kListedEach; ++j) sum += l.in[j] ? l.mass[j] : 0;
+        return block_sum(sum, sh);
+    };
+    const auto keep = [&](uint32_t least, uint32_t count, uint32_t ties) {
+        const uint32_t last = ties < count ? last_tie(sh, l, least, ties) : ~0u;
 #pragma unroll
-    for (uint32_t j = 0; j < kListedEach; ++j) {
-        const uint32_t e = threadIdx.x * kListedEach + j;
-        if (e < listed) {
-            const uint64_t x = sh.list[e];
-            const bool stays = e == 0 || ((!limit_p || double(before) < limit) && uint32_t(x >> 32) >= min_key);
-            sum += stays ? mass[j] : 0;
-            // by slot, falling as its complement does: low word the rank
-            sh.held[e] = stays ? uint64_t(uint32_t(x)) << 32 | e : 0;
+        for (uint32_t j = 0; j < kListedEach; ++j) l.in[j] &= l.key[j] > least || (l.key[j] == least && ~l.place[j] <= last);
+    };
+    if (lim.top_k != 0) {
+        if (listed > lim.top_k) {
+            Range r{kNoKey + 1u, row.most, 0, 0, 0};
+            narrow_listed<false>(sh, l, l.key, r, [&](uint64_t c, uint64_t) { return c < uint64_t(lim.top_k); });
+            keep(r.lo, r.count, min(r.count, uint32_t(uint64_t(lim.top_k) - r.count_before)));
         }
-        before += mass[j];
+        lim.limit = lim.top_p * double(mass_in());
     }
-    const uint64_t total = block_sum(sum, sh), want = drawn_mass(u, total);
-    sort_falling(sh.held, size);
-    sum = 0;
-#pragma unroll
-    for (uint32_t j = 0; j < kListedEach; ++j) {
-        const uint32_t e = threadIdx.x * kListedEach + j;
-        const uint64_t x = e < size ? sh.held[e] : 0;
-        mass[j] = x != 0 ? row.units(uint32_t(sh.list[uint32_t(x)] >> 32)) : 0;
-        sum += mass[j];
+    if (lim.limit_p) {
+        Range r{kNoKey + 1u, row.most, 0, 0, 0};
+        narrow_listed<true>(sh, l, l.key, r, [&](uint64_t c, uint64_t m) { return c == 0 || double(m) < lim.limit; });
+        if (r.lo < lim.min_key) {
+            r.lo = lim.min_key;
+            r.count = 0;
+        }
+        keep(r.lo, r.count, ties_within(row, r, lim.limit));
+    } else {
+        keep(lim.min_key, 0, 0);
     }
-    before = block_before(sum, sh, all);
-    if (threadIdx.x == 0) sh.picked = 0;
-    __syncthreads();
-#pragma unroll
-    for (uint32_t j = 0; j < kListedEach; ++j) {
-        if (before <= want && before + mass[j] > want) sh.picked = threadIdx.x * kListedEach + j;
-        before += mass[j];
-    }
-    __syncthreads();
-    const uint64_t x = sh.held[sh.picked];
-    slot = int64_t(~uint32_t(x >> 32));
-    prob = float(ldexp(row.weight(uint32_t(sh.list[uint32_t(x)] >> 32)), row.shift) / double(total));
+    const uint64_t total = mass_in(), want = drawn_mass(lim.u, total);
+    Range r{0u, ~0u, 0, 0, 0};
+    narrow_listed<true>(sh, l, l.place, r, [&](uint64_t c, uint64_t m) { return c == 0 || m <= want; });
+    slot = int64_t(~r.lo);
+    prob = float(ldexp(row.weight(row.key_at(~r.lo)), row.shift) / double(total));
 }
 
 // A row's parameters.
@@ -470,14 +487,18 @@ struct Limits {
     float top_p, u;
     bool limit_k, limit_p;
     uint32_t min_key;
-    template <typename T>
-    __device__ __forceinline__ void set(const SampleArgs &p, uint32_t r, SampleRow<T> &row, uint32_t most) {
-        const float t = p.temperature == nullptr ? 1.0f : p.temperature[r], min_p = p.min_p == nullptr ? 0.0f : p.min_p[r];
-        row.set(most, t);
+    float t, min_p;
+    __device__ __forceinline__ void load(const SampleArgs &p, uint32_t r) {
+        t = p.temperature == nullptr ? 1.0f : p.temperature[r];
+        min_p = p.min_p == nullptr ? 0.0f : p.min_p[r];
         top_k = p.top_k == nullptr ? 0 : p.top_k[r];
         top_p = p.top_p == nullptr ? 1.0f : p.top_p[r];
-        if (!(t > 0.0f)) { top_k = 1; top_p = 1.0f; }       // the best alone
         u = p.u[r];
+        if (!(t > 0.0f)) { top_k = 1; top_p = 1.0f; }       // the best alone
+    }
+    template <typename T>
+    __device__ __forceinline__ void set(SampleRow<T> &row, uint32_t most) {
+        row.set(most, t);
         limit_k = top_k > 0 && uint32_t(top_k) < row.n;
         limit_p = top_p < 1.0f;
         min_key = min_p > 0.0f ? row.least_of_weight(double(min_p), double(t)) : kNoKey + 1u;
@@ -506,8 +527,8 @@ __device__ void sample_row(const SampleRow<T> &row, SampleShared &sh, const Limi
         const uint32_t b = pick_bin<false>(row, sh, all, [&](uint32_t k) { return row.bin(k); }, first_k, total);
         all.lo = row.least_of_bin(b);
         if (all.count_before + all.count <= kListed) {
-            const uint32_t listed = gather(row, sh, all.lo, row.most);
-            return draw_from_list(row, sh, min(listed, uint32_t(top_k)), limit_p, true, double(top_p), 0.0, min_key, u, slot, prob);
+            const uint32_t listed = list_slots(row, sh, 0, row.n, all.lo, row.most);
+            return draw_from_list(row, sh, listed, ListLimits{uint32_t(top_k), min_key, limit_p, double(top_p), 0.0, u}, slot, prob);
         }
         if (b != 0) all.hi = row.least_of_bin(b - 1) - 1u;
         narrow<false>(row, sh, all, first_k);
@@ -532,8 +553,8 @@ __device__ void sample_row(const SampleRow<T> &row, SampleShared &sh, const Limi
             // of what top-p may leave, min-p leaves the slots of min_key and above
             const uint32_t from = max(all.lo, min_key);
             if (from > all.lo || all.count_before + all.count <= kListed) {
-                const uint32_t listed = gather(row, sh, from, row.most);
-                if (sh.listed <= kListed) return draw_from_list(row, sh, listed, true, false, 0.0, limit, min_key, u, slot, prob);
+                const uint32_t listed = list_slots(row, sh, 0, row.n, from, row.most);
+                if (sh.listed <= kListed) return draw_from_list(row, sh, listed, ListLimits{0u, min_key, true, 0.0, limit, u}, slot, prob);
             }
         }
         if (b != 0) all.hi = row.least_of_bin(b - 1) - 1u;
@@ -579,14 +600,15 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample(SampleArgs p) {
     SampleShared &sh = *reinterpret_cast<SampleShared *>(smem);
     for (uint32_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         SampleRow<T> row = row_of<T>(p, r);
+        Limits lim;
+        lim.load(p, r);
         uint32_t most = kNoKey;
         row.each(0, p.n, threadIdx.x, kSampleThreads, [&](uint32_t, uint32_t k) { most = max(most, k); });
         most = block_max(most, sh);
         int64_t slot = -1;
         float prob = 0.0f;
         if (most != kNoKey) {
-            Limits lim;
-            lim.set(p, r, row, most);
+            lim.set(row, most);
             sample_row(row, sh, lim, slot, prob);
         }
         if (threadIdx.x == 0) { p.out_slots[r] = slot; p.out_probs[r] = prob; }
@@ -630,13 +652,14 @@ struct Chunk {
     SampleSplit *ws;
     uint32_t r, c, from, to, most;
     __device__ __forceinline__ Chunk(const SampleArgs &p, const SplitArgs &x)
-        : row(row_of<T>(p, blockIdx.y)), ws(x.rows + blockIdx.y), r(blockIdx.y), c(blockIdx.x), from(blockIdx.x * x.chunk), to(min(p.n, from + x.chunk)) {}
+        : row(row_of<T>(p, blockIdx.x)), ws(x.rows + blockIdx.x), r(blockIdx.x), c(blockIdx.y), from(blockIdx.y * x.chunk), to(min(p.n, from + x.chunk)) {}
     __device__ __forceinline__ bool open(const SampleArgs &p, const SplitArgs &x, SampleShared &sh) {
+        lim.load(p, r);
         most = kNoKey;
         for (uint32_t i = threadIdx.x; i < x.chunks; i += kSampleThreads) most = max(most, x.chunk_most[size_t(r) * x.chunks + i]);
         most = block_max(most, sh);
         if (most == kNoKey) return false;
-        lim.set(p, r, row, most);
+        lim.set(row, most);
         return true;
     }
     __device__ __forceinline__ void write(const SampleArgs &p, int64_t slot, float prob) const {
@@ -743,14 +766,13 @@ __device__ void add_slots(const Chunk<T> &ch, SampleShared &sh, uint32_t lo, uin
     for (uint32_t i = threadIdx.x; i < listed; i += kSampleThreads)
         if (sh.found_count + i < kListed) ch.ws->list[sh.found_count + i] = sh.list[i];
 }
-// The row's list, sorted.
+// The row's list.
 template <typename T>
 __device__ uint32_t take_list(const Chunk<T> &ch, SampleShared &sh) {
     const uint32_t listed = min(ch.ws->listed, kListed);
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < listed; i += kSampleThreads) sh.list[i] = ch.ws->list[i];
     __syncthreads();
-    sort_list(sh, listed);
     return listed;
 }
 
@@ -803,8 +825,7 @@ __device__ void narrow_chunk(const SampleArgs &p, Chunk<T> &ch, SampleShared &sh
     if (listable(upto)) {
         if (ch.c != 0) return;
         const uint32_t listed = take_list(ch, sh);
-        if (MASS) draw_from_list(ch.row, sh, listed, true, false, 0.0, limit, lim.min_key, lim.u, slot, prob);
-        else draw_from_list(ch.row, sh, min(listed, uint32_t(lim.top_k)), lim.limit_p, true, double(lim.top_p), 0.0, lim.min_key, lim.u, slot, prob);
+        draw_from_list(ch.row, sh, listed, MASS ? ListLimits{0u, lim.min_key, true, 0.0, limit, lim.u} : ListLimits{uint32_t(lim.top_k), lim.min_key, lim.limit_p, double(lim.top_p), 0.0, lim.u}, slot, prob);
         return ch.write(p, slot, prob);
     }
     if (lim.limit_k && lim.limit_p) {
@@ -840,10 +861,12 @@ __device__ void find_threshold(const Chunk<T> &ch, SampleShared &sh, uint32_t &l
     Range r = first_range<MASS>(ch, sh, limit, upto, b);
     const auto reaches = [&](uint64_t c, uint64_t m) { return MASS ? c == 0 || double(m) < limit : c < uint64_t(lim.top_k); };
     r = second_range<MASS>(ch, sh, r, b, reaches);
-    const uint64_t before = r.count_before;
-    narrow_in_list<MASS>(ch.row, sh, take_list(ch, sh), r, reaches);
+    Listed l;
+    l.take<MASS>(ch.row, sh, take_list(ch, sh));
+    narrow_listed<MASS>(sh, l, l.key, r, reaches);
+    const uint32_t ties = ties_of<MASS>(ch, r, limit);
     least = r.lo;
-    tie_last = ~uint32_t(sh.list[uint32_t(r.count_before - before) + ties_of<MASS>(ch, r, limit) - 1u]);
+    tie_last = ties < r.count ? last_tie(sh, l, least, ties) : ~0u;
 }
 template <typename T>
 __global__ __launch_bounds__(kSampleThreads) void k_sample_mass(SampleArgs p, SplitArgs x) {
@@ -907,7 +930,7 @@ static hipError_t sample(const SampleArgs &a, hipStream_t s) {
     const SplitArgs x{reinterpret_cast<SampleSplit *>(a.ws), reinterpret_cast<uint64_t *>(a.ws + split.masses), reinterpret_cast<uint2 *>(a.ws + split.cuts),
                       reinterpret_cast<uint32_t *>(a.ws + split.mosts),
                       split.chunk, split.chunks};
-    const dim3 grid(split.chunks, a.rows);
+    const dim3 grid(a.rows, split.chunks);      // (rows next to each other: their first chunks, which work alone at times, on all XCDs)
     const auto go = [&](void (*kernel)(SampleArgs, SplitArgs), dim3 g, size_t bytes) {
         const hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), bytes);
         return e != hipSuccess ? e : launch(kernel, g, kSampleThreads, bytes, s, a, x);
@@ -918,7 +941,7 @@ static hipError_t sample(const SampleArgs &a, hipStream_t s) {
     if (a.top_k == nullptr && a.top_p == nullptr && a.temperature == nullptr) return hipSuccess;      // nothing limits any row
     if (const hipError_t e = go(k_sample_narrow<T>, grid, lds); e != hipSuccess) return e;
     if (const hipError_t e = go(k_sample_mass<T>, grid, lds); e != hipSuccess) return e;
-    return go(k_sample_draw<T>, dim3(1, a.rows), unlisted);
+    return go(k_sample_draw<T>, dim3(a.rows), unlisted);
 }
 hipError_t launch_sample(const SampleArgs &a, int score_type, hipStream_t s) {
     if (score_type == kF32) return sample<float>(a, s);
