@@ -252,7 +252,7 @@ int tv_fp8_rescore_dev(int device, void *stream, const void *d_queries, int q_ty
                        const uint8_t *d_rows, size_t row_stride, const void *d_scales, size_t scale_stride, size_t n, int group, size_t dim, int scale_type,
                        const int64_t *d_slots, size_t slot_stride, size_t m, size_t k, float *d_out_scores, int64_t *d_out_slots,
                        void *d_workspace, size_t workspace_bytes);
-size_t tv_fp8_rescore_workspace(size_t nq, size_t m);
+size_t tv_fp8_rescore_workspace(size_t nq, size_t m, size_t dim);
 /* Draws one slot from each row of n scores.  Allowed are the slots whose mask bit is set (d_mask_words NULL: all;
  * 64 slots a word, as tv_pack_mask makes them; mask_stride 0: one mask for all rows) and whose score is neither NaN nor
  * -infinity.  With slots ranked by score, ties to the lower slot, and w = exp((score - best) / temperature):

@@ -84,7 +84,7 @@ extern "C" {
     pub fn tv_fp8_quantize_dev(device: c_int, stream: *mut c_void, d_x: *const c_void, x_type: c_int, x_stride: usize, rows: usize, dim: usize, scale_type: c_int, group: c_int, d_codes: *mut u8, code_stride: usize, d_scales: *mut c_void, scale_stride: usize) -> c_int;
     pub fn tv_fp8_matmul_dev(device: c_int, stream: *mut c_void, d_a: *const u8, a_stride: usize, d_a_scales: *const c_void, a_scale_stride: usize, m: usize, d_b: *const u8, b_stride: usize, d_b_scales: *const c_void, b_scale_stride: usize, n: usize, group: c_int, dim: usize, scale_type: c_int, d_out: *mut c_void, out_type: c_int, out_stride: usize) -> c_int;
     pub fn tv_fp8_rescore_dev(device: c_int, stream: *mut c_void, d_queries: *const c_void, q_type: c_int, q_stride: usize, nq: usize, d_rows: *const u8, row_stride: usize, d_scales: *const c_void, scale_stride: usize, n: usize, group: c_int, dim: usize, scale_type: c_int, d_slots: *const i64, slot_stride: usize, m: usize, k: usize, d_out_scores: *mut c_float, d_out_slots: *mut i64, d_workspace: *mut c_void, workspace_bytes: usize) -> c_int;
-    pub fn tv_fp8_rescore_workspace(nq: usize, m: usize) -> usize;
+    pub fn tv_fp8_rescore_workspace(nq: usize, m: usize, dim: usize) -> usize;
     pub fn tv_sample_dev(device: c_int, stream: *mut c_void, d_scores: *const c_void, score_type: c_int, score_stride: usize, rows: usize, n: usize, d_mask_words: *const u64, mask_stride: usize, d_u: *const c_float, d_temperature: *const c_float, d_top_k: *const i32, d_top_p: *const c_float, d_min_p: *const c_float, d_out_slots: *mut i64, d_out_probs: *mut c_float, d_workspace: *mut c_void, workspace_bytes: usize) -> c_int;
     pub fn tv_sample_workspace(rows: usize, n: usize) -> usize;
 

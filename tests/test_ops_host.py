@@ -48,8 +48,8 @@ def test_matmul_refuses(change, text):
 
 @pytest.mark.parametrize("change,text", [
     (dict(dim=20000), "dim"), (dict(k=9), "k exceeds"), (dict(m=16385, ws_bytes=1 << 30), "16384"), (dict(q=None), "null"), (dict(q=P + 2), "aligned"),
-    (dict(slots=None), "null"), (dict(slots=P + 4), "aligned"), (dict(s=None), "null"), (dict(i=P + 4), "aligned"), (dict(ws=None), "workspace"),
-    (dict(ws_bytes=127), "workspace"), (dict(rows=None), "null"), (dict(group=3), "128"), (dict(q_type=7), "values"), (dict(nq=1 << 31, ws_bytes=1 << 40), "queries")])
+    (dict(slots=None), "null"), (dict(slots=P + 4), "aligned"), (dict(s=None), "null"), (dict(i=P + 4), "aligned"), (dict(ws=None, m=300), "workspace"),
+    (dict(ws_bytes=2 * 300 * 8 - 1, m=300), "workspace"), (dict(ws=P + 4, m=300), "workspace"), (dict(rows=None), "null"), (dict(group=3), "128"), (dict(q_type=7), "values"), (dict(nq=1 << 31, ws_bytes=1 << 40), "queries")])
 def test_rescore_refuses(change, text):
     refused(rescore(**change), text)
 

@@ -120,7 +120,7 @@ def lib():
     L.tv_fp8_matmul_dev.argtypes = [i32, vp, vp, sz, vp, sz, sz, vp, sz, vp, sz, sz, i32, sz, i32, vp, i32, sz]
     L.tv_fp8_rescore_dev.argtypes = [i32, vp, vp, i32, sz, sz, vp, sz, vp, sz, sz, i32, sz, i32, vp, sz, sz, sz, vp, vp, vp, sz]
     L.tv_fp8_rescore_workspace.restype = sz
-    L.tv_fp8_rescore_workspace.argtypes = [sz, sz]
+    L.tv_fp8_rescore_workspace.argtypes = [sz, sz, sz]
     L.tv_sample_dev.argtypes = [i32, vp, vp, i32, sz, sz, sz, vp, sz, vp, vp, vp, vp, vp, vp, vp, vp, sz]
     L.tv_sample_workspace.restype = sz
     L.tv_sample_workspace.argtypes = [sz, sz]

@@ -7,6 +7,8 @@
 #include <cstdint>
 #include <tuple>
 
+#include "tv_device.h"
+
 namespace tv {
 
 constexpr int kScaleBlock = 128;      // coordinates that share a scale
@@ -48,9 +50,10 @@ struct RescoreArgs {
     uint32_t dim, nq, m, k;
     float *out_scores;
     int64_t *out_slots;
-    uint64_t *keys;                   // workspace: nq * m sort keys
+    uint64_t *keys;                   // workspace: nq * m sort keys, or none (rescore_workspace)
 };
 constexpr uint32_t kMaxRescore = 16384;      // candidates of a query: their sort keys fit a workgroup's LDS
+size_t rescore_workspace(size_t nq, size_t m, size_t dim);
 hipError_t launch_fp8_rescore(const RescoreArgs &a, int q_type, int scale_type, hipStream_t s);
 
 struct SampleArgs {
@@ -87,5 +90,33 @@ hipError_t launch(void (*kernel)(P...), dim3 grid, dim3 threads, size_t lds, hip
 
 typedef _Float16 f16;
 typedef __bf16 bf16;
+
+typedef int v4i_any __attribute__((ext_vector_type(4), aligned(1)));
+
+// 16 bytes moved down by so many, zeros from above; 16 and more leave nothing.
+__device__ __forceinline__ v4i bytes_down(v4i v, uint32_t bytes) {
+    uint64_t lo = uint64_t(uint32_t(v[0])) | uint64_t(uint32_t(v[1])) << 32, hi = uint64_t(uint32_t(v[2])) | uint64_t(uint32_t(v[3])) << 32;
+    if (bytes & 8u) { lo = hi; hi = 0; }
+    const uint32_t bits = (bytes & 7u) * 8u;
+    lo = lo >> bits | (hi << 1) << (63u - bits);
+    hi >>= bits;
+    if (bytes >= 16u) lo = hi = 0;
+    return v4i{int(uint32_t(lo)), int(uint32_t(lo >> 32)), int(uint32_t(hi)), int(uint32_t(hi >> 32))};
+}
+// 16 codes of a row from k on, those past `dim` zero, without touching what lies behind the row: a run that the row ends in is
+// the end of the row's last 16 codes.
+__device__ __forceinline__ v4i codes16(const uint8_t *row, uint32_t k, uint32_t dim) {
+    if (dim >= 16u) {
+        const uint32_t at = min(k, dim - 16u);
+        return bytes_down(*reinterpret_cast<const v4i_any *>(row + at), k - at);
+    }
+    v4i v{0, 0, 0, 0};
+    for (uint32_t i = 0; k + i < dim; ++i) {
+        const v4i x = bytes_down(v4i{0, 0, 0, int(uint32_t(row[k + i]) << 24)}, 15u - i);
+        v |= x;
+    }
+    return v;
+}
+
 
 }  // namespace tv

@@ -94,7 +94,7 @@ int tv_fp8_matmul_dev(int device, void *stream, const uint8_t *d_a, size_t a_str
     return e == hipSuccess ? TV_OK : op_failed(e, "tv_fp8_matmul_dev");
 }
 
-size_t tv_fp8_rescore_workspace(size_t nq, size_t m) { return nq * m * sizeof(uint64_t); }
+size_t tv_fp8_rescore_workspace(size_t nq, size_t m, size_t dim) { return tv::rescore_workspace(nq, m, dim); }
 
 int tv_fp8_rescore_dev(int device, void *stream, const void *d_queries, int q_type, size_t q_stride, size_t nq,
                        const uint8_t *d_rows, size_t row_stride, const void *d_scales, size_t scale_stride, size_t n, int group, size_t dim, int scale_type,
@@ -109,7 +109,7 @@ int tv_fp8_rescore_dev(int device, void *stream, const void *d_queries, int q_ty
     if (d_queries == nullptr || off(d_queries, value_bytes(q_type))) return op_refused("queries are null or not aligned");
     if (d_slots == nullptr || d_out_scores == nullptr || d_out_slots == nullptr || off(d_slots, 8) || off(d_out_scores, 4) || off(d_out_slots, 8))
         return op_refused("slots or results are null or not aligned");
-    if (workspace_bytes < tv_fp8_rescore_workspace(nq, m) || d_workspace == nullptr || off(d_workspace, 8))
+    if (const size_t need = tv::rescore_workspace(nq, m, dim); need != 0 && (workspace_bytes < need || d_workspace == nullptr || off(d_workspace, 8)))
         return op_refused("workspace is null, not aligned or smaller than tv_fp8_rescore_workspace()");
     OnDevice on(device);
     if (on.rc != TV_OK) return on.rc;

@@ -5,8 +5,6 @@ answer what the index's codes are too coarse for: exact-to-8-bits scores of ever
 of a search (`rescore`).  Everything is a torch tensor on the GPU; calls run on the current stream of the tensors' device
 and do not wait.
 """
-from dataclasses import dataclass
-
 import torch
 
 from . import _lib as T
@@ -34,55 +32,78 @@ def _gpu(name, t, dtypes, ndim=2):
         raise TypeError(f"{name} must be a {ndim}-D {wanted} tensor, got {_desc(t)}")
     if not t.is_cuda:
         raise ValueError(f"{name} must be on a GPU, got {t.device}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name}: elements of a row must lie next to each other; call contiguous() first")
     return t
 
 
-def _same_device(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
+def _same_device(device, name, t):
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
 
 
 def _call(fn, device, *args):
-    T.check(fn(device.index, torch.cuda.current_stream(device).cuda_stream, *args))
+    at = device.index
+    status = fn(at, _stream_of(at), *args)
+    if status != T.OK:
+        T.check(status)
 
 
-@dataclass(frozen=True)
+# (the pointer itself, where this torch hands it out: a Stream object takes a fifth of a short call's time)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream_of(index):
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def _workspace(size, device):
+    """(tensor, address, bytes) of a call's workspace.  It is given back when the call has been made: what the stream runs
+    later may take it over, and comes later."""
+    if size == 0:
+        return None, None, 0
+    t = torch.empty(size, dtype=torch.uint8, device=device)
+    return t, t.data_ptr(), size
+
+
 class Fp8Rows:
     """`codes` float8_e4m3fn [rows, dim], `scales` [ceil(rows / group), ceil(dim / 128)] of float8_e8m0fnu or float32; a
     coordinate is code * scale.  `group`: rows that share a scale, 1 or 128."""
-    codes: torch.Tensor
-    scales: torch.Tensor
-    group: int = 1
 
-    def __post_init__(self):
-        _gpu("codes", self.codes, (torch.float8_e4m3fn,))
-        _gpu("scales", self.scales, tuple(_SCALE_TYPES))
-        if self.group not in (1, BLOCK):
-            raise ValueError(f"group must be 1 or {BLOCK}, got {self.group}")
-        rows, dim = self.codes.shape
+    __slots__ = ("_codes", "_scales", "_group", "_scale_type")
+
+    def __init__(self, codes, scales, group=1):
+        _gpu("codes", codes, (torch.float8_e4m3fn,))
+        _gpu("scales", scales, tuple(_SCALE_TYPES))
+        if group not in (1, BLOCK):
+            raise ValueError(f"group must be 1 or {BLOCK}, got {group}")
+        rows, dim = codes.shape
         if not 1 <= dim <= _MAX_DIM:
             raise ValueError(f"dim must be 1 to {_MAX_DIM}, got {dim}")
-        if tuple(self.scales.shape) != (-(-rows // self.group), _blocks(dim)):
-            raise ValueError(f"scales of {rows} x {dim} codes in groups of {self.group} rows must be "
-                             f"{(-(-rows // self.group), _blocks(dim))}, got {tuple(self.scales.shape)}")
-        _same_device(self.codes.device, scales=self.scales)
+        if tuple(scales.shape) != (-(-rows // group), _blocks(dim)):
+            raise ValueError(f"scales of {rows} x {dim} codes in groups of {group} rows must be "
+                             f"{(-(-rows // group), _blocks(dim))}, got {tuple(scales.shape)}")
+        _same_device(codes.device, "scales", scales)
+        self._set(codes, scales, group, _SCALE_TYPES[scales.dtype])
+
+    def _set(self, codes, scales, group, scale_type):
+        self._codes, self._scales, self._group, self._scale_type = codes, scales, group, scale_type
+        return self
+
+    codes = property(lambda self: self._codes)
+    scales = property(lambda self: self._scales)
+    group = property(lambda self: self._group)
+    dim = property(lambda self: self._codes.shape[1])
 
     def __len__(self):
-        return self.codes.shape[0]
-
-    @property
-    def dim(self):
-        return self.codes.shape[1]
-
-    @property
-    def _scale_type(self):
-        return _SCALE_TYPES[self.scales.dtype]
+        return self._codes.shape[0]
 
     def _args(self):
-        return self.codes.data_ptr(), self.codes.stride(0), self.scales.data_ptr(), self.scales.stride(0), len(self)
+        c, s = self._codes, self._scales
+        return c.data_ptr(), c.stride(0), s.data_ptr(), s.stride(0), c.shape[0]
+
+    def __repr__(self):
+        return f"Fp8Rows({len(self)} x {self.dim}, scales {self.scales.dtype} of {self.group} rows, {self.codes.device})"
 
 
 def quantize(x, *, scale="e8m0", group=1):
@@ -97,11 +118,12 @@ def quantize(x, *, scale="e8m0", group=1):
     if not 1 <= dim <= _MAX_DIM:
         raise ValueError(f"dim must be 1 to {_MAX_DIM}, got {dim}")
     kind, dtype = _SCALES[scale]
-    codes = torch.empty(rows, -(-dim // _ROW_ALIGN) * _ROW_ALIGN, dtype=torch.float8_e4m3fn, device=x.device)[:, :dim]
-    scales = torch.empty(-(-rows // group), _blocks(dim), dtype=dtype, device=x.device)
-    _call(T.lib().tv_fp8_quantize_dev, x.device, x.data_ptr(), _VALUES[x.dtype], x.stride(0), rows, dim, kind, group,
-          codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(0))
-    return Fp8Rows(codes, scales, group)
+    device = x.device
+    codes = torch.empty_strided((rows, dim), (-(-dim // _ROW_ALIGN) * _ROW_ALIGN, 1), dtype=torch.float8_e4m3fn, device=device)
+    scales = torch.empty((-(-rows // group), _blocks(dim)), dtype=dtype, device=device)
+    made = Fp8Rows.__new__(Fp8Rows)._set(codes, scales, group, kind)
+    _call(T.lib().tv_fp8_quantize_dev, device, x.data_ptr(), _VALUES[x.dtype], x.stride(0), rows, dim, kind, group, *made._args()[:4])
+    return made
 
 
 def matmul(a, b, *, dtype=torch.float32, out=None):
@@ -115,17 +137,18 @@ def matmul(a, b, *, dtype=torch.float32, out=None):
         raise ValueError(f"dim {a.dim} of a does not match dim {b.dim} of b")
     if a.scales.dtype != b.scales.dtype:
         raise ValueError(f"scales of a are {a.scales.dtype}, of b {b.scales.dtype}")
-    _same_device(a.codes.device, b=b.codes)
+    device = a.codes.device
+    _same_device(device, "b", b.codes)
     if out is None:
         if dtype not in _VALUES:
             raise TypeError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
-        out = torch.empty(len(a), len(b), dtype=dtype, device=a.codes.device)
+        out = torch.empty((len(a), len(b)), dtype=dtype, device=device)
     else:
         _gpu("out", out, tuple(_VALUES))
         if tuple(out.shape) != (len(a), len(b)):
             raise ValueError(f"out must be {(len(a), len(b))}, got {tuple(out.shape)}")
-        _same_device(a.codes.device, out=out)
-    _call(T.lib().tv_fp8_matmul_dev, a.codes.device, *a._args(), *b._args(), b.group, a.dim, a._scale_type,
+        _same_device(device, "out", out)
+    _call(T.lib().tv_fp8_matmul_dev, device, *a._args(), *b._args(), b.group, a.dim, a._scale_type,
           out.data_ptr(), _VALUES[out.dtype], out.stride(0))
     return out
 
@@ -145,11 +168,12 @@ def rescore(queries, rows, slots, k):
     if not 0 <= k <= m:
         raise ValueError(f"k must be 0 to {m}, the number of candidates, got {k}")
     device = queries.device
-    _same_device(device, rows=rows.codes, slots=slots)
-    scores = torch.empty(nq, k, dtype=torch.float32, device=device)
-    best = torch.empty(nq, k, dtype=torch.int64, device=device)
-    ws = torch.empty(T.lib().tv_fp8_rescore_workspace(nq, m), dtype=torch.uint8, device=device)
+    _same_device(device, "rows", rows.codes)
+    _same_device(device, "slots", slots)
+    scores = torch.empty((nq, k), dtype=torch.float32, device=device)
+    best = torch.empty((nq, k), dtype=torch.int64, device=device)
+    ws = _workspace(T.lib().tv_fp8_rescore_workspace(nq, m, rows.dim), device)
     _call(T.lib().tv_fp8_rescore_dev, device, queries.data_ptr(), _VALUES[queries.dtype], queries.stride(0), nq,
           *rows._args(), rows.group, rows.dim, rows._scale_type, slots.data_ptr(), slots.stride(0), m, k,
-          scores.data_ptr(), best.data_ptr(), ws.data_ptr(), ws.numel())
+          scores.data_ptr(), best.data_ptr(), *ws[1:])
     return scores, best

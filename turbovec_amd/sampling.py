@@ -7,7 +7,7 @@ tensor on the GPU; calls run on the current stream of the tensors' device and do
 import torch
 
 from . import _lib as T
-from .fp8 import _VALUES, _call, _gpu, _same_device
+from .fp8 import _VALUES, _call, _gpu, _same_device, _workspace
 
 
 def _a_row(name, value, rows, dtype, device):
@@ -19,7 +19,7 @@ def _a_row(name, value, rows, dtype, device):
     _gpu(name, value, (dtype,), ndim=1)
     if len(value) != rows:
         raise ValueError(f"{name} must have a value a row, {rows}, got {len(value)}")
-    _same_device(device, **{name: value})
+    _same_device(device, name, value)
     return value
 
 
@@ -45,11 +45,11 @@ def sample(scores, u, *, temperature=None, top_k=None, top_p=None, min_p=None, m
         _gpu("mask", mask, (torch.int64,), ndim=2 if isinstance(mask, torch.Tensor) and mask.dim() == 2 else 1)
         if tuple(mask.shape) not in ((words,), (rows, words)):
             raise ValueError(f"mask must be {(words,)} or {(rows, words)}, got {tuple(mask.shape)}")
-        _same_device(device, mask=mask)
+        _same_device(device, "mask", mask)
         mask_ptr, mask_stride = mask.data_ptr(), mask.stride(0) if mask.dim() == 2 else 0
     slots = torch.empty(rows, dtype=torch.int64, device=device)
     probs = torch.empty(rows, dtype=torch.float32, device=device)
-    ws = torch.empty(T.lib().tv_sample_workspace(rows, n), dtype=torch.uint8, device=device)
+    ws = _workspace(T.lib().tv_sample_workspace(rows, n), device)
     _call(T.lib().tv_sample_dev, device, scores.data_ptr(), _VALUES[scores.dtype], scores.stride(0), rows, n, mask_ptr, mask_stride,
-          u.data_ptr(), *(None if p is None else p.data_ptr() for p in params), slots.data_ptr(), probs.data_ptr(), ws.data_ptr(), ws.numel())
+          u.data_ptr(), *(None if p is None else p.data_ptr() for p in params), slots.data_ptr(), probs.data_ptr(), *ws[1:])
     return slots, probs
