@@ -5,9 +5,13 @@
 // whatever order threads arrive in.  What top-k, top-p and min-p leave is a prefix of the slots ranked by score, ties to the lower
 // slot: the slots above some score, and the first few of those that have it.
 //
-// A histogram over the distance to the best score, whose bins widen with it, finds the bin that top-k or top-p end in.  Where the slots
-// down to that bin are few, they are gathered, sorted, and everything else happens among them.  Where they are many, the bin is
-// divided again until what is left in it is one score or few slots; then the row is walked once more to draw from what stays.
+// All of it is one kind of search: of values in falling order (keys of scores, or complements of slots), the last one before which less
+// than so many slots, or so much mass, lies.  A histogram of 1024 bins narrows the values to one bin, the next one divides that.  The first
+// histogram of a row goes by the distance to the best score, its bins widening with it; where the slots down to the bin it finds are
+// few, they are gathered, and everything else happens among them.  Bound by the passes over the row and the exponentials; a
+// single row by what a pass takes at least, and by the fetching of its own instructions (one loop serves every search for that).
+#include <algorithm>
+
 #include "tv_device.h"
 #include "tv_ops.h"
 
@@ -16,8 +20,7 @@ namespace tv {
 constexpr int kSampleThreads = 1024, kSampleWaves = kSampleThreads / 64;
 constexpr uint32_t kNoKey = 0x007fffffu;     // -infinity's; what is not allowed has it too
 constexpr uint32_t kBins = 1024;             // a bin to a thread
-constexpr uint32_t kListed = 4000, kListedEach = 4;     // slots that are gathered, at most: four to a thread, and two workgroups' LDS to a compute unit
-constexpr uint32_t kSorted = 512;            // of which so many are sorted
+constexpr uint32_t kListed = 4000;           // slots that are gathered, at most: two workgroups' LDS to a compute unit
 
 // The scores' order as unsigned numbers; -0 counts as +0, NaN as -infinity.
 __device__ __forceinline__ uint32_t score_key(float s) {
@@ -158,24 +161,14 @@ __device__ __forceinline__ uint64_t wave_upto(uint64_t v) {
 constexpr uint32_t kCopies = 4;
 struct SampleShared {
     uint64_t part[kSampleWaves], found_mass;
-    uint32_t part32[kSampleWaves], listed, picked, found_count, last;
+    uint32_t part32[kSampleWaves], listed, picked, found_count, found_before, found_value;
     uint32_t count[kBins * kCopies];
     uint64_t mass[kBins * kCopies];
-    uint64_t list[kListed];       // (last: kernels that list nothing leave it out)
+    uint64_t list[kListed];       // key, complement of the slot.  (Last: kernels that list nothing leave it out.)
 };
 
-__device__ uint64_t block_sum(uint64_t v, SampleShared &sh) {
-    v = wave_upto(v);
-    __syncthreads();
-    if ((threadIdx.x & 63u) == 63u) sh.part[threadIdx.x >> 6] = v;
-    __syncthreads();
-    uint64_t all = 0;
-#pragma unroll
-    for (int w = 0; w < kSampleWaves; ++w) all += sh.part[w];
-    return all;
-}
 // The sum over the threads before this one; `all` the sum over all of them.
-__device__ uint64_t block_before(uint64_t v, SampleShared &sh, uint64_t &all) {
+__device__ __forceinline__ uint64_t block_before(uint64_t v, SampleShared &sh, uint64_t &all) {
     const uint32_t wave = threadIdx.x >> 6;
     const uint64_t upto = wave_upto(v);
     __syncthreads();
@@ -183,7 +176,6 @@ __device__ uint64_t block_before(uint64_t v, SampleShared &sh, uint64_t &all) {
     __syncthreads();
     uint64_t before = upto - v;
     all = 0;
-#pragma unroll
     for (uint32_t w = 0; w < uint32_t(kSampleWaves); ++w) {
         const uint64_t x = sh.part[w];
         before += w < wave ? x : 0;
@@ -191,303 +183,26 @@ __device__ uint64_t block_before(uint64_t v, SampleShared &sh, uint64_t &all) {
     }
     return before;
 }
-
-// Sorts up to kSorted different words, none of them 0, falling, by counting those above each.
-__device__ void sort_falling(uint64_t *x, uint32_t size) {
-    __syncthreads();
-    const uint64_t mine = threadIdx.x < size ? x[threadIdx.x] : 0;
-    uint32_t above = 0;
-    if (mine != 0)
-        for (uint32_t i = 0; i < size; ++i) above += uint32_t(x[i] > mine);
-    __syncthreads();
-    if (mine != 0) x[above] = mine;
-    __syncthreads();
-}
-
-// In slot order, the first slot whose f, summed up to it from lo on, exceeds `want`; it is one of the `len` from lo on.  All threads return it.
-template <typename T, typename F>
-__device__ uint32_t locate_in(const SampleRow<T> &row, SampleShared &sh, uint32_t lo, uint32_t len, uint64_t want, F &&f) {
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    while (len > uint32_t(kSampleThreads)) {
-        const uint32_t seg = ((len + kSampleWaves - 1) / kSampleWaves + 63u) & ~63u;
-        const uint32_t from = min(len, wave * seg), to = min(len, from + seg);
-        uint64_t sum = 0;
-        row.each(lo + from, lo + to, lane, 64u, [&](uint32_t i, uint32_t k) { if (k != kNoKey) sum += f(i, k); });
-        sum = wave_upto(sum);
-        __syncthreads();
-        if (lane == 63u) sh.part[wave] = sum;
-        __syncthreads();
-        uint32_t w = 0;
-        uint64_t upto = sh.part[0], before = 0;
-        while (w + 1 < uint32_t(kSampleWaves) && upto <= want) {
-            before = upto;
-            upto += sh.part[++w];
-        }
-        want -= before;
-        lo += min(len, w * seg);
-        len = min(seg, len - min(len, w * seg));
-    }
-    // at most one slot to a thread
-    const uint32_t i = lo + threadIdx.x, k = threadIdx.x < len ? row.key_at(i) : kNoKey;
-    const uint64_t mine = k != kNoKey ? f(i, k) : 0;
+__device__ __forceinline__ uint64_t block_sum(uint64_t v, SampleShared &sh) {
     uint64_t all;
-    const uint64_t before = block_before(mine, sh, all);
-    if (threadIdx.x == 0) sh.picked = 0;
+    block_before(v, sh, all);
+    return all;
+}
+__device__ __forceinline__ uint32_t block_max(uint32_t v, SampleShared &sh) {
+    v = wave_umax(v);
     __syncthreads();
-    if (before <= want && before + mine > want) sh.picked = threadIdx.x;
+    if ((threadIdx.x & 63u) == 0) sh.part32[threadIdx.x >> 6] = v;
     __syncthreads();
-    return lo + sh.picked;
-}
-// f summed over the slots lo .. hi - 1.
-template <typename T, typename F>
-__device__ uint64_t sum_of(const SampleRow<T> &row, SampleShared &sh, uint32_t lo, uint32_t hi, F &&f) {
-    uint64_t sum = 0;
-    row.each(lo, hi, threadIdx.x, kSampleThreads, [&](uint32_t i, uint32_t k) { if (k != kNoKey) sum += f(i, k); });
-    return block_sum(sum, sh);
-}
-
-// What a threshold is looked for by: its keys lo .. hi, how many slots have one of them, and what lies above.
-struct Range {
-    uint32_t lo, hi, count;
-    uint64_t count_before, mass_before;
-};
-
-template <bool MASS>
-__device__ void clear_bins(SampleShared &sh) {
-    __syncthreads();
-#pragma unroll
-    for (uint32_t c = 0; c < kCopies; ++c) {
-        sh.count[c * kBins + threadIdx.x] = 0;
-        if (MASS) sh.mass[c * kBins + threadIdx.x] = 0;
-    }
-    __syncthreads();
-}
-// One histogram: of the slots lo .. hi - 1 whose keys lie in r, the bins by bin_of.
-template <bool MASS, typename T, typename B>
-__device__ void fill_bins(const SampleRow<T> &row, SampleShared &sh, const Range &r, uint32_t lo, uint32_t hi, B &&bin_of) {
-    clear_bins<MASS>(sh);
-    const uint32_t copy = threadIdx.x % kCopies;
-    row.each(lo, hi, threadIdx.x, kSampleThreads, [&](uint32_t, uint32_t k) {
-        if (k < r.lo || k > r.hi) return;
-        const uint32_t at = bin_of(k) * kCopies + copy;
-        atomicAdd(&sh.count[at], 1u);
-        if (MASS) atomicAdd(reinterpret_cast<unsigned long long *>(&sh.mass[at]), (unsigned long long)row.units(k));
-    });
-    __syncthreads();
-}
-// A thread's bin, all copies.
-template <bool MASS>
-__device__ __forceinline__ void own_bin(const SampleShared &sh, uint32_t &count, uint64_t &mass) {
-    count = 0;
-    mass = 0;
-#pragma unroll
-    for (uint32_t c = 0; c < kCopies; ++c) {
-        count += sh.count[threadIdx.x * kCopies + c];
-        if (MASS) mass += sh.mass[threadIdx.x * kCopies + c];
-    }
-}
-// The last bin that has slots and that reaches(count before, mass before) says yes to; r's counts become that bin's, total the mass of all.
-template <bool MASS, typename F>
-__device__ uint32_t pick_bin(SampleShared &sh, Range &r, uint32_t count, uint64_t mass, F &&reaches, uint64_t &total) {
-    const uint32_t t = threadIdx.x;
-    if (t == 0) sh.picked = 0;
-    uint64_t all;
-    const uint64_t count_before = r.count_before + block_before(count, sh, all);
-    const uint64_t mass_before = MASS ? r.mass_before + block_before(mass, sh, total) : 0;
-    if (count != 0 && (t == 0 || reaches(count_before, mass_before))) atomicMax(&sh.picked, t);
-    __syncthreads();
-    const uint32_t pick = sh.picked;
-    if (t == pick) { sh.found_count = uint32_t(count_before); sh.found_mass = mass_before; sh.listed = count; }
-    __syncthreads();
-    r.count = sh.listed;
-    r.count_before = sh.found_count;
-    r.mass_before = sh.found_mass;
-    return pick;
-}
-template <bool MASS, typename T, typename B, typename F>
-__device__ uint32_t pick_bin(const SampleRow<T> &row, SampleShared &sh, Range &r, B &&bin_of, F &&reaches, uint64_t &total) {
-    fill_bins<MASS>(row, sh, r, 0, row.n, bin_of);
-    uint32_t count;
-    uint64_t mass;
-    own_bin<MASS>(sh, count, mass);
-    return pick_bin<MASS>(sh, r, count, mass, reaches, total);
-}
-// The keys of bin b of the histogram that narrows r, whose bins are 2^shift keys each.
-__device__ __forceinline__ uint32_t narrow_shift(const Range &r) { return uint32_t(max(0, 22 - __clz(int(r.hi - r.lo)))); }
-__device__ __forceinline__ void narrow_to(Range &r, uint32_t b, uint32_t shift) {
-    r.hi -= b << shift;
-    r.lo = max(r.lo, r.hi - min(r.hi, (1u << shift) - 1u));
-}
-
-// Lists the slots of from .. to - 1 whose keys lie in lo .. hi, kListed at most; returns how many.
-template <typename T>
-__device__ uint32_t list_slots(const SampleRow<T> &row, SampleShared &sh, uint32_t from, uint32_t to, uint32_t lo, uint32_t hi) {
-    __syncthreads();
-    if (threadIdx.x == 0) sh.listed = 0;
-    __syncthreads();
-    row.each(from, to, threadIdx.x, kSampleThreads, [&](uint32_t i, uint32_t k) {
-        if (k < lo || k > hi) return;
-        const uint32_t at = atomicAdd(&sh.listed, 1u);
-        if (at < kListed) sh.list[at] = uint64_t(k) << 32 | uint32_t(~i);
-    });
-    __syncthreads();
-    return min(sh.listed, kListed);
-}
-// A thread's slots of the list.
-struct Listed {
-    uint32_t key[kListedEach], place[kListedEach];      // place: the complement of the slot, which falls as the slot rises
-    uint64_t mass[kListedEach];
-    bool in[kListedEach];
-    template <bool MASS, typename T>
-    __device__ __forceinline__ void take(const SampleRow<T> &row, const SampleShared &sh, uint32_t listed) {
-#pragma unroll
-        for (uint32_t j = 0; j < kListedEach; ++j) {
-            const uint32_t e = j * kSampleThreads + threadIdx.x;
-            in[j] = e < listed;
-            const uint64_t x = in[j] ? sh.list[e] : 0;
-            key[j] = uint32_t(x >> 32);
-            place[j] = uint32_t(x);
-            mass[j] = MASS && in[j] ? row.units(key[j]) : 0;
-        }
-    }
-};
-// Narrows r to one value v: the last, in falling order, that has slots that are in and that reaches(count before, mass before) says yes to.
-template <bool MASS, typename F>
-__device__ void narrow_listed(SampleShared &sh, const Listed &l, const uint32_t (&v)[kListedEach], Range &r, F &&reaches) {
-    do {      // (once at least: r's count may not be known yet)
-        const uint32_t shift = narrow_shift(r), copy = threadIdx.x % kCopies;
-        clear_bins<MASS>(sh);
-#pragma unroll
-        for (uint32_t j = 0; j < kListedEach; ++j) {
-            if (!l.in[j] || v[j] < r.lo || v[j] > r.hi) continue;
-            const uint32_t at = ((r.hi - v[j]) >> shift) * kCopies + copy;
-            atomicAdd(&sh.count[at], 1u);
-            if (MASS) atomicAdd(reinterpret_cast<unsigned long long *>(&sh.mass[at]), (unsigned long long)l.mass[j]);
-        }
-        __syncthreads();
-        uint32_t count;
-        uint64_t mass, total;
-        own_bin<MASS>(sh, count, mass);
-        narrow_to(r, pick_bin<MASS>(sh, r, count, mass, reaches, total), shift);
-    } while (r.lo < r.hi);
-}
-// The slot up to which `ties` of those that are in and have this key lie.
-__device__ uint32_t last_tie(SampleShared &sh, Listed l, uint32_t key, uint32_t ties) {
-#pragma unroll
-    for (uint32_t j = 0; j < kListedEach; ++j) l.in[j] &= l.key[j] == key;
-    Range r{0u, ~0u, 0, 0, 0};
-    narrow_listed<false>(sh, l, l.place, r, [&](uint64_t c, uint64_t) { return c < uint64_t(ties); });
-    return ~r.lo;
-}
-
-// Narrows r to one key: the last, in falling order, that has slots and that reaches(count before, mass before) says yes to.
-template <bool MASS, typename T, typename F>
-__device__ void narrow(const SampleRow<T> &row, SampleShared &sh, Range &r, F &&reaches) {
-    uint64_t total;
-    while (r.lo < r.hi && r.count > kListed) {
-        const uint32_t hi = r.hi, shift = narrow_shift(r);
-        const uint32_t b = pick_bin<MASS>(row, sh, r, [=](uint32_t k) { return (hi - k) >> shift; }, reaches, total);
-        narrow_to(r, b, shift);
-    }
-    if (r.lo == r.hi) return;
-    Listed l;
-    l.take<MASS>(row, sh, list_slots(row, sh, 0, row.n, r.lo, r.hi));
-    narrow_listed<MASS>(sh, l, l.key, r, reaches);
-}
-
-__device__ __forceinline__ uint64_t drawn_mass(float u, uint64_t sum) {
-    const double want = double(u) * double(sum);
-    return want >= double(sum) ? sum - 1 : want > 0.0 ? uint64_t(want) : uint64_t(0);
-}
-
-// Draws from the slots of sh.list: of the first top_k in the order of their rank (0: all), those that less than a limit of mass lies before
-// (limit_p), and of those the ones of at least min_key.  The limit is top_p of the mass of the first top_k, or given.
-struct ListLimits {
-    uint32_t top_k, min_key;
-    bool limit_p;
-    double top_p, limit;
-    float u;
-};
-
-// Few slots: sorted by rank, then, what stays of them, by slot.
-template <typename T>
-__device__ void draw_sorted(const SampleRow<T> &row, SampleShared &sh, uint32_t listed, ListLimits lim, int64_t &slot, float &prob) {
-    const uint32_t t = threadIdx.x;
-    sort_falling(sh.list, listed);
-    if (lim.top_k != 0) listed = min(listed, lim.top_k);
-    const uint64_t x = t < listed ? sh.list[t] : 0;
-    const uint32_t key = uint32_t(x >> 32);
-    const uint64_t mass = x != 0 ? row.units(key) : 0;
-    uint64_t all, total;
-    const uint64_t before = block_before(mass, sh, all);
-    if (lim.top_k != 0) lim.limit = lim.top_p * double(all);
-    const bool stays = x != 0 && (t == 0 || ((!lim.limit_p || double(before) < lim.limit) && key >= lim.min_key));
-    // (what stays is a prefix: min-p and top-p both leave one)
-    block_before(stays, sh, all);
-    const uint32_t kept = uint32_t(all);
-    if (stays) sh.list[t] = uint64_t(uint32_t(x)) << 32 | key;
-    sort_falling(sh.list, kept);
-    const uint64_t y = t < kept ? sh.list[t] : 0;
-    const uint64_t own = y != 0 ? row.units(uint32_t(y)) : 0, upto = block_before(own, sh, total), want = drawn_mass(lim.u, total);
-    if (t == 0) sh.picked = 0;
-    __syncthreads();
-    if (upto <= want && upto + own > want) sh.picked = t;
-    __syncthreads();
-    const uint64_t z = sh.list[sh.picked];
-    slot = int64_t(~uint32_t(z >> 32));
-    prob = float(ldexp(row.weight(uint32_t(z)), row.shift) / double(total));
-}
-
-template <typename T>
-__device__ void draw_from_list(const SampleRow<T> &row, SampleShared &sh, uint32_t listed, ListLimits lim, int64_t &slot, float &prob) {
-    if (listed <= kSorted) return draw_sorted(row, sh, listed, lim, slot, prob);
-    Listed l;
-    l.take<true>(row, sh, listed);
-    uint64_t sum;
-    const auto mass_in = [&] {
-        sum = 0;
-#pragma unroll
-        for (uint32_t j = 0; j < kListedEach; ++j) sum += l.in[j] ? l.mass[j] : 0;
-        return block_sum(sum, sh);
-    };
-    const auto keep = [&](uint32_t least, uint32_t count, uint32_t ties) {
-        const uint32_t last = ties < count ? last_tie(sh, l, least, ties) : ~0u;
-#pragma unroll
-        for (uint32_t j = 0; j < kListedEach; ++j) l.in[j] &= l.key[j] > least || (l.key[j] == least && ~l.place[j] <= last);
-    };
-    if (lim.top_k != 0) {
-        if (listed > lim.top_k) {
-            Range r{kNoKey + 1u, row.most, 0, 0, 0};
-            narrow_listed<false>(sh, l, l.key, r, [&](uint64_t c, uint64_t) { return c < uint64_t(lim.top_k); });
-            keep(r.lo, r.count, min(r.count, uint32_t(uint64_t(lim.top_k) - r.count_before)));
-        }
-        lim.limit = lim.top_p * double(mass_in());
-    }
-    if (lim.limit_p) {
-        Range r{kNoKey + 1u, row.most, 0, 0, 0};
-        narrow_listed<true>(sh, l, l.key, r, [&](uint64_t c, uint64_t m) { return c == 0 || double(m) < lim.limit; });
-        if (r.lo < lim.min_key) {
-            r.lo = lim.min_key;
-            r.count = 0;
-        }
-        keep(r.lo, r.count, ties_within(row, r, lim.limit));
-    } else {
-        keep(lim.min_key, 0, 0);
-    }
-    const uint64_t total = mass_in(), want = drawn_mass(lim.u, total);
-    Range r{0u, ~0u, 0, 0, 0};
-    narrow_listed<true>(sh, l, l.place, r, [&](uint64_t c, uint64_t m) { return c == 0 || m <= want; });
-    slot = int64_t(~r.lo);
-    prob = float(ldexp(row.weight(row.key_at(~r.lo)), row.shift) / double(total));
+    for (int w = 0; w < kSampleWaves; ++w) v = max(v, sh.part32[w]);
+    return v;
 }
 
 // A row's parameters.
 struct Limits {
     int32_t top_k;
-    float top_p, u;
+    float top_p, u, t, min_p;
     bool limit_k, limit_p;
     uint32_t min_key;
-    float t, min_p;
     __device__ __forceinline__ void load(const SampleArgs &p, uint32_t r) {
         t = p.temperature == nullptr ? 1.0f : p.temperature[r];
         min_p = p.min_p == nullptr ? 0.0f : p.min_p[r];
@@ -505,75 +220,273 @@ struct Limits {
     }
 };
 
-// How many of r's slots, which all have its one key, stay: those that less than `limit` of mass lies before.
+// What stays: slots of keys above `least`, and of those of that key the ones up to tie_last.
+struct Cut {
+    uint32_t least, tie_last;
+    __device__ __forceinline__ bool leaves(uint32_t i, uint32_t k) const { return k > least || (k == least && i <= tie_last); }
+};
+// The values that the one sought is among, in falling order from hi; of a bin that was picked, its slots, and the slots and the mass before it.
+struct Search {
+    uint32_t lo, hi, count;
+    uint64_t before, mass_before;
+};
+__device__ __forceinline__ uint32_t shift_of(const Search &s) { return uint32_t(max(0, 22 - __clz(int(s.hi - s.lo)))); }      // 1024 bins of 2^shift
+__device__ __forceinline__ void narrow_to(Search &s, uint32_t bin) {
+    const uint32_t shift = shift_of(s);
+    s.hi -= bin << shift;
+    s.lo = max(s.lo, s.hi - min(s.hi, (1u << shift) - 1u));
+}
+
+enum { kByDistance, kByKey, kByPlace };
+struct Pass {
+    int mode;
+    bool mass, ties;          // ties: of the cut's slots only those of its least key
+};
+// A histogram of the cut's slots whose values lie in s: of those of the list, or those lo .. hi - 1 of the row.
 template <typename T>
-__device__ __forceinline__ uint32_t ties_within(const SampleRow<T> &row, const Range &r, double limit) {
-    const uint64_t each = row.units(r.lo);
-    const double fit = each == 0 ? double(r.count) : ceil((limit - double(r.mass_before)) / double(each));
-    return fit < 1.0 ? 1u : fit < double(r.count) ? uint32_t(fit) : r.count;
+__device__ __forceinline__ void fill(const SampleRow<T> &row, SampleShared &sh, bool listed, uint32_t lo, uint32_t hi, const Cut &cut, const Search &s, const Pass &pass) {
+    __syncthreads();
+#pragma unroll
+    for (uint32_t c = 0; c < kCopies; ++c) {
+        sh.count[c * kBins + threadIdx.x] = 0;
+        if (pass.mass) sh.mass[c * kBins + threadIdx.x] = 0;
+    }
+    __syncthreads();
+    const uint32_t shift = shift_of(s), copy = threadIdx.x % kCopies;
+    const auto add = [&](uint32_t i, uint32_t k) {
+        if (!cut.leaves(i, k) || (pass.ties && k != cut.least)) return;
+        const uint32_t v = pass.mode == kByPlace ? ~i : k;
+        if (v < s.lo || v > s.hi) return;
+        const uint32_t at = (pass.mode == kByDistance ? row.bin(k) : (s.hi - v) >> shift) * kCopies + copy;
+        atomicAdd(&sh.count[at], 1u);
+        if (pass.mass) atomicAdd(reinterpret_cast<unsigned long long *>(&sh.mass[at]), (unsigned long long)row.units(k));
+    };
+    if (listed) {
+#pragma unroll 1
+        for (uint32_t e = threadIdx.x; e < hi; e += kSampleThreads) add(~uint32_t(sh.list[e]), uint32_t(sh.list[e] >> 32));
+    } else {
+        row.each(lo, hi, threadIdx.x, kSampleThreads, add);
+    }
+    __syncthreads();
+}
+// A thread's bin, all copies.
+__device__ __forceinline__ void own_bin(const SampleShared &sh, bool with_mass, uint32_t &count, uint64_t &mass) {
+    count = 0;
+    mass = 0;
+#pragma unroll
+    for (uint32_t c = 0; c < kCopies; ++c) {
+        count += sh.count[threadIdx.x * kCopies + c];
+        if (with_mass) mass += sh.mass[threadIdx.x * kCopies + c];
+    }
+}
+
+__device__ __forceinline__ uint64_t drawn_mass(float u, uint64_t sum) {
+    const double want = double(u) * double(sum);
+    return want >= double(sum) ? sum - 1 : want > 0.0 ? uint64_t(want) : uint64_t(0);
+}
+// A row's searches, one after the other.
+enum { kTopK, kTopP, kTies, kDraw };
+struct State {
+    int phase, after;         // after: the phase that ends in ties
+    bool whole;               // the search has not been narrowed yet
+    bool listed;
+    uint32_t n;               // slots in the list
+    Search s;
+    Cut cut;
+    uint64_t bound, total;    // total: the mass of what the phase's first histogram counted
+};
+__device__ __forceinline__ bool by_mass(int phase) { return phase == kTopP || phase == kDraw; }
+
+// Of the bins, a thread each, the last that has slots and that less than the bound lies before; the first one always.
+__device__ __forceinline__ uint32_t pick(SampleShared &sh, State &st, const Limits &lim, uint32_t count, uint64_t mass) {
+    const uint32_t t = threadIdx.x;
+    if (t == 0) sh.picked = 0;
+    uint64_t all;
+    const uint64_t before = st.s.before + block_before(count, sh, all);
+    uint64_t upto = before, mass_before = 0;
+    if (by_mass(st.phase)) {
+        upto = mass_before = st.s.mass_before + block_before(mass, sh, all);
+        if (st.whole) {
+            st.total = all;
+            st.bound = st.phase == kTopP ? uint64_t(ceil(double(lim.top_p) * double(all))) : drawn_mass(lim.u, all) + 1;
+        }
+    }
+    if (count != 0 && (before == 0 || upto < st.bound)) atomicMax(&sh.picked, t);
+    __syncthreads();
+    const uint32_t bin = sh.picked;
+    if (t == bin) { sh.found_count = count; sh.found_before = uint32_t(before); sh.found_mass = mass_before; }
+    __syncthreads();
+    st.s.count = sh.found_count;
+    st.s.before = sh.found_before;
+    st.s.mass_before = sh.found_mass;
+    st.whole = false;
+    return bin;
+}
+
+// Lists the cut's slots of lo .. hi - 1 whose keys are from .. upto, kListed at most; returns how many.
+template <typename T>
+__device__ __forceinline__ uint32_t list_slots(const SampleRow<T> &row, SampleShared &sh, uint32_t lo, uint32_t hi, const Cut &cut, uint32_t from, uint32_t upto) {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.listed = 0;
+    __syncthreads();
+    row.each(lo, hi, threadIdx.x, kSampleThreads, [&](uint32_t i, uint32_t k) {
+        if (k < from || k > upto || !cut.leaves(i, k)) return;
+        const uint32_t at = atomicAdd(&sh.listed, 1u);
+        if (at < kListed) sh.list[at] = uint64_t(k) << 32 | uint32_t(~i);
+    });
+    __syncthreads();
+    return min(sh.listed, kListed);
+}
+// The one value in s of the list's slots that count.
+__device__ __forceinline__ uint32_t only_value(SampleShared &sh, const State &st) {
+    for (uint32_t e = threadIdx.x; e < st.n; e += kSampleThreads) {
+        const uint32_t k = uint32_t(sh.list[e] >> 32), place = uint32_t(sh.list[e]), v = st.phase >= kTies ? place : k;
+        if (v >= st.s.lo && v <= st.s.hi && st.cut.leaves(~place, k) && (st.phase != kTies || k == st.cut.least)) sh.found_value = v;
+    }
+    __syncthreads();
+    const uint32_t v = sh.found_value;
+    __syncthreads();
+    return v;
+}
+
+// Of the cut's slots from lo on (ties: those of its least key, each counting 1; otherwise their mass), in slot order the first that the sum up to it
+// exceeds `want` at; it is one of the `len` from lo on.
+template <typename T>
+__device__ __forceinline__ uint32_t locate(const SampleRow<T> &row, SampleShared &sh, uint32_t lo, uint32_t len, const Cut &cut, bool ties, uint64_t want) {
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const auto value = [&](uint32_t i, uint32_t k) { return !cut.leaves(i, k) ? uint64_t(0) : ties ? uint64_t(k == cut.least) : row.units(k); };
+    while (len > uint32_t(kSampleThreads)) {
+        const uint32_t seg = ((len + kSampleWaves - 1) / kSampleWaves + 63u) & ~63u;
+        const uint32_t from = min(len, wave * seg), to = min(len, from + seg);
+        uint64_t sum = 0;
+        row.each(lo + from, lo + to, lane, 64u, [&](uint32_t i, uint32_t k) { sum += value(i, k); });
+        sum = wave_upto(sum);
+        __syncthreads();
+        if (lane == 63u) sh.part[wave] = sum;
+        __syncthreads();
+        uint32_t w = 0;
+        uint64_t upto = sh.part[0], before = 0;
+        while (w + 1 < uint32_t(kSampleWaves) && upto <= want) {
+            before = upto;
+            upto += sh.part[++w];
+        }
+        want -= before;
+        lo += min(len, w * seg);
+        len = min(seg, len - min(len, w * seg));
+    }
+    // at most one slot to a thread
+    const uint64_t mine = threadIdx.x < len ? value(lo + threadIdx.x, row.key_at(lo + threadIdx.x)) : 0;
+    uint64_t all;
+    const uint64_t before = block_before(mine, sh, all);
+    if (threadIdx.x == 0) sh.picked = 0;
+    __syncthreads();
+    if (before <= want && before + mine > want) sh.picked = threadIdx.x;
+    __syncthreads();
+    return lo + sh.picked;
+}
+// The mass that the cut leaves of the slots lo .. hi - 1.
+template <typename T>
+__device__ __forceinline__ uint64_t mass_of(const SampleRow<T> &row, SampleShared &sh, uint32_t lo, uint32_t hi, const Cut &cut) {
+    uint64_t sum = 0;
+    row.each(lo, hi, threadIdx.x, kSampleThreads, [&](uint32_t i, uint32_t k) { sum += cut.leaves(i, k) ? row.units(k) : 0; });
+    return block_sum(sum, sh);
 }
 
 template <typename T>
-__device__ void sample_row(const SampleRow<T> &row, SampleShared &sh, const Limits &lim, int64_t &slot, float &prob) {
-    const int32_t top_k = lim.top_k;
-    const float top_p = lim.top_p, u = lim.u;
-    const bool limit_k = lim.limit_k, limit_p = lim.limit_p;
-    const uint32_t min_key = lim.min_key;
-    const auto first_k = [&](uint64_t c, uint64_t) { return c < uint64_t(top_k); };
-    uint64_t total = 0;
-    uint32_t least = kNoKey + 1u, equal = 0, ties = 0;      // slots of a higher key stay, and so many of those of this one
-    if (limit_k) {
-        Range all{kNoKey + 1u, row.most, 0, 0, 0};
-        const uint32_t b = pick_bin<false>(row, sh, all, [&](uint32_t k) { return row.bin(k); }, first_k, total);
-        all.lo = row.least_of_bin(b);
-        if (all.count_before + all.count <= kListed) {
-            const uint32_t listed = list_slots(row, sh, 0, row.n, all.lo, row.most);
-            return draw_from_list(row, sh, listed, ListLimits{uint32_t(top_k), min_key, limit_p, double(top_p), 0.0, u}, slot, prob);
+__device__ __forceinline__ State first_state(const SampleRow<T> &row, const Limits &lim) {
+    State st;
+    st.phase = lim.limit_k ? kTopK : lim.limit_p ? kTopP : kDraw;
+    st.after = kDraw;
+    st.whole = true;
+    st.listed = false;
+    st.n = 0;
+    st.s = Search{kNoKey + 1u, row.most, 0, 0, 0};
+    st.cut = Cut{kNoKey + 1u, ~0u};
+    st.bound = uint64_t(lim.top_k);
+    st.total = 0;
+    return st;
+}
+// The search goes from the row's first histogram to the bin it picked.  `down`: slots that can still be drawn, down to that bin.
+template <typename T>
+__device__ __forceinline__ void to_bin(const SampleRow<T> &row, SampleShared &sh, State &st, const Limits &lim, uint32_t bin, uint32_t count, uint32_t &down) {
+    // (min-p leaves fewer, but top-p after top-k needs all of top-k's)
+    const uint32_t last = st.phase == kTopP ? min(bin, row.bin(lim.min_key)) : bin;
+    down = uint32_t(block_sum(threadIdx.x <= last ? count : 0, sh));
+    st.s.lo = max(st.cut.least, row.least_of_bin(bin));
+    st.s.hi = bin == 0 ? row.most : row.least_of_bin(bin - 1) - 1u;
+}
+// From which key on a row's slots are listed.  Where min-p leaves nothing of the bin, the search is over.
+__device__ __forceinline__ uint32_t list_from(State &st, const Limits &lim) {
+    if (st.phase != kTopP || lim.min_key <= st.s.lo) return st.s.lo;
+    st.s.lo = min(lim.min_key, st.s.hi);
+    if (lim.min_key > st.s.hi) st.s.count = 0;
+    return lim.min_key;
+}
+
+// The searches that are left, to the draw, or (to_cut) to the end of the one that st is in.
+template <typename T>
+__device__ void search(const SampleRow<T> &row, SampleShared &sh, const Limits &lim, State &st, bool to_cut, int64_t &slot, float &prob) {
+    while (true) {
+        if (st.phase >= kTies && !st.listed) {
+            // slots next to each other fall into one bin, a row's are walked instead
+            if (st.phase == kDraw) {
+                st.total = mass_of(row, sh, 0, row.n, st.cut);
+                st.bound = drawn_mass(lim.u, st.total) + 1;
+            }
+            st.s.lo = st.s.hi = ~locate(row, sh, 0, row.n, st.cut, st.phase == kTies, st.bound - 1);
+        } else if (st.whole || (st.s.lo < st.s.hi && st.s.count != 0)) {
+            const bool first = st.whole && !st.listed;
+            if (!st.whole && st.listed && st.s.count == 1) {
+                st.s.lo = st.s.hi = only_value(sh, st);
+                continue;
+            }
+            fill(row, sh, st.listed, 0, st.listed ? st.n : row.n, st.cut, st.s, Pass{first ? kByDistance : st.phase >= kTies ? kByPlace : kByKey, by_mass(st.phase), st.phase == kTies});
+            uint32_t count, down;
+            uint64_t mass;
+            own_bin(sh, by_mass(st.phase), count, mass);
+            const uint32_t bin = pick(sh, st, lim, count, mass);
+            if (!first) {
+                narrow_to(st.s, bin);
+                continue;
+            }
+            to_bin(row, sh, st, lim, bin, count, down);
+            if (down <= kListed) {
+                st.n = list_slots(row, sh, 0, row.n, st.cut, list_from(st, lim), row.most);
+                st.listed = true;
+            }
+            continue;
         }
-        if (b != 0) all.hi = row.least_of_bin(b - 1) - 1u;
-        narrow<false>(row, sh, all, first_k);
-        least = all.lo;
-        equal = all.count;
-        ties = min(equal, uint32_t(uint64_t(top_k) - all.count_before));
-    }
-    if (limit_p) {
-        double limit = 0.0;
-        if (limit_k) {
-            const uint64_t above = sum_of(row, sh, 0, row.n, [&](uint32_t, uint32_t k) { return k > least ? row.units(k) : uint64_t(0); });
-            limit = double(top_p) * double(above + row.units(least) * ties);
+        // one value is left
+        if (st.phase == kDraw) {
+            slot = int64_t(~st.s.lo);
+            prob = float(ldexp(row.weight(row.key_at(~st.s.lo)), row.shift) / double(st.total));
+            return;
         }
-        const auto first_p = [&](uint64_t c, uint64_t m) { return c == 0 || double(m) < limit; };
-        Range all{least, row.most, 0, 0, 0};
-        // (the limit is a share of the mass that the histogram itself adds up, where top-k has left everything)
-        const uint32_t b = pick_bin<true>(row, sh, all, [&](uint32_t k) { return row.bin(k); },
-            [&](uint64_t c, uint64_t m) { return c == 0 || double(m) < (limit_k ? limit : double(top_p) * double(total)); }, total);
-        if (!limit_k) limit = double(top_p) * double(total);
-        all.lo = max(least, row.least_of_bin(b));
-        if (!limit_k) {
-            // of what top-p may leave, min-p leaves the slots of min_key and above
-            const uint32_t from = max(all.lo, min_key);
-            if (from > all.lo || all.count_before + all.count <= kListed) {
-                const uint32_t listed = list_slots(row, sh, 0, row.n, from, row.most);
-                if (sh.listed <= kListed) return draw_from_list(row, sh, listed, ListLimits{0u, min_key, true, 0.0, limit, u}, slot, prob);
+        int next = kDraw;
+        if (st.phase == kTies) {
+            st.cut.tie_last = ~st.s.lo;
+            next = st.after;
+        } else {
+            next = st.phase == kTopK && lim.limit_p ? kTopP : kDraw;
+            uint32_t ties = uint32_t(min(uint64_t(st.s.count), st.bound - min(st.bound, st.s.before)));
+            if (st.phase == kTopP) {
+                const uint64_t each = row.units(st.s.lo);
+                const double fit = each == 0 ? double(st.s.count) : ceil((double(st.bound) - double(st.s.mass_before)) / double(each));
+                ties = fit < 1.0 ? min(1u, st.s.count) : fit < double(st.s.count) ? uint32_t(fit) : st.s.count;
+            }
+            st.cut = Cut{st.s.lo, st.s.lo == st.cut.least ? st.cut.tie_last : ~0u};
+            if (ties < st.s.count) {
+                st.after = next;
+                next = kTies;
+                st.bound = ties;
             }
         }
-        if (b != 0) all.hi = row.least_of_bin(b - 1) - 1u;
-        narrow<true>(row, sh, all, first_p);
-        const uint32_t stay = ties_within(row, all, limit);
-        // (never below top-k's class: the mass up to its end is all that top-k left, or more)
-        ties = limit_k && all.lo == least ? min(stay, ties) : stay;
-        least = all.lo;
-        equal = all.count;
+        if (to_cut && next != kTies) return;
+        if (next == kDraw && lim.min_key > st.cut.least) st.cut = Cut{lim.min_key, ~0u};
+        st.phase = next;
+        st.whole = true;
+        st.s = next >= kTies ? Search{~(row.n - 1u), ~0u, 0, 0, 0} : Search{st.cut.least, row.most, 0, 0, 0};
     }
-    uint32_t tie_last = ~0u;
-    if (ties < equal) {
-        tie_last = locate_in(row, sh, 0, row.n, ties - 1u, [&](uint32_t, uint32_t k) { return uint64_t(k == least); });
-    }
-    const auto kept = [&](uint32_t i, uint32_t k) { return k < least || k < min_key || (k == least && i > tie_last) ? uint64_t(0) : row.units(k); };
-    total = sum_of(row, sh, 0, row.n, kept);
-    const uint32_t at = locate_in(row, sh, 0, row.n, drawn_mass(u, total), kept);
-    slot = at;
-    prob = float(ldexp(row.weight(row.key_at(at)), row.shift) / double(total));
 }
 
 template <typename T>
@@ -583,14 +496,6 @@ __device__ __forceinline__ SampleRow<T> row_of(const SampleArgs &p, uint32_t r) 
     row.mask = p.mask == nullptr ? nullptr : p.mask + size_t(r) * p.mask_stride;
     row.n = p.n;
     return row;
-}
-__device__ __forceinline__ uint32_t block_max(uint32_t v, SampleShared &sh) {
-    v = wave_umax(v);
-    __syncthreads();
-    if ((threadIdx.x & 63u) == 0) sh.part32[threadIdx.x >> 6] = v;
-    __syncthreads();
-    for (int w = 0; w < kSampleWaves; ++w) v = max(v, sh.part32[w]);
-    return v;
 }
 
 // Short rows, and many: a workgroup to a row.
@@ -609,7 +514,9 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample(SampleArgs p) {
         float prob = 0.0f;
         if (most != kNoKey) {
             lim.set(row, most);
-            sample_row(row, sh, lim, slot, prob);
+            State st = first_state(row, lim);
+            if (st.phase == kDraw && lim.min_key > st.cut.least) st.cut.least = lim.min_key;
+            search(row, sh, lim, st, false, slot, prob);
         }
         if (threadIdx.x == 0) { p.out_slots[r] = slot; p.out_probs[r] = prob; }
         __syncthreads();
@@ -618,10 +525,10 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample(SampleArgs p) {
 
 // Long rows, not many: a row goes in chunks to workgroups, through six kernels that each walk it once at most.
 //   max     the best score of each chunk
-//   bins    the histogram, added up over the row's chunks; where nothing limits the row, the mass of each chunk
-//   list    few slots down to the threshold's bin: gathered.  Many: the bin's own histogram.  Where nothing limits the row, the draw.
-//   narrow  a draw from the gathered slots, by the first chunk; or the slots of the second histogram's bin.  (top-k that leaves many and
-//           top-p together: the first chunk takes the row alone.)
+//   bins    the first histogram, added up over the row's chunks; where nothing limits the row, the mass of each chunk
+//   list    few slots down to the bin it leaves: gathered.  Many: the bin's own histogram.  Where nothing limits the row, the draw.
+//   narrow  the rest of the search among the gathered slots, by the first chunk; or the slots of the second histogram's bin.  (top-k that
+//           leaves many and top-p together: the first chunk takes the row alone.)
 //   mass    the threshold from the slots of that bin, by each chunk for itself; what stays in the chunk
 //   draw    from those masses, by the first chunk
 // A kernel's chunks add to what lies in the workspace with whole numbers, so that their order does not show.  What they hand on passes from
@@ -631,15 +538,16 @@ struct SampleSplit {
     // zeroed by the first kernel
     uint64_t mass[2][kBins];
     uint32_t count[2][kBins];
-    uint32_t listed, state, least, tie_last;
+    uint32_t listed, state;
+    Cut cut;
     uint64_t list[kListed];
 };
 constexpr uint32_t kSplitZeroed = offsetof(SampleSplit, list) / 4;
-enum { kRowOpen = 0, kRowDone = 1, kRowThreshold = 2 };
+enum { kRowOpen = 0, kRowDone = 1, kRowCut = 2 };
 struct SplitArgs {
     SampleSplit *rows;
     uint64_t *chunk_mass;     // [row][chunk]
-    uint2 *chunk_cut;         // the threshold's key, and the last slot of that key that stays
+    Cut *chunk_cut;
     uint32_t *chunk_most;
     uint32_t chunk, chunks;   // slots of a chunk, chunks of a row
 };
@@ -650,12 +558,15 @@ struct Chunk {
     SampleRow<T> row;
     Limits lim;
     SampleSplit *ws;
-    uint32_t r, c, from, to, most;
+    uint32_t r, c, from, to, most, count;
+    uint64_t mass;            // count, mass: a thread's bin of the first histogram
     __device__ __forceinline__ Chunk(const SampleArgs &p, const SplitArgs &x)
         : row(row_of<T>(p, blockIdx.x)), ws(x.rows + blockIdx.x), r(blockIdx.x), c(blockIdx.y), from(blockIdx.y * x.chunk), to(min(p.n, from + x.chunk)) {}
-    __device__ __forceinline__ bool open(const SampleArgs &p, const SplitArgs &x, SampleShared &sh) {
+    __device__ __forceinline__ bool open(const SampleArgs &p, const SplitArgs &x, SampleShared &sh, bool bins) {
         lim.load(p, r);
         most = kNoKey;
+        count = bins ? ws->count[0][threadIdx.x] : 0;
+        mass = bins ? ws->mass[0][threadIdx.x] : 0;
         for (uint32_t i = threadIdx.x; i < x.chunks; i += kSampleThreads) most = max(most, x.chunk_most[size_t(r) * x.chunks + i]);
         most = block_max(most, sh);
         if (most == kNoKey) return false;
@@ -665,21 +576,46 @@ struct Chunk {
     __device__ __forceinline__ void write(const SampleArgs &p, int64_t slot, float prob) const {
         if (threadIdx.x == 0) { p.out_slots[r] = slot; p.out_probs[r] = prob; ws->state = kRowDone; }
     }
+    // After the first histogram.
+    __device__ __forceinline__ State first_bin(SampleShared &sh, uint32_t &down) {
+        State st = first_state(row, lim);
+        to_bin(row, sh, st, lim, pick(sh, st, lim, count, mass), count, down);
+        return st;
+    }
+    __device__ __forceinline__ bool limited() const { return lim.limit_k || lim.limit_p; }
 };
 
-template <bool MASS>
-__device__ void add_bins(SampleShared &sh, SampleSplit *ws, int which) {
+template <typename T>
+__device__ __forceinline__ void add_bins(const Chunk<T> &ch, SampleShared &sh, int which, bool with_mass) {
     uint32_t count;
     uint64_t mass;
-    own_bin<MASS>(sh, count, mass);
+    own_bin(sh, with_mass, count, mass);
     if (count == 0) return;
-    atomicAdd(&ws->count[which][threadIdx.x], count);
-    if (MASS) atomicAdd(reinterpret_cast<unsigned long long *>(&ws->mass[which][threadIdx.x]), (unsigned long long)mass);
+    atomicAdd(&ch.ws->count[which][threadIdx.x], count);
+    if (with_mass) atomicAdd(reinterpret_cast<unsigned long long *>(&ch.ws->mass[which][threadIdx.x]), (unsigned long long)mass);
+}
+// Adds the chunk's slots with keys from .. upto to the row's list, which has room for them.
+template <typename T>
+__device__ __forceinline__ void add_slots(const Chunk<T> &ch, SampleShared &sh, uint32_t from, uint32_t upto) {
+    const uint32_t listed = list_slots(ch.row, sh, ch.from, ch.to, Cut{kNoKey + 1u, ~0u}, from, upto);
+    if (threadIdx.x == 0) sh.found_count = listed == 0u ? 0u : atomicAdd(&ch.ws->listed, listed);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < listed; i += kSampleThreads)
+        if (sh.found_count + i < kListed) ch.ws->list[sh.found_count + i] = sh.list[i];
+}
+// The search goes on among the row's list.
+template <typename T>
+__device__ __forceinline__ void take_list(const Chunk<T> &ch, SampleShared &sh, State &st) {
+    st.n = min(ch.ws->listed, kListed);
+    st.listed = true;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < st.n; i += kSampleThreads) sh.list[i] = ch.ws->list[i];
+    __syncthreads();
 }
 
 // The row's draw from the masses of its chunks.
-template <typename T, typename F>
-__device__ void draw_by_chunks(const SampleArgs &p, const SplitArgs &x, const Chunk<T> &ch, SampleShared &sh, F &&kept) {
+template <typename T>
+__device__ __forceinline__ void draw_by_chunks(const SampleArgs &p, const SplitArgs &x, const Chunk<T> &ch, SampleShared &sh, const Cut &cut) {
     const uint64_t *const masses = x.chunk_mass + size_t(ch.r) * x.chunks;
     uint64_t sum = 0;
     for (uint32_t i = threadIdx.x; i < x.chunks; i += kSampleThreads) sum += masses[i];
@@ -697,7 +633,7 @@ __device__ void draw_by_chunks(const SampleArgs &p, const SplitArgs &x, const Ch
     const uint32_t c = sh.picked, lo = c * x.chunk;
     want -= sh.found_mass;
     __syncthreads();
-    const uint32_t at = locate_in(ch.row, sh, lo, min(x.chunk, p.n - lo), want, kept);
+    const uint32_t at = locate(ch.row, sh, lo, min(x.chunk, p.n - lo), cut, false, want);
     ch.write(p, at, float(ldexp(ch.row.weight(ch.row.key_at(at)), ch.row.shift) / double(total)));
 }
 
@@ -718,195 +654,112 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_bins(SampleArgs p, Sp
     extern __shared__ uint8_t smem[];
     SampleShared &sh = *reinterpret_cast<SampleShared *>(smem);
     Chunk<T> ch(p, x);
-    if (!ch.open(p, x, sh)) {
+    if (!ch.open(p, x, sh, false)) {
         if (ch.c == 0) ch.write(p, -1, 0.0f);
         return;
     }
-    const Range all{kNoKey + 1u, ch.most, 0, 0, 0};
-    const auto bin_of = [&](uint32_t k) { return ch.row.bin(k); };
-    if (ch.lim.limit_k) {
-        fill_bins<false>(ch.row, sh, all, ch.from, ch.to, bin_of);
-        add_bins<false>(sh, ch.ws, 0);
-    } else if (ch.lim.limit_p) {
-        fill_bins<true>(ch.row, sh, all, ch.from, ch.to, bin_of);
-        add_bins<true>(sh, ch.ws, 0);
+    if (ch.limited()) {
+        const State st = first_state(ch.row, ch.lim);
+        fill(ch.row, sh, false, ch.from, ch.to, st.cut, st.s, Pass{kByDistance, !ch.lim.limit_k, false});
+        add_bins(ch, sh, 0, !ch.lim.limit_k);
     } else {
-        const uint32_t min_key = ch.lim.min_key;
-        const uint64_t mass = sum_of(ch.row, sh, ch.from, ch.to, [&](uint32_t, uint32_t k) { return k < min_key ? uint64_t(0) : ch.row.units(k); });
+        const uint64_t mass = mass_of(ch.row, sh, ch.from, ch.to, Cut{ch.lim.min_key, ~0u});
         if (threadIdx.x == 0) x.chunk_mass[size_t(ch.r) * x.chunks + ch.c] = mass;
     }
 }
 
-// The bin b that the histogram leaves the threshold in, as keys from its least one up to the row's largest.  limit: of top-p's mass.  upto: slots
-// down to that bin, or to min-p's.
-template <bool MASS, typename T>
-__device__ Range first_range(const Chunk<T> &ch, SampleShared &sh, double &limit, uint32_t &upto, uint32_t &b) {
-    const uint32_t count = ch.ws->count[0][threadIdx.x];
-    const uint64_t mass = MASS ? ch.ws->mass[0][threadIdx.x] : 0;
-    uint64_t total = 0;
-    Range r{kNoKey + 1u, ch.most, 0, 0, 0};
-    b = pick_bin<MASS>(sh, r, count, mass,
-        [&](uint64_t c, uint64_t m) { return MASS ? c == 0 || double(m) < double(ch.lim.top_p) * double(total) : c < uint64_t(ch.lim.top_k); }, total);
-    limit = double(ch.lim.top_p) * double(total);
-    const uint32_t down_to = MASS ? min(b, ch.row.bin(ch.lim.min_key)) : b;
-    upto = uint32_t(min(block_sum(threadIdx.x <= down_to ? count : 0, sh), uint64_t(0xffffffffu)));
-    r.lo = ch.row.least_of_bin(b);
-    return r;
-}
-
-// Whether so few slots are left that the row is drawn from them.
-__device__ __forceinline__ bool listable(uint32_t upto) { return upto <= kListed; }
-
-// Adds the chunk's slots with keys lo .. hi to the row's list, which has room for them.
-template <typename T>
-__device__ void add_slots(const Chunk<T> &ch, SampleShared &sh, uint32_t lo, uint32_t hi) {
-    const uint32_t listed = list_slots(ch.row, sh, ch.from, ch.to, lo, hi);
-    if (threadIdx.x == 0) sh.found_count = listed == 0u ? 0u : atomicAdd(&ch.ws->listed, listed);
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < listed; i += kSampleThreads)
-        if (sh.found_count + i < kListed) ch.ws->list[sh.found_count + i] = sh.list[i];
-}
-// The row's list.
-template <typename T>
-__device__ uint32_t take_list(const Chunk<T> &ch, SampleShared &sh) {
-    const uint32_t listed = min(ch.ws->listed, kListed);
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < listed; i += kSampleThreads) sh.list[i] = ch.ws->list[i];
-    __syncthreads();
-    return listed;
-}
-
-template <bool MASS, typename T>
-__device__ void list_chunk(Chunk<T> &ch, SampleShared &sh) {
-    double limit;
-    uint32_t upto, b;
-    Range r = first_range<MASS>(ch, sh, limit, upto, b);
-    if (listable(upto)) return add_slots(ch, sh, MASS ? max(r.lo, ch.lim.min_key) : r.lo, ch.most);
-    if (ch.lim.limit_k && ch.lim.limit_p) return;
-    if (b != 0) r.hi = ch.row.least_of_bin(b - 1) - 1u;
-    const uint32_t shift = narrow_shift(r);
-    fill_bins<MASS>(ch.row, sh, r, ch.from, ch.to, [&](uint32_t k) { return (r.hi - k) >> shift; });
-    add_bins<MASS>(sh, ch.ws, 1);
-}
 template <typename T>
 __global__ __launch_bounds__(kSampleThreads) void k_sample_list(SampleArgs p, SplitArgs x) {
     extern __shared__ uint8_t smem[];
     SampleShared &sh = *reinterpret_cast<SampleShared *>(smem);
     Chunk<T> ch(p, x);
-    if (!ch.open(p, x, sh)) return;
-    if (ch.lim.limit_k) return list_chunk<false>(ch, sh);
-    if (ch.lim.limit_p) return list_chunk<true>(ch, sh);
-    const uint32_t min_key = ch.lim.min_key;
-    if (ch.c == 0) draw_by_chunks(p, x, ch, sh, [&](uint32_t, uint32_t k) { return k < min_key ? uint64_t(0) : ch.row.units(k); });
+    if (!ch.open(p, x, sh, true)) return;
+    if (!ch.limited()) {
+        if (ch.c == 0) draw_by_chunks(p, x, ch, sh, Cut{ch.lim.min_key, ~0u});
+        return;
+    }
+    uint32_t down;
+    State st = ch.first_bin(sh, down);
+    if (down <= kListed) return add_slots(ch, sh, list_from(st, ch.lim), ch.most);
+    if (ch.lim.limit_k && ch.lim.limit_p) return;
+    fill(ch.row, sh, false, ch.from, ch.to, st.cut, st.s, Pass{kByKey, by_mass(st.phase), false});
+    add_bins(ch, sh, 1, by_mass(st.phase));
 }
 
-// The range that the second histogram leaves.
-template <bool MASS, typename T, typename F>
-__device__ Range second_range(const Chunk<T> &ch, SampleShared &sh, Range r, uint32_t b, F &&reaches) {
-    if (b != 0) r.hi = ch.row.least_of_bin(b - 1) - 1u;
-    uint64_t total;
-    const uint32_t shift = narrow_shift(r);
-    narrow_to(r, pick_bin<MASS>(sh, r, ch.ws->count[1][threadIdx.x], MASS ? ch.ws->mass[1][threadIdx.x] : 0, reaches, total), shift);
-    return r;
-}
-template <bool MASS, typename T>
-__device__ __forceinline__ uint32_t ties_of(const Chunk<T> &ch, const Range &r, double limit) {
-    return MASS ? ties_within(ch.row, r, limit) : min(r.count, uint32_t(uint64_t(ch.lim.top_k) - r.count_before));
-}
-
-template <bool MASS, typename T>
-__device__ void narrow_chunk(const SampleArgs &p, Chunk<T> &ch, SampleShared &sh) {
-    const Limits &lim = ch.lim;
-    double limit;
-    uint32_t upto, b;
-    int64_t slot;
-    float prob;
-    Range r = first_range<MASS>(ch, sh, limit, upto, b);
-    if (listable(upto)) {
-        if (ch.c != 0) return;
-        const uint32_t listed = take_list(ch, sh);
-        draw_from_list(ch.row, sh, listed, MASS ? ListLimits{0u, lim.min_key, true, 0.0, limit, lim.u} : ListLimits{uint32_t(lim.top_k), lim.min_key, lim.limit_p, double(lim.top_p), 0.0, lim.u}, slot, prob);
-        return ch.write(p, slot, prob);
-    }
-    if (lim.limit_k && lim.limit_p) {
-        if (ch.c != 0) return;
-        sample_row(ch.row, sh, lim, slot, prob);
-        return ch.write(p, slot, prob);
-    }
-    const auto reaches = [&](uint64_t c, uint64_t m) { return MASS ? c == 0 || double(m) < limit : c < uint64_t(lim.top_k); };
-    r = second_range<MASS>(ch, sh, r, b, reaches);
-    if (r.count <= kListed) return add_slots(ch, sh, r.lo, r.hi);
-    // more than that with keys next to each other: one workgroup goes on
-    if (ch.c != 0) return;
-    narrow<MASS>(ch.row, sh, r, reaches);
-    const uint32_t ties = ties_of<MASS>(ch, r, limit), key = r.lo;
-    const uint32_t last = ties < r.count ? locate_in(ch.row, sh, 0, ch.row.n, ties - 1u, [&](uint32_t, uint32_t k) { return uint64_t(k == key); }) : ~0u;
-    if (threadIdx.x == 0) { ch.ws->least = key; ch.ws->tie_last = last; ch.ws->state = kRowThreshold; }
-}
 template <typename T>
 __global__ __launch_bounds__(kSampleThreads) void k_sample_narrow(SampleArgs p, SplitArgs x) {
     extern __shared__ uint8_t smem[];
     SampleShared &sh = *reinterpret_cast<SampleShared *>(smem);
     Chunk<T> ch(p, x);
-    if (!ch.open(p, x, sh)) return;
-    if (ch.lim.limit_k) narrow_chunk<false>(p, ch, sh);
-    else if (ch.lim.limit_p) narrow_chunk<true>(p, ch, sh);
+    if (!ch.open(p, x, sh, true) || !ch.limited()) return;
+    uint32_t down;
+    State st = ch.first_bin(sh, down);
+    bool to_cut = false;
+    if (down <= kListed) {
+        if (ch.c != 0) return;
+        list_from(st, ch.lim);
+        take_list(ch, sh, st);
+    } else if (ch.lim.limit_k && ch.lim.limit_p) {
+        if (ch.c != 0) return;
+        st = first_state(ch.row, ch.lim);
+    } else {
+        narrow_to(st.s, pick(sh, st, ch.lim, ch.ws->count[1][threadIdx.x], ch.ws->mass[1][threadIdx.x]));
+        if (st.s.count <= kListed) return add_slots(ch, sh, st.s.lo, st.s.hi);
+        // more than that with keys next to each other: one workgroup goes on
+        if (ch.c != 0) return;
+        to_cut = true;
+    }
+    int64_t slot;
+    float prob;
+    search(ch.row, sh, ch.lim, st, to_cut, slot, prob);
+    if (!to_cut) return ch.write(p, slot, prob);
+    if (threadIdx.x == 0) { ch.ws->cut = st.cut; ch.ws->state = kRowCut; }
 }
 
-template <bool MASS, typename T>
-__device__ void find_threshold(const Chunk<T> &ch, SampleShared &sh, uint32_t &least, uint32_t &tie_last) {
-    const Limits &lim = ch.lim;
-    double limit;
-    uint32_t upto, b;
-    Range r = first_range<MASS>(ch, sh, limit, upto, b);
-    const auto reaches = [&](uint64_t c, uint64_t m) { return MASS ? c == 0 || double(m) < limit : c < uint64_t(lim.top_k); };
-    r = second_range<MASS>(ch, sh, r, b, reaches);
-    Listed l;
-    l.take<MASS>(ch.row, sh, take_list(ch, sh));
-    narrow_listed<MASS>(sh, l, l.key, r, reaches);
-    const uint32_t ties = ties_of<MASS>(ch, r, limit);
-    least = r.lo;
-    tie_last = ties < r.count ? last_tie(sh, l, least, ties) : ~0u;
-}
 template <typename T>
 __global__ __launch_bounds__(kSampleThreads) void k_sample_mass(SampleArgs p, SplitArgs x) {
     extern __shared__ uint8_t smem[];
     SampleShared &sh = *reinterpret_cast<SampleShared *>(smem);
     Chunk<T> ch(p, x);
-    if (ch.ws->state == kRowDone || !ch.open(p, x, sh)) return;
-    uint32_t least, tie_last;
-    if (ch.ws->state == kRowThreshold) { least = ch.ws->least; tie_last = ch.ws->tie_last; }
-    else if (ch.lim.limit_k) find_threshold<false>(ch, sh, least, tie_last);
-    else find_threshold<true>(ch, sh, least, tie_last);
-    const uint32_t min_key = ch.lim.min_key;
-    const uint64_t mass = sum_of(ch.row, sh, ch.from, ch.to,
-        [&](uint32_t i, uint32_t k) { return k < least || k < min_key || (k == least && i > tie_last) ? uint64_t(0) : ch.row.units(k); });
+    const uint32_t state = ch.ws->state;
+    if (state == kRowDone || !ch.open(p, x, sh, state != kRowCut)) return;
+    Cut cut = ch.ws->cut;
+    if (state != kRowCut) {
+        uint32_t down;
+        State st = ch.first_bin(sh, down);
+        narrow_to(st.s, pick(sh, st, ch.lim, ch.ws->count[1][threadIdx.x], ch.ws->mass[1][threadIdx.x]));
+        take_list(ch, sh, st);
+        int64_t slot;
+        float prob;
+        search(ch.row, sh, ch.lim, st, true, slot, prob);
+        cut = st.cut;
+    }
+    if (ch.lim.min_key > cut.least) cut = Cut{ch.lim.min_key, ~0u};
+    const uint64_t mass = mass_of(ch.row, sh, ch.from, ch.to, cut);
     if (threadIdx.x != 0) return;
     x.chunk_mass[size_t(ch.r) * x.chunks + ch.c] = mass;
-    x.chunk_cut[size_t(ch.r) * x.chunks + ch.c] = make_uint2(least, tie_last);
+    x.chunk_cut[size_t(ch.r) * x.chunks + ch.c] = cut;
 }
 template <typename T>
 __global__ __launch_bounds__(kSampleThreads) void k_sample_draw(SampleArgs p, SplitArgs x) {
     extern __shared__ uint8_t smem[];
     SampleShared &sh = *reinterpret_cast<SampleShared *>(smem);
     Chunk<T> ch(p, x);
-    if (ch.ws->state == kRowDone || !ch.open(p, x, sh)) return;
-    const uint2 cut = x.chunk_cut[size_t(ch.r) * x.chunks];
-    const uint32_t min_key = ch.lim.min_key;
-    draw_by_chunks(p, x, ch, sh, [&](uint32_t i, uint32_t k) { return k < cut.x || k < min_key || (k == cut.x && i > cut.y) ? uint64_t(0) : ch.row.units(k); });
+    if (ch.ws->state == kRowDone || !ch.open(p, x, sh, false)) return;
+    draw_by_chunks(p, x, ch, sh, x.chunk_cut[size_t(ch.r) * x.chunks]);
 }
 
 // Rows of more slots than this go in chunks, as long as there are no more than kSplitRows of them.
-constexpr size_t kSplitSlots = 16384, kSplitRows = 512;
-constexpr uint32_t kChunk = 8192;
+constexpr size_t kSplitSlots = 16384, kSplitRows = 128;
+constexpr size_t kChunk = 8192;
 struct Split {
     uint32_t chunk, chunks;
     size_t masses, cuts, mosts, bytes;
 };
 static Split split_of(size_t rows, size_t n) {
-    // chunks for a thousand workgroups
-    size_t chunk = kChunk;
-    while (rows * ((n + chunk - 1) / chunk) > 1024 && chunk < n) chunk *= 2;
+    // chunks for a workgroup a compute unit: what a kernel does before it walks its chunk takes as long as 16384 slots
+    const size_t most = rows < 128 ? 256 / rows : 2;
+    const size_t chunk = std::max(kChunk, ((n + most - 1) / most + kChunk - 1) / kChunk * kChunk);
     Split x;
     x.chunk = uint32_t(chunk);
     x.chunks = uint32_t((n + chunk - 1) / chunk);
@@ -927,7 +780,7 @@ static hipError_t sample(const SampleArgs &a, hipStream_t s) {
         return launch(k_sample<T>, a.rows < 65536u ? a.rows : 65536u, kSampleThreads, lds, s, a);
     }
     const Split split = split_of(a.rows, a.n);
-    const SplitArgs x{reinterpret_cast<SampleSplit *>(a.ws), reinterpret_cast<uint64_t *>(a.ws + split.masses), reinterpret_cast<uint2 *>(a.ws + split.cuts),
+    const SplitArgs x{reinterpret_cast<SampleSplit *>(a.ws), reinterpret_cast<uint64_t *>(a.ws + split.masses), reinterpret_cast<Cut *>(a.ws + split.cuts),
                       reinterpret_cast<uint32_t *>(a.ws + split.mosts),
                       split.chunk, split.chunks};
     const dim3 grid(a.rows, split.chunks);      // (rows next to each other: their first chunks, which work alone at times, on all XCDs)
