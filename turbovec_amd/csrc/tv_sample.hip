@@ -30,11 +30,12 @@ __device__ __forceinline__ float key_score(uint32_t k) { return order_unkey(int(
 
 template <typename T>
 struct SampleRow {
-    static constexpr int kEach = 16 / int(sizeof(T));
+    static constexpr int kEach = 16 / int(sizeof(T)), kFirstBin = (127 - 20) * 32;
     const T *scores;
     const uint64_t *mask;
     uint32_t n, most;         // most: the key of the largest score
-    double top, inverse, inverse2;      // that score, 1 / T, and that times log2(e)
+    float best;               // that score
+    double top, inverse, inverse2;      // the same, 1 / T, and that times log2(e)
     int shift;
     struct Load {
         T v[kEach];
@@ -54,11 +55,11 @@ struct SampleRow {
             else l.bits &= ~(1u << j);
         }
     }
-    __device__ __forceinline__ uint32_t key(const Load &l, int j) const { return (l.bits >> j) & 1u ? score_key(float(l.v[j])) : kNoKey; }
     __device__ __forceinline__ uint32_t key_at(uint32_t i) const {
         return mask == nullptr || ((mask[i >> 6] >> (i & 63u)) & 1u) ? score_key(float(scores[i])) : kNoKey;
     }
-    // f(slot, key) for every slot of lo .. hi - 1 (multiples of kEach, or the end), a worker of `workers`.
+    // f(slot, score) for every allowed slot of lo .. hi - 1 (multiples of kEach, or the end) whose score is neither NaN nor -infinity, a worker of
+    // `workers`.
     template <typename F>
     __device__ __forceinline__ void each(uint32_t lo, uint32_t hi, uint32_t worker, uint32_t workers, F &&f) const {
         const uint32_t step = workers * kEach;
@@ -70,7 +71,10 @@ struct SampleRow {
             const bool more = hi - i > step;
             if (more) load(next, i + step);
 #pragma unroll
-            for (int j = 0; j < kEach; ++j) f(i + j, key(now, j));
+            for (int j = 0; j < kEach; ++j) {
+                const float v = float(now.v[j]);
+                if (((now.bits >> j) & 1u) && v > -__int_as_float(0x7f800000)) f(i + j, v);
+            }
             if (!more) return;
             now = next;
             i += step;
@@ -81,8 +85,8 @@ struct SampleRow {
     // The same as a whole number of 2^-shift, which is what sums are made of: 2^y = 2^e * 2^f, |f| <= 1/2, with the exponential series up to
     // its tenth power (off by 2.2e-13 at most); adding 2 leaves its value in the low 52 bits.  A library exponential and a
     // conversion to 64 bits take three times as long.
-    __device__ __forceinline__ uint64_t units(uint32_t k) const {
-        const double y = fmax((double(key_score(k)) - top) * inverse2, -200.0);
+    __device__ __forceinline__ uint64_t units(float score) const {
+        const double y = fmax((double(score) - top) * inverse2, -200.0);
         const double e = rint(y), f = (y - e) * 0.69314718055994530942;
         double v = 1.0 / 3628800.0;
         v = fma(v, f, 1.0 / 362880.0);
@@ -98,20 +102,18 @@ struct SampleRow {
         const uint64_t bits = uint64_t(__double_as_longlong(v + 2.0)) & 0xfffffffffffffull;      // v * 2^51
         const int down = 62 - shift - int(e);
         const uint64_t x = bits << 11;
-        return k == most ? 1ull << shift : down >= 64 ? 0ull : (x + ((1ull << down) >> 1)) >> down;
+        return score == best ? 1ull << shift : down >= 64 ? 0ull : (x + ((1ull << down) >> 1)) >> down;
     }
-    // The bin of a key: 32 for each power of two that the distance to the best score spans, from 2^-20 to 2^12.
-    __device__ __forceinline__ uint32_t bin(uint32_t k) const {
-        const float d = key_score(most) - key_score(k);
-        const int x = k == most ? 0 : int(__float_as_uint(d) >> 18) - (127 - 20) * 32;
-        return uint32_t(min(max(x, 0), int(kBins) - 1));
-    }
-    // The least key of those in bins up to b (keys rise as bins fall): every lane of a wave tries one of 64 places, until a step is one key.
-    __device__ __forceinline__ uint32_t least_of_bin(uint32_t b) const {
+    // How far a score lies below the best, as the bits of that distance: a number that rises with it.
+    __device__ __forceinline__ uint32_t distance(float v) const { return v == best ? 0u : __float_as_uint(best - v); }
+    // The bin of a distance: 32 for each power of two that it spans, from 2^-20 to 2^12; what is nearer or further is in the first or the last.
+    __device__ __forceinline__ static uint32_t bin(uint32_t d) { return uint32_t(min(max(int(d >> 18) - kFirstBin, 0), int(kBins) - 1)); }
+    // The least key no further than d (keys rise as distances fall): every lane of a wave tries one of 64 places, until a step is one key.
+    __device__ __forceinline__ uint32_t least_within(uint32_t d) const {
         uint32_t lo = kNoKey + 1u, left = most - lo;           // it is one of lo .. lo + left
         while (left != 0u) {
             const uint32_t step = left / 64u + 1u, mine = lo + min(left, (threadIdx.x & 63u) * step);
-            const uint64_t yes = __ballot(bin(mine) <= b);
+            const uint64_t yes = __ballot(distance(key_score(mine)) <= d);
             const uint32_t first = yes == 0ull ? 64u : uint32_t(__builtin_ctzll(yes));
             if (first == 0u) return lo;
             // above the place before the first that is, and no further
@@ -131,7 +133,8 @@ struct SampleRow {
     // Of a row's scores, given the largest one's key.
     __device__ __forceinline__ void set(uint32_t most_, float t) {
         most = most_;
-        top = double(key_score(most));
+        best = key_score(most);
+        top = double(best);
         // (an infinite best leaves the others nothing)
         inverse = t > 0.0f && top < __longlong_as_double(0x7ff0000000000000ll) ? 1.0 / double(t) : 1.0;
         inverse2 = inverse * 1.44269504088896340736;
@@ -223,21 +226,22 @@ struct Limits {
 // What stays: slots of keys above `least`, and of those of that key the ones up to tie_last.
 struct Cut {
     uint32_t least, tie_last;
-    __device__ __forceinline__ bool leaves(uint32_t i, uint32_t k) const { return k > least || (k == least && i <= tie_last); }
 };
-// The values that the one sought is among, in falling order from hi; of a bin that was picked, its slots, and the slots and the mass before it.
+struct CutScores {
+    float least;
+    uint32_t tie_last;
+    __device__ __forceinline__ explicit CutScores(const Cut &c) : least(key_score(c.least)), tie_last(c.tie_last) {}
+    __device__ __forceinline__ bool leaves(uint32_t i, float v) const { return v > least || (v == least && i <= tie_last); }
+};
+// The values that the one sought is among, in falling order from hi: keys of scores, near to far within distances `near` to `far`, or complements of
+// slots.  Of a bin that was picked: its slots, and the slots and the mass before it.
 struct Search {
-    uint32_t lo, hi, count;
+    uint32_t lo, hi, near, far, count;
     uint64_t before, mass_before;
 };
-__device__ __forceinline__ uint32_t shift_of(const Search &s) { return uint32_t(max(0, 22 - __clz(int(s.hi - s.lo)))); }      // 1024 bins of 2^shift
-__device__ __forceinline__ void narrow_to(Search &s, uint32_t bin) {
-    const uint32_t shift = shift_of(s);
-    s.hi -= bin << shift;
-    s.lo = max(s.lo, s.hi - min(s.hi, (1u << shift) - 1u));
-}
+__device__ __forceinline__ uint32_t shift_of(uint32_t range) { return uint32_t(max(0, 22 - __clz(int(range)))); }      // 1024 bins of 2^shift
 
-enum { kByDistance, kByKey, kByPlace };
+enum { kFirst, kByDistance, kByKey, kByPlace };
 struct Pass {
     int mode;
     bool mass, ties;          // ties: of the cut's slots only those of its least key
@@ -252,18 +256,31 @@ __device__ __forceinline__ void fill(const SampleRow<T> &row, SampleShared &sh, 
         if (pass.mass) sh.mass[c * kBins + threadIdx.x] = 0;
     }
     __syncthreads();
-    const uint32_t shift = shift_of(s), copy = threadIdx.x % kCopies;
-    const auto add = [&](uint32_t i, uint32_t k) {
-        if (!cut.leaves(i, k) || (pass.ties && k != cut.least)) return;
-        const uint32_t v = pass.mode == kByPlace ? ~i : k;
-        if (v < s.lo || v > s.hi) return;
-        const uint32_t at = (pass.mode == kByDistance ? row.bin(k) : (s.hi - v) >> shift) * kCopies + copy;
+    const CutScores scores(cut);
+    const uint32_t by_distance = shift_of(s.far - s.near), by_value = shift_of(s.hi - s.lo), copy = threadIdx.x % kCopies;
+    const auto add = [&](uint32_t i, float v) {
+        if (!scores.leaves(i, v)) return;
+        uint32_t bin;
+        if (pass.mode <= kByDistance) {
+            const uint32_t d = row.distance(v);
+            bin = row.bin(d);
+            if (pass.mode == kByDistance) {
+                if (d < s.near || d > s.far) return;
+                bin = (d - s.near) >> by_distance;
+            }
+        } else {
+            if (pass.ties && v != scores.least) return;
+            const uint32_t x = pass.mode == kByPlace ? ~i : score_key(v);
+            if (x < s.lo || x > s.hi) return;
+            bin = (s.hi - x) >> by_value;
+        }
+        const uint32_t at = bin * kCopies + copy;
         atomicAdd(&sh.count[at], 1u);
-        if (pass.mass) atomicAdd(reinterpret_cast<unsigned long long *>(&sh.mass[at]), (unsigned long long)row.units(k));
+        if (pass.mass) atomicAdd(reinterpret_cast<unsigned long long *>(&sh.mass[at]), (unsigned long long)row.units(v));
     };
     if (listed) {
 #pragma unroll 1
-        for (uint32_t e = threadIdx.x; e < hi; e += kSampleThreads) add(~uint32_t(sh.list[e]), uint32_t(sh.list[e] >> 32));
+        for (uint32_t e = threadIdx.x; e < hi; e += kSampleThreads) add(~uint32_t(sh.list[e]), key_score(uint32_t(sh.list[e] >> 32)));
     } else {
         row.each(lo, hi, threadIdx.x, kSampleThreads, add);
     }
@@ -289,6 +306,7 @@ enum { kTopK, kTopP, kTies, kDraw };
 struct State {
     int phase, after;         // after: the phase that ends in ties
     bool whole;               // the search has not been narrowed yet
+    int histograms;           // of the row by distance so far; two, then by key
     bool listed;
     uint32_t n;               // slots in the list
     Search s;
@@ -329,10 +347,12 @@ __device__ __forceinline__ uint32_t list_slots(const SampleRow<T> &row, SampleSh
     __syncthreads();
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
-    row.each(lo, hi, threadIdx.x, kSampleThreads, [&](uint32_t i, uint32_t k) {
-        if (k < from || k > upto || !cut.leaves(i, k)) return;
+    const CutScores scores(cut);
+    const float least = key_score(from), most = key_score(upto);
+    row.each(lo, hi, threadIdx.x, kSampleThreads, [&](uint32_t i, float v) {
+        if (v < least || v > most || !scores.leaves(i, v)) return;
         const uint32_t at = atomicAdd(&sh.listed, 1u);
-        if (at < kListed) sh.list[at] = uint64_t(k) << 32 | uint32_t(~i);
+        if (at < kListed) sh.list[at] = uint64_t(score_key(v)) << 32 | uint32_t(~i);
     });
     __syncthreads();
     return min(sh.listed, kListed);
@@ -341,7 +361,8 @@ __device__ __forceinline__ uint32_t list_slots(const SampleRow<T> &row, SampleSh
 __device__ __forceinline__ uint32_t only_value(SampleShared &sh, const State &st) {
     for (uint32_t e = threadIdx.x; e < st.n; e += kSampleThreads) {
         const uint32_t k = uint32_t(sh.list[e] >> 32), place = uint32_t(sh.list[e]), v = st.phase >= kTies ? place : k;
-        if (v >= st.s.lo && v <= st.s.hi && st.cut.leaves(~place, k) && (st.phase != kTies || k == st.cut.least)) sh.found_value = v;
+        const bool stays = k > st.cut.least || (k == st.cut.least && ~place <= st.cut.tie_last);
+        if (v >= st.s.lo && v <= st.s.hi && stays && (st.phase != kTies || k == st.cut.least)) sh.found_value = v;
     }
     __syncthreads();
     const uint32_t v = sh.found_value;
@@ -354,12 +375,13 @@ __device__ __forceinline__ uint32_t only_value(SampleShared &sh, const State &st
 template <typename T>
 __device__ __forceinline__ uint32_t locate(const SampleRow<T> &row, SampleShared &sh, uint32_t lo, uint32_t len, const Cut &cut, bool ties, uint64_t want) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const auto value = [&](uint32_t i, uint32_t k) { return !cut.leaves(i, k) ? uint64_t(0) : ties ? uint64_t(k == cut.least) : row.units(k); };
+    const CutScores scores(cut);
+    const auto value = [&](uint32_t i, float v) { return !scores.leaves(i, v) ? uint64_t(0) : ties ? uint64_t(v == scores.least) : row.units(v); };
     while (len > uint32_t(kSampleThreads)) {
         const uint32_t seg = ((len + kSampleWaves - 1) / kSampleWaves + 63u) & ~63u;
         const uint32_t from = min(len, wave * seg), to = min(len, from + seg);
         uint64_t sum = 0;
-        row.each(lo + from, lo + to, lane, 64u, [&](uint32_t i, uint32_t k) { sum += value(i, k); });
+        row.each(lo + from, lo + to, lane, 64u, [&](uint32_t i, float v) { sum += value(i, v); });
         sum = wave_upto(sum);
         __syncthreads();
         if (lane == 63u) sh.part[wave] = sum;
@@ -375,7 +397,11 @@ __device__ __forceinline__ uint32_t locate(const SampleRow<T> &row, SampleShared
         len = min(seg, len - min(len, w * seg));
     }
     // at most one slot to a thread
-    const uint64_t mine = threadIdx.x < len ? value(lo + threadIdx.x, row.key_at(lo + threadIdx.x)) : 0;
+    uint64_t mine = 0;
+    if (threadIdx.x < len) {
+        const uint32_t k = row.key_at(lo + threadIdx.x);
+        mine = k != kNoKey ? value(lo + threadIdx.x, key_score(k)) : 0;
+    }
     uint64_t all;
     const uint64_t before = block_before(mine, sh, all);
     if (threadIdx.x == 0) sh.picked = 0;
@@ -384,12 +410,13 @@ __device__ __forceinline__ uint32_t locate(const SampleRow<T> &row, SampleShared
     __syncthreads();
     return lo + sh.picked;
 }
-// The mass that the cut leaves of the slots lo .. hi - 1.
+// The mass that the cut leaves of the slots lo .. hi - 1 that are this worker's.
 template <typename T>
-__device__ __forceinline__ uint64_t mass_of(const SampleRow<T> &row, SampleShared &sh, uint32_t lo, uint32_t hi, const Cut &cut) {
+__device__ __forceinline__ uint64_t mass_of(const SampleRow<T> &row, uint32_t lo, uint32_t hi, uint32_t worker, uint32_t workers, const Cut &cut) {
+    const CutScores scores(cut);
     uint64_t sum = 0;
-    row.each(lo, hi, threadIdx.x, kSampleThreads, [&](uint32_t i, uint32_t k) { sum += cut.leaves(i, k) ? row.units(k) : 0; });
-    return block_sum(sum, sh);
+    row.each(lo, hi, worker, workers, [&](uint32_t i, float v) { sum += scores.leaves(i, v) ? row.units(v) : 0; });
+    return sum;
 }
 
 template <typename T>
@@ -398,22 +425,35 @@ __device__ __forceinline__ State first_state(const SampleRow<T> &row, const Limi
     st.phase = lim.limit_k ? kTopK : lim.limit_p ? kTopP : kDraw;
     st.after = kDraw;
     st.whole = true;
+    st.histograms = 0;
     st.listed = false;
     st.n = 0;
-    st.s = Search{kNoKey + 1u, row.most, 0, 0, 0};
+    st.s = Search{kNoKey + 1u, row.most, 0, ~0u, 0, 0, 0};
     st.cut = Cut{kNoKey + 1u, ~0u};
     st.bound = uint64_t(lim.top_k);
     st.total = 0;
     return st;
 }
-// The search goes from the row's first histogram to the bin it picked.  `down`: slots that can still be drawn, down to that bin.
+// The search goes from a histogram by distance to the bin it picked.
 template <typename T>
-__device__ __forceinline__ void to_bin(const SampleRow<T> &row, SampleShared &sh, State &st, const Limits &lim, uint32_t bin, uint32_t count, uint32_t &down) {
-    // (min-p leaves fewer, but top-p after top-k needs all of top-k's)
-    const uint32_t last = st.phase == kTopP ? min(bin, row.bin(lim.min_key)) : bin;
-    down = uint32_t(block_sum(threadIdx.x <= last ? count : 0, sh));
-    st.s.lo = max(st.cut.least, row.least_of_bin(bin));
-    st.s.hi = bin == 0 ? row.most : row.least_of_bin(bin - 1) - 1u;
+__device__ __forceinline__ void to_bin(const SampleRow<T> &row, State &st, uint32_t bin) {
+    Search &s = st.s;
+    if (st.histograms++ == 0) {
+        s.near = bin == 0 ? 0u : uint32_t(row.kFirstBin + int(bin)) << 18;
+        s.far = bin == kBins - 1 ? 0x7f800000u : (uint32_t(row.kFirstBin + int(bin) + 1) << 18) - 1u;
+    } else {
+        const uint32_t shift = shift_of(s.far - s.near);
+        s.near += bin << shift;
+        s.far = min(s.far, s.near + ((1u << shift) - 1u));
+    }
+    s.lo = max(st.cut.least, row.least_within(s.far));
+    s.hi = s.near == 0 ? row.most : row.least_within(s.near - 1u) - 1u;
+}
+// Of the first histogram, the slots down to the picked bin that can still be drawn.  (Min-p leaves fewer, but top-p after top-k needs all of top-k's.)
+template <typename T>
+__device__ __forceinline__ uint32_t slots_down_to(const SampleRow<T> &row, SampleShared &sh, const State &st, const Limits &lim, uint32_t bin, uint32_t count) {
+    const uint32_t last = st.phase == kTopP ? min(bin, row.bin(row.distance(key_score(lim.min_key)))) : bin;
+    return uint32_t(block_sum(threadIdx.x <= last ? count : 0, sh));
 }
 // From which key on a row's slots are listed.  Where min-p leaves nothing of the bin, the search is over.
 __device__ __forceinline__ uint32_t list_from(State &st, const Limits &lim) {
@@ -430,26 +470,30 @@ __device__ void search(const SampleRow<T> &row, SampleShared &sh, const Limits &
         if (st.phase >= kTies && !st.listed) {
             // slots next to each other fall into one bin, a row's are walked instead
             if (st.phase == kDraw) {
-                st.total = mass_of(row, sh, 0, row.n, st.cut);
+                st.total = block_sum(mass_of(row, 0, row.n, threadIdx.x, kSampleThreads, st.cut), sh);
                 st.bound = drawn_mass(lim.u, st.total) + 1;
             }
             st.s.lo = st.s.hi = ~locate(row, sh, 0, row.n, st.cut, st.phase == kTies, st.bound - 1);
         } else if (st.whole || (st.s.lo < st.s.hi && st.s.count != 0)) {
-            const bool first = st.whole && !st.listed;
+            const bool distances = !st.listed && st.histograms < 2, first = distances && st.histograms == 0;
             if (!st.whole && st.listed && st.s.count == 1) {
                 st.s.lo = st.s.hi = only_value(sh, st);
                 continue;
             }
-            fill(row, sh, st.listed, 0, st.listed ? st.n : row.n, st.cut, st.s, Pass{first ? kByDistance : st.phase >= kTies ? kByPlace : kByKey, by_mass(st.phase), st.phase == kTies});
-            uint32_t count, down;
+            const int mode = first ? kFirst : distances ? kByDistance : st.phase >= kTies ? kByPlace : kByKey;
+            fill(row, sh, st.listed, 0, st.listed ? st.n : row.n, st.cut, st.s, Pass{mode, by_mass(st.phase), st.phase == kTies});
+            uint32_t count;
             uint64_t mass;
             own_bin(sh, by_mass(st.phase), count, mass);
             const uint32_t bin = pick(sh, st, lim, count, mass);
-            if (!first) {
-                narrow_to(st.s, bin);
+            if (!distances) {
+                const uint32_t shift = shift_of(st.s.hi - st.s.lo);
+                st.s.hi -= bin << shift;
+                st.s.lo = max(st.s.lo, st.s.hi - min(st.s.hi, (1u << shift) - 1u));
                 continue;
             }
-            to_bin(row, sh, st, lim, bin, count, down);
+            to_bin(row, st, bin);
+            const uint32_t down = first ? slots_down_to(row, sh, st, lim, bin, count) : uint32_t(min(st.s.before + st.s.count, uint64_t(~0u)));
             if (down <= kListed) {
                 st.n = list_slots(row, sh, 0, row.n, st.cut, list_from(st, lim), row.most);
                 st.listed = true;
@@ -470,7 +514,7 @@ __device__ void search(const SampleRow<T> &row, SampleShared &sh, const Limits &
             next = st.phase == kTopK && lim.limit_p ? kTopP : kDraw;
             uint32_t ties = uint32_t(min(uint64_t(st.s.count), st.bound - min(st.bound, st.s.before)));
             if (st.phase == kTopP) {
-                const uint64_t each = row.units(st.s.lo);
+                const uint64_t each = row.units(key_score(st.s.lo));
                 const double fit = each == 0 ? double(st.s.count) : ceil((double(st.bound) - double(st.s.mass_before)) / double(each));
                 ties = fit < 1.0 ? min(1u, st.s.count) : fit < double(st.s.count) ? uint32_t(fit) : st.s.count;
             }
@@ -485,7 +529,9 @@ __device__ void search(const SampleRow<T> &row, SampleShared &sh, const Limits &
         if (next == kDraw && lim.min_key > st.cut.least) st.cut = Cut{lim.min_key, ~0u};
         st.phase = next;
         st.whole = true;
-        st.s = next >= kTies ? Search{~(row.n - 1u), ~0u, 0, 0, 0} : Search{st.cut.least, row.most, 0, 0, 0};
+        st.histograms = 0;
+        st.s = Search{st.cut.least, row.most, 0, ~0u, 0, 0, 0};
+        if (next >= kTies) { st.s.lo = ~(row.n - 1u); st.s.hi = ~0u; }
     }
 }
 
@@ -507,9 +553,9 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample(SampleArgs p) {
         SampleRow<T> row = row_of<T>(p, r);
         Limits lim;
         lim.load(p, r);
-        uint32_t most = kNoKey;
-        row.each(0, p.n, threadIdx.x, kSampleThreads, [&](uint32_t, uint32_t k) { most = max(most, k); });
-        most = block_max(most, sh);
+        float best = -__int_as_float(0x7f800000);
+        row.each(0, p.n, threadIdx.x, kSampleThreads, [&](uint32_t, float v) { best = fmaxf(best, v); });
+        const uint32_t most = block_max(score_key(best), sh);
         int64_t slot = -1;
         float prob = 0.0f;
         if (most != kNoKey) {
@@ -525,7 +571,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample(SampleArgs p) {
 
 // Long rows, not many: a row goes in chunks to workgroups, through six kernels that each walk it once at most.
 //   max     the best score of each chunk
-//   bins    the first histogram, added up over the row's chunks; where nothing limits the row, the mass of each chunk
+//   bins    the first histogram, added up over the row's chunks; where nothing limits the row, the mass of each part of a chunk
 //   list    few slots down to the bin it leaves: gathered.  Many: the bin's own histogram.  Where nothing limits the row, the draw.
 //   narrow  the rest of the search among the gathered slots, by the first chunk; or the slots of the second histogram's bin.  (top-k that
 //           leaves many and top-p together: the first chunk takes the row alone.)
@@ -546,8 +592,8 @@ constexpr uint32_t kSplitZeroed = offsetof(SampleSplit, list) / 4;
 enum { kRowOpen = 0, kRowDone = 1, kRowCut = 2 };
 struct SplitArgs {
     SampleSplit *rows;
-    uint64_t *chunk_mass;     // [row][chunk]
-    Cut *chunk_cut;
+    uint64_t *part_mass;      // [row][part]: kSampleWaves parts a chunk, a wave each
+    Cut *chunk_cut;           // [row][chunk]
     uint32_t *chunk_most;
     uint32_t chunk, chunks;   // slots of a chunk, chunks of a row
 };
@@ -579,7 +625,9 @@ struct Chunk {
     // After the first histogram.
     __device__ __forceinline__ State first_bin(SampleShared &sh, uint32_t &down) {
         State st = first_state(row, lim);
-        to_bin(row, sh, st, lim, pick(sh, st, lim, count, mass), count, down);
+        const uint32_t bin = pick(sh, st, lim, count, mass);
+        to_bin(row, st, bin);
+        down = slots_down_to(row, sh, st, lim, bin, count);
         return st;
     }
     __device__ __forceinline__ bool limited() const { return lim.limit_k || lim.limit_p; }
@@ -613,27 +661,35 @@ __device__ __forceinline__ void take_list(const Chunk<T> &ch, SampleShared &sh, 
     __syncthreads();
 }
 
-// The row's draw from the masses of its chunks.
+// The mass of each part of the chunk.
 template <typename T>
-__device__ __forceinline__ void draw_by_chunks(const SampleArgs &p, const SplitArgs &x, const Chunk<T> &ch, SampleShared &sh, const Cut &cut) {
-    const uint64_t *const masses = x.chunk_mass + size_t(ch.r) * x.chunks;
+__device__ __forceinline__ void put_masses(const SplitArgs &x, const Chunk<T> &ch, const Cut &cut) {
+    const uint32_t part = x.chunk / kSampleWaves, wave = threadIdx.x >> 6, lo = min(ch.to, ch.from + wave * part);
+    const uint64_t mass = wave_upto(mass_of(ch.row, lo, min(ch.to, lo + part), threadIdx.x & 63u, 64u, cut));
+    if ((threadIdx.x & 63u) == 63u) x.part_mass[(size_t(ch.r) * x.chunks + ch.c) * kSampleWaves + wave] = mass;
+}
+// The row's draw from those of its chunks.
+template <typename T>
+__device__ __forceinline__ void draw_by_parts(const SampleArgs &p, const SplitArgs &x, const Chunk<T> &ch, SampleShared &sh, const Cut &cut) {
+    const uint32_t parts = x.chunks * kSampleWaves, part = x.chunk / kSampleWaves;
+    const uint64_t *const masses = x.part_mass + size_t(ch.r) * parts;
     uint64_t sum = 0;
-    for (uint32_t i = threadIdx.x; i < x.chunks; i += kSampleThreads) sum += masses[i];
+    for (uint32_t i = threadIdx.x; i < parts; i += kSampleThreads) sum += masses[i];
     const uint64_t total = block_sum(sum, sh);
     uint64_t want = drawn_mass(ch.lim.u, total), before = 0;
     if (threadIdx.x == 0) { sh.picked = 0; sh.found_mass = 0; }
-    for (uint32_t i = 0; i < x.chunks; i += kSampleThreads) {
-        const uint64_t mine = i + threadIdx.x < x.chunks ? masses[i + threadIdx.x] : 0;
+    for (uint32_t i = 0; i < parts; i += kSampleThreads) {
+        const uint64_t mine = i + threadIdx.x < parts ? masses[i + threadIdx.x] : 0;
         uint64_t all;
         const uint64_t upto = before + block_before(mine, sh, all);
         if (upto <= want && upto + mine > want) { sh.picked = i + threadIdx.x; sh.found_mass = upto; }
         before += all;
     }
     __syncthreads();
-    const uint32_t c = sh.picked, lo = c * x.chunk;
+    const uint32_t lo = sh.picked * part;
     want -= sh.found_mass;
     __syncthreads();
-    const uint32_t at = locate(ch.row, sh, lo, min(x.chunk, p.n - lo), cut, false, want);
+    const uint32_t at = locate(ch.row, sh, lo, min(part, p.n - lo), cut, false, want);
     ch.write(p, at, float(ldexp(ch.row.weight(ch.row.key_at(at)), ch.row.shift) / double(total)));
 }
 
@@ -643,9 +699,9 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_max(SampleArgs p, Spl
     SampleShared &sh = *reinterpret_cast<SampleShared *>(smem);
     const Chunk<T> ch(p, x);
     for (uint32_t i = ch.c * kSampleThreads + threadIdx.x; i < kSplitZeroed; i += x.chunks * kSampleThreads) reinterpret_cast<uint32_t *>(ch.ws)[i] = 0;
-    uint32_t most = kNoKey;
-    ch.row.each(ch.from, ch.to, threadIdx.x, kSampleThreads, [&](uint32_t, uint32_t k) { most = max(most, k); });
-    most = block_max(most, sh);
+    float best = -__int_as_float(0x7f800000);
+    ch.row.each(ch.from, ch.to, threadIdx.x, kSampleThreads, [&](uint32_t, float v) { best = fmaxf(best, v); });
+    const uint32_t most = block_max(score_key(best), sh);
     if (threadIdx.x == 0) x.chunk_most[size_t(ch.r) * x.chunks + ch.c] = most;
 }
 
@@ -660,11 +716,10 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_bins(SampleArgs p, Sp
     }
     if (ch.limited()) {
         const State st = first_state(ch.row, ch.lim);
-        fill(ch.row, sh, false, ch.from, ch.to, st.cut, st.s, Pass{kByDistance, !ch.lim.limit_k, false});
+        fill(ch.row, sh, false, ch.from, ch.to, st.cut, st.s, Pass{kFirst, !ch.lim.limit_k, false});
         add_bins(ch, sh, 0, !ch.lim.limit_k);
     } else {
-        const uint64_t mass = mass_of(ch.row, sh, ch.from, ch.to, Cut{ch.lim.min_key, ~0u});
-        if (threadIdx.x == 0) x.chunk_mass[size_t(ch.r) * x.chunks + ch.c] = mass;
+        put_masses(x, ch, Cut{ch.lim.min_key, ~0u});
     }
 }
 
@@ -675,14 +730,14 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_list(SampleArgs p, Sp
     Chunk<T> ch(p, x);
     if (!ch.open(p, x, sh, true)) return;
     if (!ch.limited()) {
-        if (ch.c == 0) draw_by_chunks(p, x, ch, sh, Cut{ch.lim.min_key, ~0u});
+        if (ch.c == 0) draw_by_parts(p, x, ch, sh, Cut{ch.lim.min_key, ~0u});
         return;
     }
     uint32_t down;
     State st = ch.first_bin(sh, down);
     if (down <= kListed) return add_slots(ch, sh, list_from(st, ch.lim), ch.most);
     if (ch.lim.limit_k && ch.lim.limit_p) return;
-    fill(ch.row, sh, false, ch.from, ch.to, st.cut, st.s, Pass{kByKey, by_mass(st.phase), false});
+    fill(ch.row, sh, false, ch.from, ch.to, st.cut, st.s, Pass{kByDistance, by_mass(st.phase), false});
     add_bins(ch, sh, 1, by_mass(st.phase));
 }
 
@@ -703,7 +758,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_narrow(SampleArgs p, 
         if (ch.c != 0) return;
         st = first_state(ch.row, ch.lim);
     } else {
-        narrow_to(st.s, pick(sh, st, ch.lim, ch.ws->count[1][threadIdx.x], ch.ws->mass[1][threadIdx.x]));
+        to_bin(ch.row, st, pick(sh, st, ch.lim, ch.ws->count[1][threadIdx.x], ch.ws->mass[1][threadIdx.x]));
         if (st.s.count <= kListed) return add_slots(ch, sh, st.s.lo, st.s.hi);
         // more than that with keys next to each other: one workgroup goes on
         if (ch.c != 0) return;
@@ -727,7 +782,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_mass(SampleArgs p, Sp
     if (state != kRowCut) {
         uint32_t down;
         State st = ch.first_bin(sh, down);
-        narrow_to(st.s, pick(sh, st, ch.lim, ch.ws->count[1][threadIdx.x], ch.ws->mass[1][threadIdx.x]));
+        to_bin(ch.row, st, pick(sh, st, ch.lim, ch.ws->count[1][threadIdx.x], ch.ws->mass[1][threadIdx.x]));
         take_list(ch, sh, st);
         int64_t slot;
         float prob;
@@ -735,10 +790,8 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_mass(SampleArgs p, Sp
         cut = st.cut;
     }
     if (ch.lim.min_key > cut.least) cut = Cut{ch.lim.min_key, ~0u};
-    const uint64_t mass = mass_of(ch.row, sh, ch.from, ch.to, cut);
-    if (threadIdx.x != 0) return;
-    x.chunk_mass[size_t(ch.r) * x.chunks + ch.c] = mass;
-    x.chunk_cut[size_t(ch.r) * x.chunks + ch.c] = cut;
+    put_masses(x, ch, cut);
+    if (threadIdx.x == 0) x.chunk_cut[size_t(ch.r) * x.chunks + ch.c] = cut;
 }
 template <typename T>
 __global__ __launch_bounds__(kSampleThreads) void k_sample_draw(SampleArgs p, SplitArgs x) {
@@ -746,7 +799,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_draw(SampleArgs p, Sp
     SampleShared &sh = *reinterpret_cast<SampleShared *>(smem);
     Chunk<T> ch(p, x);
     if (ch.ws->state == kRowDone || !ch.open(p, x, sh, false)) return;
-    draw_by_chunks(p, x, ch, sh, x.chunk_cut[size_t(ch.r) * x.chunks]);
+    draw_by_parts(p, x, ch, sh, x.chunk_cut[size_t(ch.r) * x.chunks]);
 }
 
 // Rows of more slots than this go in chunks, as long as there are no more than kSplitRows of them.
@@ -764,7 +817,7 @@ static Split split_of(size_t rows, size_t n) {
     x.chunk = uint32_t(chunk);
     x.chunks = uint32_t((n + chunk - 1) / chunk);
     x.masses = rows * sizeof(SampleSplit);
-    x.cuts = x.masses + rows * x.chunks * 8;
+    x.cuts = x.masses + rows * x.chunks * kSampleWaves * 8;
     x.mosts = x.cuts + rows * x.chunks * 8;
     x.bytes = x.mosts + rows * x.chunks * 4;
     return x;
