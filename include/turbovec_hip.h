@@ -260,7 +260,7 @@ size_t tv_fp8_rescore_workspace(size_t nq, size_t m, size_t dim);
  * top_p of their mass; of those, min_p > 0 keeps w >= min(min_p, 1); the best one always stays.  Drawn is the first
  * slot, in order of slots, at which the running sum of the kept w exceeds u times their sum, 0 <= u < 1.  A temperature
  * that is not above 0 draws the best.  out_probs: w over the sum of the kept ones.  A row that allows nothing: slot -1,
- * probability 0.  Weights are taken in 64 bits and held as multiples of 2^-(63 - ceil(log2 n)); sums of them are exact,
+ * probability 0.  Weights are taken in 64 bits and held in whole multiples of 2^-(63 - ceil(log2 n)), rounded down; sums of them are exact,
  * so that a draw never depends on the order of additions.  d_u holds a value a row; each of the four parameters does
  * too, or is NULL: temperature 1, no limit. */
 int tv_sample_dev(int device, void *stream, const void *d_scores, int score_type, size_t score_stride, size_t rows, size_t n,

@@ -1,6 +1,6 @@
 // Drawing a slot from rows of scores, with temperature, top-k, top-p and min-p, from given random numbers.
 //
-// The weight of a slot is exp((score - max) / T), taken in 64 bits and held as a whole number of 2^-shift, shift = 63 -
+// The weight of a slot is exp((score - max) / T), taken in 64 bits and held in whole units of 2^-shift (what is left over is dropped), shift = 63 -
 // ceil(log2 n): sums of any number of them fit 64 bits and do not depend on the order of the additions, so that a draw is the same
 // whatever order threads arrive in.  What top-k, top-p and min-p leave is a prefix of the slots ranked by score, ties to the lower
 // slot: the slots above some score, and the first few of those that have it.
@@ -22,11 +22,24 @@ constexpr uint32_t kNoKey = 0x007fffffu;     // -infinity's; what is not allowed
 constexpr uint32_t kBins = 1024;             // a bin to a thread
 constexpr uint32_t kListed = 4000;           // slots that are gathered, at most: two workgroups' LDS to a compute unit
 
+// The same value in all lanes, said to the compiler: it keeps it in scalar registers and branches on it without masks.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return uint32_t(__builtin_amdgcn_readfirstlane(int(v))); }
+__device__ __forceinline__ uint64_t uniform(uint64_t v) { return uint64_t(uniform(uint32_t(v >> 32))) << 32 | uniform(uint32_t(v)); }
+__device__ __forceinline__ float uniform(float v) { return __uint_as_float(uniform(__float_as_uint(v))); }
+__device__ __forceinline__ double uniform(double v) { return __longlong_as_double((long long)(uniform(uint64_t(__double_as_longlong(v))))); }
+
 // The scores' order as unsigned numbers; -0 counts as +0, NaN as -infinity.
 __device__ __forceinline__ uint32_t score_key(float s) {
     return s > -__int_as_float(0x7f800000) ? uint32_t(order_key(s + 0.0f)) ^ 0x80000000u : kNoKey;
 }
 __device__ __forceinline__ float key_score(uint32_t k) { return order_unkey(int(k ^ 0x80000000u)); }
+
+// a * b + c, c the same in all lanes.  (The compiler copies each coefficient first, to add into it.)
+__device__ __forceinline__ double fma_of(double a, double b, double c) {
+    double r;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+    return r;
+}
 
 template <typename T>
 struct SampleRow {
@@ -58,8 +71,8 @@ struct SampleRow {
     __device__ __forceinline__ uint32_t key_at(uint32_t i) const {
         return mask == nullptr || ((mask[i >> 6] >> (i & 63u)) & 1u) ? score_key(float(scores[i])) : kNoKey;
     }
-    // f(slot, score) for every allowed slot of lo .. hi - 1 (multiples of kEach, or the end) whose score is neither NaN nor -infinity, a worker of
-    // `workers`.
+    // f(slot, score, whether it counts) for the slots of lo .. hi - 1 (multiples of kEach, or the end), a worker of `workers`: those count that
+    // are allowed and whose score is neither NaN nor -infinity.
     template <typename F>
     __device__ __forceinline__ void each(uint32_t lo, uint32_t hi, uint32_t worker, uint32_t workers, F &&f) const {
         const uint32_t step = workers * kEach;
@@ -73,7 +86,7 @@ struct SampleRow {
 #pragma unroll
             for (int j = 0; j < kEach; ++j) {
                 const float v = float(now.v[j]);
-                if (((now.bits >> j) & 1u) && v > -__int_as_float(0x7f800000)) f(i + j, v);
+                f(i + j, v, ((now.bits >> j) & 1u) != 0u && v > -__int_as_float(0x7f800000));
             }
             if (!more) return;
             now = next;
@@ -82,27 +95,25 @@ struct SampleRow {
     }
     // exp((score - max) / T); for scores whose largest is +infinity, 1 for those that have it
     __device__ __forceinline__ double weight(uint32_t k) const { return k == most ? 1.0 : exp((double(key_score(k)) - top) * inverse); }
-    // The same as a whole number of 2^-shift, which is what sums are made of: 2^y = 2^e * 2^f, |f| <= 1/2, with the exponential series up to
-    // its tenth power (off by 2.2e-13 at most); adding 2 leaves its value in the low 52 bits.  A library exponential and a
-    // conversion to 64 bits take three times as long.
+    // The same in whole units of 2^-shift, which is what sums are made of: 2^y = 2^e * 2^f, |f| <= 1/2, with the exponential series up to
+    // its ninth power (off by 7e-12 at most), then its high and its low 32 bits.  A library exponential and a conversion to 64 bits
+    // take three times as long.
     __device__ __forceinline__ uint64_t units(float score) const {
-        const double y = fmax((double(score) - top) * inverse2, -200.0);
-        const double e = rint(y), f = (y - e) * 0.69314718055994530942;
-        double v = 1.0 / 3628800.0;
-        v = fma(v, f, 1.0 / 362880.0);
-        v = fma(v, f, 1.0 / 40320.0);
-        v = fma(v, f, 1.0 / 5040.0);
-        v = fma(v, f, 1.0 / 720.0);
-        v = fma(v, f, 1.0 / 120.0);
-        v = fma(v, f, 1.0 / 24.0);
-        v = fma(v, f, 1.0 / 6.0);
-        v = fma(v, f, 0.5);
-        v = fma(v, f, 1.0);
-        v = fma(v, f, 1.0);
-        const uint64_t bits = uint64_t(__double_as_longlong(v + 2.0)) & 0xfffffffffffffull;      // v * 2^51
-        const int down = 62 - shift - int(e);
-        const uint64_t x = bits << 11;
-        return score == best ? 1ull << shift : down >= 64 ? 0ull : (x + ((1ull << down) >> 1)) >> down;
+        if (!(best < __int_as_float(0x7f800000))) return score == best ? 1ull << shift : 0ull;
+        constexpr double k1 = 0.69314718055994530942, k2 = k1 * k1 / 2, k3 = k2 * k1 / 3, k4 = k3 * k1 / 4, k5 = k4 * k1 / 5, k6 = k5 * k1 / 6, k7 = k6 * k1 / 7,
+                         k8 = k7 * k1 / 8, k9 = k8 * k1 / 9;
+        const double y = (double(score) - top) * inverse2, e = rint(y), f = y - e;
+        double v = fma_of(k9, f, k8);
+        v = fma_of(v, f, k7);
+        v = fma_of(v, f, k6);
+        v = fma_of(v, f, k5);
+        v = fma_of(v, f, k4);
+        v = fma_of(v, f, k3);
+        v = fma_of(v, f, k2);
+        v = fma_of(v, f, k1);
+        v = ldexp(fma(v, f, 1.0), int(e) + (shift - 32));
+        const uint32_t hi = uint32_t(v);
+        return uint64_t(hi) << 32 | uint32_t((v - double(hi)) * 4294967296.0);
     }
     // How far a score lies below the best, as the bits of that distance: a number that rises with it.
     __device__ __forceinline__ uint32_t distance(float v) const { return v == best ? 0u : __float_as_uint(best - v); }
@@ -113,7 +124,7 @@ struct SampleRow {
         uint32_t lo = kNoKey + 1u, left = most - lo;           // it is one of lo .. lo + left
         while (left != 0u) {
             const uint32_t step = left / 64u + 1u, mine = lo + min(left, (threadIdx.x & 63u) * step);
-            const uint64_t yes = __ballot(distance(key_score(mine)) <= d);
+            const uint64_t yes = uniform(uint64_t(__ballot(distance(key_score(mine)) <= d)));
             const uint32_t first = yes == 0ull ? 64u : uint32_t(__builtin_ctzll(yes));
             if (first == 0u) return lo;
             // above the place before the first that is, and no further
@@ -134,10 +145,10 @@ struct SampleRow {
     __device__ __forceinline__ void set(uint32_t most_, float t) {
         most = most_;
         best = key_score(most);
-        top = double(best);
+        top = uniform(double(best));
         // (an infinite best leaves the others nothing)
-        inverse = t > 0.0f && top < __longlong_as_double(0x7ff0000000000000ll) ? 1.0 / double(t) : 1.0;
-        inverse2 = inverse * 1.44269504088896340736;
+        inverse = t > 0.0f && top < __longlong_as_double(0x7ff0000000000000ll) ? uniform(1.0 / double(t)) : 1.0;
+        inverse2 = uniform(inverse * 1.44269504088896340736);
         shift = 63 - (32 - __clz(int((n - 1u) | 1u)));
     }
 };
@@ -184,6 +195,7 @@ __device__ __forceinline__ uint64_t block_before(uint64_t v, SampleShared &sh, u
         before += w < wave ? x : 0;
         all += x;
     }
+    all = uniform(all);
     return before;
 }
 __device__ __forceinline__ uint64_t block_sum(uint64_t v, SampleShared &sh) {
@@ -197,7 +209,7 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, SampleShared &sh) {
     if ((threadIdx.x & 63u) == 0) sh.part32[threadIdx.x >> 6] = v;
     __syncthreads();
     for (int w = 0; w < kSampleWaves; ++w) v = max(v, sh.part32[w]);
-    return v;
+    return uniform(v);
 }
 
 // A row's parameters.
@@ -207,11 +219,11 @@ struct Limits {
     bool limit_k, limit_p;
     uint32_t min_key;
     __device__ __forceinline__ void load(const SampleArgs &p, uint32_t r) {
-        t = p.temperature == nullptr ? 1.0f : p.temperature[r];
-        min_p = p.min_p == nullptr ? 0.0f : p.min_p[r];
-        top_k = p.top_k == nullptr ? 0 : p.top_k[r];
-        top_p = p.top_p == nullptr ? 1.0f : p.top_p[r];
-        u = p.u[r];
+        t = p.temperature == nullptr ? 1.0f : uniform(p.temperature[r]);
+        min_p = p.min_p == nullptr ? 0.0f : uniform(p.min_p[r]);
+        top_k = p.top_k == nullptr ? 0 : int32_t(uniform(uint32_t(p.top_k[r])));
+        top_p = p.top_p == nullptr ? 1.0f : uniform(p.top_p[r]);
+        u = uniform(p.u[r]);
         if (!(t > 0.0f)) { top_k = 1; top_p = 1.0f; }       // the best alone
     }
     template <typename T>
@@ -219,7 +231,7 @@ struct Limits {
         row.set(most, t);
         limit_k = top_k > 0 && uint32_t(top_k) < row.n;
         limit_p = top_p < 1.0f;
-        min_key = min_p > 0.0f ? row.least_of_weight(double(min_p), double(t)) : kNoKey + 1u;
+        min_key = min_p > 0.0f ? uniform(row.least_of_weight(double(min_p), double(t))) : kNoKey + 1u;
     }
 };
 
@@ -258,29 +270,29 @@ __device__ __forceinline__ void fill(const SampleRow<T> &row, SampleShared &sh, 
     __syncthreads();
     const CutScores scores(cut);
     const uint32_t by_distance = shift_of(s.far - s.near), by_value = shift_of(s.hi - s.lo), copy = threadIdx.x % kCopies;
-    const auto add = [&](uint32_t i, float v) {
-        if (!scores.leaves(i, v)) return;
+    const auto add = [&](uint32_t i, float v, bool in) {
+        in = in && scores.leaves(i, v);
         uint32_t bin;
         if (pass.mode <= kByDistance) {
             const uint32_t d = row.distance(v);
             bin = row.bin(d);
             if (pass.mode == kByDistance) {
-                if (d < s.near || d > s.far) return;
+                in = in && d >= s.near && d <= s.far;
                 bin = (d - s.near) >> by_distance;
             }
         } else {
-            if (pass.ties && v != scores.least) return;
             const uint32_t x = pass.mode == kByPlace ? ~i : score_key(v);
-            if (x < s.lo || x > s.hi) return;
+            in = in && x >= s.lo && x <= s.hi && (!pass.ties || v == scores.least);
             bin = (s.hi - x) >> by_value;
         }
+        if (!in) return;
         const uint32_t at = bin * kCopies + copy;
         atomicAdd(&sh.count[at], 1u);
         if (pass.mass) atomicAdd(reinterpret_cast<unsigned long long *>(&sh.mass[at]), (unsigned long long)row.units(v));
     };
     if (listed) {
 #pragma unroll 1
-        for (uint32_t e = threadIdx.x; e < hi; e += kSampleThreads) add(~uint32_t(sh.list[e]), key_score(uint32_t(sh.list[e] >> 32)));
+        for (uint32_t e = threadIdx.x; e < hi; e += kSampleThreads) add(~uint32_t(sh.list[e]), key_score(uint32_t(sh.list[e] >> 32)), true);
     } else {
         row.each(lo, hi, threadIdx.x, kSampleThreads, add);
     }
@@ -326,17 +338,17 @@ __device__ __forceinline__ uint32_t pick(SampleShared &sh, State &st, const Limi
         upto = mass_before = st.s.mass_before + block_before(mass, sh, all);
         if (st.whole) {
             st.total = all;
-            st.bound = st.phase == kTopP ? uint64_t(ceil(double(lim.top_p) * double(all))) : drawn_mass(lim.u, all) + 1;
+            st.bound = uniform(st.phase == kTopP ? uint64_t(ceil(double(lim.top_p) * double(all))) : drawn_mass(lim.u, all) + 1);
         }
     }
     if (count != 0 && (before == 0 || upto < st.bound)) atomicMax(&sh.picked, t);
     __syncthreads();
-    const uint32_t bin = sh.picked;
+    const uint32_t bin = uniform(sh.picked);
     if (t == bin) { sh.found_count = count; sh.found_before = uint32_t(before); sh.found_mass = mass_before; }
     __syncthreads();
-    st.s.count = sh.found_count;
-    st.s.before = sh.found_before;
-    st.s.mass_before = sh.found_mass;
+    st.s.count = uniform(sh.found_count);
+    st.s.before = uniform(sh.found_before);
+    st.s.mass_before = uniform(sh.found_mass);
     st.whole = false;
     return bin;
 }
@@ -349,13 +361,13 @@ __device__ __forceinline__ uint32_t list_slots(const SampleRow<T> &row, SampleSh
     __syncthreads();
     const CutScores scores(cut);
     const float least = key_score(from), most = key_score(upto);
-    row.each(lo, hi, threadIdx.x, kSampleThreads, [&](uint32_t i, float v) {
-        if (v < least || v > most || !scores.leaves(i, v)) return;
+    row.each(lo, hi, threadIdx.x, kSampleThreads, [&](uint32_t i, float v, bool in) {
+        if (!in || v < least || v > most || !scores.leaves(i, v)) return;
         const uint32_t at = atomicAdd(&sh.listed, 1u);
         if (at < kListed) sh.list[at] = uint64_t(score_key(v)) << 32 | uint32_t(~i);
     });
     __syncthreads();
-    return min(sh.listed, kListed);
+    return uniform(min(sh.listed, kListed));
 }
 // The one value in s of the list's slots that count.
 __device__ __forceinline__ uint32_t only_value(SampleShared &sh, const State &st) {
@@ -365,7 +377,7 @@ __device__ __forceinline__ uint32_t only_value(SampleShared &sh, const State &st
         if (v >= st.s.lo && v <= st.s.hi && stays && (st.phase != kTies || k == st.cut.least)) sh.found_value = v;
     }
     __syncthreads();
-    const uint32_t v = sh.found_value;
+    const uint32_t v = uniform(sh.found_value);
     __syncthreads();
     return v;
 }
@@ -376,21 +388,26 @@ template <typename T>
 __device__ __forceinline__ uint32_t locate(const SampleRow<T> &row, SampleShared &sh, uint32_t lo, uint32_t len, const Cut &cut, bool ties, uint64_t want) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const CutScores scores(cut);
-    const auto value = [&](uint32_t i, float v) { return !scores.leaves(i, v) ? uint64_t(0) : ties ? uint64_t(v == scores.least) : row.units(v); };
+    const auto value = [&](uint32_t i, float v, bool in) {
+        in = in && scores.leaves(i, v);
+        if (__ballot(in) == 0ull) return uint64_t(0);
+        const uint64_t x = ties ? uint64_t(v == scores.least) : row.units(v);
+        return in ? x : uint64_t(0);
+    };
     while (len > uint32_t(kSampleThreads)) {
         const uint32_t seg = ((len + kSampleWaves - 1) / kSampleWaves + 63u) & ~63u;
         const uint32_t from = min(len, wave * seg), to = min(len, from + seg);
         uint64_t sum = 0;
-        row.each(lo + from, lo + to, lane, 64u, [&](uint32_t i, float v) { sum += value(i, v); });
+        row.each(lo + from, lo + to, lane, 64u, [&](uint32_t i, float v, bool in) { sum += value(i, v, in); });
         sum = wave_upto(sum);
         __syncthreads();
         if (lane == 63u) sh.part[wave] = sum;
         __syncthreads();
         uint32_t w = 0;
-        uint64_t upto = sh.part[0], before = 0;
+        uint64_t upto = uniform(sh.part[0]), before = 0;
         while (w + 1 < uint32_t(kSampleWaves) && upto <= want) {
             before = upto;
-            upto += sh.part[++w];
+            upto += uniform(sh.part[++w]);
         }
         want -= before;
         lo += min(len, w * seg);
@@ -400,7 +417,7 @@ __device__ __forceinline__ uint32_t locate(const SampleRow<T> &row, SampleShared
     uint64_t mine = 0;
     if (threadIdx.x < len) {
         const uint32_t k = row.key_at(lo + threadIdx.x);
-        mine = k != kNoKey ? value(lo + threadIdx.x, key_score(k)) : 0;
+        mine = value(lo + threadIdx.x, key_score(k), k != kNoKey);
     }
     uint64_t all;
     const uint64_t before = block_before(mine, sh, all);
@@ -408,14 +425,19 @@ __device__ __forceinline__ uint32_t locate(const SampleRow<T> &row, SampleShared
     __syncthreads();
     if (before <= want && before + mine > want) sh.picked = threadIdx.x;
     __syncthreads();
-    return lo + sh.picked;
+    return lo + uniform(sh.picked);
 }
 // The mass that the cut leaves of the slots lo .. hi - 1 that are this worker's.
 template <typename T>
 __device__ __forceinline__ uint64_t mass_of(const SampleRow<T> &row, uint32_t lo, uint32_t hi, uint32_t worker, uint32_t workers, const Cut &cut) {
     const CutScores scores(cut);
     uint64_t sum = 0;
-    row.each(lo, hi, worker, workers, [&](uint32_t i, float v) { sum += scores.leaves(i, v) ? row.units(v) : 0; });
+    row.each(lo, hi, worker, workers, [&](uint32_t i, float v, bool in) {
+        in = in && scores.leaves(i, v);
+        if (__ballot(in) == 0ull) return;
+        const uint64_t x = row.units(v);
+        sum += in ? x : 0;
+    });
     return sum;
 }
 
@@ -471,7 +493,7 @@ __device__ void search(const SampleRow<T> &row, SampleShared &sh, const Limits &
             // slots next to each other fall into one bin, a row's are walked instead
             if (st.phase == kDraw) {
                 st.total = block_sum(mass_of(row, 0, row.n, threadIdx.x, kSampleThreads, st.cut), sh);
-                st.bound = drawn_mass(lim.u, st.total) + 1;
+                st.bound = uniform(drawn_mass(lim.u, st.total) + 1);
             }
             st.s.lo = st.s.hi = ~locate(row, sh, 0, row.n, st.cut, st.phase == kTies, st.bound - 1);
         } else if (st.whole || (st.s.lo < st.s.hi && st.s.count != 0)) {
@@ -516,7 +538,7 @@ __device__ void search(const SampleRow<T> &row, SampleShared &sh, const Limits &
             if (st.phase == kTopP) {
                 const uint64_t each = row.units(key_score(st.s.lo));
                 const double fit = each == 0 ? double(st.s.count) : ceil((double(st.bound) - double(st.s.mass_before)) / double(each));
-                ties = fit < 1.0 ? min(1u, st.s.count) : fit < double(st.s.count) ? uint32_t(fit) : st.s.count;
+                ties = uniform(fit < 1.0 ? min(1u, st.s.count) : fit < double(st.s.count) ? uint32_t(fit) : st.s.count);
             }
             st.cut = Cut{st.s.lo, st.s.lo == st.cut.least ? st.cut.tie_last : ~0u};
             if (ties < st.s.count) {
@@ -554,7 +576,9 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample(SampleArgs p) {
         Limits lim;
         lim.load(p, r);
         float best = -__int_as_float(0x7f800000);
-        row.each(0, p.n, threadIdx.x, kSampleThreads, [&](uint32_t, float v) { best = fmaxf(best, v); });
+        row.each(0, p.n, threadIdx.x, kSampleThreads, [&](uint32_t, float v, bool in) {
+        if (in) best = fmaxf(best, v);
+    });
         const uint32_t most = block_max(score_key(best), sh);
         int64_t slot = -1;
         float prob = 0.0f;
@@ -654,7 +678,7 @@ __device__ __forceinline__ void add_slots(const Chunk<T> &ch, SampleShared &sh, 
 // The search goes on among the row's list.
 template <typename T>
 __device__ __forceinline__ void take_list(const Chunk<T> &ch, SampleShared &sh, State &st) {
-    st.n = min(ch.ws->listed, kListed);
+    st.n = uniform(min(ch.ws->listed, kListed));
     st.listed = true;
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < st.n; i += kSampleThreads) sh.list[i] = ch.ws->list[i];
@@ -686,8 +710,8 @@ __device__ __forceinline__ void draw_by_parts(const SampleArgs &p, const SplitAr
         before += all;
     }
     __syncthreads();
-    const uint32_t lo = sh.picked * part;
-    want -= sh.found_mass;
+    const uint32_t lo = uniform(sh.picked) * part;
+    want -= uniform(sh.found_mass);
     __syncthreads();
     const uint32_t at = locate(ch.row, sh, lo, min(part, p.n - lo), cut, false, want);
     ch.write(p, at, float(ldexp(ch.row.weight(ch.row.key_at(at)), ch.row.shift) / double(total)));
@@ -700,7 +724,9 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_max(SampleArgs p, Spl
     const Chunk<T> ch(p, x);
     for (uint32_t i = ch.c * kSampleThreads + threadIdx.x; i < kSplitZeroed; i += x.chunks * kSampleThreads) reinterpret_cast<uint32_t *>(ch.ws)[i] = 0;
     float best = -__int_as_float(0x7f800000);
-    ch.row.each(ch.from, ch.to, threadIdx.x, kSampleThreads, [&](uint32_t, float v) { best = fmaxf(best, v); });
+    ch.row.each(ch.from, ch.to, threadIdx.x, kSampleThreads, [&](uint32_t, float v, bool in) {
+        if (in) best = fmaxf(best, v);
+    });
     const uint32_t most = block_max(score_key(best), sh);
     if (threadIdx.x == 0) x.chunk_most[size_t(ch.r) * x.chunks + ch.c] = most;
 }
@@ -776,9 +802,9 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_mass(SampleArgs p, Sp
     extern __shared__ uint8_t smem[];
     SampleShared &sh = *reinterpret_cast<SampleShared *>(smem);
     Chunk<T> ch(p, x);
-    const uint32_t state = ch.ws->state;
+    const uint32_t state = uniform(ch.ws->state);
     if (state == kRowDone || !ch.open(p, x, sh, state != kRowCut)) return;
-    Cut cut = ch.ws->cut;
+    Cut cut{uniform(ch.ws->cut.least), uniform(ch.ws->cut.tie_last)};
     if (state != kRowCut) {
         uint32_t down;
         State st = ch.first_bin(sh, down);
@@ -798,8 +824,9 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_draw(SampleArgs p, Sp
     extern __shared__ uint8_t smem[];
     SampleShared &sh = *reinterpret_cast<SampleShared *>(smem);
     Chunk<T> ch(p, x);
-    if (ch.ws->state == kRowDone || !ch.open(p, x, sh, false)) return;
-    draw_by_parts(p, x, ch, sh, x.chunk_cut[size_t(ch.r) * x.chunks]);
+    if (uniform(ch.ws->state) == kRowDone || !ch.open(p, x, sh, false)) return;
+    const Cut cut = x.chunk_cut[size_t(ch.r) * x.chunks];
+    draw_by_parts(p, x, ch, sh, Cut{uniform(cut.least), uniform(cut.tie_last)});
 }
 
 // Rows of more slots than this go in chunks, as long as there are no more than kSplitRows of them.
