@@ -319,7 +319,7 @@ struct State {
     int phase, after;         // after: the phase that ends in ties
     bool whole;               // the search has not been narrowed yet
     int histograms;           // of the row by distance so far; two, then by key
-    bool listed;
+    bool listed, bin_only;    // bin_only: the list holds one bin's slots, not all from there up
     uint32_t n;               // slots in the list
     Search s;
     Cut cut;
@@ -385,7 +385,8 @@ __device__ __forceinline__ uint32_t only_value(SampleShared &sh, const State &st
 // Of the cut's slots from lo on (ties: those of its least key, each counting 1; otherwise their mass), in slot order the first that the sum up to it
 // exceeds `want` at; it is one of the `len` from lo on.
 template <typename T>
-__device__ __forceinline__ uint32_t locate(const SampleRow<T> &row, SampleShared &sh, uint32_t lo, uint32_t len, const Cut &cut, bool ties, uint64_t want) {
+__device__ __forceinline__ uint32_t locate(const SampleRow<T> &row, SampleShared &sh, uint32_t lo, uint32_t len, const Cut &cut, bool ties, uint64_t want, bool draws = false,
+                                           float u = 0.0f, uint64_t *total = nullptr) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const CutScores scores(cut);
     const auto value = [&](uint32_t i, float v, bool in) {
@@ -403,6 +404,13 @@ __device__ __forceinline__ uint32_t locate(const SampleRow<T> &row, SampleShared
         __syncthreads();
         if (lane == 63u) sh.part[wave] = sum;
         __syncthreads();
+        if (draws) {
+            uint64_t all = 0;
+            for (uint32_t w = 0; w < uint32_t(kSampleWaves); ++w) all += uniform(sh.part[w]);
+            *total = all;
+            want = uniform(drawn_mass(u, all));
+            draws = false;
+        }
         uint32_t w = 0;
         uint64_t upto = uniform(sh.part[0]), before = 0;
         while (w + 1 < uint32_t(kSampleWaves) && upto <= want) {
@@ -412,8 +420,8 @@ __device__ __forceinline__ uint32_t locate(const SampleRow<T> &row, SampleShared
         want -= before;
         lo += min(len, w * seg);
         len = min(seg, len - min(len, w * seg));
+        __syncthreads();
     }
-    // at most one slot to a thread
     uint64_t mine = 0;
     if (threadIdx.x < len) {
         const uint32_t k = row.key_at(lo + threadIdx.x);
@@ -421,6 +429,10 @@ __device__ __forceinline__ uint32_t locate(const SampleRow<T> &row, SampleShared
     }
     uint64_t all;
     const uint64_t before = block_before(mine, sh, all);
+    if (draws) {
+        *total = all;
+        want = uniform(drawn_mass(u, all));
+    }
     if (threadIdx.x == 0) sh.picked = 0;
     __syncthreads();
     if (before <= want && before + mine > want) sh.picked = threadIdx.x;
@@ -448,7 +460,7 @@ __device__ __forceinline__ State first_state(const SampleRow<T> &row, const Limi
     st.after = kDraw;
     st.whole = true;
     st.histograms = 0;
-    st.listed = false;
+    st.listed = st.bin_only = false;
     st.n = 0;
     st.s = Search{kNoKey + 1u, row.most, 0, ~0u, 0, 0, 0};
     st.cut = Cut{kNoKey + 1u, ~0u};
@@ -491,11 +503,7 @@ __device__ void search(const SampleRow<T> &row, SampleShared &sh, const Limits &
     while (true) {
         if (st.phase >= kTies && !st.listed) {
             // slots next to each other fall into one bin, a row's are walked instead
-            if (st.phase == kDraw) {
-                st.total = block_sum(mass_of(row, 0, row.n, threadIdx.x, kSampleThreads, st.cut), sh);
-                st.bound = uniform(drawn_mass(lim.u, st.total) + 1);
-            }
-            st.s.lo = st.s.hi = ~locate(row, sh, 0, row.n, st.cut, st.phase == kTies, st.bound - 1);
+            st.s.lo = st.s.hi = ~locate(row, sh, 0, row.n, st.cut, st.phase == kTies, st.bound - 1, st.phase == kDraw, lim.u, &st.total);
         } else if (st.whole || (st.s.lo < st.s.hi && st.s.count != 0)) {
             const bool distances = !st.listed && st.histograms < 2, first = distances && st.histograms == 0;
             if (!st.whole && st.listed && st.s.count == 1) {
@@ -516,8 +524,10 @@ __device__ void search(const SampleRow<T> &row, SampleShared &sh, const Limits &
             }
             to_bin(row, st, bin);
             const uint32_t down = first ? slots_down_to(row, sh, st, lim, bin, count) : uint32_t(min(st.s.before + st.s.count, uint64_t(~0u)));
-            if (down <= kListed) {
-                st.n = list_slots(row, sh, 0, row.n, st.cut, list_from(st, lim), row.most);
+            if (down <= kListed || st.s.count <= kListed) {
+                st.bin_only = down > kListed;
+                const uint32_t from = list_from(st, lim), upto = st.bin_only ? st.s.hi : row.most;
+                st.n = from > upto ? 0 : list_slots(row, sh, 0, row.n, st.cut, from, upto);
                 st.listed = true;
             }
             continue;
@@ -550,6 +560,7 @@ __device__ void search(const SampleRow<T> &row, SampleShared &sh, const Limits &
         if (to_cut && next != kTies) return;
         if (next == kDraw && lim.min_key > st.cut.least) st.cut = Cut{lim.min_key, ~0u};
         st.phase = next;
+        if (next != kTies && st.bin_only) st.listed = st.bin_only = false;
         st.whole = true;
         st.histograms = 0;
         st.s = Search{st.cut.least, row.most, 0, ~0u, 0, 0, 0};
@@ -763,6 +774,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_list(SampleArgs p, Sp
     State st = ch.first_bin(sh, down);
     if (down <= kListed) return add_slots(ch, sh, list_from(st, ch.lim), ch.most);
     if (ch.lim.limit_k && ch.lim.limit_p) return;
+    if (st.s.count <= kListed) return add_slots(ch, sh, st.s.lo, st.s.hi);
     fill(ch.row, sh, false, ch.from, ch.to, st.cut, st.s, Pass{kByDistance, by_mass(st.phase), false});
     add_bins(ch, sh, 1, by_mass(st.phase));
 }
@@ -784,6 +796,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_narrow(SampleArgs p, 
         if (ch.c != 0) return;
         st = first_state(ch.row, ch.lim);
     } else {
+        if (st.s.count <= kListed) return;
         to_bin(ch.row, st, pick(sh, st, ch.lim, ch.ws->count[1][threadIdx.x], ch.ws->mass[1][threadIdx.x]));
         if (st.s.count <= kListed) return add_slots(ch, sh, st.s.lo, st.s.hi);
         // more than that with keys next to each other: one workgroup goes on
@@ -808,7 +821,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_mass(SampleArgs p, Sp
     if (state != kRowCut) {
         uint32_t down;
         State st = ch.first_bin(sh, down);
-        to_bin(ch.row, st, pick(sh, st, ch.lim, ch.ws->count[1][threadIdx.x], ch.ws->mass[1][threadIdx.x]));
+        if (st.s.count > kListed) to_bin(ch.row, st, pick(sh, st, ch.lim, ch.ws->count[1][threadIdx.x], ch.ws->mass[1][threadIdx.x]));
         take_list(ch, sh, st);
         int64_t slot;
         float prob;
