@@ -17,9 +17,8 @@
 
 namespace tv {
 
-constexpr int kSampleThreads = 1024, kSampleWaves = kSampleThreads / 64;
+constexpr int kSampleWaves = 16, kSampleThreads = kSampleWaves * 64;      // of a row that is not short
 constexpr uint32_t kNoKey = 0x007fffffu;     // -infinity's; what is not allowed has it too
-constexpr uint32_t kBins = 1024;             // a bin to a thread
 constexpr uint32_t kListed = 4000;           // slots that are gathered, at most: two workgroups' LDS to a compute unit
 
 // The same value in all lanes, said to the compiler: it keeps it in scalar registers and branches on it without masks.
@@ -43,7 +42,7 @@ __device__ __forceinline__ double fma_of(double a, double b, double c) {
 
 template <typename T>
 struct SampleRow {
-    static constexpr int kEach = 16 / int(sizeof(T)), kFirstBin = (127 - 20) * 32;
+    static constexpr int kEach = 16 / int(sizeof(T));
     const T *scores;
     const uint64_t *mask;
     uint32_t n, most;         // most: the key of the largest score
@@ -117,8 +116,6 @@ struct SampleRow {
     }
     // How far a score lies below the best, as the bits of that distance: a number that rises with it.
     __device__ __forceinline__ uint32_t distance(float v) const { return v == best ? 0u : __float_as_uint(best - v); }
-    // The bin of a distance: 32 for each power of two that it spans, from 2^-20 to 2^12; what is nearer or further is in the first or the last.
-    __device__ __forceinline__ static uint32_t bin(uint32_t d) { return uint32_t(min(max(int(d >> 18) - kFirstBin, 0), int(kBins) - 1)); }
     // The least key no further than d (keys rise as distances fall): every lane of a wave tries one of 64 places, until a step is one key.
     __device__ __forceinline__ uint32_t least_within(uint32_t d) const {
         uint32_t lo = kNoKey + 1u, left = most - lo;           // it is one of lo .. lo + left
@@ -173,16 +170,30 @@ __device__ __forceinline__ uint64_t wave_upto(uint64_t v) {
 // Scores crowd into some fifty bins: four copies of each keep the lanes of a wave from waiting for each other (ten million
 // scores in one row, a histogram of masses: 17.2 ms with one copy).
 constexpr uint32_t kCopies = 4;
+// What a workgroup of W waves shares; a bin to a thread.
+template <int W>
 struct SampleShared {
-    uint64_t part[kSampleWaves], found_mass;
-    uint32_t part32[kSampleWaves], listed, picked, found_count, found_before, found_value;
+    static constexpr uint32_t kThreads = 64 * W, kBins = kThreads, kBits = W == 16 ? 10 : W == 4 ? 8 : 0, kMost = W == 16 ? kListed : 2048;
+    static_assert(kBins == 1u << kBits, "a bin to a thread");
+    uint64_t part[W], found_mass;
+    uint32_t part32[W], listed, picked, found_count, found_before, found_value;
     uint32_t count[kBins * kCopies];
     uint64_t mass[kBins * kCopies];
-    uint64_t list[kListed];       // key, complement of the slot.  (Last: kernels that list nothing leave it out.)
+    uint64_t list[kMost];         // key, complement of the slot.  (Last: kernels that list nothing leave it out.)
+    // The bin of a distance: 32 of 1024 for each power of two that it spans, from 2^-20 to 2^12; what is nearer or further is in the first or the
+    // last.
+    static constexpr int kDistance = 28 - int(kBits), kFirstBin = (127 - 20) << (int(kBits) - 5);
+    __device__ __forceinline__ static uint32_t bin(uint32_t d) { return uint32_t(min(max(int(d >> kDistance) - kFirstBin, 0), int(kBins) - 1)); }
+    __device__ __forceinline__ static uint32_t nearest(uint32_t bin) { return bin == 0 ? 0u : uint32_t(kFirstBin + int(bin)) << kDistance; }
+    __device__ __forceinline__ static uint32_t furthest(uint32_t bin) { return bin == kBins - 1 ? 0x7f800000u : nearest(bin + 1) - 1u; }
+    // That many values fall into bins of 2^this.
+    __device__ __forceinline__ static uint32_t shift_of(uint32_t range) { return uint32_t(max(0, 32 - int(kBits) - __clz(int(range)))); }
 };
+using LongShared = SampleShared<kSampleWaves>;
 
 // The sum over the threads before this one; `all` the sum over all of them.
-__device__ __forceinline__ uint64_t block_before(uint64_t v, SampleShared &sh, uint64_t &all) {
+template <int W>
+__device__ __forceinline__ uint64_t block_before(uint64_t v, SampleShared<W> &sh, uint64_t &all) {
     const uint32_t wave = threadIdx.x >> 6;
     const uint64_t upto = wave_upto(v);
     __syncthreads();
@@ -190,7 +201,7 @@ __device__ __forceinline__ uint64_t block_before(uint64_t v, SampleShared &sh, u
     __syncthreads();
     uint64_t before = upto - v;
     all = 0;
-    for (uint32_t w = 0; w < uint32_t(kSampleWaves); ++w) {
+    for (uint32_t w = 0; w < uint32_t(W); ++w) {
         const uint64_t x = sh.part[w];
         before += w < wave ? x : 0;
         all += x;
@@ -198,17 +209,19 @@ __device__ __forceinline__ uint64_t block_before(uint64_t v, SampleShared &sh, u
     all = uniform(all);
     return before;
 }
-__device__ __forceinline__ uint64_t block_sum(uint64_t v, SampleShared &sh) {
+template <int W>
+__device__ __forceinline__ uint64_t block_sum(uint64_t v, SampleShared<W> &sh) {
     uint64_t all;
     block_before(v, sh, all);
     return all;
 }
-__device__ __forceinline__ uint32_t block_max(uint32_t v, SampleShared &sh) {
+template <int W>
+__device__ __forceinline__ uint32_t block_max(uint32_t v, SampleShared<W> &sh) {
     v = wave_umax(v);
     __syncthreads();
     if ((threadIdx.x & 63u) == 0) sh.part32[threadIdx.x >> 6] = v;
     __syncthreads();
-    for (int w = 0; w < kSampleWaves; ++w) v = max(v, sh.part32[w]);
+    for (int w = 0; w < W; ++w) v = max(v, sh.part32[w]);
     return uniform(v);
 }
 
@@ -251,7 +264,6 @@ struct Search {
     uint32_t lo, hi, near, far, count;
     uint64_t before, mass_before;
 };
-__device__ __forceinline__ uint32_t shift_of(uint32_t range) { return uint32_t(max(0, 22 - __clz(int(range)))); }      // 1024 bins of 2^shift
 
 enum { kFirst, kByDistance, kByKey, kByPlace };
 struct Pass {
@@ -259,23 +271,23 @@ struct Pass {
     bool mass, ties;          // ties: of the cut's slots only those of its least key
 };
 // A histogram of the cut's slots whose values lie in s: of those of the list, or those lo .. hi - 1 of the row.
-template <typename T>
-__device__ __forceinline__ void fill(const SampleRow<T> &row, SampleShared &sh, bool listed, uint32_t lo, uint32_t hi, const Cut &cut, const Search &s, const Pass &pass) {
+template <typename T, int W>
+__device__ __forceinline__ void fill(const SampleRow<T> &row, SampleShared<W> &sh, bool listed, uint32_t lo, uint32_t hi, const Cut &cut, const Search &s, const Pass &pass) {
     __syncthreads();
 #pragma unroll
     for (uint32_t c = 0; c < kCopies; ++c) {
-        sh.count[c * kBins + threadIdx.x] = 0;
-        if (pass.mass) sh.mass[c * kBins + threadIdx.x] = 0;
+        sh.count[c * sh.kBins + threadIdx.x] = 0;
+        if (pass.mass) sh.mass[c * sh.kBins + threadIdx.x] = 0;
     }
     __syncthreads();
     const CutScores scores(cut);
-    const uint32_t by_distance = shift_of(s.far - s.near), by_value = shift_of(s.hi - s.lo), copy = threadIdx.x % kCopies;
+    const uint32_t by_distance = sh.shift_of(s.far - s.near), by_value = sh.shift_of(s.hi - s.lo), copy = threadIdx.x % kCopies;
     const auto add = [&](uint32_t i, float v, bool in) {
         in = in && scores.leaves(i, v);
         uint32_t bin;
         if (pass.mode <= kByDistance) {
             const uint32_t d = row.distance(v);
-            bin = row.bin(d);
+            bin = sh.bin(d);
             if (pass.mode == kByDistance) {
                 in = in && d >= s.near && d <= s.far;
                 bin = (d - s.near) >> by_distance;
@@ -292,14 +304,15 @@ __device__ __forceinline__ void fill(const SampleRow<T> &row, SampleShared &sh, 
     };
     if (listed) {
 #pragma unroll 1
-        for (uint32_t e = threadIdx.x; e < hi; e += kSampleThreads) add(~uint32_t(sh.list[e]), key_score(uint32_t(sh.list[e] >> 32)), true);
+        for (uint32_t e = threadIdx.x; e < hi; e += sh.kThreads) add(~uint32_t(sh.list[e]), key_score(uint32_t(sh.list[e] >> 32)), true);
     } else {
-        row.each(lo, hi, threadIdx.x, kSampleThreads, add);
+        row.each(lo, hi, threadIdx.x, sh.kThreads, add);
     }
     __syncthreads();
 }
 // A thread's bin, all copies.
-__device__ __forceinline__ void own_bin(const SampleShared &sh, bool with_mass, uint32_t &count, uint64_t &mass) {
+template <int W>
+__device__ __forceinline__ void own_bin(const SampleShared<W> &sh, bool with_mass, uint32_t &count, uint64_t &mass) {
     count = 0;
     mass = 0;
 #pragma unroll
@@ -328,7 +341,8 @@ struct State {
 __device__ __forceinline__ bool by_mass(int phase) { return phase == kTopP || phase == kDraw; }
 
 // Of the bins, a thread each, the last that has slots and that less than the bound lies before; the first one always.
-__device__ __forceinline__ uint32_t pick(SampleShared &sh, State &st, const Limits &lim, uint32_t count, uint64_t mass) {
+template <int W>
+__device__ __forceinline__ uint32_t pick(SampleShared<W> &sh, State &st, const Limits &lim, uint32_t count, uint64_t mass) {
     const uint32_t t = threadIdx.x;
     if (t == 0) sh.picked = 0;
     uint64_t all;
@@ -353,25 +367,26 @@ __device__ __forceinline__ uint32_t pick(SampleShared &sh, State &st, const Limi
     return bin;
 }
 
-// Lists the cut's slots of lo .. hi - 1 whose keys are from .. upto, kListed at most; returns how many.
-template <typename T>
-__device__ __forceinline__ uint32_t list_slots(const SampleRow<T> &row, SampleShared &sh, uint32_t lo, uint32_t hi, const Cut &cut, uint32_t from, uint32_t upto) {
+// Lists the cut's slots of lo .. hi - 1 whose keys are from .. upto, sh.kMost at most; returns how many.
+template <typename T, int W>
+__device__ __forceinline__ uint32_t list_slots(const SampleRow<T> &row, SampleShared<W> &sh, uint32_t lo, uint32_t hi, const Cut &cut, uint32_t from, uint32_t upto) {
     __syncthreads();
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
     const CutScores scores(cut);
     const float least = key_score(from), most = key_score(upto);
-    row.each(lo, hi, threadIdx.x, kSampleThreads, [&](uint32_t i, float v, bool in) {
+    row.each(lo, hi, threadIdx.x, sh.kThreads, [&](uint32_t i, float v, bool in) {
         if (!in || v < least || v > most || !scores.leaves(i, v)) return;
         const uint32_t at = atomicAdd(&sh.listed, 1u);
-        if (at < kListed) sh.list[at] = uint64_t(score_key(v)) << 32 | uint32_t(~i);
+        if (at < sh.kMost) sh.list[at] = uint64_t(score_key(v)) << 32 | uint32_t(~i);
     });
     __syncthreads();
-    return uniform(min(sh.listed, kListed));
+    return uniform(min(sh.listed, sh.kMost));
 }
 // The one value in s of the list's slots that count.
-__device__ __forceinline__ uint32_t only_value(SampleShared &sh, const State &st) {
-    for (uint32_t e = threadIdx.x; e < st.n; e += kSampleThreads) {
+template <int W>
+__device__ __forceinline__ uint32_t only_value(SampleShared<W> &sh, const State &st) {
+    for (uint32_t e = threadIdx.x; e < st.n; e += sh.kThreads) {
         const uint32_t k = uint32_t(sh.list[e] >> 32), place = uint32_t(sh.list[e]), v = st.phase >= kTies ? place : k;
         const bool stays = k > st.cut.least || (k == st.cut.least && ~place <= st.cut.tie_last);
         if (v >= st.s.lo && v <= st.s.hi && stays && (st.phase != kTies || k == st.cut.least)) sh.found_value = v;
@@ -384,8 +399,8 @@ __device__ __forceinline__ uint32_t only_value(SampleShared &sh, const State &st
 
 // Of the cut's slots from lo on (ties: those of its least key, each counting 1; otherwise their mass), in slot order the first that the sum up to it
 // exceeds `want` at; it is one of the `len` from lo on.
-template <typename T>
-__device__ __forceinline__ uint32_t locate(const SampleRow<T> &row, SampleShared &sh, uint32_t lo, uint32_t len, const Cut &cut, bool ties, uint64_t want, bool draws = false,
+template <typename T, int W>
+__device__ __forceinline__ uint32_t locate(const SampleRow<T> &row, SampleShared<W> &sh, uint32_t lo, uint32_t len, const Cut &cut, bool ties, uint64_t want, bool draws = false,
                                            float u = 0.0f, uint64_t *total = nullptr) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const CutScores scores(cut);
@@ -395,8 +410,8 @@ __device__ __forceinline__ uint32_t locate(const SampleRow<T> &row, SampleShared
         const uint64_t x = ties ? uint64_t(v == scores.least) : row.units(v);
         return in ? x : uint64_t(0);
     };
-    while (len > uint32_t(kSampleThreads)) {
-        const uint32_t seg = ((len + kSampleWaves - 1) / kSampleWaves + 63u) & ~63u;
+    while (len > sh.kThreads) {
+        const uint32_t seg = ((len + uint32_t(W) - 1) / W + 63u) & ~63u;
         const uint32_t from = min(len, wave * seg), to = min(len, from + seg);
         uint64_t sum = 0;
         row.each(lo + from, lo + to, lane, 64u, [&](uint32_t i, float v, bool in) { sum += value(i, v, in); });
@@ -406,14 +421,14 @@ __device__ __forceinline__ uint32_t locate(const SampleRow<T> &row, SampleShared
         __syncthreads();
         if (draws) {
             uint64_t all = 0;
-            for (uint32_t w = 0; w < uint32_t(kSampleWaves); ++w) all += uniform(sh.part[w]);
+            for (uint32_t w = 0; w < uint32_t(W); ++w) all += uniform(sh.part[w]);
             *total = all;
             want = uniform(drawn_mass(u, all));
             draws = false;
         }
         uint32_t w = 0;
         uint64_t upto = uniform(sh.part[0]), before = 0;
-        while (w + 1 < uint32_t(kSampleWaves) && upto <= want) {
+        while (w + 1 < uint32_t(W) && upto <= want) {
             before = upto;
             upto += uniform(sh.part[++w]);
         }
@@ -469,14 +484,14 @@ __device__ __forceinline__ State first_state(const SampleRow<T> &row, const Limi
     return st;
 }
 // The search goes from a histogram by distance to the bin it picked.
-template <typename T>
-__device__ __forceinline__ void to_bin(const SampleRow<T> &row, State &st, uint32_t bin) {
+template <typename T, int W>
+__device__ __forceinline__ void to_bin(const SampleRow<T> &row, const SampleShared<W> &sh, State &st, uint32_t bin) {
     Search &s = st.s;
     if (st.histograms++ == 0) {
-        s.near = bin == 0 ? 0u : uint32_t(row.kFirstBin + int(bin)) << 18;
-        s.far = bin == kBins - 1 ? 0x7f800000u : (uint32_t(row.kFirstBin + int(bin) + 1) << 18) - 1u;
+        s.near = sh.nearest(bin);
+        s.far = sh.furthest(bin);
     } else {
-        const uint32_t shift = shift_of(s.far - s.near);
+        const uint32_t shift = sh.shift_of(s.far - s.near);
         s.near += bin << shift;
         s.far = min(s.far, s.near + ((1u << shift) - 1u));
     }
@@ -484,9 +499,9 @@ __device__ __forceinline__ void to_bin(const SampleRow<T> &row, State &st, uint3
     s.hi = s.near == 0 ? row.most : row.least_within(s.near - 1u) - 1u;
 }
 // Of the first histogram, the slots down to the picked bin that can still be drawn.  (Min-p leaves fewer, but top-p after top-k needs all of top-k's.)
-template <typename T>
-__device__ __forceinline__ uint32_t slots_down_to(const SampleRow<T> &row, SampleShared &sh, const State &st, const Limits &lim, uint32_t bin, uint32_t count) {
-    const uint32_t last = st.phase == kTopP ? min(bin, row.bin(row.distance(key_score(lim.min_key)))) : bin;
+template <typename T, int W>
+__device__ __forceinline__ uint32_t slots_down_to(const SampleRow<T> &row, SampleShared<W> &sh, const State &st, const Limits &lim, uint32_t bin, uint32_t count) {
+    const uint32_t last = st.phase == kTopP ? min(bin, sh.bin(row.distance(key_score(lim.min_key)))) : bin;
     return uint32_t(block_sum(threadIdx.x <= last ? count : 0, sh));
 }
 // From which key on a row's slots are listed.  Where min-p leaves nothing of the bin, the search is over.
@@ -498,8 +513,8 @@ __device__ __forceinline__ uint32_t list_from(State &st, const Limits &lim) {
 }
 
 // The searches that are left, to the draw, or (to_cut) to the end of the one that st is in.
-template <typename T>
-__device__ void search(const SampleRow<T> &row, SampleShared &sh, const Limits &lim, State &st, bool to_cut, int64_t &slot, float &prob) {
+template <typename T, int W>
+__device__ void search(const SampleRow<T> &row, SampleShared<W> &sh, const Limits &lim, State &st, bool to_cut, int64_t &slot, float &prob) {
     while (true) {
         if (st.phase >= kTies && !st.listed) {
             // slots next to each other fall into one bin, a row's are walked instead
@@ -517,15 +532,15 @@ __device__ void search(const SampleRow<T> &row, SampleShared &sh, const Limits &
             own_bin(sh, by_mass(st.phase), count, mass);
             const uint32_t bin = pick(sh, st, lim, count, mass);
             if (!distances) {
-                const uint32_t shift = shift_of(st.s.hi - st.s.lo);
+                const uint32_t shift = sh.shift_of(st.s.hi - st.s.lo);
                 st.s.hi -= bin << shift;
                 st.s.lo = max(st.s.lo, st.s.hi - min(st.s.hi, (1u << shift) - 1u));
                 continue;
             }
-            to_bin(row, st, bin);
+            to_bin(row, sh, st, bin);
             const uint32_t down = first ? slots_down_to(row, sh, st, lim, bin, count) : uint32_t(min(st.s.before + st.s.count, uint64_t(~0u)));
-            if (down <= kListed || st.s.count <= kListed) {
-                st.bin_only = down > kListed;
+            if (down <= sh.kMost || st.s.count <= sh.kMost) {
+                st.bin_only = down > sh.kMost;
                 const uint32_t from = list_from(st, lim), upto = st.bin_only ? st.s.hi : row.most;
                 st.n = from > upto ? 0 : list_slots(row, sh, 0, row.n, st.cut, from, upto);
                 st.listed = true;
@@ -577,19 +592,19 @@ __device__ __forceinline__ SampleRow<T> row_of(const SampleArgs &p, uint32_t r) 
     return row;
 }
 
-// Short rows, and many: a workgroup to a row.
-template <typename T>
-__global__ __launch_bounds__(kSampleThreads) void k_sample(SampleArgs p) {
+// Short rows, and many: a workgroup of W waves to a row.
+template <typename T, int W>
+__global__ __launch_bounds__(64 * W) void k_sample(SampleArgs p) {
     extern __shared__ uint8_t smem[];
-    SampleShared &sh = *reinterpret_cast<SampleShared *>(smem);
+    SampleShared<W> &sh = *reinterpret_cast<SampleShared<W> *>(smem);
     for (uint32_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         SampleRow<T> row = row_of<T>(p, r);
         Limits lim;
         lim.load(p, r);
         float best = -__int_as_float(0x7f800000);
-        row.each(0, p.n, threadIdx.x, kSampleThreads, [&](uint32_t, float v, bool in) {
-        if (in) best = fmaxf(best, v);
-    });
+        row.each(0, p.n, threadIdx.x, sh.kThreads, [&](uint32_t, float v, bool in) {
+            if (in) best = fmaxf(best, v);
+        });
         const uint32_t most = block_max(score_key(best), sh);
         int64_t slot = -1;
         float prob = 0.0f;
@@ -617,8 +632,8 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample(SampleArgs p) {
 // 256 rows of 100K take 448 us in one kernel where a launch takes 2.
 struct SampleSplit {
     // zeroed by the first kernel
-    uint64_t mass[2][kBins];
-    uint32_t count[2][kBins];
+    uint64_t mass[2][LongShared::kBins];
+    uint32_t count[2][LongShared::kBins];
     uint32_t listed, state;
     Cut cut;
     uint64_t list[kListed];
@@ -643,7 +658,7 @@ struct Chunk {
     uint64_t mass;            // count, mass: a thread's bin of the first histogram
     __device__ __forceinline__ Chunk(const SampleArgs &p, const SplitArgs &x)
         : row(row_of<T>(p, blockIdx.x)), ws(x.rows + blockIdx.x), r(blockIdx.x), c(blockIdx.y), from(blockIdx.y * x.chunk), to(min(p.n, from + x.chunk)) {}
-    __device__ __forceinline__ bool open(const SampleArgs &p, const SplitArgs &x, SampleShared &sh, bool bins) {
+    __device__ __forceinline__ bool open(const SampleArgs &p, const SplitArgs &x, LongShared &sh, bool bins) {
         lim.load(p, r);
         most = kNoKey;
         count = bins ? ws->count[0][threadIdx.x] : 0;
@@ -658,10 +673,10 @@ struct Chunk {
         if (threadIdx.x == 0) { p.out_slots[r] = slot; p.out_probs[r] = prob; ws->state = kRowDone; }
     }
     // After the first histogram.
-    __device__ __forceinline__ State first_bin(SampleShared &sh, uint32_t &down) {
+    __device__ __forceinline__ State first_bin(LongShared &sh, uint32_t &down) {
         State st = first_state(row, lim);
         const uint32_t bin = pick(sh, st, lim, count, mass);
-        to_bin(row, st, bin);
+        to_bin(row, sh, st, bin);
         down = slots_down_to(row, sh, st, lim, bin, count);
         return st;
     }
@@ -669,7 +684,7 @@ struct Chunk {
 };
 
 template <typename T>
-__device__ __forceinline__ void add_bins(const Chunk<T> &ch, SampleShared &sh, int which, bool with_mass) {
+__device__ __forceinline__ void add_bins(const Chunk<T> &ch, LongShared &sh, int which, bool with_mass) {
     uint32_t count;
     uint64_t mass;
     own_bin(sh, with_mass, count, mass);
@@ -679,7 +694,7 @@ __device__ __forceinline__ void add_bins(const Chunk<T> &ch, SampleShared &sh, i
 }
 // Adds the chunk's slots with keys from .. upto to the row's list, which has room for them.
 template <typename T>
-__device__ __forceinline__ void add_slots(const Chunk<T> &ch, SampleShared &sh, uint32_t from, uint32_t upto) {
+__device__ __forceinline__ void add_slots(const Chunk<T> &ch, LongShared &sh, uint32_t from, uint32_t upto) {
     const uint32_t listed = list_slots(ch.row, sh, ch.from, ch.to, Cut{kNoKey + 1u, ~0u}, from, upto);
     if (threadIdx.x == 0) sh.found_count = listed == 0u ? 0u : atomicAdd(&ch.ws->listed, listed);
     __syncthreads();
@@ -688,7 +703,7 @@ __device__ __forceinline__ void add_slots(const Chunk<T> &ch, SampleShared &sh, 
 }
 // The search goes on among the row's list.
 template <typename T>
-__device__ __forceinline__ void take_list(const Chunk<T> &ch, SampleShared &sh, State &st) {
+__device__ __forceinline__ void take_list(const Chunk<T> &ch, LongShared &sh, State &st) {
     st.n = uniform(min(ch.ws->listed, kListed));
     st.listed = true;
     __syncthreads();
@@ -705,7 +720,7 @@ __device__ __forceinline__ void put_masses(const SplitArgs &x, const Chunk<T> &c
 }
 // The row's draw from those of its chunks.
 template <typename T>
-__device__ __forceinline__ void draw_by_parts(const SampleArgs &p, const SplitArgs &x, const Chunk<T> &ch, SampleShared &sh, const Cut &cut) {
+__device__ __forceinline__ void draw_by_parts(const SampleArgs &p, const SplitArgs &x, const Chunk<T> &ch, LongShared &sh, const Cut &cut) {
     const uint32_t parts = x.chunks * kSampleWaves, part = x.chunk / kSampleWaves;
     const uint64_t *const masses = x.part_mass + size_t(ch.r) * parts;
     uint64_t sum = 0;
@@ -731,7 +746,7 @@ __device__ __forceinline__ void draw_by_parts(const SampleArgs &p, const SplitAr
 template <typename T>
 __global__ __launch_bounds__(kSampleThreads) void k_sample_max(SampleArgs p, SplitArgs x) {
     extern __shared__ uint8_t smem[];
-    SampleShared &sh = *reinterpret_cast<SampleShared *>(smem);
+    LongShared &sh = *reinterpret_cast<LongShared *>(smem);
     const Chunk<T> ch(p, x);
     for (uint32_t i = ch.c * kSampleThreads + threadIdx.x; i < kSplitZeroed; i += x.chunks * kSampleThreads) reinterpret_cast<uint32_t *>(ch.ws)[i] = 0;
     float best = -__int_as_float(0x7f800000);
@@ -745,7 +760,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_max(SampleArgs p, Spl
 template <typename T>
 __global__ __launch_bounds__(kSampleThreads) void k_sample_bins(SampleArgs p, SplitArgs x) {
     extern __shared__ uint8_t smem[];
-    SampleShared &sh = *reinterpret_cast<SampleShared *>(smem);
+    LongShared &sh = *reinterpret_cast<LongShared *>(smem);
     Chunk<T> ch(p, x);
     if (!ch.open(p, x, sh, false)) {
         if (ch.c == 0) ch.write(p, -1, 0.0f);
@@ -763,7 +778,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_bins(SampleArgs p, Sp
 template <typename T>
 __global__ __launch_bounds__(kSampleThreads) void k_sample_list(SampleArgs p, SplitArgs x) {
     extern __shared__ uint8_t smem[];
-    SampleShared &sh = *reinterpret_cast<SampleShared *>(smem);
+    LongShared &sh = *reinterpret_cast<LongShared *>(smem);
     Chunk<T> ch(p, x);
     if (!ch.open(p, x, sh, true)) return;
     if (!ch.limited()) {
@@ -782,7 +797,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_list(SampleArgs p, Sp
 template <typename T>
 __global__ __launch_bounds__(kSampleThreads) void k_sample_narrow(SampleArgs p, SplitArgs x) {
     extern __shared__ uint8_t smem[];
-    SampleShared &sh = *reinterpret_cast<SampleShared *>(smem);
+    LongShared &sh = *reinterpret_cast<LongShared *>(smem);
     Chunk<T> ch(p, x);
     if (!ch.open(p, x, sh, true) || !ch.limited()) return;
     uint32_t down;
@@ -797,7 +812,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_narrow(SampleArgs p, 
         st = first_state(ch.row, ch.lim);
     } else {
         if (st.s.count <= kListed) return;
-        to_bin(ch.row, st, pick(sh, st, ch.lim, ch.ws->count[1][threadIdx.x], ch.ws->mass[1][threadIdx.x]));
+        to_bin(ch.row, sh, st, pick(sh, st, ch.lim, ch.ws->count[1][threadIdx.x], ch.ws->mass[1][threadIdx.x]));
         if (st.s.count <= kListed) return add_slots(ch, sh, st.s.lo, st.s.hi);
         // more than that with keys next to each other: one workgroup goes on
         if (ch.c != 0) return;
@@ -813,7 +828,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_narrow(SampleArgs p, 
 template <typename T>
 __global__ __launch_bounds__(kSampleThreads) void k_sample_mass(SampleArgs p, SplitArgs x) {
     extern __shared__ uint8_t smem[];
-    SampleShared &sh = *reinterpret_cast<SampleShared *>(smem);
+    LongShared &sh = *reinterpret_cast<LongShared *>(smem);
     Chunk<T> ch(p, x);
     const uint32_t state = uniform(ch.ws->state);
     if (state == kRowDone || !ch.open(p, x, sh, state != kRowCut)) return;
@@ -821,7 +836,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_mass(SampleArgs p, Sp
     if (state != kRowCut) {
         uint32_t down;
         State st = ch.first_bin(sh, down);
-        if (st.s.count > kListed) to_bin(ch.row, st, pick(sh, st, ch.lim, ch.ws->count[1][threadIdx.x], ch.ws->mass[1][threadIdx.x]));
+        if (st.s.count > kListed) to_bin(ch.row, sh, st, pick(sh, st, ch.lim, ch.ws->count[1][threadIdx.x], ch.ws->mass[1][threadIdx.x]));
         take_list(ch, sh, st);
         int64_t slot;
         float prob;
@@ -835,7 +850,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_mass(SampleArgs p, Sp
 template <typename T>
 __global__ __launch_bounds__(kSampleThreads) void k_sample_draw(SampleArgs p, SplitArgs x) {
     extern __shared__ uint8_t smem[];
-    SampleShared &sh = *reinterpret_cast<SampleShared *>(smem);
+    LongShared &sh = *reinterpret_cast<LongShared *>(smem);
     Chunk<T> ch(p, x);
     if (uniform(ch.ws->state) == kRowDone || !ch.open(p, x, sh, false)) return;
     const Cut cut = x.chunk_cut[size_t(ch.r) * x.chunks];
@@ -865,12 +880,19 @@ static Split split_of(size_t rows, size_t n) {
 static bool splits(size_t rows, size_t n) { return n > kSplitSlots && rows <= kSplitRows; }
 size_t sample_workspace(size_t rows, size_t n) { return splits(rows, n) ? split_of(rows, n).bytes : 0; }
 
+// A row for four waves: a short one, whose time goes into the steps that the workgroup waits in between (one row, top-k 50 and top-p 0.9: 100
+// slots 26 -> 18 us, 4000 slots 28 -> 23, 8000 slots 30 -> 26 but 31 -> 34 with top-p alone, 16000 slots 34 -> 38).  And of more rows than compute units,
+// four of which share one then, those not too long (1024 rows of 1000: 112 -> 26, of 25000: 165 -> 74, of 100000: 331 -> 257 but 400 -> 434 with
+// top-p alone; 300 rows of 25000: 82 -> 56, of 100000: 147 -> 171).
+static bool few_waves(size_t rows, size_t n) { return n <= 6144 || (rows > 256 && n <= 64 * rows); }
 template <typename T>
 static hipError_t sample(const SampleArgs &a, hipStream_t s) {
-    const size_t lds = sizeof(SampleShared), unlisted = offsetof(SampleShared, list);
+    const size_t lds = sizeof(LongShared), unlisted = offsetof(LongShared, list);
+    const uint32_t grid_rows = a.rows < 65536u ? a.rows : 65536u;
+    if (few_waves(a.rows, a.n)) return launch(k_sample<T, 4>, grid_rows, 256, sizeof(SampleShared<4>), s, a);
     if (!splits(a.rows, a.n)) {
-        if (const hipError_t e = allow_lds(reinterpret_cast<const void *>(k_sample<T>), lds); e != hipSuccess) return e;
-        return launch(k_sample<T>, a.rows < 65536u ? a.rows : 65536u, kSampleThreads, lds, s, a);
+        if (const hipError_t e = allow_lds(reinterpret_cast<const void *>(k_sample<T, kSampleWaves>), lds); e != hipSuccess) return e;
+        return launch(k_sample<T, kSampleWaves>, grid_rows, kSampleThreads, lds, s, a);
     }
     const Split split = split_of(a.rows, a.n);
     const SplitArgs x{reinterpret_cast<SampleSplit *>(a.ws), reinterpret_cast<uint64_t *>(a.ws + split.masses), reinterpret_cast<Cut *>(a.ws + split.cuts),
