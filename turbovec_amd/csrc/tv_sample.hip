@@ -171,9 +171,9 @@ __device__ __forceinline__ uint64_t wave_upto(uint64_t v) {
 // scores in one row, a histogram of masses: 17.2 ms with one copy).
 constexpr uint32_t kCopies = 4;
 // What a workgroup of W waves shares; a bin to a thread.
-template <int W>
+template <int W, uint32_t MOST = kListed>
 struct SampleShared {
-    static constexpr uint32_t kThreads = 64 * W, kBins = kThreads, kBits = W == 16 ? 10 : W == 4 ? 8 : 0, kMost = W == 16 ? kListed : 2048;
+    static constexpr uint32_t kThreads = 64 * W, kBins = kThreads, kBits = W == 16 ? 10 : W == 4 ? 8 : 0, kMost = MOST;
     static_assert(kBins == 1u << kBits, "a bin to a thread");
     uint64_t part[W], found_mass;
     uint32_t part32[W], listed, picked, found_count, found_before, found_value;
@@ -189,11 +189,12 @@ struct SampleShared {
     // That many values fall into bins of 2^this.
     __device__ __forceinline__ static uint32_t shift_of(uint32_t range) { return uint32_t(max(0, 32 - int(kBits) - __clz(int(range)))); }
 };
+constexpr uint32_t kShortListed = 2048;     // five workgroups' LDS to a compute unit
 using LongShared = SampleShared<kSampleWaves>;
 
 // The sum over the threads before this one; `all` the sum over all of them.
-template <int W>
-__device__ __forceinline__ uint64_t block_before(uint64_t v, SampleShared<W> &sh, uint64_t &all) {
+template <int W, uint32_t MOST>
+__device__ __forceinline__ uint64_t block_before(uint64_t v, SampleShared<W, MOST> &sh, uint64_t &all) {
     const uint32_t wave = threadIdx.x >> 6;
     const uint64_t upto = wave_upto(v);
     __syncthreads();
@@ -209,14 +210,14 @@ __device__ __forceinline__ uint64_t block_before(uint64_t v, SampleShared<W> &sh
     all = uniform(all);
     return before;
 }
-template <int W>
-__device__ __forceinline__ uint64_t block_sum(uint64_t v, SampleShared<W> &sh) {
+template <int W, uint32_t MOST>
+__device__ __forceinline__ uint64_t block_sum(uint64_t v, SampleShared<W, MOST> &sh) {
     uint64_t all;
     block_before(v, sh, all);
     return all;
 }
-template <int W>
-__device__ __forceinline__ uint32_t block_max(uint32_t v, SampleShared<W> &sh) {
+template <int W, uint32_t MOST>
+__device__ __forceinline__ uint32_t block_max(uint32_t v, SampleShared<W, MOST> &sh) {
     v = wave_umax(v);
     __syncthreads();
     if ((threadIdx.x & 63u) == 0) sh.part32[threadIdx.x >> 6] = v;
@@ -271,8 +272,8 @@ struct Pass {
     bool mass, ties;          // ties: of the cut's slots only those of its least key
 };
 // A histogram of the cut's slots whose values lie in s: of those of the list, or those lo .. hi - 1 of the row.
-template <typename T, int W>
-__device__ __forceinline__ void fill(const SampleRow<T> &row, SampleShared<W> &sh, bool listed, uint32_t lo, uint32_t hi, const Cut &cut, const Search &s, const Pass &pass) {
+template <typename T, int W, uint32_t MOST>
+__device__ __forceinline__ void fill(const SampleRow<T> &row, SampleShared<W, MOST> &sh, bool listed, uint32_t lo, uint32_t hi, const Cut &cut, const Search &s, const Pass &pass) {
     __syncthreads();
 #pragma unroll
     for (uint32_t c = 0; c < kCopies; ++c) {
@@ -311,8 +312,8 @@ __device__ __forceinline__ void fill(const SampleRow<T> &row, SampleShared<W> &s
     __syncthreads();
 }
 // A thread's bin, all copies.
-template <int W>
-__device__ __forceinline__ void own_bin(const SampleShared<W> &sh, bool with_mass, uint32_t &count, uint64_t &mass) {
+template <int W, uint32_t MOST>
+__device__ __forceinline__ void own_bin(const SampleShared<W, MOST> &sh, bool with_mass, uint32_t &count, uint64_t &mass) {
     count = 0;
     mass = 0;
 #pragma unroll
@@ -341,8 +342,8 @@ struct State {
 __device__ __forceinline__ bool by_mass(int phase) { return phase == kTopP || phase == kDraw; }
 
 // Of the bins, a thread each, the last that has slots and that less than the bound lies before; the first one always.
-template <int W>
-__device__ __forceinline__ uint32_t pick(SampleShared<W> &sh, State &st, const Limits &lim, uint32_t count, uint64_t mass) {
+template <int W, uint32_t MOST>
+__device__ __forceinline__ uint32_t pick(SampleShared<W, MOST> &sh, State &st, const Limits &lim, uint32_t count, uint64_t mass) {
     const uint32_t t = threadIdx.x;
     if (t == 0) sh.picked = 0;
     uint64_t all;
@@ -368,8 +369,8 @@ __device__ __forceinline__ uint32_t pick(SampleShared<W> &sh, State &st, const L
 }
 
 // Lists the cut's slots of lo .. hi - 1 whose keys are from .. upto, sh.kMost at most; returns how many.
-template <typename T, int W>
-__device__ __forceinline__ uint32_t list_slots(const SampleRow<T> &row, SampleShared<W> &sh, uint32_t lo, uint32_t hi, const Cut &cut, uint32_t from, uint32_t upto) {
+template <typename T, int W, uint32_t MOST>
+__device__ __forceinline__ uint32_t list_slots(const SampleRow<T> &row, SampleShared<W, MOST> &sh, uint32_t lo, uint32_t hi, const Cut &cut, uint32_t from, uint32_t upto) {
     __syncthreads();
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
@@ -384,8 +385,8 @@ __device__ __forceinline__ uint32_t list_slots(const SampleRow<T> &row, SampleSh
     return uniform(min(sh.listed, sh.kMost));
 }
 // The one value in s of the list's slots that count.
-template <int W>
-__device__ __forceinline__ uint32_t only_value(SampleShared<W> &sh, const State &st) {
+template <int W, uint32_t MOST>
+__device__ __forceinline__ uint32_t only_value(SampleShared<W, MOST> &sh, const State &st) {
     for (uint32_t e = threadIdx.x; e < st.n; e += sh.kThreads) {
         const uint32_t k = uint32_t(sh.list[e] >> 32), place = uint32_t(sh.list[e]), v = st.phase >= kTies ? place : k;
         const bool stays = k > st.cut.least || (k == st.cut.least && ~place <= st.cut.tie_last);
@@ -399,8 +400,8 @@ __device__ __forceinline__ uint32_t only_value(SampleShared<W> &sh, const State 
 
 // Of the cut's slots from lo on (ties: those of its least key, each counting 1; otherwise their mass), in slot order the first that the sum up to it
 // exceeds `want` at; it is one of the `len` from lo on.
-template <typename T, int W>
-__device__ __forceinline__ uint32_t locate(const SampleRow<T> &row, SampleShared<W> &sh, uint32_t lo, uint32_t len, const Cut &cut, bool ties, uint64_t want, bool draws = false,
+template <typename T, int W, uint32_t MOST>
+__device__ __forceinline__ uint32_t locate(const SampleRow<T> &row, SampleShared<W, MOST> &sh, uint32_t lo, uint32_t len, const Cut &cut, bool ties, uint64_t want, bool draws = false,
                                            float u = 0.0f, uint64_t *total = nullptr) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const CutScores scores(cut);
@@ -484,8 +485,8 @@ __device__ __forceinline__ State first_state(const SampleRow<T> &row, const Limi
     return st;
 }
 // The search goes from a histogram by distance to the bin it picked.
-template <typename T, int W>
-__device__ __forceinline__ void to_bin(const SampleRow<T> &row, const SampleShared<W> &sh, State &st, uint32_t bin) {
+template <typename T, int W, uint32_t MOST>
+__device__ __forceinline__ void to_bin(const SampleRow<T> &row, const SampleShared<W, MOST> &sh, State &st, uint32_t bin) {
     Search &s = st.s;
     if (st.histograms++ == 0) {
         s.near = sh.nearest(bin);
@@ -499,8 +500,8 @@ __device__ __forceinline__ void to_bin(const SampleRow<T> &row, const SampleShar
     s.hi = s.near == 0 ? row.most : row.least_within(s.near - 1u) - 1u;
 }
 // Of the first histogram, the slots down to the picked bin that can still be drawn.  (Min-p leaves fewer, but top-p after top-k needs all of top-k's.)
-template <typename T, int W>
-__device__ __forceinline__ uint32_t slots_down_to(const SampleRow<T> &row, SampleShared<W> &sh, const State &st, const Limits &lim, uint32_t bin, uint32_t count) {
+template <typename T, int W, uint32_t MOST>
+__device__ __forceinline__ uint32_t slots_down_to(const SampleRow<T> &row, SampleShared<W, MOST> &sh, const State &st, const Limits &lim, uint32_t bin, uint32_t count) {
     const uint32_t last = st.phase == kTopP ? min(bin, sh.bin(row.distance(key_score(lim.min_key)))) : bin;
     return uint32_t(block_sum(threadIdx.x <= last ? count : 0, sh));
 }
@@ -512,9 +513,10 @@ __device__ __forceinline__ uint32_t list_from(State &st, const Limits &lim) {
     return lim.min_key;
 }
 
-// The searches that are left, to the draw, or (to_cut) to the end of the one that st is in.
-template <typename T, int W>
-__device__ void search(const SampleRow<T> &row, SampleShared<W> &sh, const Limits &lim, State &st, bool to_cut, int64_t &slot, float &prob) {
+// The searches that are left, to the draw, or (to_cut) to the end of the one that st is in, or (to_list) to where the slots that can still be drawn
+// are listed: then false.
+template <typename T, int W, uint32_t MOST>
+__device__ __forceinline__ bool search(const SampleRow<T> &row, SampleShared<W, MOST> &sh, const Limits &lim, State &st, bool to_cut, bool to_list, int64_t &slot, float &prob) {
     while (true) {
         if (st.phase >= kTies && !st.listed) {
             // slots next to each other fall into one bin, a row's are walked instead
@@ -544,6 +546,7 @@ __device__ void search(const SampleRow<T> &row, SampleShared<W> &sh, const Limit
                 const uint32_t from = list_from(st, lim), upto = st.bin_only ? st.s.hi : row.most;
                 st.n = from > upto ? 0 : list_slots(row, sh, 0, row.n, st.cut, from, upto);
                 st.listed = true;
+                if (to_list && !st.bin_only) return false;
             }
             continue;
         }
@@ -551,7 +554,7 @@ __device__ void search(const SampleRow<T> &row, SampleShared<W> &sh, const Limit
         if (st.phase == kDraw) {
             slot = int64_t(~st.s.lo);
             prob = float(ldexp(row.weight(row.key_at(~st.s.lo)), row.shift) / double(st.total));
-            return;
+            return true;
         }
         int next = kDraw;
         if (st.phase == kTies) {
@@ -572,7 +575,7 @@ __device__ void search(const SampleRow<T> &row, SampleShared<W> &sh, const Limit
                 st.bound = ties;
             }
         }
-        if (to_cut && next != kTies) return;
+        if (to_cut && next != kTies) return true;
         if (next == kDraw && lim.min_key > st.cut.least) st.cut = Cut{lim.min_key, ~0u};
         st.phase = next;
         if (next != kTies && st.bin_only) st.listed = st.bin_only = false;
@@ -593,10 +596,10 @@ __device__ __forceinline__ SampleRow<T> row_of(const SampleArgs &p, uint32_t r) 
 }
 
 // Short rows, and many: a workgroup of W waves to a row.
-template <typename T, int W>
+template <typename T, int W, uint32_t MOST>
 __global__ __launch_bounds__(64 * W) void k_sample(SampleArgs p) {
     extern __shared__ uint8_t smem[];
-    SampleShared<W> &sh = *reinterpret_cast<SampleShared<W> *>(smem);
+    SampleShared<W, MOST> &sh = *reinterpret_cast<SampleShared<W, MOST> *>(smem);
     for (uint32_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         SampleRow<T> row = row_of<T>(p, r);
         Limits lim;
@@ -612,7 +615,16 @@ __global__ __launch_bounds__(64 * W) void k_sample(SampleArgs p) {
             lim.set(row, most);
             State st = first_state(row, lim);
             if (st.phase == kDraw && lim.min_key > st.cut.least) st.cut.least = lim.min_key;
-            search(row, sh, lim, st, false, slot, prob);
+            if (!search(row, sh, lim, st, false, W == kSampleWaves && r + gridDim.x >= p.rows, slot, prob)) {
+                // Four waves go on: they wait less for each other, and a barrier counts the waves that have not ended.
+                SampleShared<4, MOST> &few = *reinterpret_cast<SampleShared<4, MOST> *>(smem);
+                static_assert(sizeof(few) <= offsetof(SampleShared<kSampleWaves>, list), "the list moves down past itself");
+                __syncthreads();
+                if (threadIdx.x >= few.kThreads) return;
+                for (uint32_t i = threadIdx.x; i < st.n; i += few.kThreads) few.list[i] = sh.list[i];
+                __syncthreads();
+                search(row, few, lim, st, false, false, slot, prob);
+            }
         }
         if (threadIdx.x == 0) { p.out_slots[r] = slot; p.out_probs[r] = prob; }
         __syncthreads();
@@ -702,12 +714,12 @@ __device__ __forceinline__ void add_slots(const Chunk<T> &ch, LongShared &sh, ui
         if (sh.found_count + i < kListed) ch.ws->list[sh.found_count + i] = sh.list[i];
 }
 // The search goes on among the row's list.
-template <typename T>
-__device__ __forceinline__ void take_list(const Chunk<T> &ch, LongShared &sh, State &st) {
+template <typename T, int W>
+__device__ __forceinline__ void take_list(const Chunk<T> &ch, SampleShared<W> &sh, State &st) {
     st.n = uniform(min(ch.ws->listed, kListed));
     st.listed = true;
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < st.n; i += kSampleThreads) sh.list[i] = ch.ws->list[i];
+    for (uint32_t i = threadIdx.x; i < st.n; i += sh.kThreads) sh.list[i] = ch.ws->list[i];
     __syncthreads();
 }
 
@@ -806,7 +818,15 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_narrow(SampleArgs p, 
     if (down <= kListed) {
         if (ch.c != 0) return;
         list_from(st, ch.lim);
-        take_list(ch, sh, st);
+        // Four waves go on: they wait less for each other, and a barrier counts the waves that have not ended.
+        __syncthreads();
+        SampleShared<4> &few = *reinterpret_cast<SampleShared<4> *>(smem);
+        if (threadIdx.x >= few.kThreads) return;
+        take_list(ch, few, st);
+        int64_t slot;
+        float prob;
+        search(ch.row, few, ch.lim, st, false, false, slot, prob);
+        return ch.write(p, slot, prob);
     } else if (ch.lim.limit_k && ch.lim.limit_p) {
         if (ch.c != 0) return;
         st = first_state(ch.row, ch.lim);
@@ -820,7 +840,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_narrow(SampleArgs p, 
     }
     int64_t slot;
     float prob;
-    search(ch.row, sh, ch.lim, st, to_cut, slot, prob);
+    search(ch.row, sh, ch.lim, st, to_cut, false, slot, prob);
     if (!to_cut) return ch.write(p, slot, prob);
     if (threadIdx.x == 0) { ch.ws->cut = st.cut; ch.ws->state = kRowCut; }
 }
@@ -840,7 +860,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_mass(SampleArgs p, Sp
         take_list(ch, sh, st);
         int64_t slot;
         float prob;
-        search(ch.row, sh, ch.lim, st, true, slot, prob);
+        search(ch.row, sh, ch.lim, st, true, false, slot, prob);
         cut = st.cut;
     }
     if (ch.lim.min_key > cut.least) cut = Cut{ch.lim.min_key, ~0u};
@@ -889,10 +909,10 @@ template <typename T>
 static hipError_t sample(const SampleArgs &a, hipStream_t s) {
     const size_t lds = sizeof(LongShared), unlisted = offsetof(LongShared, list);
     const uint32_t grid_rows = a.rows < 65536u ? a.rows : 65536u;
-    if (few_waves(a.rows, a.n)) return launch(k_sample<T, 4>, grid_rows, 256, sizeof(SampleShared<4>), s, a);
+    if (few_waves(a.rows, a.n)) return launch(k_sample<T, 4, kShortListed>, grid_rows, 256, sizeof(SampleShared<4, kShortListed>), s, a);
     if (!splits(a.rows, a.n)) {
-        if (const hipError_t e = allow_lds(reinterpret_cast<const void *>(k_sample<T, kSampleWaves>), lds); e != hipSuccess) return e;
-        return launch(k_sample<T, kSampleWaves>, grid_rows, kSampleThreads, lds, s, a);
+        if (const hipError_t e = allow_lds(reinterpret_cast<const void *>(k_sample<T, kSampleWaves, kListed>), lds); e != hipSuccess) return e;
+        return launch(k_sample<T, kSampleWaves, kListed>, grid_rows, kSampleThreads, lds, s, a);
     }
     const Split split = split_of(a.rows, a.n);
     const SplitArgs x{reinterpret_cast<SampleSplit *>(a.ws), reinterpret_cast<uint64_t *>(a.ws + split.masses), reinterpret_cast<Cut *>(a.ws + split.cuts),
