@@ -513,6 +513,17 @@ __device__ __forceinline__ uint32_t list_from(State &st, const Limits &lim) {
     return lim.min_key;
 }
 
+// Gathers what is in the bin, or, of few slots down to it, those from there up; where there are few.
+template <typename T, int W, uint32_t MOST>
+__device__ __forceinline__ bool list_bin(const SampleRow<T> &row, SampleShared<W, MOST> &sh, State &st, const Limits &lim, uint32_t down) {
+    if (down > sh.kMost && st.s.count > sh.kMost) return false;
+    st.bin_only = down > sh.kMost;
+    const uint32_t from = list_from(st, lim), upto = st.bin_only ? st.s.hi : row.most;
+    st.n = from > upto ? 0 : list_slots(row, sh, 0, row.n, st.cut, from, upto);
+    st.listed = true;
+    return true;
+}
+
 // The searches that are left, to the draw, or (to_cut) to the end of the one that st is in, or (to_list) to where the slots that can still be drawn
 // are listed: then false.
 template <typename T, int W, uint32_t MOST>
@@ -541,11 +552,7 @@ __device__ __forceinline__ bool search(const SampleRow<T> &row, SampleShared<W, 
             }
             to_bin(row, sh, st, bin);
             const uint32_t down = first ? slots_down_to(row, sh, st, lim, bin, count) : uint32_t(min(st.s.before + st.s.count, uint64_t(~0u)));
-            if (down <= sh.kMost || st.s.count <= sh.kMost) {
-                st.bin_only = down > sh.kMost;
-                const uint32_t from = list_from(st, lim), upto = st.bin_only ? st.s.hi : row.most;
-                st.n = from > upto ? 0 : list_slots(row, sh, 0, row.n, st.cut, from, upto);
-                st.listed = true;
+            if (list_bin(row, sh, st, lim, down)) {
                 if (to_list && !st.bin_only) return false;
             }
             continue;
@@ -635,17 +642,17 @@ __global__ __launch_bounds__(64 * W) void k_sample(SampleArgs p) {
 //   max     the best score of each chunk
 //   bins    the first histogram, added up over the row's chunks; where nothing limits the row, the mass of each part of a chunk
 //   list    few slots down to the bin it leaves: gathered.  Many: the bin's own histogram.  Where nothing limits the row, the draw.
-//   narrow  the rest of the search among the gathered slots, by the first chunk; or the slots of the second histogram's bin.  (top-k that
-//           leaves many and top-p together: the first chunk takes the row alone.)
-//   mass    the threshold from the slots of that bin, by each chunk for itself; what stays in the chunk
-//   draw    from those masses, by the first chunk
+//   narrow  the rest of the search among the gathered slots, by the first chunk; or, where the second histogram was made, its bin's slots
+//   mass    the threshold from the slots of that bin, by each chunk for itself; what stays in the chunk.  Where that was top-k's and top-p follows,
+//           top-p's first histogram
+//   draw    from those masses, by the first chunk; or the rest of top-p's search (ten million, top-k 20000 and top-p 0.9: 3.3 of 3.4 ms)
 // A kernel's chunks add to what lies in the workspace with whole numbers, so that their order does not show.  What they hand on passes from
 // kernel to kernel: handing it to the last chunk to finish, within one, takes a write-back of the XCD's cache a chunk, which made
 // 256 rows of 100K take 448 us in one kernel where a launch takes 2.
 struct SampleSplit {
     // zeroed by the first kernel
-    uint64_t mass[2][LongShared::kBins];
-    uint32_t count[2][LongShared::kBins];
+    uint64_t mass[3][LongShared::kBins];
+    uint32_t count[3][LongShared::kBins];
     uint32_t listed, state;
     Cut cut;
     uint64_t list[kListed];
@@ -693,7 +700,17 @@ struct Chunk {
         return st;
     }
     __device__ __forceinline__ bool limited() const { return lim.limit_k || lim.limit_p; }
+    __device__ __forceinline__ bool both() const { return lim.limit_k && lim.limit_p; }
 };
+// Top-p's search after top-k's cut.
+template <typename T>
+__device__ __forceinline__ State second_state(const Chunk<T> &ch, const Cut &cut) {
+    State st = first_state(ch.row, ch.lim);
+    st.phase = kTopP;
+    st.cut = cut;
+    st.s.lo = cut.least;
+    return st;
+}
 
 template <typename T>
 __device__ __forceinline__ void add_bins(const Chunk<T> &ch, LongShared &sh, int which, bool with_mass) {
@@ -800,7 +817,6 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_list(SampleArgs p, Sp
     uint32_t down;
     State st = ch.first_bin(sh, down);
     if (down <= kListed) return add_slots(ch, sh, list_from(st, ch.lim), ch.most);
-    if (ch.lim.limit_k && ch.lim.limit_p) return;
     if (st.s.count <= kListed) return add_slots(ch, sh, st.s.lo, st.s.hi);
     fill(ch.row, sh, false, ch.from, ch.to, st.cut, st.s, Pass{kByDistance, by_mass(st.phase), false});
     add_bins(ch, sh, 1, by_mass(st.phase));
@@ -827,9 +843,6 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_narrow(SampleArgs p, 
         float prob;
         search(ch.row, few, ch.lim, st, false, false, slot, prob);
         return ch.write(p, slot, prob);
-    } else if (ch.lim.limit_k && ch.lim.limit_p) {
-        if (ch.c != 0) return;
-        st = first_state(ch.row, ch.lim);
     } else {
         if (st.s.count <= kListed) return;
         to_bin(ch.row, sh, st, pick(sh, st, ch.lim, ch.ws->count[1][threadIdx.x], ch.ws->mass[1][threadIdx.x]));
@@ -863,8 +876,15 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_mass(SampleArgs p, Sp
         search(ch.row, sh, ch.lim, st, true, false, slot, prob);
         cut = st.cut;
     }
-    if (ch.lim.min_key > cut.least) cut = Cut{ch.lim.min_key, ~0u};
-    put_masses(x, ch, cut);
+    if (ch.both()) {
+        // top-p's first histogram, of what top-k leaves
+        const State after = second_state(ch, cut);
+        fill(ch.row, sh, false, ch.from, ch.to, cut, after.s, Pass{kFirst, true, false});
+        add_bins(ch, sh, 2, true);
+    } else {
+        if (ch.lim.min_key > cut.least) cut = Cut{ch.lim.min_key, ~0u};
+        put_masses(x, ch, cut);
+    }
     if (threadIdx.x == 0) x.chunk_cut[size_t(ch.r) * x.chunks + ch.c] = cut;
 }
 template <typename T>
@@ -873,8 +893,17 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_draw(SampleArgs p, Sp
     LongShared &sh = *reinterpret_cast<LongShared *>(smem);
     Chunk<T> ch(p, x);
     if (uniform(ch.ws->state) == kRowDone || !ch.open(p, x, sh, false)) return;
-    const Cut cut = x.chunk_cut[size_t(ch.r) * x.chunks];
-    draw_by_parts(p, x, ch, sh, Cut{uniform(cut.least), uniform(cut.tie_last)});
+    Cut cut = x.chunk_cut[size_t(ch.r) * x.chunks];
+    cut = Cut{uniform(cut.least), uniform(cut.tie_last)};
+    if (!ch.both()) return draw_by_parts(p, x, ch, sh, cut);
+    State st = second_state(ch, cut);
+    const uint32_t count = ch.ws->count[2][threadIdx.x], bin = pick(sh, st, ch.lim, count, ch.ws->mass[2][threadIdx.x]);
+    to_bin(ch.row, sh, st, bin);
+    list_bin(ch.row, sh, st, ch.lim, slots_down_to(ch.row, sh, st, ch.lim, bin, count));
+    int64_t slot;
+    float prob;
+    search(ch.row, sh, ch.lim, st, false, false, slot, prob);
+    ch.write(p, slot, prob);
 }
 
 // Rows of more slots than this go in chunks, as long as there are no more than kSplitRows of them.
@@ -929,7 +958,7 @@ static hipError_t sample(const SampleArgs &a, hipStream_t s) {
     if (a.top_k == nullptr && a.top_p == nullptr && a.temperature == nullptr) return hipSuccess;      // nothing limits any row
     if (const hipError_t e = go(k_sample_narrow<T>, grid, lds); e != hipSuccess) return e;
     if (const hipError_t e = go(k_sample_mass<T>, grid, lds); e != hipSuccess) return e;
-    return go(k_sample_draw<T>, dim3(a.rows), unlisted);
+    return go(k_sample_draw<T>, dim3(a.rows), lds);
 }
 hipError_t launch_sample(const SampleArgs &a, int score_type, hipStream_t s) {
     if (score_type == kF32) return sample<float>(a, s);
