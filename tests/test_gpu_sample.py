@@ -20,8 +20,8 @@ def gen(seed):
 
 
 def plain_row(s, u, t, k, p, m, allowed):
-    """(slot, probability) of one row; s float64.  Weights are multiples of 2^-(63 - ceil(log2 n)): one below half of that is
-    never drawn, not even by u = 0."""
+    """(slot, probability) of one row; s float64.  Weights are whole multiples of 2^-(63 - ceil(log2 n)), rounded down: one below
+    that is never drawn, not even by u = 0."""
     unit = 2.0 ** -(63 - max(1, int(len(s) - 1).bit_length()))
     s = np.where(allowed & ~np.isnan(s), s, -np.inf)
     if np.all(s == -np.inf):
@@ -36,14 +36,14 @@ def plain_row(s, u, t, k, p, m, allowed):
     if k > 0:
         order = order[:k]
     if p < 1:
-        mass = np.cumsum(np.rint(w[order] / unit) * unit)
+        mass = np.cumsum(np.floor(w[order] / unit) * unit)
         stays = np.concatenate(([0.0], mass[:-1])) < p * mass[-1]
         stays[0] = True
         order = order[stays]
     if m > 0:
         order = order[w[order] >= min(m, 1.0)]
     kept = np.sort(order)
-    mass = np.cumsum(np.rint(w[kept] / unit) * unit)
+    mass = np.cumsum(np.floor(w[kept] / unit) * unit)
     want = u * mass[-1]
     at = min(int(np.searchsorted(mass, want, side="right")), len(kept) - 1)
     return int(kept[at]), w[kept[at]] / mass[-1]
@@ -65,8 +65,9 @@ def check(sample, scores, u, mask=None, **params):
         allowed = bits(mask if mask is None or mask.dim() == 1 else mask[r], n)
         slot, prob = plain_row(host[r], float(u[r]), value("temperature", r, 1.0), int(value("top_k", r, 0)), value("top_p", r, 1.0), value("min_p", r, 0.0), allowed)
         assert int(slots[r]) == slot, (r, int(slots[r]), slot)
-        # weights are rounded to multiples of 2^-(63 - ceil(log2 n)), at most half of one each against a sum of at least 1; the quotient once to 32 bits
-        assert abs(float(probs[r]) - prob) <= prob * (2.0 ** -24 + n * 2.0 ** -(62 - int(n - 1).bit_length()) + 1e-12) + 2.0 ** -149, (r, float(probs[r]), prob)
+        # weights lose less than 2^-(63 - ceil(log2 n)) each against a sum of at least 1, and are off by their series' first term left out,
+        # (ln 2 / 2)^10 / 10! = 6.9e-12 against 2^-1/2 at least; the quotient is rounded once to 32 bits
+        assert abs(float(probs[r]) - prob) <= prob * (2.0 ** -24 + n * 2.0 ** -(63 - int(n - 1).bit_length()) + 1e-11) + 2.0 ** -149, (r, float(probs[r]), prob)
     return slots, probs
 
 
@@ -94,6 +95,93 @@ def test_long_rows(sample, n, rows):
         u = torch.rand(rows, generator=gen(6), device="cuda")
         for limits in (dict(), dict(top_k=40), dict(top_k=60_000), dict(top_p=0.9), dict(top_k=5000, top_p=0.7, min_p=0.01), dict(temperature=0.2, top_p=0.95)):
             check(sample, scores, u, **limits)
+
+
+@pytest.mark.parametrize("rows,n", [(2, 6144), (2, 6145), (257, 6145), (2, 16384), (2, 16385), (128, 16385), (129, 16385), (257, 16448), (257, 16449)])
+def test_where_the_forms_meet(sample, rows, n):
+    """Sizes on both sides of where a row gets more waves, or is cut into chunks."""
+    for dtype in (torch.float32, torch.bfloat16):
+        scores = (3 * torch.randn(rows, n, generator=gen(rows), device="cuda")).to(dtype)
+        u = torch.rand(rows, generator=gen(n), device="cuda")
+        k = torch.randint(0, 6000, (rows,), generator=gen(n + 1), device="cuda", dtype=torch.int32)
+        k[::3] = 0
+        t = 0.3 + torch.rand(rows, generator=gen(n + 2), device="cuda")
+        check(sample, scores, u)
+        check(sample, scores, u, temperature=t, top_k=k, top_p=0.9, min_p=1e-4)
+
+
+@pytest.mark.parametrize("rows,n", [(1, 20_000), (1, 250_000), (3, 100_000), (140, 12_000), (140, 30_000), (600, 30_000)])
+def test_thousands_stay(sample, rows, n):
+    """Limits that leave more slots than are gathered: by number, by mass, by both, and by min-p."""
+    scores = 2 * torch.randn(rows, n, generator=gen(rows + n), device="cuda")
+    u = torch.rand(rows, generator=gen(n), device="cuda")
+    some = torch.arange(0, rows, 15 if rows > 40 else 1, device="cuda")
+    for limits in (dict(top_k=n // 2), dict(top_p=0.97, temperature=4.0), dict(top_k=n - 1, top_p=0.8, temperature=9.0), dict(top_k=5000, top_p=0.999, temperature=5.0, min_p=0.3),
+                   dict(top_p=0.9, min_p=0.02, temperature=2.0), dict(min_p=0.01, temperature=1e4)):
+        slots, probs = sample(scores, u, **limits)
+        check(lambda *a, **b: (slots[some], probs[some]), scores[some], u[some], **limits)
+
+
+@pytest.mark.parametrize("rows,n", [(1, 50_000), (2, 300_000), (150, 20_000)])
+def test_crowded_scores(sample, rows, n):
+    """Thousands of equal scores at the threshold, scores that differ in their last bits, that cross zero, that are subnormal, and one far above the others."""
+    g = gen(rows)
+    base = torch.randn(rows, n, generator=g, device="cuda")
+    cases = [(0.5 * torch.round(2 * base), 1.0),                                   # about 20 values
+             (1.0 + 2.0 ** -23 * torch.randint(0, 50, (rows, n), generator=g, device="cuda"), 1e-6),
+             (1e-3 * base, 1e-3),
+             (1e-41 * torch.randint(-500, 500, (rows, n), generator=g, device="cuda"), 1e-39),
+             (torch.where(torch.arange(n, device="cuda") == n // 3, 1e6, base), 3e4)]
+    u = torch.rand(rows, generator=g, device="cuda")
+    some = torch.arange(0, rows, 50, device="cuda")
+    for scores, t in cases:
+        for limits in (dict(top_p=0.5), dict(top_k=n // 3), dict(top_k=6000, top_p=0.9), dict(top_k=100, top_p=0.999), dict(min_p=0.5, top_p=0.7)):
+            slots, probs = sample(scores, u, temperature=t, **limits)
+            check(lambda *a, **b: (slots[some], probs[some]), scores[some], u[some], temperature=t, **limits)
+
+
+def test_long_rows_with_masks(sample):
+    n, rows = 90_001, 5
+    g = gen(50)
+    scores = 3 * torch.randn(rows, n, generator=g, device="cuda")
+    scores[1, 100:80_000] = float("nan")
+    scores[2, 7] = scores[2, 70_000] = float("inf")
+    scores[3] = -float("inf")
+    words = -(-n // 64)
+    half = torch.randint(-2 ** 63, 2 ** 63 - 1, (rows, words), generator=g, device="cuda", dtype=torch.int64)
+    half[4] = 0
+    half[4, -1] = -1 << (n % 64)                     # only bits past the row's end
+    u = torch.rand(rows, generator=g, device="cuda")
+    for mask in (half, half[0], half[4]):
+        for limits in (dict(), dict(top_k=50, top_p=0.9), dict(top_p=0.95, temperature=2.0), dict(top_k=20_000, top_p=0.5), dict(temperature=0.0), dict(min_p=0.2)):
+            check(sample, scores, u, mask=mask, **limits)
+
+
+def test_draws_by_two_threads(sample):
+    """Calls at once, each thread on a stream of its own: each gives what it gives alone."""
+    import threading
+    sets = []
+    for i, (rows, n) in enumerate(((3, 60_000), (200, 3000))):
+        scores = 3 * torch.randn(rows, n, generator=gen(60 + i), device="cuda")
+        u = torch.rand(rows, generator=gen(70 + i), device="cuda")
+        sets.append((scores, u, sample(scores, u, top_k=100, top_p=0.9)))
+    torch.cuda.synchronize()
+    same = [0, 0]
+
+    def work(i):
+        scores, u, want = sets[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = sample(scores, u, top_k=100, top_p=0.9)
+                torch.cuda.current_stream().synchronize()
+                same[i] += all(torch.equal(x, y) for x, y in zip(got, want))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert same == [20, 20]
 
 
 def test_many_rows(sample):
