@@ -586,6 +586,7 @@ static hipError_t tile(const MatmulArgs &a, hipStream_t s) {
     const uint64_t grid = by_n ? (uint64_t(nt) + 7) / 8 * 8 * mt : (uint64_t(mt) + 7) / 8 * 8 * nt;
     // 16 bytes at a time past the registers: rows at multiples of 16 bytes, and a tile's offsets in 32 bits
     const bool direct16 = ((uintptr_t(a.a.codes) | uintptr_t(a.b.codes) | a.a.stride | a.b.stride) & 15) == 0 && a.a.stride < (1u << 23) && a.b.stride < (1u << 23);
+    if ((grid * (64 * WM * WN)) >> 32) return hipErrorInvalidConfiguration;      // (a result of 130 GB, or a narrow one of a billion columns)
     const size_t size = EXACT ? 4 : 2;
     const bool wide = ((uintptr_t(a.out) | a.out_stride * size) & 15) == 0;
     const auto kernel = k_fp8_tile<EXACT, SC, TM, TN, WM, WN>;

@@ -92,6 +92,28 @@ struct SampleRow {
             i += step;
         }
     }
+    // The same, four loads at a time, for a pass that does little with a score: one load at a time it waits for each.
+    template <typename F>
+    __device__ __forceinline__ void scan(uint32_t lo, uint32_t hi, uint32_t worker, uint32_t workers, F &&f) const {
+        const uint32_t step = workers * kEach;
+        uint32_t i = lo + worker * kEach;
+        for (; i < hi && hi - i >= 3u * step + kEach; i += 4u * step) {
+            Load l[4];
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                l[a].bits = mask == nullptr ? ~0u : uint32_t(mask[(i + a * step) >> 6] >> ((i + a * step) & 63u));
+                __builtin_memcpy(l[a].v, scores + i + a * step, 16);
+            }
+#pragma unroll
+            for (int a = 0; a < 4; ++a)
+#pragma unroll
+                for (int j = 0; j < kEach; ++j) {
+                    const float v = float(l[a].v[j]);
+                    f(i + a * step + j, v, ((l[a].bits >> j) & 1u) != 0u && v > -__int_as_float(0x7f800000));
+                }
+        }
+        each(i, hi, 0, workers, f);
+    }
     // exp((score - max) / T); for scores whose largest is +infinity, 1 for those that have it
     __device__ __forceinline__ double weight(uint32_t k) const { return k == most ? 1.0 : exp((double(key_score(k)) - top) * inverse); }
     // The same in whole units of 2^-shift, which is what sums are made of: 2^y = 2^e * 2^f, |f| <= 1/2, with the exponential series up to
@@ -376,7 +398,7 @@ __device__ __forceinline__ uint32_t list_slots(const SampleRow<T> &row, SampleSh
     __syncthreads();
     const CutScores scores(cut);
     const float least = key_score(from), most = key_score(upto);
-    row.each(lo, hi, threadIdx.x, sh.kThreads, [&](uint32_t i, float v, bool in) {
+    row.scan(lo, hi, threadIdx.x, sh.kThreads, [&](uint32_t i, float v, bool in) {
         if (!in || v < least || v > most || !scores.leaves(i, v)) return;
         const uint32_t at = atomicAdd(&sh.listed, 1u);
         if (at < sh.kMost) sh.list[at] = uint64_t(score_key(v)) << 32 | uint32_t(~i);
@@ -612,7 +634,7 @@ __global__ __launch_bounds__(64 * W) void k_sample(SampleArgs p) {
         Limits lim;
         lim.load(p, r);
         float best = -__int_as_float(0x7f800000);
-        row.each(0, p.n, threadIdx.x, sh.kThreads, [&](uint32_t, float v, bool in) {
+        row.scan(0, p.n, threadIdx.x, sh.kThreads, [&](uint32_t, float v, bool in) {
             if (in) best = fmaxf(best, v);
         });
         const uint32_t most = block_max(score_key(best), sh);
@@ -779,7 +801,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_max(SampleArgs p, Spl
     const Chunk<T> ch(p, x);
     for (uint32_t i = ch.c * kSampleThreads + threadIdx.x; i < kSplitZeroed; i += x.chunks * kSampleThreads) reinterpret_cast<uint32_t *>(ch.ws)[i] = 0;
     float best = -__int_as_float(0x7f800000);
-    ch.row.each(ch.from, ch.to, threadIdx.x, kSampleThreads, [&](uint32_t, float v, bool in) {
+    ch.row.scan(ch.from, ch.to, threadIdx.x, kSampleThreads, [&](uint32_t, float v, bool in) {
         if (in) best = fmaxf(best, v);
     });
     const uint32_t most = block_max(score_key(best), sh);
