@@ -16,6 +16,9 @@ def _a_row(name, value, rows, dtype, device):
         return None
     if not isinstance(value, torch.Tensor):
         return torch.full((rows,), value, dtype=dtype, device=device)
+    if value.dtype is dtype and value.shape == (rows,) and value.device == device and value.is_contiguous():
+        return value
+    # (what is wrong with it)
     _gpu(name, value, (dtype,), ndim=1)
     if len(value) != rows:
         raise ValueError(f"{name} must have a value a row, {rows}, got {len(value)}")
