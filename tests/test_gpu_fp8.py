@@ -296,6 +296,16 @@ def test_rescore_many_candidates(fp8, m, k):
     check_best(fp8, q, rows, torch.randint(0, 20000, (2, m), generator=gen(42), device="cuda"), k)
 
 
+@pytest.mark.parametrize("nq,m", [(1, 128), (1, 129), (127, 129), (128, 129), (128, 256), (128, 257), (256, 40), (257, 40), (257, 256), (300, 257)])
+@pytest.mark.parametrize("dim", [96, 2000])
+def test_rescore_where_the_forms_meet(fp8, nq, m, dim):
+    """Numbers of queries and candidates on both sides of where a call takes two launches, and a query fewer waves."""
+    rows = fp8.quantize(torch.randn(700, dim, generator=gen(51), device="cuda"))
+    q = torch.randn(nq, dim, generator=gen(52), device="cuda")
+    slots = torch.randint(-3, 703, (nq, m), generator=gen(53), device="cuda")
+    check_best(fp8, q, rows, slots, min(m, 30))
+
+
 @pytest.mark.parametrize("dim,pad,offset", [(256, 257, 0), (200, 201, 3), (16384, 16384, 0), (10000, 10000, 0)])
 def test_rescore_odd_places_and_long_rows(fp8, dim, pad, offset):
     rows = stored(fp8, torch.randn(50, dim, generator=gen(43), device="cuda"), "e8m0", 1, pad, offset)

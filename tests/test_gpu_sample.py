@@ -97,7 +97,7 @@ def test_long_rows(sample, n, rows):
             check(sample, scores, u, **limits)
 
 
-@pytest.mark.parametrize("rows,n", [(2, 6144), (2, 6145), (257, 6145), (2, 16384), (2, 16385), (128, 16385), (129, 16385), (257, 16448), (257, 16449)])
+@pytest.mark.parametrize("rows,n", [(2, 6144), (2, 6145), (257, 6145), (2, 16384), (2, 16385), (128, 16385), (129, 16385), (2, 40960), (2, 40961), (128, 40961), (129, 40961), (257, 16448), (257, 16449)])
 def test_where_the_forms_meet(sample, rows, n):
     """Sizes on both sides of where a row gets more waves, or is cut into chunks."""
     for dtype in (torch.float32, torch.bfloat16):
