@@ -72,7 +72,7 @@ def check(sample, scores, u, mask=None, **params):
 
 
 LIMITS = [dict(), dict(top_k=1), dict(top_k=7), dict(top_k=1000), dict(top_p=0.5), dict(top_p=0.99), dict(min_p=0.1), dict(top_k=50, top_p=0.9),
-          dict(top_k=50, top_p=0.9, min_p=0.05), dict(temperature=0.1), dict(temperature=3.0, top_p=0.3), dict(temperature=0.0), dict(top_p=1e-6), dict(top_p=0.0),
+          dict(top_k=50, top_p=0.9, min_p=0.05), dict(temperature=0.1), dict(temperature=3.0, top_p=0.3), dict(temperature=0.0), dict(top_p=1e-6), dict(top_p=0.0), dict(top_p=-0.5), dict(top_p=-float("inf")),
           dict(min_p=1.0), dict(min_p=5.0), dict(top_k=-3), dict(top_p=2.0), dict(temperature=float("inf"), top_k=30)]
 
 
@@ -184,6 +184,11 @@ def test_draws_by_two_threads(sample):
     assert same == [20, 20]
 
 
+def test_no_rows(sample):
+    slots, probs = sample(torch.empty(0, 100_000, device="cuda"), torch.empty(0, device="cuda"), top_k=5)
+    assert slots.shape == probs.shape == (0,)
+
+
 def test_many_rows(sample):
     scores = torch.randn(700, 1500, generator=gen(8), device="cuda")
     u = torch.rand(700, generator=gen(9), device="cuda")
@@ -203,6 +208,28 @@ def test_ties(sample, n):
     for scores in (few, same, signs, -1e30 * few):
         for limits in (dict(), dict(top_k=5), dict(top_k=n // 2 + 1), dict(top_p=0.5), dict(top_p=0.25, top_k=n - 1), dict(min_p=1.0), dict(temperature=0.0)):
             check(sample, scores, u, **limits)
+
+
+@pytest.mark.parametrize("rows,n", [(1, 1000), (1, 10_000), (200, 10_000), (2, 200_000)])
+def test_min_p_above_the_slot_that_top_p_ends_at(sample, rows, n):
+    """Top-p ends at a slot that is alone between its neighbours, and min-p lies closely above it: one slot is left, whatever an
+    earlier call found in that place."""
+    u = torch.rand(rows, generator=gen(80), device="cuda")
+    for far in (-20.0, -1.3):
+        scores = torch.full((rows, n), far, device="cuda")
+        scores[:, n // 2] = 0.0
+        scores[:, n // 3] = -1.01                      # weight 0.3642
+        if far == -1.3:
+            scores[:, :n // 4] = scores[:, n - n // 4:] = -30.0
+            scores[:, n // 4:n // 3] = -30.0
+            scores[:, n // 3 + 1:n // 3 + 3] = -1.3
+            scores[:, n // 3 + 3:n // 2] = scores[:, n // 2 + 1:n - n // 4] = -30.0
+        for before in (5.0, 90.0, -0.4):
+            other = torch.full((rows, n), before - 60.0, device="cuda")
+            other[:, 5], other[:, 9] = before, before - 0.3
+            check(sample, other, u, top_p=0.8)
+            slots, probs = check(sample, scores, u, top_p=0.6 if far == -1.3 else 0.9, min_p=0.36604)
+            assert slots.tolist() == [n // 2] * rows and probs.tolist() == [1.0] * rows
 
 
 def test_masked_and_not_numbers(sample):

@@ -70,6 +70,7 @@ def test_no_rows_do_nothing():
     assert rescore(k=0) == T.OK
     assert rescore(m=0, k=0, slots=None) == T.OK
     assert sample(rows=0, scores=None) == T.OK
+    assert T.lib().tv_sample_workspace(0, 1 << 20) == 0 and T.lib().tv_fp8_rescore_workspace(0, 1000, 256) == 0
 
 
 @pytest.mark.skipif(torch.cuda.is_available(), reason="what a call says where there is no GPU")

@@ -377,7 +377,7 @@ __device__ __forceinline__ uint32_t pick(SampleShared<W, MOST> &sh, State &st, c
         upto = mass_before = st.s.mass_before + block_before(mass, sh, all);
         if (st.whole) {
             st.total = all;
-            st.bound = uniform(st.phase == kTopP ? uint64_t(ceil(double(lim.top_p) * double(all))) : drawn_mass(lim.u, all) + 1);
+            st.bound = uniform(st.phase == kTopP ? uint64_t(ceil(fmax(double(lim.top_p), 0.0) * double(all))) : drawn_mass(lim.u, all) + 1);
         }
     }
     if (count != 0 && (before == 0 || upto < st.bound)) atomicMax(&sh.picked, t);
@@ -408,9 +408,11 @@ __device__ __forceinline__ uint32_t list_slots(const SampleRow<T> &row, SampleSh
     __syncthreads();
     return uniform(min(sh.listed, sh.kMost));
 }
-// The one value in s of the list's slots that count.
+// The one value in s of the list's slots that count; where min-p has kept it out of the list, the least that would be there.
 template <int W, uint32_t MOST>
 __device__ __forceinline__ uint32_t only_value(SampleShared<W, MOST> &sh, const State &st) {
+    if (threadIdx.x == 0) sh.found_value = st.s.lo;
+    __syncthreads();
     for (uint32_t e = threadIdx.x; e < st.n; e += sh.kThreads) {
         const uint32_t k = uint32_t(sh.list[e] >> 32), place = uint32_t(sh.list[e]), v = st.phase >= kTies ? place : k;
         const bool stays = k > st.cut.least || (k == st.cut.least && ~place <= st.cut.tie_last);
@@ -952,7 +954,7 @@ static Split split_of(size_t rows, size_t n) {
     x.bytes = x.mosts + rows * x.chunks * 4;
     return x;
 }
-static bool splits(size_t rows, size_t n) { return n > kSplitSlots && rows <= kSplitRows; }
+static bool splits(size_t rows, size_t n) { return n > kSplitSlots && rows != 0 && rows <= kSplitRows; }
 size_t sample_workspace(size_t rows, size_t n) { return splits(rows, n) ? split_of(rows, n).bytes : 0; }
 
 // A row for four waves: a short one, whose time goes into the steps that the workgroup waits in between (one row, top-k 50 and top-p 0.9: 100
