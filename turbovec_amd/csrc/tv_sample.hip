@@ -140,8 +140,12 @@ struct SampleRow {
     }
     // How far a score lies below the best, as the bits of that distance: a number that rises with it.
     __device__ __forceinline__ uint32_t distance(float v) const { return v == best ? 0u : __float_as_uint(best - v); }
-    // The least key no further than d (keys rise as distances fall): every lane of a wave tries one of 64 places, until a step is one key.
+    // The least key no further than d (keys rise as distances fall): among the 64 around best - d, a lane each; where rounding has put it further
+    // away, every lane tries one of 64 places, until a step is one key.
     __device__ __forceinline__ uint32_t least_within(uint32_t d) const {
+        const uint32_t base = min(max(score_key(best - __uint_as_float(d)) - 32u, kNoKey + 1u), most);
+        const uint64_t near = uniform(uint64_t(__ballot(distance(key_score(min(base + (threadIdx.x & 63u), most))) <= d)));
+        if (near != 0ull && ((near & 1u) == 0u || base == kNoKey + 1u)) return base + uint32_t(__builtin_ctzll(near));
         uint32_t lo = kNoKey + 1u, left = most - lo;           // it is one of lo .. lo + left
         while (left != 0u) {
             const uint32_t step = left / 64u + 1u, mine = lo + min(left, (threadIdx.x & 63u) * step);
@@ -181,8 +185,13 @@ __device__ __forceinline__ uint64_t plus_moved(uint64_t v) {
     const uint32_t hi = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(v >> 32)), CTRL, ROWS, 0xf, false));
     return v + (uint64_t(hi) << 32 | lo);
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t plus_moved(uint32_t v) {
+    return v + uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CTRL, ROWS, 0xf, false));
+}
 // The sum over the lanes up to this one (all 64 active): within rows of 16, then the row ends handed on.
-__device__ __forceinline__ uint64_t wave_upto(uint64_t v) {
+template <typename N>
+__device__ __forceinline__ N wave_upto(N v) {
     v = plus_moved<0x111, 0xf>(v);      // row_shr 1, 2, 4, 8
     v = plus_moved<0x112, 0xf>(v);
     v = plus_moved<0x114, 0xf>(v);
@@ -200,7 +209,7 @@ struct SampleShared {
     static constexpr uint32_t kThreads = 64 * W, kBins = kThreads, kBits = W == 16 ? 10 : W == 4 ? 8 : 0, kMost = MOST;
     static_assert(kBins == 1u << kBits, "a bin to a thread");
     uint64_t part[W], found_mass;
-    uint32_t part32[W], listed, picked, found_count, found_before, found_value;
+    uint32_t part32[W], listed, picked, found_count, found_before, found_down, found_value;
     uint32_t count[kBins * kCopies];
     uint64_t mass[kBins * kCopies];
     uint64_t list[kMost];         // key, complement of the slot.  (Last: kernels that list nothing leave it out.)
@@ -365,30 +374,46 @@ struct State {
 };
 __device__ __forceinline__ bool by_mass(int phase) { return phase == kTopP || phase == kDraw; }
 
-// Of the bins, a thread each, the last that has slots and that less than the bound lies before; the first one always.
+// Of the bins, a thread each, the last that has slots and that less than the bound lies before; the first one always.  `down`: the slots down to
+// it, or to the bin `cap` if that comes before.
 template <int W, uint32_t MOST>
-__device__ __forceinline__ uint32_t pick(SampleShared<W, MOST> &sh, State &st, const Limits &lim, uint32_t count, uint64_t mass) {
-    const uint32_t t = threadIdx.x;
+__device__ __forceinline__ uint32_t pick(SampleShared<W, MOST> &sh, State &st, const Limits &lim, uint32_t count, uint64_t mass, uint32_t cap, uint32_t &down) {
+    const uint32_t t = threadIdx.x, wave = t >> 6;
+    const bool masses = by_mass(st.phase);
+    const uint32_t counts = wave_upto(count);
+    const uint64_t sums = masses ? wave_upto(mass) : 0;
+    __syncthreads();
     if (t == 0) sh.picked = 0;
-    uint64_t all;
-    const uint64_t before = st.s.before + block_before(count, sh, all);
-    uint64_t upto = before, mass_before = 0;
-    if (by_mass(st.phase)) {
-        upto = mass_before = st.s.mass_before + block_before(mass, sh, all);
+    if ((t & 63u) == 63u) { sh.part32[wave] = counts; sh.part[wave] = sums; }
+    __syncthreads();
+    uint32_t before = counts - count;
+    for (uint32_t w = 0; w < wave; ++w) before += sh.part32[w];
+    uint64_t upto = st.s.before + before, mass_before = 0;
+    if (masses) {
+        uint64_t all = 0;
+        mass_before = st.s.mass_before + sums - mass;
+        for (uint32_t w = 0; w < uint32_t(W); ++w) {
+            const uint64_t x = sh.part[w];
+            mass_before += w < wave ? x : 0;
+            all += x;
+        }
+        upto = mass_before;
         if (st.whole) {
-            st.total = all;
+            st.total = all = uniform(all);
             st.bound = uniform(st.phase == kTopP ? uint64_t(ceil(fmax(double(lim.top_p), 0.0) * double(all))) : drawn_mass(lim.u, all) + 1);
         }
     }
-    if (count != 0 && (before == 0 || upto < st.bound)) atomicMax(&sh.picked, t);
+    if (count != 0 && (st.s.before + before == 0 || upto < st.bound)) atomicMax(&sh.picked, t);
     __syncthreads();
     const uint32_t bin = uniform(sh.picked);
-    if (t == bin) { sh.found_count = count; sh.found_before = uint32_t(before); sh.found_mass = mass_before; }
+    if (t == bin) { sh.found_count = count; sh.found_before = uint32_t(st.s.before) + before; sh.found_mass = mass_before; }
+    if (t == min(bin, cap)) sh.found_down = uint32_t(st.s.before) + before + count;
     __syncthreads();
     st.s.count = uniform(sh.found_count);
     st.s.before = uniform(sh.found_before);
     st.s.mass_before = uniform(sh.found_mass);
     st.whole = false;
+    down = uniform(sh.found_down);
     return bin;
 }
 
@@ -525,11 +550,10 @@ __device__ __forceinline__ void to_bin(const SampleRow<T> &row, const SampleShar
     s.lo = max(st.cut.least, row.least_within(s.far));
     s.hi = s.near == 0 ? row.most : row.least_within(s.near - 1u) - 1u;
 }
-// Of the first histogram, the slots down to the picked bin that can still be drawn.  (Min-p leaves fewer, but top-p after top-k needs all of top-k's.)
+// The last bin of the first histogram that can matter for what is drawn.  (Min-p leaves fewer, but top-p after top-k needs all of top-k's.)
 template <typename T, int W, uint32_t MOST>
-__device__ __forceinline__ uint32_t slots_down_to(const SampleRow<T> &row, SampleShared<W, MOST> &sh, const State &st, const Limits &lim, uint32_t bin, uint32_t count) {
-    const uint32_t last = st.phase == kTopP ? min(bin, sh.bin(row.distance(key_score(lim.min_key)))) : bin;
-    return uint32_t(block_sum(threadIdx.x <= last ? count : 0, sh));
+__device__ __forceinline__ uint32_t last_bin(const SampleRow<T> &row, const SampleShared<W, MOST> &sh, const State &st, const Limits &lim) {
+    return st.phase == kTopP ? sh.bin(row.distance(key_score(lim.min_key))) : sh.kBins - 1;
 }
 // From which key on a row's slots are listed.  Where min-p leaves nothing of the bin, the search is over.
 __device__ __forceinline__ uint32_t list_from(State &st, const Limits &lim) {
@@ -569,7 +593,8 @@ __device__ __forceinline__ bool search(const SampleRow<T> &row, SampleShared<W, 
             uint32_t count;
             uint64_t mass;
             own_bin(sh, by_mass(st.phase), count, mass);
-            const uint32_t bin = pick(sh, st, lim, count, mass);
+            uint32_t down;
+            const uint32_t bin = pick(sh, st, lim, count, mass, first ? last_bin(row, sh, st, lim) : sh.kBins - 1, down);
             if (!distances) {
                 const uint32_t shift = sh.shift_of(st.s.hi - st.s.lo);
                 st.s.hi -= bin << shift;
@@ -577,7 +602,6 @@ __device__ __forceinline__ bool search(const SampleRow<T> &row, SampleShared<W, 
                 continue;
             }
             to_bin(row, sh, st, bin);
-            const uint32_t down = first ? slots_down_to(row, sh, st, lim, bin, count) : uint32_t(min(st.s.before + st.s.count, uint64_t(~0u)));
             if (list_bin(row, sh, st, lim, down)) {
                 if (to_list && !st.bin_only) return false;
             }
@@ -720,9 +744,8 @@ struct Chunk {
     // After the first histogram.
     __device__ __forceinline__ State first_bin(LongShared &sh, uint32_t &down) {
         State st = first_state(row, lim);
-        const uint32_t bin = pick(sh, st, lim, count, mass);
+        const uint32_t bin = pick(sh, st, lim, count, mass, last_bin(row, sh, st, lim), down);
         to_bin(row, sh, st, bin);
-        down = slots_down_to(row, sh, st, lim, bin, count);
         return st;
     }
     __device__ __forceinline__ bool limited() const { return lim.limit_k || lim.limit_p; }
@@ -871,7 +894,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_narrow(SampleArgs p, 
         return ch.write(p, slot, prob);
     } else {
         if (st.s.count <= kListed) return;
-        to_bin(ch.row, sh, st, pick(sh, st, ch.lim, ch.ws->count[1][threadIdx.x], ch.ws->mass[1][threadIdx.x]));
+        to_bin(ch.row, sh, st, pick(sh, st, ch.lim, ch.ws->count[1][threadIdx.x], ch.ws->mass[1][threadIdx.x], sh.kBins - 1, down));
         if (st.s.count <= kListed) return add_slots(ch, sh, st.s.lo, st.s.hi);
         // more than that with keys next to each other: one workgroup goes on
         if (ch.c != 0) return;
@@ -895,7 +918,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_mass(SampleArgs p, Sp
     if (state != kRowCut) {
         uint32_t down;
         State st = ch.first_bin(sh, down);
-        if (st.s.count > kListed) to_bin(ch.row, sh, st, pick(sh, st, ch.lim, ch.ws->count[1][threadIdx.x], ch.ws->mass[1][threadIdx.x]));
+        if (st.s.count > kListed) to_bin(ch.row, sh, st, pick(sh, st, ch.lim, ch.ws->count[1][threadIdx.x], ch.ws->mass[1][threadIdx.x], sh.kBins - 1, down));
         take_list(ch, sh, st);
         int64_t slot;
         float prob;
@@ -923,9 +946,10 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_draw(SampleArgs p, Sp
     cut = Cut{uniform(cut.least), uniform(cut.tie_last)};
     if (!ch.both()) return draw_by_parts(p, x, ch, sh, cut);
     State st = second_state(ch, cut);
-    const uint32_t count = ch.ws->count[2][threadIdx.x], bin = pick(sh, st, ch.lim, count, ch.ws->mass[2][threadIdx.x]);
+    uint32_t down;
+    const uint32_t bin = pick(sh, st, ch.lim, ch.ws->count[2][threadIdx.x], ch.ws->mass[2][threadIdx.x], last_bin(ch.row, sh, st, ch.lim), down);
     to_bin(ch.row, sh, st, bin);
-    list_bin(ch.row, sh, st, ch.lim, slots_down_to(ch.row, sh, st, ch.lim, bin, count));
+    list_bin(ch.row, sh, st, ch.lim, down);
     int64_t slot;
     float prob;
     search(ch.row, sh, ch.lim, st, false, false, slot, prob);
