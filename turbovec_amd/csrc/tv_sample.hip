@@ -799,19 +799,20 @@ __device__ __forceinline__ void put_masses(const SplitArgs &x, const Chunk<T> &c
 // The row's draw from those of its chunks.
 template <typename T>
 __device__ __forceinline__ void draw_by_parts(const SampleArgs &p, const SplitArgs &x, const Chunk<T> &ch, LongShared &sh, const Cut &cut) {
-    const uint32_t parts = x.chunks * kSampleWaves, part = x.chunk / kSampleWaves;
+    // (a thread to parts that follow each other)
+    const uint32_t parts = x.chunks * kSampleWaves, part = x.chunk / kSampleWaves, each = (parts + kSampleThreads - 1) / kSampleThreads;
     const uint64_t *const masses = x.part_mass + size_t(ch.r) * parts;
-    uint64_t sum = 0;
-    for (uint32_t i = threadIdx.x; i < parts; i += kSampleThreads) sum += masses[i];
-    const uint64_t total = block_sum(sum, sh);
-    uint64_t want = drawn_mass(ch.lim.u, total), before = 0;
+    uint32_t at_part = min(parts, threadIdx.x * each);
+    uint64_t sum = 0, total;
+    for (uint32_t i = at_part; i < min(parts, (threadIdx.x + 1u) * each); ++i) sum += masses[i];
+    uint64_t before = block_before(sum, sh, total);
+    uint64_t want = drawn_mass(ch.lim.u, total);
     if (threadIdx.x == 0) { sh.picked = 0; sh.found_mass = 0; }
-    for (uint32_t i = 0; i < parts; i += kSampleThreads) {
-        const uint64_t mine = i + threadIdx.x < parts ? masses[i + threadIdx.x] : 0;
-        uint64_t all;
-        const uint64_t upto = before + block_before(mine, sh, all);
-        if (upto <= want && upto + mine > want) { sh.picked = i + threadIdx.x; sh.found_mass = upto; }
-        before += all;
+    __syncthreads();
+    if (before <= want && before + sum > want) {
+        for (; before + masses[at_part] <= want; ++at_part) before += masses[at_part];
+        sh.picked = at_part;
+        sh.found_mass = before;
     }
     __syncthreads();
     const uint32_t lo = uniform(sh.picked) * part;
