@@ -699,12 +699,19 @@ __global__ __launch_bounds__(64 * W) void k_sample(SampleArgs p) {
 // A kernel's chunks add to what lies in the workspace with whole numbers, so that their order does not show.  What they hand on passes from
 // kernel to kernel: handing it to the last chunk to finish, within one, takes a write-back of the XCD's cache a chunk, which made
 // 256 rows of 100K take 448 us in one kernel where a launch takes 2.
+// Where a row's search stands between kernels.
+struct Kept {
+    uint32_t most, down;      // the key of the largest score, 0 where there is nothing to search; slots down to the bin (first_bin)
+    Search s;
+    uint64_t bound, total;
+};
 struct SampleSplit {
     // zeroed by the first kernel
     uint64_t mass[3][LongShared::kBins];
     uint32_t count[3][LongShared::kBins];
     uint32_t listed, state;
     Cut cut;
+    Kept kept[2];             // after the first histogram; after the second, or the first where its bin's slots are listed
     uint64_t list[kListed];
 };
 constexpr uint32_t kSplitZeroed = offsetof(SampleSplit, list) / 4;
@@ -736,6 +743,25 @@ struct Chunk {
         most = block_max(most, sh);
         if (most == kNoKey) return false;
         lim.set(row, most);
+        return true;
+    }
+    __device__ __forceinline__ void keep(int at, const State &st, uint32_t down) const {
+        if (c == 0 && threadIdx.x == 0) ws->kept[at] = Kept{most, down, st.s, st.bound, st.total};
+    }
+    // Instead of open() and first_bin(), in a kernel behind the one that kept it.
+    __device__ __forceinline__ bool open_kept(const SampleArgs &p, int at, State &st, uint32_t &down) {
+        const Kept k = ws->kept[at];
+        most = uniform(k.most);
+        if (most == 0u) return false;
+        lim.load(p, r);
+        lim.set(row, most);
+        st = first_state(row, lim);
+        st.whole = false;
+        st.histograms = 1;
+        st.s = Search{uniform(k.s.lo), uniform(k.s.hi), uniform(k.s.near), uniform(k.s.far), uniform(k.s.count), uniform(k.s.before), uniform(k.s.mass_before)};
+        st.bound = uniform(k.bound);
+        st.total = uniform(k.total);
+        down = uniform(k.down);
         return true;
     }
     __device__ __forceinline__ void write(const SampleArgs &p, int64_t slot, float prob) const {
@@ -866,6 +892,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_list(SampleArgs p, Sp
     }
     uint32_t down;
     State st = ch.first_bin(sh, down);
+    ch.keep(0, st, down);
     if (down <= kListed) return add_slots(ch, sh, list_from(st, ch.lim), ch.most);
     if (st.s.count <= kListed) return add_slots(ch, sh, st.s.lo, st.s.hi);
     fill(ch.row, sh, false, ch.from, ch.to, st.cut, st.s, Pass{kByDistance, by_mass(st.phase), false});
@@ -877,34 +904,28 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_narrow(SampleArgs p, 
     extern __shared__ uint8_t smem[];
     LongShared &sh = *reinterpret_cast<LongShared *>(smem);
     Chunk<T> ch(p, x);
-    if (!ch.open(p, x, sh, true) || !ch.limited()) return;
+    State st;
     uint32_t down;
-    State st = ch.first_bin(sh, down);
-    bool to_cut = false;
+    int64_t slot;
+    float prob;
+    if (!ch.open_kept(p, 0, st, down)) return;
     if (down <= kListed) {
         if (ch.c != 0) return;
         list_from(st, ch.lim);
         // Four waves go on: they wait less for each other, and a barrier counts the waves that have not ended.
-        __syncthreads();
         SampleShared<4> &few = *reinterpret_cast<SampleShared<4> *>(smem);
         if (threadIdx.x >= few.kThreads) return;
         take_list(ch, few, st);
-        int64_t slot;
-        float prob;
         search(ch.row, few, ch.lim, st, false, false, slot, prob);
         return ch.write(p, slot, prob);
-    } else {
-        if (st.s.count <= kListed) return;
-        to_bin(ch.row, sh, st, pick(sh, st, ch.lim, ch.ws->count[1][threadIdx.x], ch.ws->mass[1][threadIdx.x], sh.kBins - 1, down));
-        if (st.s.count <= kListed) return add_slots(ch, sh, st.s.lo, st.s.hi);
-        // more than that with keys next to each other: one workgroup goes on
-        if (ch.c != 0) return;
-        to_cut = true;
     }
-    int64_t slot;
-    float prob;
-    search(ch.row, sh, ch.lim, st, to_cut, false, slot, prob);
-    if (!to_cut) return ch.write(p, slot, prob);
+    if (st.s.count <= kListed) return ch.keep(1, st, down);
+    to_bin(ch.row, sh, st, pick(sh, st, ch.lim, ch.ws->count[1][threadIdx.x], ch.ws->mass[1][threadIdx.x], sh.kBins - 1, down));
+    ch.keep(1, st, down);
+    if (st.s.count <= kListed) return add_slots(ch, sh, st.s.lo, st.s.hi);
+    // more than that with keys next to each other: one workgroup goes on
+    if (ch.c != 0) return;
+    search(ch.row, sh, ch.lim, st, true, false, slot, prob);
     if (threadIdx.x == 0) { ch.ws->cut = st.cut; ch.ws->state = kRowCut; }
 }
 
@@ -914,15 +935,14 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_mass(SampleArgs p, Sp
     LongShared &sh = *reinterpret_cast<LongShared *>(smem);
     Chunk<T> ch(p, x);
     const uint32_t state = uniform(ch.ws->state);
-    if (state == kRowDone || !ch.open(p, x, sh, state != kRowCut)) return;
+    State st;
+    uint32_t down;
+    if (state == kRowDone || !ch.open_kept(p, 1, st, down)) return;
     Cut cut{uniform(ch.ws->cut.least), uniform(ch.ws->cut.tie_last)};
     if (state != kRowCut) {
-        uint32_t down;
-        State st = ch.first_bin(sh, down);
-        if (st.s.count > kListed) to_bin(ch.row, sh, st, pick(sh, st, ch.lim, ch.ws->count[1][threadIdx.x], ch.ws->mass[1][threadIdx.x], sh.kBins - 1, down));
-        take_list(ch, sh, st);
         int64_t slot;
         float prob;
+        take_list(ch, sh, st);
         search(ch.row, sh, ch.lim, st, true, false, slot, prob);
         cut = st.cut;
     }
