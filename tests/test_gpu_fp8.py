@@ -175,6 +175,16 @@ def test_matmul_larger(fp8, scale, group, m, n, dim):
 
 
 @pytest.mark.parametrize("scale,group", [("e8m0", 1), ("f32", 1), ("f32", 128)])
+@pytest.mark.parametrize("m,n,dim", [(16, 300, 3900), (16, 300, 4096), (16, 4097, 8192), (15, 700, 8900), (16, 130, 9500), (8, 100, 16384), (9, 100, 16384), (3, 8200, 16384), (4, 8200, 16384)])
+def test_matmul_few_long_rows(fp8, scale, group, m, n, dim):
+    """Few rows of a as long as fit a compute unit's memory, and longer."""
+    a = fp8.quantize(torch.randn(m, dim, generator=gen(13), device="cuda"), scale=scale)
+    b = fp8.quantize(torch.randn(n, dim, generator=gen(14), device="cuda"), scale=scale, group=group)
+    for dtype in DTYPES:
+        check_product(a, b, fp8.matmul(a, b, dtype=dtype))
+
+
+@pytest.mark.parametrize("scale,group", [("e8m0", 1), ("f32", 1), ("f32", 128)])
 @pytest.mark.parametrize("dim,pad,offset", [(256, 272, 0), (256, 256, 4), (256, 257, 0), (200, 208, 0), (200, 201, 3), (1000, 1008, 0), (129, 130, 1), (100, 4096, 16)])
 @pytest.mark.parametrize("m,n", [(2, 70), (70, 300), (300, 290)])
 def test_matmul_strided(fp8, scale, group, dim, pad, offset, m, n):

@@ -236,7 +236,8 @@ __device__ __forceinline__ void store_out(void *out, size_t at, float v, int typ
 // One row against 1M of 1536 coordinates, into floats: 266 us, 5.8 TB/s where a pure read reaches 6.5.
 constexpr int kDirectThreads = 256, kDirectWaves = kDirectThreads / 64, kDirectBlocks = 4;
 constexpr uint32_t kDirectGroups = 4;         // workgroups of a compute unit at a time
-constexpr size_t kDirectLds = 64 << 10;      // of a's rows, at most
+constexpr size_t kDirectLds = 64 << 10;      // of a's rows, at most, where workgroups stream
+constexpr size_t kMostLds = 160 << 10;        // of a compute unit
 
 // Scales of kDirectBlocks blocks from k on, of `blocks` in the row; those past the end are whatever.
 struct Scales4 {
@@ -602,10 +603,15 @@ static hipError_t tile(const MatmulArgs &a, hipStream_t s) {
 
 template <bool EXACT, int SC>
 static hipError_t matmul(const MatmulArgs &a, hipStream_t s) {
-    if (a.a.rows <= 16 && a.dim >= 16 && size_t(a.a.rows) * direct_row(a.dim) <= kDirectLds) {
-        // (Sixteen rows to a wave leave waves without any.  One row against 4096 and 16384 of 1536: 9 us either way; 65536: 22 shared out, 19 with a
-        // wave to sixteen.  In tiles of 64, sixteen rows of a against 100000 take 31 us where these take 33, one row 36 where it takes 28.)
-        return a.b.rows < 256 * 4 * 16 ? direct<EXACT, SC == kScaleBytes, true>(a, s) : direct<EXACT, SC == kScaleBytes, false>(a, s);
+    if (a.a.rows <= 16 && a.dim >= 16) {
+        // Sixteen rows to a wave leave waves without any.  One row against 4096 and 16384 of 1536: 9 us either way; 65536: 22 shared out, 19 with a
+        // wave to sixteen.  In tiles of 64, sixteen rows of a against 100000 take 31 us where these take 33, one row 36 where it takes 28.
+        const bool few = a.b.rows < 256 * 4 * 16;
+        if (size_t(a.a.rows) * direct_row(a.dim) <= kDirectLds) return few ? direct<EXACT, SC == kScaleBytes, true>(a, s) : direct<EXACT, SC == kScaleBytes, false>(a, s);
+        // More of a than that leaves a compute unit one workgroup or two: as long as none waits for its turn.  (8 rows of 16384 against 4000, 8000
+        // and 16000 into bfloat16: 30, 55 and 109 us; in tiles 65, 65 and 93.)
+        const size_t lds = direct_lds(a.a.rows, a.dim);
+        if (lds <= kMostLds && (a.b.rows + 15) / 16 <= 256 * (kMostLds / lds)) return direct<EXACT, SC == kScaleBytes, true>(a, s);
     }
     // A CU's time: the tiles it gets times what one takes.  The rates are those of 1024 by 100000 of 1536: tiles of 256, 128 and 64 take 198, 242 and
     // 339 us into bfloat16, 333, 366 and 444 into floats.  Where few tiles fill the card the small ones win: 300 by 3000 36, 18 and 10 us.  (Float
