@@ -614,13 +614,13 @@ static hipError_t matmul(const MatmulArgs &a, hipStream_t s) {
         if (lds <= kMostLds && (a.b.rows + 15) / 16 <= 256 * (kMostLds / lds)) return direct<EXACT, SC == kScaleBytes, true>(a, s);
     }
     // A CU's time: the tiles it gets times what one takes.  The rates are those of 1024 by 100000 of 1536: tiles of 256, 128 and 64 take 198, 242 and
-    // 339 us into bfloat16, 333, 366 and 444 into floats.  Where few tiles fill the card the small ones win: 300 by 3000 36, 18 and 10 us.  (Float
+    // 339 us into bfloat16, 333, 366 and 444 into floats (a little less for 128: rounds are counted whole, 7 for 6.1 of the 256).  Where few tiles fill the card the small ones win: 300 by 3000 36, 18 and 10 us.  (Float
     // scales and bfloat16 operands of a 256 x 256 tile do not fit the registers.)
     auto time = [&](uint32_t tm, uint32_t tn, double rate) {
         const uint64_t tiles = uint64_t((a.a.rows + tm - 1) / tm) * ((a.b.rows + tn - 1) / tn);
         return double((tiles + 255) / 256) * tm * tn / rate;
     };
-    const double l = time(256, 256, 1.0), m = time(128, 128, EXACT ? 0.9 : 0.8), sm = time(64, 64, EXACT ? 0.75 : 0.58);
+    const double l = time(256, 256, 1.0), m = time(128, 128, EXACT ? 0.85 : 0.8), sm = time(64, 64, EXACT ? 0.75 : 0.58);
     if constexpr (!EXACT || SC == kScaleBytes) {
         if (l <= m && l <= sm) return tile<EXACT, SC, 256, 256, 2, 4>(a, s);
     }
