@@ -11,6 +11,7 @@ from . import _lib as T
 
 _VALUES = {torch.float32: T.F32, torch.float16: T.F16, torch.bfloat16: T.BF16}
 _SCALES = {"e8m0": (T.SCALE_E8M0, torch.float8_e8m0fnu), "f32": (T.SCALE_F32, torch.float32)}
+_CODES = (torch.float8_e4m3fn,)
 _SCALE_TYPES = {torch.float8_e8m0fnu: T.SCALE_E8M0, torch.float32: T.SCALE_F32}
 BLOCK = 128                     # coordinates that share a scale
 _MAX_DIM = 16384
@@ -73,18 +74,18 @@ class Fp8Rows:
     __slots__ = ("_codes", "_scales", "_group", "_scale_type")
 
     def __init__(self, codes, scales, group=1):
-        _gpu("codes", codes, (torch.float8_e4m3fn,))
-        _gpu("scales", scales, tuple(_SCALE_TYPES))
+        _gpu("codes", codes, _CODES)
+        _gpu("scales", scales, _SCALE_TYPES)
         if group not in (1, BLOCK):
             raise ValueError(f"group must be 1 or {BLOCK}, got {group}")
         rows, dim = codes.shape
         if not 1 <= dim <= _MAX_DIM:
             raise ValueError(f"dim must be 1 to {_MAX_DIM}, got {dim}")
-        if tuple(scales.shape) != (-(-rows // group), _blocks(dim)):
+        if scales.shape != (-(-rows // group), -(-dim // BLOCK)):
             raise ValueError(f"scales of {rows} x {dim} codes in groups of {group} rows must be "
                              f"{(-(-rows // group), _blocks(dim))}, got {tuple(scales.shape)}")
         _same_device(codes.device, "scales", scales)
-        self._set(codes, scales, group, _SCALE_TYPES[scales.dtype])
+        self._codes, self._scales, self._group, self._scale_type = codes, scales, group, _SCALE_TYPES[scales.dtype]
 
     def _set(self, codes, scales, group, scale_type):
         self._codes, self._scales, self._group, self._scale_type = codes, scales, group, scale_type
@@ -109,7 +110,7 @@ class Fp8Rows:
 def quantize(x, *, scale="e8m0", group=1):
     """8-bit rows of `x` (float32, float16 or bfloat16 [rows, dim]; tv_fp8_quantize_dev).  `scale`: "e8m0", powers of two, which
     the matrix units apply at no cost, or "f32"; `group`: rows that share a scale, 1 or 128."""
-    _gpu("x", x, tuple(_VALUES))
+    _gpu("x", x, _VALUES)
     if scale not in _SCALES:
         raise ValueError(f"scale must be 'e8m0' or 'f32', got {scale!r}")
     if group not in (1, BLOCK):
@@ -131,24 +132,25 @@ def matmul(a, b, *, dtype=torch.float32, out=None):
     rows of `a` have scales of their own, `b` may share them; both have the same type of scales."""
     if not isinstance(a, Fp8Rows) or not isinstance(b, Fp8Rows):
         raise TypeError(f"a and b must be Fp8Rows, got {type(a).__name__} and {type(b).__name__}")
-    if a.group != 1:
+    if a._group != 1:
         raise ValueError("rows of a must have scales of their own (group 1)")
-    if a.dim != b.dim:
-        raise ValueError(f"dim {a.dim} of a does not match dim {b.dim} of b")
-    if a.scales.dtype != b.scales.dtype:
+    (m, dim), (n, b_dim) = a._codes.shape, b._codes.shape
+    if dim != b_dim:
+        raise ValueError(f"dim {dim} of a does not match dim {b_dim} of b")
+    if a._scale_type != b._scale_type:
         raise ValueError(f"scales of a are {a.scales.dtype}, of b {b.scales.dtype}")
-    device = a.codes.device
-    _same_device(device, "b", b.codes)
+    device = a._codes.device
+    _same_device(device, "b", b._codes)
     if out is None:
         if dtype not in _VALUES:
             raise TypeError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
-        out = torch.empty((len(a), len(b)), dtype=dtype, device=device)
+        out = torch.empty((m, n), dtype=dtype, device=device)
     else:
-        _gpu("out", out, tuple(_VALUES))
-        if tuple(out.shape) != (len(a), len(b)):
-            raise ValueError(f"out must be {(len(a), len(b))}, got {tuple(out.shape)}")
+        _gpu("out", out, _VALUES)
+        if out.shape != (m, n):
+            raise ValueError(f"out must be {(m, n)}, got {tuple(out.shape)}")
         _same_device(device, "out", out)
-    _call(T.lib().tv_fp8_matmul_dev, device, *a._args(), *b._args(), b.group, a.dim, a._scale_type,
+    _call(T.lib().tv_fp8_matmul_dev, device, *a._args(), *b._args(), b._group, dim, a._scale_type,
           out.data_ptr(), _VALUES[out.dtype], out.stride(0))
     return out
 
@@ -159,21 +161,22 @@ def rescore(queries, rows, slots, k):
     rows count as absent; a query with fewer than `k` present ends in (-inf, -1)."""
     if not isinstance(rows, Fp8Rows):
         raise TypeError(f"rows must be Fp8Rows, got {type(rows).__name__}")
-    _gpu("queries", queries, tuple(_VALUES))
+    _gpu("queries", queries, _VALUES)
     _gpu("slots", slots, (torch.int64,))
     nq, m = slots.shape
-    if tuple(queries.shape) != (nq, rows.dim):
-        raise ValueError(f"queries must be {(nq, rows.dim)}, got {tuple(queries.shape)}")
+    dim = rows._codes.shape[1]
+    if queries.shape != (nq, dim):
+        raise ValueError(f"queries must be {(nq, dim)}, got {tuple(queries.shape)}")
     k = int(k)
     if not 0 <= k <= m:
         raise ValueError(f"k must be 0 to {m}, the number of candidates, got {k}")
     device = queries.device
-    _same_device(device, "rows", rows.codes)
+    _same_device(device, "rows", rows._codes)
     _same_device(device, "slots", slots)
     scores = torch.empty((nq, k), dtype=torch.float32, device=device)
     best = torch.empty((nq, k), dtype=torch.int64, device=device)
-    ws = _workspace(T.lib().tv_fp8_rescore_workspace(nq, m, rows.dim), device)
+    ws = _workspace(T.lib().tv_fp8_rescore_workspace(nq, m, dim), device)
     _call(T.lib().tv_fp8_rescore_dev, device, queries.data_ptr(), _VALUES[queries.dtype], queries.stride(0), nq,
-          *rows._args(), rows.group, rows.dim, rows._scale_type, slots.data_ptr(), slots.stride(0), m, k,
+          *rows._args(), rows._group, dim, rows._scale_type, slots.data_ptr(), slots.stride(0), m, k,
           scores.data_ptr(), best.data_ptr(), *ws[1:])
     return scores, best

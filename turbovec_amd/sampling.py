@@ -32,7 +32,7 @@ def sample(scores, u, *, temperature=None, top_k=None, top_p=None, min_p=None, m
     (float32, `top_k` int32); None: temperature 1, no limit.  `mask`: int64 words of 64 slots, as `pack_mask` makes
     them, [ceil(n / 64)] for all rows or [rows, ceil(n / 64)].  Slots are limited by top-k, then top-p, then min-p, and drawn in
     the order of slots; a row that allows nothing gives (-1, 0)."""
-    _gpu("scores", scores, tuple(_VALUES))
+    _gpu("scores", scores, _VALUES)
     rows, n = scores.shape
     if n == 0:
         raise ValueError("rows without scores")
