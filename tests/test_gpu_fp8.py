@@ -174,6 +174,16 @@ def test_matmul_larger(fp8, scale, group, m, n, dim):
         check_product(a, b, fp8.matmul(a, b, dtype=dtype))
 
 
+@pytest.mark.parametrize("scale,group", [("e8m0", 1), ("f32", 1), ("e8m0", 128), ("f32", 128)])
+@pytest.mark.parametrize("m,n,dim", [(17, 130, 200), (31, 1000, 129), (32, 4097, 256), (33, 140_000, 128), (64, 70_003, 130), (129, 45_000, 256), (192, 23_000, 40), (250, 20_001, 384)])
+def test_matmul_narrow_tiles(fp8, scale, group, m, n, dim):
+    """Sizes that go to tiles of 32 or 64 rows of a by 128 of b."""
+    a = fp8.quantize(torch.randn(m, dim, generator=gen(15), device="cuda"), scale=scale)
+    b = fp8.quantize(torch.randn(n, dim, generator=gen(16), device="cuda") * torch.exp2(torch.arange(n, device="cuda") % 5 - 2.0)[:, None], scale=scale, group=group)
+    for dtype in DTYPES:
+        check_product(a, b, fp8.matmul(a, b, dtype=dtype))
+
+
 @pytest.mark.parametrize("scale,group", [("e8m0", 1), ("f32", 1), ("f32", 128)])
 @pytest.mark.parametrize("m,n,dim", [(16, 300, 3900), (16, 300, 4096), (16, 4097, 8192), (15, 700, 8900), (16, 130, 9500), (8, 100, 16384), (9, 100, 16384), (3, 8200, 16384), (4, 8200, 16384)])
 def test_matmul_few_long_rows(fp8, scale, group, m, n, dim):

@@ -3,6 +3,8 @@
 // A row's coordinates are e4m3 codes (4 exponent bits, 3 of mantissa, largest value 448); each block of 128 coordinates has
 // a scale, of its own row or of the tile of 128 rows it lies in: a float, or the exponent alone of a power of two (e8m0), which
 // the matrix unit applies itself.
+#include <cmath>
+
 #include "tv_device.h"
 #include "tv_ops.h"
 
@@ -613,18 +615,28 @@ static hipError_t matmul(const MatmulArgs &a, hipStream_t s) {
         const size_t lds = direct_lds(a.a.rows, a.dim);
         if (lds <= kMostLds && (a.b.rows + 15) / 16 <= 256 * (kMostLds / lds)) return direct<EXACT, SC == kScaleBytes, true>(a, s);
     }
-    // A CU's time: the tiles it gets times what one takes.  The rates are those of 1024 by 100000 of 1536: tiles of 256, 128 and 64 take 198, 242 and
-    // 339 us into bfloat16, 333, 366 and 444 into floats (a little less for 128: rounds are counted whole, 7 for 6.1 of the 256).  Where few tiles fill the card the small ones win: 300 by 3000 36, 18 and 10 us.  (Float
-    // scales and bfloat16 operands of a 256 x 256 tile do not fit the registers.)
-    auto time = [&](uint32_t tm, uint32_t tn, double rate) {
-        const uint64_t tiles = uint64_t((a.a.rows + tm - 1) / tm) * ((a.b.rows + tn - 1) / tn);
-        return double((tiles + 255) / 256) * tm * tn / rate;
-    };
-    const double l = time(256, 256, 1.0), m = time(128, 128, EXACT ? 0.85 : 0.8), sm = time(64, 64, EXACT ? 0.75 : 0.58);
-    if constexpr (!EXACT || SC == kScaleBytes) {
-        if (l <= m && l <= sm) return tile<EXACT, SC, 256, 256, 2, 4>(a, s);
+    // Up to 32 rows of a into floats: a tile that does not convert rows that are not there.  (32 by 77777 of 1000 22 us, by 1M of 1536 343; in tiles of 64
+    // 27 and 371.  Into bfloat16 it is 23 and 24, 303 and 319, but 30 and 27 by 100000 of 1536.)
+    if constexpr (EXACT) {
+        if (a.a.rows <= 32) return tile<EXACT, SC, 32, 128, 1, 4>(a, s);
     }
-    return m <= sm ? tile<EXACT, SC, 128, 128, 2, 2>(a, s) : tile<EXACT, SC, 64, 64, 2, 2>(a, s);
+    // A CU's time: the tiles it gets, which come in rounds of as many as it holds at a time, times what one takes.  The rates are those of 1024 by 100000
+    // of 1536: tiles of 256, 128 and 64 take 198, 242 and 339 us into bfloat16, 333, 366 and 444 into floats (a little less for 128: 6.1 rounds of the
+    // 256 count as 7), and of 256 by 1M for 64 x 128: 733 us where 256 takes 526 and 64 900.  A started round costs a whole one: 64 by 100000 takes 28 us
+    // in tiles of 64, 32 of 64 x 128, by 77777 of 1000 29 and 26.  Where few tiles fill the card the small ones win: 300 by 3000 36, 18 and
+    // 10 us, 64 by 20000 18 in tiles of 64 x 128 and 14 of 64.  (Float scales and bfloat16 operands of a 256 x 256 tile do not fit the registers.)
+    auto tiles = [&](uint32_t tm, uint32_t tn) { return uint64_t((a.a.rows + tm - 1) / tm) * ((a.b.rows + tn - 1) / tn); };
+    auto time = [&](uint32_t tm, uint32_t tn, uint32_t held, double rate) {
+        const uint64_t n = tiles(tm, tn), one = 256 * held;
+        return double(n <= one ? (n + 255) / 256 : (n + one - 1) / one * held) * tm * tn / rate;
+    };
+    const double l = EXACT && SC != kScaleBytes ? HUGE_VAL : time(256, 256, 1, 1.0), m = time(128, 128, 2, EXACT ? 0.85 : 0.8), sm = time(64, 64, 4, EXACT ? 0.75 : 0.58);
+    const double wide = tiles(64, 128) < 512 ? HUGE_VAL : time(64, 128, 3, EXACT ? 0.78 : 0.72);
+    if constexpr (!EXACT || SC == kScaleBytes) {
+        if (l <= m && l <= sm && l <= wide) return tile<EXACT, SC, 256, 256, 2, 4>(a, s);
+    }
+    if (m <= sm && m <= wide) return tile<EXACT, SC, 128, 128, 2, 2>(a, s);
+    return wide <= sm ? tile<EXACT, SC, 64, 128, 2, 2>(a, s) : tile<EXACT, SC, 64, 64, 2, 2>(a, s);
 }
 template <bool EXACT>
 static hipError_t matmul_as(const MatmulArgs &a, int scale_type, hipStream_t s) {
