@@ -79,7 +79,7 @@ __device__ __forceinline__ void store_scale(void *scales, size_t at, uint32_t st
     else static_cast<uint32_t *>(scales)[at] = stored;
 }
 
-// A scale for each row: half a wave to a block, four blocks at a time.  Bound by memory: 400K rows of 1536 floats take 578 us, 5.3 TB/s read and
+// A scale for each row: half a wave to a block, four blocks at a time.  Bound by memory: 400K rows of 1536 floats take 578 to 610 us, 5.0 to 5.3 TB/s read and
 // written (a copy reaches 4.9, half of it writes).
 constexpr int kQuantThreads = 256, kQuantUnits = 4;
 constexpr uint64_t kMostGroups = 1 << 20;    // workgroups of a launch: a grid of 2^32 threads is not allowed
@@ -393,8 +393,8 @@ static hipError_t direct(const MatmulArgs &a, hipStream_t s) {
 // run that belongs there.
 //
 // Bound by the matrix unit and what feeds it: 4096 rows by 4096 of 4096 coordinates into bfloat16 56 us with e8m0 scales (2.4 PFLOP/s) and
-// 66 with floats (2.1; their multiply-adds), where the library's 8-bit product of that size, one scale for all of it, takes 49.  1024 by 100000
-// of 1536 into floats 320 us, 0.98 PFLOP/s; the library's bfloat16 product of a large size reaches 1.16.
+// 66 to 73 with floats (1.9 to 2.1; their multiply-adds), where the library's 8-bit product of that size, one scale for all of it, takes 49.  1024 by 100000
+// of 1536 into floats 320 to 336 us, 0.94 to 0.98 PFLOP/s; the library's bfloat16 product of a large size reaches 1.16.
 enum { kScaleBytes = 0, kScaleRows = 1, kScaleTiles = 2 };      // e8m0; floats of each row of b; floats of 128 rows of b
 
 __device__ __forceinline__ void load16_to_lds(uint32_t lds, const uint8_t *base, uint32_t offset) {

@@ -10,8 +10,8 @@
 // histogram of a row goes by the distance to the best score, its bins widening with it; where the slots down to the bin it finds are
 // few, they are gathered, and everything else happens among them.  Bound by the passes over the row, three to six, and the exponentials (20 64-bit
 // instructions each); a single row by what a pass takes at least, and by the fetching of its own instructions (one loop serves every
-// search for that).  256 rows of 100000 bfloat16 scores, top-p 0.95 and min-p 0.001: 105 us; one row of 100000, top-k 50 and top-p 0.9: 37;
-// ten million, half of them masked, top-p 0.5: 134.
+// search for that).  256 rows of 100000 bfloat16 scores, top-p 0.95 and min-p 0.001: 102 us; one row of 100000, top-k 50 and top-p 0.9: 30 to
+// 34; ten million, half of them masked, top-p 0.5: 103.
 #include <algorithm>
 
 #include "tv_device.h"
