@@ -431,3 +431,23 @@ def test_a_buffer_past_four_gigabytes(fp8):
     slots = torch.randint(32_000, n, (3, 50), generator=gen(92), device="cuda")
     for x, y in zip(fp8.rescore(x[:3], far, slots, 9), fp8.rescore(x[:3], r, slots, 9)):
         assert torch.equal(x, y)
+
+
+def test_more_rows_and_queries_than_a_grid_has(fp8):
+    """Numbers of rows and queries for which workgroups go round: each part gives what it gives in a call of its own."""
+    x = torch.randn(34_000_000, 1, generator=gen(93), device="cuda")
+    for group in (1, 128):
+        r = fp8.quantize(x, group=group)
+        for lo in (0, 33_553_408, 33_999_872 - 128):
+            part = fp8.quantize(x[lo:lo + 128], group=group)
+            assert torch.equal(r.codes[lo:lo + 128].view(torch.uint8), part.codes.view(torch.uint8))
+            assert torch.equal(r.scales[lo // group:lo // group + len(part.scales)].view(torch.uint8), part.scales.view(torch.uint8))
+    del x, r
+    rows = fp8.quantize(torch.randn(500, 40, generator=gen(94), device="cuda"))
+    q = torch.randn(70_000, 40, generator=gen(95), device="cuda")
+    for m in (3, 300):
+        slots = torch.randint(0, 500, (70_000, m), generator=gen(96), device="cuda")
+        got = fp8.rescore(q, rows, slots, 3)
+        for lo in (0, 65_500, 69_900):
+            for a, b in zip(got, fp8.rescore(q[lo:lo + 100], rows, slots[lo:lo + 100], 3)):
+                assert torch.equal(a[lo:lo + 100], b)

@@ -184,6 +184,17 @@ def test_draws_by_two_threads(sample):
     assert same == [20, 20]
 
 
+def test_more_rows_than_a_grid_has(sample):
+    for n in (5, 7000):
+        scores = (3 * torch.randn(66_000, n, generator=gen(81), device="cuda")).half()
+        u = torch.rand(66_000, generator=gen(82), device="cuda")
+        got = sample(scores, u, top_k=3, top_p=0.9)
+        for lo in (0, 65_400, 65_900):
+            for a, b in zip(got, sample(scores[lo:lo + 100], u[lo:lo + 100], top_k=3, top_p=0.9)):
+                assert torch.equal(a[lo:lo + 100], b)
+        check(sample, scores[65_530:65_545], u[65_530:65_545], top_k=3, top_p=0.9)
+
+
 def test_no_rows(sample):
     slots, probs = sample(torch.empty(0, 100_000, device="cuda"), torch.empty(0, device="cuda"), top_k=5)
     assert slots.shape == probs.shape == (0,)
