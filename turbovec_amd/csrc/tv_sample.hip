@@ -222,6 +222,7 @@ struct SampleShared {
     // That many values fall into bins of 2^this.
     __device__ __forceinline__ static uint32_t shift_of(uint32_t range) { return uint32_t(max(0, 32 - int(kBits) - __clz(int(range)))); }
 };
+constexpr uint32_t kTopEach = 16;           // slots of a thread from which on its best one tells enough (list_top)
 constexpr uint32_t kShortListed = 2048;     // five workgroups' LDS to a compute unit
 using LongShared = SampleShared<kSampleWaves>;
 
@@ -574,6 +575,30 @@ __device__ __forceinline__ bool list_bin(const SampleRow<T> &row, SampleShared<W
     return true;
 }
 
+// Top-k's slots and a few more, without a histogram of the row: of its threads' best scores (each of slots of its own) as many as k
+// reach down to some bin, so that many slots do too.  False where that leaves too many, or fewer threads than k have a slot.
+template <typename T, int W, uint32_t MOST>
+__device__ __forceinline__ bool list_top(const SampleRow<T> &row, SampleShared<W, MOST> &sh, const Limits &lim, State &st, float own_best) {
+    __syncthreads();
+#pragma unroll
+    for (uint32_t c = 0; c < kCopies; ++c) sh.count[c * sh.kBins + threadIdx.x] = 0;
+    __syncthreads();
+    if (own_best > -__int_as_float(0x7f800000)) atomicAdd(&sh.count[sh.bin(row.distance(own_best)) * kCopies + threadIdx.x % kCopies], 1u);
+    __syncthreads();
+    uint32_t count, down;
+    uint64_t mass;
+    own_bin(sh, false, count, mass);
+    State of_threads = st;
+    const uint32_t bin = pick(sh, of_threads, lim, count, 0, sh.kBins - 1, down);
+    if (down < uint32_t(lim.top_k)) return false;
+    to_bin(row, sh, of_threads, bin);
+    st.n = list_slots(row, sh, 0, row.n, st.cut, of_threads.s.lo, row.most);
+    if (uniform(sh.listed) > sh.kMost) return false;
+    st.s.lo = of_threads.s.lo;
+    st.listed = true;
+    return true;
+}
+
 // The searches that are left, to the draw, or (to_cut) to the end of the one that st is in, or (to_list) to where the slots that can still be drawn
 // are listed: then false.
 template <typename T, int W, uint32_t MOST>
@@ -672,7 +697,9 @@ __global__ __launch_bounds__(64 * W) void k_sample(SampleArgs p) {
             lim.set(row, most);
             State st = first_state(row, lim);
             if (st.phase == kDraw && lim.min_key > st.cut.least) st.cut.least = lim.min_key;
-            if (!search(row, sh, lim, st, false, W == kSampleWaves && r + gridDim.x >= p.rows, slot, prob)) {
+            const bool last = W == kSampleWaves && r + gridDim.x >= p.rows;
+            const bool top = st.phase == kTopK && uint32_t(lim.top_k) <= sh.kThreads / 2 && p.n >= kTopEach * sh.kThreads && list_top(row, sh, lim, st, best);
+            if ((top && last) || !search(row, sh, lim, st, false, last, slot, prob)) {
                 // Four waves go on: they wait less for each other, and a barrier counts the waves that have not ended.
                 SampleShared<4, MOST> &few = *reinterpret_cast<SampleShared<4, MOST> *>(smem);
                 static_assert(sizeof(few) <= offsetof(SampleShared<kSampleWaves>, list), "the list moves down past itself");
