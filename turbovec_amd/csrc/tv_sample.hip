@@ -9,9 +9,9 @@
 // than so many slots, or so much mass, lies.  A histogram of 1024 bins narrows the values to one bin, the next one divides that.  The first
 // histogram of a row goes by the distance to the best score, its bins widening with it; where the slots down to the bin it finds are
 // few, they are gathered, and everything else happens among them.  Top-k's slots are gathered without it where the best scores of the threads tell
-// which (list_top).  Bound by the passes over the row, two to six, and the exponentials (20 64-bit
+// which (list_top), top-p's where min-p does (list_kept).  Bound by the passes over the row, two to six, and the exponentials (20 64-bit
 // instructions each); a single row by what a pass takes at least, and by the fetching of its own instructions (one loop serves every
-// search for that).  256 rows of 100000 bfloat16 scores, top-p 0.95 and min-p 0.001: 102 us; one row of 100000, top-k 50 and top-p 0.9: 30 to
+// search for that).  256 rows of 100000 bfloat16 scores, top-p 0.95 and min-p 0.001: 92 us, top-k 50 and top-p 0.9: 43; one row of 100000, top-k 50 and top-p 0.9: 30 to
 // 34; ten million, half of them masked, top-p 0.5: 103.
 #include <algorithm>
 
@@ -22,7 +22,7 @@ namespace tv {
 
 constexpr int kSampleWaves = 16, kSampleThreads = kSampleWaves * 64;      // of a row that is not short
 constexpr uint32_t kNoKey = 0x007fffffu;     // -infinity's; what is not allowed has it too
-constexpr uint32_t kListed = 4000;           // slots that are gathered, at most: two workgroups' LDS to a compute unit
+constexpr uint32_t kListed = 4000;           // slots that are gathered of a row in chunks, at most: two workgroups' LDS to a compute unit
 
 // The same value in all lanes, said to the compiler: it keeps it in scalar registers and branches on it without masks.
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return uint32_t(__builtin_amdgcn_readfirstlane(int(v))); }
@@ -204,16 +204,16 @@ __device__ __forceinline__ N wave_upto(N v) {
 // Scores crowd into some fifty bins: four copies of each keep the lanes of a wave from waiting for each other (ten million
 // scores in one row, a histogram of masses: 17.2 ms with one copy).
 constexpr uint32_t kCopies = 4;
-// What a workgroup of W waves shares; a bin to a thread.
-template <int W, uint32_t MOST = kListed>
+// What a workgroup of W waves shares; a bin to a thread.  ROOM: for so many bins, so that fewer waves find the list in the same place.
+template <int W, uint32_t MOST = kListed, uint32_t ROOM = 64 * W>
 struct SampleShared {
     static constexpr uint32_t kThreads = 64 * W, kBins = kThreads, kBits = W == 16 ? 10 : W == 4 ? 8 : 0, kMost = MOST;
     static_assert(kBins == 1u << kBits, "a bin to a thread");
-    uint64_t part[W], found_mass;
-    uint32_t part32[W], listed, picked, found_count, found_before, found_down, found_value;
-    uint32_t count[kBins * kCopies];
-    uint64_t mass[kBins * kCopies];
-    uint64_t list[kMost];         // key, complement of the slot.  (Last: kernels that list nothing leave it out.)
+    uint64_t part[ROOM / 64], found_mass;
+    uint32_t part32[ROOM / 64], listed, picked, found_count, found_before, found_down, found_value;
+    uint32_t count[ROOM * kCopies];
+    uint64_t mass[ROOM * kCopies];
+    uint64_t list[MOST];          // key, complement of the slot.  (Last: what lies within 64 KiB is addressed at no cost.)
     // The bin of a distance: 32 of 1024 for each power of two that it spans, from 2^-20 to 2^12; what is nearer or further is in the first or the
     // last.
     static constexpr int kDistance = 28 - int(kBits), kFirstBin = (127 - 20) << (int(kBits) - 5);
@@ -227,11 +227,13 @@ struct SampleShared {
 // 15000 26 and 22; rows of 1000 16 either way.)
 constexpr uint32_t kTopEach = 4;
 constexpr uint32_t kShortListed = 2048;     // five workgroups' LDS to a compute unit
+constexpr uint32_t kRowListed = 8000;        // a compute unit has one workgroup of sixteen waves
 using LongShared = SampleShared<kSampleWaves>;
+using BinsShared = SampleShared<kSampleWaves, 1>;      // of kernels that list nothing
 
 // The sum over the threads before this one; `all` the sum over all of them.
-template <int W, uint32_t MOST>
-__device__ __forceinline__ uint64_t block_before(uint64_t v, SampleShared<W, MOST> &sh, uint64_t &all) {
+template <int W, uint32_t MOST, uint32_t ROOM>
+__device__ __forceinline__ uint64_t block_before(uint64_t v, SampleShared<W, MOST, ROOM> &sh, uint64_t &all) {
     const uint32_t wave = threadIdx.x >> 6;
     const uint64_t upto = wave_upto(v);
     __syncthreads();
@@ -247,14 +249,14 @@ __device__ __forceinline__ uint64_t block_before(uint64_t v, SampleShared<W, MOS
     all = uniform(all);
     return before;
 }
-template <int W, uint32_t MOST>
-__device__ __forceinline__ uint64_t block_sum(uint64_t v, SampleShared<W, MOST> &sh) {
+template <int W, uint32_t MOST, uint32_t ROOM>
+__device__ __forceinline__ uint64_t block_sum(uint64_t v, SampleShared<W, MOST, ROOM> &sh) {
     uint64_t all;
     block_before(v, sh, all);
     return all;
 }
-template <int W, uint32_t MOST>
-__device__ __forceinline__ uint32_t block_max(uint32_t v, SampleShared<W, MOST> &sh) {
+template <int W, uint32_t MOST, uint32_t ROOM>
+__device__ __forceinline__ uint32_t block_max(uint32_t v, SampleShared<W, MOST, ROOM> &sh) {
     v = wave_umax(v);
     __syncthreads();
     if ((threadIdx.x & 63u) == 0) sh.part32[threadIdx.x >> 6] = v;
@@ -309,8 +311,8 @@ struct Pass {
     bool mass, ties;          // ties: of the cut's slots only those of its least key
 };
 // A histogram of the cut's slots whose values lie in s: of those of the list, or those lo .. hi - 1 of the row.
-template <typename T, int W, uint32_t MOST>
-__device__ __forceinline__ void fill(const SampleRow<T> &row, SampleShared<W, MOST> &sh, bool listed, uint32_t lo, uint32_t hi, const Cut &cut, const Search &s, const Pass &pass) {
+template <typename T, int W, uint32_t MOST, uint32_t ROOM>
+__device__ __forceinline__ void fill(const SampleRow<T> &row, SampleShared<W, MOST, ROOM> &sh, bool listed, uint32_t lo, uint32_t hi, const Cut &cut, const Search &s, const Pass &pass) {
     __syncthreads();
 #pragma unroll
     for (uint32_t c = 0; c < kCopies; ++c) {
@@ -349,8 +351,8 @@ __device__ __forceinline__ void fill(const SampleRow<T> &row, SampleShared<W, MO
     __syncthreads();
 }
 // A thread's bin, all copies.
-template <int W, uint32_t MOST>
-__device__ __forceinline__ void own_bin(const SampleShared<W, MOST> &sh, bool with_mass, uint32_t &count, uint64_t &mass) {
+template <int W, uint32_t MOST, uint32_t ROOM>
+__device__ __forceinline__ void own_bin(const SampleShared<W, MOST, ROOM> &sh, bool with_mass, uint32_t &count, uint64_t &mass) {
     count = 0;
     mass = 0;
 #pragma unroll
@@ -364,6 +366,7 @@ __device__ __forceinline__ uint64_t drawn_mass(float u, uint64_t sum) {
     const double want = double(u) * double(sum);
     return want >= double(sum) ? sum - 1 : want > 0.0 ? uint64_t(want) : uint64_t(0);
 }
+__device__ __forceinline__ uint64_t top_p_bound(const Limits &lim, uint64_t sum) { return uniform(uint64_t(ceil(fmax(double(lim.top_p), 0.0) * double(sum)))); }
 // A row's searches, one after the other.
 enum { kTopK, kTopP, kTies, kDraw };
 struct State {
@@ -380,8 +383,8 @@ __device__ __forceinline__ bool by_mass(int phase) { return phase == kTopP || ph
 
 // Of the bins, a thread each, the last that has slots and that less than the bound lies before; the first one always.  `down`: the slots down to
 // it, or to the bin `cap` if that comes before.
-template <int W, uint32_t MOST>
-__device__ __forceinline__ uint32_t pick(SampleShared<W, MOST> &sh, State &st, const Limits &lim, uint32_t count, uint64_t mass, uint32_t cap, uint32_t &down) {
+template <int W, uint32_t MOST, uint32_t ROOM>
+__device__ __forceinline__ uint32_t pick(SampleShared<W, MOST, ROOM> &sh, State &st, const Limits &lim, uint32_t count, uint64_t mass, uint32_t cap, uint32_t &down) {
     const uint32_t t = threadIdx.x, wave = t >> 6;
     const bool masses = by_mass(st.phase);
     const uint32_t counts = wave_upto(count);
@@ -404,7 +407,7 @@ __device__ __forceinline__ uint32_t pick(SampleShared<W, MOST> &sh, State &st, c
         upto = mass_before;
         if (st.whole) {
             st.total = all = uniform(all);
-            st.bound = uniform(st.phase == kTopP ? uint64_t(ceil(fmax(double(lim.top_p), 0.0) * double(all))) : drawn_mass(lim.u, all) + 1);
+            st.bound = st.phase == kTopP ? top_p_bound(lim, all) : uniform(drawn_mass(lim.u, all)) + 1;
         }
     }
     if (count != 0 && (st.s.before + before == 0 || upto < st.bound)) atomicMax(&sh.picked, t);
@@ -422,8 +425,8 @@ __device__ __forceinline__ uint32_t pick(SampleShared<W, MOST> &sh, State &st, c
 }
 
 // Lists the cut's slots of lo .. hi - 1 whose keys are from .. upto, sh.kMost at most; returns how many.
-template <typename T, int W, uint32_t MOST>
-__device__ __forceinline__ uint32_t list_slots(const SampleRow<T> &row, SampleShared<W, MOST> &sh, uint32_t lo, uint32_t hi, const Cut &cut, uint32_t from, uint32_t upto) {
+template <typename T, int W, uint32_t MOST, uint32_t ROOM>
+__device__ __forceinline__ uint32_t list_slots(const SampleRow<T> &row, SampleShared<W, MOST, ROOM> &sh, uint32_t lo, uint32_t hi, const Cut &cut, uint32_t from, uint32_t upto) {
     __syncthreads();
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
@@ -438,8 +441,8 @@ __device__ __forceinline__ uint32_t list_slots(const SampleRow<T> &row, SampleSh
     return uniform(min(sh.listed, sh.kMost));
 }
 // The one value in s of the list's slots that count; where min-p has kept it out of the list, the least that would be there.
-template <int W, uint32_t MOST>
-__device__ __forceinline__ uint32_t only_value(SampleShared<W, MOST> &sh, const State &st) {
+template <int W, uint32_t MOST, uint32_t ROOM>
+__device__ __forceinline__ uint32_t only_value(SampleShared<W, MOST, ROOM> &sh, const State &st) {
     if (threadIdx.x == 0) sh.found_value = st.s.lo;
     __syncthreads();
     for (uint32_t e = threadIdx.x; e < st.n; e += sh.kThreads) {
@@ -455,8 +458,8 @@ __device__ __forceinline__ uint32_t only_value(SampleShared<W, MOST> &sh, const 
 
 // Of the cut's slots from lo on (ties: those of its least key, each counting 1; otherwise their mass), in slot order the first that the sum up to it
 // exceeds `want` at; it is one of the `len` from lo on.
-template <typename T, int W, uint32_t MOST>
-__device__ __forceinline__ uint32_t locate(const SampleRow<T> &row, SampleShared<W, MOST> &sh, uint32_t lo, uint32_t len, const Cut &cut, bool ties, uint64_t want, bool draws = false,
+template <typename T, int W, uint32_t MOST, uint32_t ROOM>
+__device__ __forceinline__ uint32_t locate(const SampleRow<T> &row, SampleShared<W, MOST, ROOM> &sh, uint32_t lo, uint32_t len, const Cut &cut, bool ties, uint64_t want, bool draws = false,
                                            float u = 0.0f, uint64_t *total = nullptr) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     const CutScores scores(cut);
@@ -540,8 +543,8 @@ __device__ __forceinline__ State first_state(const SampleRow<T> &row, const Limi
     return st;
 }
 // The search goes from a histogram by distance to the bin it picked.
-template <typename T, int W, uint32_t MOST>
-__device__ __forceinline__ void to_bin(const SampleRow<T> &row, const SampleShared<W, MOST> &sh, State &st, uint32_t bin) {
+template <typename T, int W, uint32_t MOST, uint32_t ROOM>
+__device__ __forceinline__ void to_bin(const SampleRow<T> &row, const SampleShared<W, MOST, ROOM> &sh, State &st, uint32_t bin) {
     Search &s = st.s;
     if (st.histograms++ == 0) {
         s.near = sh.nearest(bin);
@@ -555,8 +558,8 @@ __device__ __forceinline__ void to_bin(const SampleRow<T> &row, const SampleShar
     s.hi = s.near == 0 ? row.most : row.least_within(s.near - 1u) - 1u;
 }
 // The last bin of the first histogram that can matter for what is drawn.  (Min-p leaves fewer, but top-p after top-k needs all of top-k's.)
-template <typename T, int W, uint32_t MOST>
-__device__ __forceinline__ uint32_t last_bin(const SampleRow<T> &row, const SampleShared<W, MOST> &sh, const State &st, const Limits &lim) {
+template <typename T, int W, uint32_t MOST, uint32_t ROOM>
+__device__ __forceinline__ uint32_t last_bin(const SampleRow<T> &row, const SampleShared<W, MOST, ROOM> &sh, const State &st, const Limits &lim) {
     return st.phase == kTopP ? sh.bin(row.distance(key_score(lim.min_key))) : sh.kBins - 1;
 }
 // From which key on a row's slots are listed.  Where min-p leaves nothing of the bin, the search is over.
@@ -568,8 +571,8 @@ __device__ __forceinline__ uint32_t list_from(State &st, const Limits &lim) {
 }
 
 // Gathers what is in the bin, or, of few slots down to it, those from there up; where there are few.
-template <typename T, int W, uint32_t MOST>
-__device__ __forceinline__ bool list_bin(const SampleRow<T> &row, SampleShared<W, MOST> &sh, State &st, const Limits &lim, uint32_t down) {
+template <typename T, int W, uint32_t MOST, uint32_t ROOM>
+__device__ __forceinline__ bool list_bin(const SampleRow<T> &row, SampleShared<W, MOST, ROOM> &sh, State &st, const Limits &lim, uint32_t down) {
     if (down > sh.kMost && st.s.count > sh.kMost) return false;
     st.bin_only = down > sh.kMost;
     const uint32_t from = list_from(st, lim), upto = st.bin_only ? st.s.hi : row.most;
@@ -580,8 +583,8 @@ __device__ __forceinline__ bool list_bin(const SampleRow<T> &row, SampleShared<W
 
 // Top-k's slots and a few more, without a histogram of the row: of its threads' best scores (each of slots of its own) as many as k
 // reach down to some bin, so that many slots do too.  False where that leaves too many, or fewer threads than k have a slot.
-template <typename T, int W, uint32_t MOST>
-__device__ __forceinline__ bool list_top(const SampleRow<T> &row, SampleShared<W, MOST> &sh, const Limits &lim, State &st, float own_best) {
+template <typename T, int W, uint32_t MOST, uint32_t ROOM>
+__device__ __forceinline__ bool list_top(const SampleRow<T> &row, SampleShared<W, MOST, ROOM> &sh, const Limits &lim, State &st, float own_best) {
     __syncthreads();
 #pragma unroll
     for (uint32_t c = 0; c < kCopies; ++c) sh.count[c * sh.kBins + threadIdx.x] = 0;
@@ -602,10 +605,39 @@ __device__ __forceinline__ bool list_top(const SampleRow<T> &row, SampleShared<W
     return true;
 }
 
+// What min-p leaves, listed along with the sum of all masses, which is what top-p goes by.  False where that is too much.
+template <typename T, int W, uint32_t MOST, uint32_t ROOM>
+__device__ __forceinline__ bool list_kept(const SampleRow<T> &row, SampleShared<W, MOST, ROOM> &sh, const Limits &lim, State &st) {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.listed = 0;
+    __syncthreads();
+    const float least = key_score(lim.min_key);
+    uint64_t sum = 0;
+    row.each(0, row.n, threadIdx.x, sh.kThreads, [&](uint32_t i, float v, bool in) {
+        if (__ballot(in) == 0ull) return;
+        const uint64_t x = row.units(v);
+        sum += in ? x : 0;
+        if (!in || v < least) return;
+        const uint32_t at = atomicAdd(&sh.listed, 1u);
+        if (at < sh.kMost) sh.list[at] = uint64_t(score_key(v)) << 32 | uint32_t(~i);
+    });
+    const uint64_t total = block_sum(sum, sh);
+    const uint32_t listed = uniform(sh.listed);
+    if (listed > sh.kMost) return false;
+    st.total = total;
+    st.bound = top_p_bound(lim, total);
+    st.n = listed;
+    st.listed = true;
+    st.whole = false;
+    st.s.lo = lim.min_key;
+    st.s.count = listed;
+    return true;
+}
+
 // The searches that are left, to the draw, or (to_cut) to the end of the one that st is in, or (to_list) to where the slots that can still be drawn
 // are listed: then false.
-template <typename T, int W, uint32_t MOST>
-__device__ __forceinline__ bool search(const SampleRow<T> &row, SampleShared<W, MOST> &sh, const Limits &lim, State &st, bool to_cut, bool to_list, int64_t &slot, float &prob) {
+template <typename T, int W, uint32_t MOST, uint32_t ROOM>
+__device__ __forceinline__ bool search(const SampleRow<T> &row, SampleShared<W, MOST, ROOM> &sh, const Limits &lim, State &st, bool to_cut, bool to_list, int64_t &slot, float &prob) {
     while (true) {
         if (st.phase >= kTies && !st.listed) {
             // slots next to each other fall into one bin, a row's are walked instead
@@ -702,14 +734,12 @@ __global__ __launch_bounds__(64 * W) void k_sample(SampleArgs p) {
             if (st.phase == kDraw && lim.min_key > st.cut.least) st.cut.least = lim.min_key;
             const bool last = W == kSampleWaves && r + gridDim.x >= p.rows;
             const bool top = st.phase == kTopK && uint32_t(lim.top_k) <= sh.kThreads / 2 && p.n >= kTopEach * sh.kThreads && list_top(row, sh, lim, st, best);
-            if ((top && last) || !search(row, sh, lim, st, false, last, slot, prob)) {
+            const bool kept = st.phase == kTopP && lim.min_key > kNoKey + 1u && list_kept(row, sh, lim, st);
+            if (((top || kept) && last) || !search(row, sh, lim, st, false, last, slot, prob)) {
                 // Four waves go on: they wait less for each other, and a barrier counts the waves that have not ended.
-                SampleShared<4, MOST> &few = *reinterpret_cast<SampleShared<4, MOST> *>(smem);
-                static_assert(sizeof(few) <= offsetof(SampleShared<kSampleWaves>, list), "the list moves down past itself");
+                SampleShared<4, MOST, 64 * W> &few = *reinterpret_cast<SampleShared<4, MOST, 64 * W> *>(smem);
                 __syncthreads();
                 if (threadIdx.x >= few.kThreads) return;
-                for (uint32_t i = threadIdx.x; i < st.n; i += few.kThreads) few.list[i] = sh.list[i];
-                __syncthreads();
                 search(row, few, lim, st, false, false, slot, prob);
             }
         }
@@ -764,7 +794,8 @@ struct Chunk {
     uint64_t mass;            // count, mass: a thread's bin of the first histogram
     __device__ __forceinline__ Chunk(const SampleArgs &p, const SplitArgs &x)
         : row(row_of<T>(p, blockIdx.x)), ws(x.rows + blockIdx.x), r(blockIdx.x), c(blockIdx.y), from(blockIdx.y * x.chunk), to(min(p.n, from + x.chunk)) {}
-    __device__ __forceinline__ bool open(const SampleArgs &p, const SplitArgs &x, LongShared &sh, bool bins) {
+    template <uint32_t MOST>
+    __device__ __forceinline__ bool open(const SampleArgs &p, const SplitArgs &x, SampleShared<kSampleWaves, MOST> &sh, bool bins) {
         lim.load(p, r);
         most = kNoKey;
         count = bins ? ws->count[0][threadIdx.x] : 0;
@@ -817,8 +848,8 @@ __device__ __forceinline__ State second_state(const Chunk<T> &ch, const Cut &cut
     return st;
 }
 
-template <typename T>
-__device__ __forceinline__ void add_bins(const Chunk<T> &ch, LongShared &sh, int which, bool with_mass) {
+template <typename T, uint32_t MOST>
+__device__ __forceinline__ void add_bins(const Chunk<T> &ch, SampleShared<kSampleWaves, MOST> &sh, int which, bool with_mass) {
     uint32_t count;
     uint64_t mass;
     own_bin(sh, with_mass, count, mass);
@@ -881,7 +912,7 @@ __device__ __forceinline__ void draw_by_parts(const SampleArgs &p, const SplitAr
 template <typename T>
 __global__ __launch_bounds__(kSampleThreads) void k_sample_max(SampleArgs p, SplitArgs x) {
     extern __shared__ uint8_t smem[];
-    LongShared &sh = *reinterpret_cast<LongShared *>(smem);
+    BinsShared &sh = *reinterpret_cast<BinsShared *>(smem);
     const Chunk<T> ch(p, x);
     for (uint32_t i = ch.c * kSampleThreads + threadIdx.x; i < kSplitZeroed; i += x.chunks * kSampleThreads) reinterpret_cast<uint32_t *>(ch.ws)[i] = 0;
     float best = -__int_as_float(0x7f800000);
@@ -895,7 +926,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_max(SampleArgs p, Spl
 template <typename T>
 __global__ __launch_bounds__(kSampleThreads) void k_sample_bins(SampleArgs p, SplitArgs x) {
     extern __shared__ uint8_t smem[];
-    LongShared &sh = *reinterpret_cast<LongShared *>(smem);
+    BinsShared &sh = *reinterpret_cast<BinsShared *>(smem);
     Chunk<T> ch(p, x);
     if (!ch.open(p, x, sh, false)) {
         if (ch.c == 0) ch.write(p, -1, 0.0f);
@@ -1039,12 +1070,13 @@ size_t sample_workspace(size_t rows, size_t n) { return splits(rows, n) ? split_
 static bool few_waves(size_t rows, size_t n) { return n <= 6144 || (rows > 256 && n <= 64 * rows); }
 template <typename T>
 static hipError_t sample(const SampleArgs &a, hipStream_t s) {
-    const size_t lds = sizeof(LongShared), unlisted = offsetof(LongShared, list);
+    const size_t lds = sizeof(LongShared), unlisted = sizeof(BinsShared), row_lds = sizeof(SampleShared<kSampleWaves, kRowListed>);
     const uint32_t grid_rows = a.rows < 65536u ? a.rows : 65536u;
     if (few_waves(a.rows, a.n)) return launch(k_sample<T, 4, kShortListed>, grid_rows, 256, sizeof(SampleShared<4, kShortListed>), s, a);
     if (!splits(a.rows, a.n)) {
-        if (const hipError_t e = allow_lds(reinterpret_cast<const void *>(k_sample<T, kSampleWaves, kListed>), lds); e != hipSuccess) return e;
-        return launch(k_sample<T, kSampleWaves, kListed>, grid_rows, kSampleThreads, lds, s, a);
+        const auto kernel = k_sample<T, kSampleWaves, kRowListed>;
+        if (const hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), row_lds); e != hipSuccess) return e;
+        return launch(kernel, grid_rows, kSampleThreads, row_lds, s, a);
     }
     const Split split = split_of(a.rows, a.n);
     const SplitArgs x{reinterpret_cast<SampleSplit *>(a.ws), reinterpret_cast<uint64_t *>(a.ws + split.masses), reinterpret_cast<Cut *>(a.ws + split.cuts),
