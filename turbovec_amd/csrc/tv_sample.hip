@@ -1038,9 +1038,10 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample_draw(SampleArgs p, Sp
     ch.write(p, slot, prob);
 }
 
-// Rows of more slots than this go in chunks, as long as there are no more than kSplitRows of them.  (Top-k 50 and top-p 0.9, in chunks and in one
-// workgroup: one row of 32768 45 and 40 us, of 65536 47 and 51, of 131072 46 and 76; 128 rows of 65536 57 and 58, of 131072 76 and 84; 192 rows of
-// 131072 99 and 89.)
+// Rows of more slots than this go in chunks, as long as there are no more than kSplitRows of them.  Which limit holds is on the device; by mass the
+// chunks gain more than they lose by number.  (In chunks and in one workgroup, the parameters' filling counted: top-p 0.9, one row of 32768 41 and 47
+// us, of 65536 44 and 69, of 131072 45 and 106, 128 rows of 65536 64 and 72; top-k 50 and top-p 0.9, one row of 32768 43 and 30, of 65536 44 and 34,
+// of 131072 44 and 42, 128 rows of 65536 52 and 38.)
 constexpr size_t kSplitSlots = 40960, kSplitRows = 128;
 constexpr size_t kChunk = 8192;
 struct Split {

@@ -3,7 +3,7 @@
 An index holds 2 to 4 bits a coordinate.  These rows hold 8 (e4m3, with a scale for every block of 128 coordinates) and
 answer what the index's codes are too coarse for: exact-to-8-bits scores of every row (`matmul`), and of the candidates
 of a search (`rescore`).  Everything is a torch tensor on the GPU; calls run on the current stream of the tensors' device
-and do not wait.
+and do not wait.  Results carry no gradient.
 """
 import torch
 

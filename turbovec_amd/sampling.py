@@ -2,7 +2,7 @@
 
 Where a search returns the best rows, a draw returns each row with its probability under a softmax of the scores: hard
 negatives for training, varied retrieval, the next token where the rows are an output embedding.  Everything is a torch
-tensor on the GPU; calls run on the current stream of the tensors' device and do not wait.
+tensor on the GPU; calls run on the current stream of the tensors' device and do not wait.  Results carry no gradient.
 """
 import torch
 
