@@ -19,10 +19,10 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 // ---------------------------------------------------------------------------
 
 // Four values from p, those of them past `left` zero.
-template <typename T, bool VEC>
+template <typename T>
 __device__ __forceinline__ void load4(float (&v)[4], const T *p, int left) {
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    if (VEC && left >= 4) {
+    typedef T T4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    if (left >= 4) {
         const T4 x = *reinterpret_cast<const T4 *>(p);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = float(x[i]);
@@ -56,17 +56,20 @@ __device__ __forceinline__ float scale_of(float most, uint32_t &stored) {
     stored = uint32_t(power + 127);
     return __uint_as_float(stored << 23);
 }
+template <bool E8>
 __device__ __forceinline__ uint32_t codes_of(const float (&v)[4], float s) {
+    // (the inverse of a power of two from 2^-126 to 2^120 is one, so that the product is the quotient)
+    const float inverse = E8 ? __uint_as_float((254u << 23) - __float_as_uint(s)) : 0.0f;
     float q[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = fabsf(v[i]) < __int_as_float(0x7f800000) ? v[i] / s : __int_as_float(0x7fc00000);
+    for (int i = 0; i < 4; ++i) q[i] = fabsf(v[i]) < __int_as_float(0x7f800000) ? (E8 ? v[i] * inverse : v[i] / s) : __int_as_float(0x7fc00000);
     int r = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
     return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], r, true));
 }
-template <bool VEC>
 __device__ __forceinline__ void store4(uint8_t *p, uint32_t c, int left) {
-    if (VEC && left >= 4) {
-        *reinterpret_cast<uint32_t *>(p) = c;
+    typedef uint32_t Four __attribute__((aligned(1)));
+    if (left >= 4) {
+        *reinterpret_cast<Four *>(p) = c;
         return;
     }
 #pragma unroll
@@ -79,11 +82,12 @@ __device__ __forceinline__ void store_scale(void *scales, size_t at, uint32_t st
     else static_cast<uint32_t *>(scales)[at] = stored;
 }
 
-// A scale for each row: half a wave to a block, four blocks at a time.  Bound by memory: 400K rows of 1536 floats take 578 to 610 us, 5.0 to 5.3 TB/s read and
+// A scale for each row: half a wave to a block, four blocks at a time, 16 bytes of floats a lane wherever a row starts (100K of 1535: 158 us, 207 an
+// element at a time).  Bound by memory: 400K rows of 1536 floats take 578 to 610 us, 5.0 to 5.3 TB/s read and
 // written (a copy reaches 4.9, half of it writes).
 constexpr int kQuantThreads = 256, kQuantUnits = 4;
 constexpr uint64_t kMostGroups = 1 << 20;    // workgroups of a launch: a grid of 2^32 threads is not allowed
-template <typename T, bool E8, bool VEC>
+template <typename T, bool E8>
 __global__ __launch_bounds__(kQuantThreads) void k_fp8_quantize_rows(QuantizeArgs a) {
     const uint32_t blocks = (a.dim + kScaleBlock - 1) / kScaleBlock;
     const uint64_t units = uint64_t(a.rows) * blocks;
@@ -98,7 +102,7 @@ __global__ __launch_bounds__(kQuantThreads) void k_fp8_quantize_rows(QuantizeArg
         row[i] = unit < units ? uint32_t(unit / blocks) : ~0u;
         block[i] = uint32_t(unit % blocks);
         const uint32_t at = block[i] * kScaleBlock + lane * 4;
-        load4<T, VEC>(v[i], static_cast<const T *>(a.x) + size_t(row[i]) * a.x_stride + at, row[i] == ~0u ? 0 : int(a.dim) - int(at));
+        load4<T>(v[i], static_cast<const T *>(a.x) + size_t(row[i]) * a.x_stride + at, row[i] == ~0u ? 0 : int(a.dim) - int(at));
     }
 #pragma unroll
     for (int i = 0; i < kQuantUnits; ++i) {
@@ -107,14 +111,14 @@ __global__ __launch_bounds__(kQuantThreads) void k_fp8_quantize_rows(QuantizeArg
         uint32_t stored;
         const float s = scale_of<E8>(most, stored);
         const uint32_t at = block[i] * kScaleBlock + lane * 4;
-        store4<VEC>(a.codes + size_t(row[i]) * a.code_stride + at, codes_of(v[i], s), int(a.dim) - int(at));
+        store4(a.codes + size_t(row[i]) * a.code_stride + at, codes_of<E8>(v[i], s), int(a.dim) - int(at));
         if (lane == 0) store_scale<E8>(a.scales, size_t(row[i]) * a.scale_stride + block[i], stored);
     }
     }
 }
 
 // A scale for each 128 x 128 tile: a workgroup to a tile, sixteen rows to half a wave, which holds them until the scale is known.
-template <typename T, bool E8, bool VEC>
+template <typename T, bool E8>
 __global__ __launch_bounds__(kQuantThreads) void k_fp8_quantize_tiles(QuantizeArgs a) {
     __shared__ float part[kQuantThreads / 32];
     constexpr int kRows = 128 / (kQuantThreads / 32);
@@ -128,7 +132,7 @@ __global__ __launch_bounds__(kQuantThreads) void k_fp8_quantize_tiles(QuantizeAr
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
         const uint32_t row = tile * 128u + uint32_t(i * (kQuantThreads / 32) + half);
-        load4<T, VEC>(v[i], static_cast<const T *>(a.x) + size_t(row) * a.x_stride + at, row < a.rows ? int(a.dim) - int(at) : 0);
+        load4<T>(v[i], static_cast<const T *>(a.x) + size_t(row) * a.x_stride + at, row < a.rows ? int(a.dim) - int(at) : 0);
 #pragma unroll
         for (int j = 0; j < 4; ++j) most = fmaxf(most, finite_abs(v[i][j]));
     }
@@ -142,31 +146,28 @@ __global__ __launch_bounds__(kQuantThreads) void k_fp8_quantize_tiles(QuantizeAr
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
         const uint32_t row = tile * 128u + uint32_t(i * (kQuantThreads / 32) + half);
-        if (row < a.rows) store4<VEC>(a.codes + size_t(row) * a.code_stride + at, codes_of(v[i], s), int(a.dim) - int(at));
+        if (row < a.rows) store4(a.codes + size_t(row) * a.code_stride + at, codes_of<E8>(v[i], s), int(a.dim) - int(at));
     }
     if (threadIdx.x == 0) store_scale<E8>(a.scales, size_t(tile) * a.scale_stride + block, stored);
     __syncthreads();
     }
 }
 
-template <typename T, bool E8, bool VEC>
+template <typename T, bool E8>
 static hipError_t quantize(const QuantizeArgs &a, int group_shift, hipStream_t s) {
     const uint64_t blocks = (a.dim + kScaleBlock - 1) / kScaleBlock;
     if (group_shift == 0) {
         constexpr uint64_t per = kQuantThreads / 32 * kQuantUnits;
         const uint64_t groups = (a.rows * blocks + per - 1) / per;
-        return launch(k_fp8_quantize_rows<T, E8, VEC>, uint32_t(groups < kMostGroups ? groups : kMostGroups), kQuantThreads, 0, s, a);
+        return launch(k_fp8_quantize_rows<T, E8>, uint32_t(groups < kMostGroups ? groups : kMostGroups), kQuantThreads, 0, s, a);
     } else {
         const uint64_t groups = (uint64_t(a.rows) + 127) / 128 * blocks;
-        return launch(k_fp8_quantize_tiles<T, E8, VEC>, uint32_t(groups < kMostGroups ? groups : kMostGroups), kQuantThreads, 0, s, a);
+        return launch(k_fp8_quantize_tiles<T, E8>, uint32_t(groups < kMostGroups ? groups : kMostGroups), kQuantThreads, 0, s, a);
     }
 }
 template <typename T>
 static hipError_t quantize_as(const QuantizeArgs &a, int scale_type, int group_shift, hipStream_t s) {
-    // four values at a time where every row starts at a multiple of four
-    const bool vec = (uintptr_t(a.x) % (4 * sizeof(T)) | a.x_stride % 4 | uintptr_t(a.codes) % 4 | a.code_stride % 4) == 0;
-    if (scale_type == kScaleE8M0) return vec ? quantize<T, true, true>(a, group_shift, s) : quantize<T, true, false>(a, group_shift, s);
-    return vec ? quantize<T, false, true>(a, group_shift, s) : quantize<T, false, false>(a, group_shift, s);
+    return scale_type == kScaleE8M0 ? quantize<T, true>(a, group_shift, s) : quantize<T, false>(a, group_shift, s);
 }
 hipError_t launch_fp8_quantize(const QuantizeArgs &a, int x_type, int scale_type, int group_shift, hipStream_t s) {
     if (x_type == kF32) return quantize_as<float>(a, scale_type, group_shift, s);
