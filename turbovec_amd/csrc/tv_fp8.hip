@@ -36,10 +36,16 @@ __device__ __forceinline__ float finite_abs(float x) {
     return a < __int_as_float(0x7f800000) ? a : 0.0f;      // (a comparison with NaN is false)
 }
 // Largest over the half wave.
+template <int CTRL>
+__device__ __forceinline__ float max_moved(float v) {
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true)));
+}
 __device__ __forceinline__ float half_wave_max(float v) {
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor(v, d));
-    return v;
+    v = max_moved<0xb1>(v);       // quad_perm: the neighbour, the pair beside
+    v = max_moved<0x4e>(v);
+    v = max_moved<0x141>(v);      // row_half_mirror, row_mirror: the other half of 8 and of 16
+    v = max_moved<0x140>(v);
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(v), 0x401f)));      // lane ^ 16
 }
 // The scale of a block whose largest finite magnitude is `most`; `stored` is what goes to memory.
 template <bool E8>
@@ -82,8 +88,8 @@ __device__ __forceinline__ void store_scale(void *scales, size_t at, uint32_t st
     else static_cast<uint32_t *>(scales)[at] = stored;
 }
 
-// A scale for each row: half a wave to a block, four blocks at a time, 16 bytes of floats a lane wherever a row starts (100K of 1535: 158 us, 207 an
-// element at a time).  Bound by memory: 400K rows of 1536 floats take 578 to 610 us, 5.0 to 5.3 TB/s read and
+// A scale for each row: half a wave to a block, four blocks at a time, 16 bytes of floats a lane wherever a row starts (100K of 1535: 145 us, 207 an
+// element at a time).  Bound by memory: 400K rows of 1536 floats take 549 us, 5.6 TB/s read and
 // written (a copy reaches 4.9, half of it writes).
 constexpr int kQuantThreads = 256, kQuantUnits = 4;
 constexpr uint64_t kMostGroups = 1 << 20;    // workgroups of a launch: a grid of 2^32 threads is not allowed
