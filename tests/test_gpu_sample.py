@@ -339,3 +339,31 @@ def test_scores_then_a_draw(sample):
     place, _ = check(sample, s, u, temperature=0.02, top_k=20)
     drawn = slots.gather(1, place[:, None])
     assert bool((drawn >= 0).all())
+
+
+@pytest.mark.parametrize("rows,n", [(3, 1), (3, 100), (3, 5000), (3, 20_000), (3, 50_000), (300, 15_000)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_temperature_that_is_not_above_zero_draws_the_best(sample, rows, n, dtype):
+    """Whatever the other limits say, min-p above all: log(min_p) * T is above 0 there."""
+    g = gen(100 + n)
+    scores = (3 * torch.randn(rows, n, generator=g, device="cuda")).to(dtype)
+    u = torch.rand(rows, generator=g, device="cuda")
+    mask = torch.randint(-2 ** 63, 2 ** 63 - 1, (rows, -(-n // 64)), generator=g, device="cuda", dtype=torch.int64)
+    mask[1] = 0
+    allowed = ((mask[:, :, None] >> torch.arange(64, device="cuda")) & 1).reshape(rows, -1)[:, :n].bool()
+    for m, best in ((None, scores.argmax(1)), (mask, torch.where(allowed.any(1), torch.where(allowed, scores, -torch.inf).argmax(1), -1))):
+        for t in (-1.0, -1e-30, -1e30, -float("inf"), 0.0, -0.0, float("nan")):
+            for limits in (dict(min_p=0.1), dict(min_p=0.9), dict(min_p=1e-30, top_k=7, top_p=0.5), dict(min_p=0.5, top_k=n + 1)):
+                slots, probs = sample(scores, u, mask=m, temperature=t, **limits)
+                assert torch.equal(slots, best), (t, limits)
+                assert torch.equal(probs, (best >= 0).float()), (t, limits)
+
+
+def test_temperatures_of_both_signs_in_one_call(sample):
+    for rows, n in ((40, 3000), (6, 60_000)):
+        g = gen(110 + rows)
+        scores = 3 * torch.randn(rows, n, generator=g, device="cuda")
+        u = torch.rand(rows, generator=g, device="cuda")
+        t = torch.randn(rows, generator=g, device="cuda")
+        check(sample, scores, u, temperature=t, min_p=0.05)
+        check(sample, scores, u, temperature=t, min_p=0.3, top_p=0.9, top_k=torch.arange(rows, device="cuda", dtype=torch.int32) * 3)

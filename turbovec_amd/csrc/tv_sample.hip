@@ -160,12 +160,12 @@ struct SampleRow {
         }
         return lo;
     }
-    // The least key whose weight is min_p (above 0) or more.
+    // The least key whose weight is min_p (above 0) or more; t is above 0.
     __device__ __forceinline__ uint32_t least_of_weight(double min_p, double t) const {
         if (min_p >= 1.0 || !(top < __longlong_as_double(0x7ff0000000000000ll))) return most;
         const double from = top + log(min_p) * t;
         const uint32_t k = score_key(float(from));
-        return max(k + (k != kNoKey && double(float(from)) < from ? 1u : 0u), kNoKey + 1u);
+        return min(max(k + (k != kNoKey && double(float(from)) < from ? 1u : 0u), kNoKey + 1u), most);
     }
     // Of a row's scores, given the largest one's key.
     __device__ __forceinline__ void set(uint32_t most_, float t) {
@@ -277,7 +277,7 @@ struct Limits {
         top_k = p.top_k == nullptr ? 0 : int32_t(uniform(uint32_t(p.top_k[r])));
         top_p = p.top_p == nullptr ? 1.0f : uniform(p.top_p[r]);
         u = uniform(p.u[r]);
-        if (!(t > 0.0f)) { top_k = 1; top_p = 1.0f; }       // the best alone
+        if (!(t > 0.0f)) { top_k = 1; top_p = 1.0f; min_p = 0.0f; }       // the best alone
     }
     template <typename T>
     __device__ __forceinline__ void set(SampleRow<T> &row, uint32_t most) {
