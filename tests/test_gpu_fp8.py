@@ -451,3 +451,98 @@ def test_more_rows_and_queries_than_a_grid_has(fp8):
         for lo in (0, 65_500, 69_900):
             for a, b in zip(got, fp8.rescore(q[lo:lo + 100], rows, slots[lo:lo + 100], 3)):
                 assert torch.equal(a[lo:lo + 100], b)
+
+
+# ---- scales far from 1 -----------------------------------------------------------------------------
+
+# (each sum of rows of b, tiles of 32, 64, 128 and 256, rows of a in LDS)
+FAR_SIZES = [(1, 300), (5, 40), (16, 17_000), (20, 300), (70, 300), (64, 70_000), (1000, 3000), (129, 45_000)]
+
+
+def check_far(a, b, got):
+    """Like check_product, but nothing is lost to subnormal numbers other than the result's own."""
+    x, y = values(a), values(b)
+    want, sums = x @ y.t(), x.abs() @ y.abs().t()
+    dim, blocks = x.shape[1], -(-x.shape[1] // 128)
+    step = torch.finfo(got.dtype).eps / 2
+    # sums in 32 bits, as in check_product; a rounding of each block's sum and of each addition to the smallest 32-bit number, 2^-149, the former
+    # times what is left of the scales when powers of two have been taken out, no more than 2^2 where such a sum is that small; half the result type's own
+    bound = (2 * dim + 3 * blocks) * 2.0 ** -23 * sums + 8 * blocks * 2.0 ** -149 + (0 if got.dtype == torch.float32 else 7 * 2.0 ** -13) * sums
+    bound = bound + (want.abs() + bound) * step + torch.finfo(got.dtype).smallest_normal * step
+    off = (got.double() - want).abs()
+    assert bool((off <= bound).all()), float((off / bound).max())
+
+
+@pytest.mark.parametrize("scale,group", [("f32", 1), ("f32", 128), ("e8m0", 1)])
+@pytest.mark.parametrize("m,n", FAR_SIZES)
+def test_matmul_products_of_scales_that_32_bits_do_not_hold(fp8, scale, group, m, n):
+    """Tiny rows on both sides, whose products are numbers though the products of their scales are not."""
+    x, y = torch.randn(m, 300, generator=gen(200), device="cuda"), torch.randn(n, 300, generator=gen(201), device="cuda")
+    for size in (1e-17, 1e-18, 1e-19, 1e-20):
+        a, b = fp8.quantize(x * size, scale=scale), fp8.quantize(y * size, scale=scale, group=group)
+        for dtype in (torch.float32, torch.bfloat16):
+            got = fp8.matmul(a, b, dtype=dtype)
+            check_far(a, b, got)
+            assert size < 1e-19 or bool((got.abs() > 1e-40).any())
+
+
+@pytest.mark.parametrize("scale,group", [("f32", 1), ("f32", 128), ("e8m0", 1)])
+@pytest.mark.parametrize("m,n", FAR_SIZES)
+def test_matmul_of_huge_rows_that_do_not_meet(fp8, scale, group, m, n):
+    """Coordinates of which one factor is 0 everywhere: 0, however large the scales are."""
+    for size in (1e10, 1e22, 1e23, 1e30, 1e33):
+        x, y = torch.zeros(m, 300, device="cuda"), torch.zeros(n, 300, device="cuda")
+        x[:, ::2], y[:, 1::2] = size, -size
+        a, b = fp8.quantize(x, scale=scale), fp8.quantize(y, scale=scale, group=group)
+        for dtype in DTYPES:
+            assert bool((fp8.matmul(a, b, dtype=dtype) == 0).all()), (size, dtype)
+
+
+@pytest.mark.parametrize("scale,group", [("f32", 1), ("f32", 128), ("e8m0", 1), ("e8m0", 128)])
+@pytest.mark.parametrize("m,n", FAR_SIZES)
+def test_matmul_of_scales_that_make_up_for_each_other(fp8, scale, group, m, n):
+    """Blocks whose scale is far above 1 on one side and as far below on the other: each counts as much as the next."""
+    dim = 128 * 12 + 40
+    power = torch.tensor([0, 60, -60, 63, -63, 64, -64, 65, -65, 90, -90, 102, -102], device="cuda").float()
+
+    def rows(count, group, sign, seed):
+        codes = torch.randint(0, 256, (count, dim), generator=gen(seed), device="cuda").to(torch.uint8)
+        codes[(codes & 0x7f) == 0x7f] = 0x3c
+        s = torch.exp2(sign * power).repeat(-(-count // group), 1)
+        if scale == "f32":
+            s *= 1 + 0.99 * torch.rand(s.shape, generator=gen(seed + 1), device="cuda")
+            return fp8.Fp8Rows(codes.view(torch.float8_e4m3fn), s, group)
+        bytes_ = (127 + sign * power).to(torch.uint8).repeat(len(s), 1)
+        return fp8.Fp8Rows(codes.view(torch.float8_e4m3fn), bytes_.view(torch.float8_e8m0fnu), group)
+
+    a, b = rows(m, 1, 1, 210), rows(n, group, -1, 220)
+    for dtype in (torch.float32, torch.bfloat16):
+        check_far(a, b, fp8.matmul(a, b, dtype=dtype))
+
+
+@pytest.mark.parametrize("group", [1, 128])
+@pytest.mark.parametrize("m,n", FAR_SIZES)
+def test_matmul_scales_that_are_no_numbers(fp8, group, m, n):
+    """A scale of b that is infinite or NaN, negative, 0, or the smallest and the largest there are."""
+    codes = lambda rows, seed: (torch.randint(0x28, 0x48, (rows, 256), generator=gen(seed), device="cuda")).to(torch.uint8).view(torch.float8_e4m3fn)  # noqa: E731
+    inf, nan, tiny = float("inf"), float("nan"), 2.0 ** -149
+    sa = torch.ones(m, 2, device="cuda")
+    sb = torch.ones(-(-n // group), 2, device="cuda")
+    sb[0, 1] = nan
+    if len(sb) > 2:
+        sb[1, 0], sb[2, 0] = inf, -3.0
+    if len(sb) > 20:
+        sb[3], sb[4], sb[5] = 0.0, tiny, 1e-10
+    a, b = fp8.Fp8Rows(codes(m, 230), sa), fp8.Fp8Rows(codes(n, 231), sb, group)
+    for dtype in (torch.float32, torch.bfloat16):
+        got = fp8.matmul(a, b, dtype=dtype)
+        row = torch.arange(n, device="cuda") // group
+        assert bool(torch.isnan(got[:, row == 0]).all())
+        if len(sb) > 2:
+            assert bool((got[:, row == 1] == inf).all())
+        plain = (row != 0) & ((row != 1) | (len(sb) <= 2))
+        if bool(plain.any()):
+            check_far(a, fp8.Fp8Rows(b.codes[plain], sb[row[plain]]), got[:, plain])
+    for x, y in ((2.0 ** 103, tiny), (2.0 ** -108, 3.4e38)):
+        x, y = fp8.Fp8Rows(a.codes, torch.full_like(sa, x)), fp8.Fp8Rows(b.codes, torch.full_like(sb, y), group)
+        check_far(x, y, fp8.matmul(x, y))
