@@ -240,7 +240,8 @@ int tv_fp8_quantize_dev(int device, void *stream, const void *d_x, int x_type, s
 /* out[i][j] = the inner product of row i of a (m rows, a scale of each row) with row j of b (n rows, scales of
  * `group` rows): sums of products of codes within a block times both scales, blocks added in 32 bits, rounded
  * once to out_type.  Float scales multiply a block's sum in 32 bits, a's first: as long as a's lie between 2^-108 and 2^103, nothing is lost
- * to numbers that 32 bits do not hold, but for the result itself.  Rows that start at multiples of 16 bytes (codes and stride) are read fastest.  A result of
+ * to numbers that 32 bits do not hold, but for the result itself.  With e8m0 scales and 32-bit results a coordinate, code * scale, counts as
+ * bfloat16 holds it: infinite from 2^128 on, in multiples of 2^-133.  Rows that start at multiples of 16 bytes (codes and stride) are read fastest.  A result of
  * more tiles than one launch has (2^24 of 64 x 64) fails before anything is written. */
 int tv_fp8_matmul_dev(int device, void *stream, const uint8_t *d_a, size_t a_stride, const void *d_a_scales, size_t a_scale_stride, size_t m,
                       const uint8_t *d_b, size_t b_stride, const void *d_b_scales, size_t b_scale_stride, size_t n, int group,

@@ -546,3 +546,29 @@ def test_matmul_scales_that_are_no_numbers(fp8, group, m, n):
     for x, y in ((2.0 ** 103, tiny), (2.0 ** -108, 3.4e38)):
         x, y = fp8.Fp8Rows(a.codes, torch.full_like(sa, x)), fp8.Fp8Rows(b.codes, torch.full_like(sb, y), group)
         check_far(x, y, fp8.matmul(x, y))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n_scales", [(1, 255), (40, 255), (300, 255)])
+def test_matmul_scale_bytes_at_both_ends(fp8, dtype, m, n_scales):
+    """Every e8m0 scale against those at either end and in between, wherever the products are ordinary numbers.  32-bit results take coordinates as numbers that
+    32 bits hold: 448 * 2^119, byte 246, is the last that they do."""
+    codes = torch.randint(0, 256, (n_scales, 128), generator=gen(240), device="cuda").to(torch.uint8)
+    codes[(codes & 0x78) < 0x30] = 0x38                    # magnitudes of 1/2 and more: their last bit is 2^-4, times 2^-127 a number of bfloat16
+    codes[(codes & 0x7f) == 0x7f] = 0x3e
+    codes[:, 0] = 0x7e                                     # 448
+    scale = torch.arange(n_scales, device="cuda", dtype=torch.uint8)
+    b = fp8.Fp8Rows(codes.view(torch.float8_e4m3fn), scale[:, None].view(torch.float8_e8m0fnu))
+    compared = torch.zeros(n_scales, dtype=torch.bool, device="cuda")
+    for e in (0, 1, 2, 3, 20, 127, 235, 245, 246, 247, 253, 254):
+        a = fp8.Fp8Rows(codes[7:8].expand(m, -1).contiguous().view(torch.float8_e4m3fn), torch.full((m, 1), e, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu))
+        got = fp8.matmul(a, b, dtype=dtype)
+        held = (scale <= 246) & (e <= 246) if dtype == torch.float32 else scale <= 254
+        near = ((scale.long() + e - 254).abs() < 100) & held
+        compared |= near
+        if bool(near.any()):
+            check_far(a, fp8.Fp8Rows(b.codes[near], scale[near][:, None].view(torch.float8_e8m0fnu)), got[:, near])
+        assert bool(near.any()) or (dtype == torch.float32 and e > 246)
+        if dtype == torch.float32:
+            assert not bool(torch.isfinite(got[:, ~held]).any())
+    assert bool(compared[:247].all()) and (dtype == torch.float32 or bool(compared.all()))
