@@ -239,9 +239,13 @@ int tv_fp8_quantize_dev(int device, void *stream, const void *d_x, int x_type, s
                         int scale_type, int group, uint8_t *d_codes, size_t code_stride, void *d_scales, size_t scale_stride);
 /* out[i][j] = the inner product of row i of a (m rows, a scale of each row) with row j of b (n rows, scales of
  * `group` rows): sums of products of codes within a block times both scales, blocks added in 32 bits, rounded
- * once to out_type.  Float scales multiply a block's sum in 32 bits, a's first: as long as a's lie between 2^-108 and 2^103, nothing is lost
- * to numbers that 32 bits do not hold, but for the result itself.  With e8m0 scales and 32-bit results a coordinate, code * scale, counts as
- * bfloat16 holds it: infinite from 2^128 on, in multiples of 2^-133.  Rows that start at multiples of 16 bytes (codes and stride) are read fastest.  A result of
+ * once to out_type.  For 16-bit results the products are added in groups of eight neighbouring coordinates, each
+ * cut off towards zero at 2^-13 of the group's largest (whose factors count as the powers of two at or below them):
+ * on random rows 1.4e-5 of the usual result, so that results close to 0 are off by more of themselves.  32-bit
+ * results lose what 32-bit sums do.  Float scales multiply a block's sum in 32 bits, a's first: as long as a's lie
+ * between 2^-108 and 2^103, nothing is lost to numbers that 32 bits do not hold, but for the result itself.  With e8m0
+ * scales and 32-bit results a coordinate, code * scale, counts as bfloat16 holds it: infinite from 2^128 on, in
+ * multiples of 2^-133.  Rows that start at multiples of 16 bytes (codes and stride) are read fastest.  A result of
  * more tiles than one launch has (2^24 of 64 x 64) fails before anything is written. */
 int tv_fp8_matmul_dev(int device, void *stream, const uint8_t *d_a, size_t a_stride, const void *d_a_scales, size_t a_scale_stride, size_t m,
                       const uint8_t *d_b, size_t b_stride, const void *d_b_scales, size_t b_scale_stride, size_t n, int group,
@@ -250,7 +254,7 @@ int tv_fp8_matmul_dev(int device, void *stream, const uint8_t *d_a, size_t a_str
  * (score desc, slot asc), as the search does: nq * k scores and slots.  Products and sums are taken in 64 bits,
  * a score is rounded once.  A slot below 0 or not below n counts as absent, the same slot twice as two
  * candidates; a query with fewer than k present ends in scores of -infinity at slot -1.  NaN scores come last.
- * Scales that are NaN or infinite make their rows' scores so. */
+ * A scale that is NaN or infinite makes its rows' scores NaN or infinite. */
 int tv_fp8_rescore_dev(int device, void *stream, const void *d_queries, int q_type, size_t q_stride, size_t nq,
                        const uint8_t *d_rows, size_t row_stride, const void *d_scales, size_t scale_stride, size_t n, int group, size_t dim, int scale_type,
                        const int64_t *d_slots, size_t slot_stride, size_t m, size_t k, float *d_out_scores, int64_t *d_out_slots,
@@ -264,7 +268,8 @@ size_t tv_fp8_rescore_workspace(size_t nq, size_t m, size_t dim);
  * slot, in order of slots, at which the running sum of the kept w exceeds u times their sum, 0 <= u < 1.  A temperature
  * that is not above 0 draws the best.  out_probs: w over the sum of the kept ones.  A row that allows nothing: slot -1,
  * probability 0.  Weights are taken in 64 bits and held in whole multiples of 2^-(63 - ceil(log2 n)), rounded down; sums of them are exact,
- * so that a draw never depends on the order of additions.  d_u holds a value a row; each of the four parameters does
+ * so that a draw never depends on the order of additions.  A slot of less weight than that is never drawn, and a row loses less than n times that in all: 2e-5
+ * of the best slot's weight at ten million slots, 0.15 % at 10^8, half of it at 2^31 - 1.  d_u holds a value a row; each of the four parameters does
  * too, or is NULL: temperature 1, no limit. */
 int tv_sample_dev(int device, void *stream, const void *d_scores, int score_type, size_t score_stride, size_t rows, size_t n,
                   const uint64_t *d_mask_words, size_t mask_stride, const float *d_u, const float *d_temperature, const int32_t *d_top_k,

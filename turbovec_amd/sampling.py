@@ -31,7 +31,8 @@ def sample(scores, u, *, temperature=None, top_k=None, top_p=None, min_p=None, m
     float32).  `u` (float32 [rows], in [0, 1)) are the random numbers.  Each parameter is a number or a tensor of a value a row
     (float32, `top_k` int32); None: temperature 1, no limit.  `mask`: int64 words of 64 slots, as `pack_mask` makes
     them, [ceil(n / 64)] for all rows or [rows, ceil(n / 64)].  Slots are limited by top-k, then top-p, then min-p, and drawn in
-    the order of slots; a row that allows nothing gives (-1, 0)."""
+    the order of slots; a row that allows nothing gives (-1, 0).  A slot whose weight is less than 2^-(63 - ceil(log2 n)) of the best one's
+    is never drawn (less than 2e-5 of a draw in all at ten million slots, a third at most at 2^31 - 1)."""
     _gpu("scores", scores, _VALUES)
     rows, n = scores.shape
     if n == 0:
