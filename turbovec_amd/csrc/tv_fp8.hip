@@ -639,17 +639,19 @@ static hipError_t matmul(const MatmulArgs &a, hipStream_t s) {
     if constexpr (EXACT) {
         if (a.a.rows <= 32) return tile<EXACT, SC, 32, 128, 1, 4>(a, s);
     }
-    // A CU's time: the tiles it gets, which come in rounds of as many as it holds at a time, times what one takes.  The rates are those of 1024 by 100000
-    // of 1536: tiles of 256, 128 and 64 take 198, 242 and 339 us into bfloat16, 333, 366 and 444 into floats (a little less for 128: 6.1 rounds of the
-    // 256 count as 7), and of 256 by 1M for 64 x 128: 733 us where 256 takes 526 and 64 900.  A started round costs a whole one: 64 by 100000 takes 28 us
-    // in tiles of 64, 32 of 64 x 128, by 77777 of 1000 29 and 26.  Where few tiles fill the card the small ones win: 300 by 3000 36, 18 and
-    // 10 us, 64 by 20000 18 in tiles of 64 x 128 and 14 of 64.  (Float scales and bfloat16 operands of a 256 x 256 tile do not fit the registers.)
+    // A CU's time: the tiles it gets, which come in rounds of as many as it holds at a time, times what one takes.  The rates come from 24 sizes of 65 to 6000 rows
+    // by 1500 to 200000, of 384 to 4096, each scale kind: at three rounds and more 128 x 128 has 0.88 of the rate of 256 x 256 into floats on the mean
+    // (0.79 to 1.10), 0.86 into 16 bits (0.58 to 1.00), 64 x 128 0.75 and 0.76, 64 x 64 0.70 and 0.61; those taken lose least over all sizes, 1.5 and
+    // 2.3 % of the best tile's time.  6000 by 6000 of 4096 into floats: 266 us in tiles of 256, 282 of 128, 346 of 64 x 128; 1024 by 100000 of 1536 333, 366 and 444
+    // of 64.  A started round costs a whole one: 64 by 100000 takes 28 us in tiles of 64, 32 of 64 x 128, by 77777 of 1000 29 and 26.  Where few tiles fill the card
+    // the small ones win: 300 by 3000 36, 18 and 10 us, 64 by 20000 18 in tiles of 64 x 128 and 14 of 64.  (Float scales and bfloat16 operands of
+    // a 256 x 256 tile do not fit the registers.)
     auto tiles = [&](uint32_t tm, uint32_t tn) { return uint64_t((a.a.rows + tm - 1) / tm) * ((a.b.rows + tn - 1) / tn); };
     auto time = [&](uint32_t tm, uint32_t tn, uint32_t held, double rate) {
         const uint64_t n = tiles(tm, tn), one = 256 * held;
         return double(n <= one ? (n + 255) / 256 : (n + one - 1) / one * held) * tm * tn / rate;
     };
-    const double l = EXACT && SC != kScaleBytes ? HUGE_VAL : time(256, 256, 1, 1.0), m = time(128, 128, 2, EXACT ? 0.85 : 0.8), sm = time(64, 64, 4, EXACT ? 0.75 : 0.58);
+    const double l = EXACT && SC != kScaleBytes ? HUGE_VAL : time(256, 256, 1, 1.0), m = time(128, 128, 2, EXACT ? 0.88 : 0.8), sm = time(64, 64, 4, EXACT ? 0.75 : 0.58);
     const double wide = tiles(64, 128) < 512 ? HUGE_VAL : time(64, 128, 3, EXACT ? 0.78 : 0.72);
     if constexpr (!EXACT || SC == kScaleBytes) {
         if (l <= m && l <= sm && l <= wide) return tile<EXACT, SC, 256, 256, 2, 4>(a, s);
