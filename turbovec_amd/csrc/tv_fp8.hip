@@ -642,7 +642,7 @@ static hipError_t matmul(const MatmulArgs &a, hipStream_t s) {
     // A CU's time: the tiles it gets, which come in rounds of as many as it holds at a time, times what one takes.  The rates come from 24 sizes of 65 to 6000 rows
     // by 1500 to 200000, of 384 to 4096, each scale kind: at three rounds and more 128 x 128 has 0.88 of the rate of 256 x 256 into floats on the mean
     // (0.79 to 1.10), 0.86 into 16 bits (0.58 to 1.00), 64 x 128 0.75 and 0.76, 64 x 64 0.70 and 0.61; those taken lose least over all sizes, 1.5 and
-    // 2.3 % of the best tile's time.  6000 by 6000 of 4096 into floats: 266 us in tiles of 256, 282 of 128, 346 of 64 x 128; 1024 by 100000 of 1536 333, 366 and 444
+    // 2.3 % of the best tile's time.  6000 by 6000 of 4096 into floats: 321 us in tiles of 256, 282 of 128, 346 of 64 x 128; 1024 by 100000 of 1536 333, 366 and 444
     // of 64.  A started round costs a whole one: 64 by 100000 takes 28 us in tiles of 64, 32 of 64 x 128, by 77777 of 1000 29 and 26.  Where few tiles fill the card
     // the small ones win: 300 by 3000 36, 18 and 10 us, 64 by 20000 18 in tiles of 64 x 128 and 14 of 64.  (Float scales and bfloat16 operands of
     // a 256 x 256 tile do not fit the registers.)
