@@ -613,3 +613,35 @@ def test_matmul_16_bit_results_lose_what_is_said(fp8, scale, group, m, n, dim):
     off = root_mean_square((got - said)[small]) / size
     # half a step of float16 of 1/64 of the size and of what is cut off, 2^-13 of a product at most; and of sums of groups and blocks 2^-23 each
     assert off <= 2.0 ** -11 * (1 / 64 + 2.0 ** -13) + 2.0 ** -23 * (dim / 8 + 2 * -(-dim // 128)) ** 0.5, off
+
+
+def test_the_documented_path_from_an_index(fp8):
+    """Numpy slots of a TurboQuantIndex to re-scoring, a mask packed for it to a draw, and rows that move as its slots do."""
+    from turbovec_amd import _lib as T
+    from turbovec_amd.index import TurboQuantIndex
+    from turbovec_amd.sampling import sample
+    n, dim, nq = 3000, 200, 6
+    x = torch.nn.functional.normalize(torch.randn(n, dim, generator=gen(260), device="cuda"))
+    queries = torch.nn.functional.normalize(x[-nq:] + 0.02 * torch.randn(nq, dim, generator=gen(261), device="cuda"))
+    index, rows = TurboQuantIndex(dim, 4), fp8.quantize(x)
+    index.add(x.cpu().numpy())
+
+    def look():
+        slots = torch.from_numpy(index.search(queries.cpu().numpy(), 50)[1]).cuda()
+        check_best(fp8, queries, rows, slots, 10)
+        return fp8.rescore(queries, rows, slots, 10)[1]
+
+    assert torch.equal(look()[:, 0], torch.arange(n - nq, n, device="cuda"))
+    allowed = np.zeros(n, bool)
+    allowed[n - nq:] = allowed[5] = True
+    words = torch.from_numpy(T.pack_mask(allowed)[0].view(np.int64)).cuda()
+    drawn, probs = sample(fp8.matmul(fp8.quantize(queries), rows), torch.rand(nq, generator=gen(262), device="cuda"), temperature=1e-3, mask=words)
+    assert torch.equal(drawn, torch.arange(n - nq, n, device="cuda")) and bool((probs > 0.99).all())
+    for slot in (17, n - nq - 2, n - 2 - 2, 0):
+        last = index.swap_remove(slot)
+        rows.codes.view(torch.uint8)[slot] = rows.codes.view(torch.uint8)[last]
+        rows.scales.view(torch.uint8)[slot] = rows.scales.view(torch.uint8)[last]
+        rows = fp8.Fp8Rows(rows.codes[:last], rows.scales[:last])
+        x[slot] = x[last]
+        x = x[:last]
+        assert torch.equal(look()[:, 0], (queries @ x.t()).argmax(1))

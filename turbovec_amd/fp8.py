@@ -69,7 +69,10 @@ def _workspace(size, device):
 
 class Fp8Rows:
     """`codes` float8_e4m3fn [rows, dim], `scales` [ceil(rows / group), ceil(dim / 128)] of float8_e8m0fnu or float32; a
-    coordinate is code * scale.  `group`: rows that share a scale, 1 or 128."""
+    coordinate is code * scale.  `group`: rows that share a scale, 1 or 128.
+
+    Beside an index row i is its slot i, which is the caller's to keep so: an index's `add` puts new rows at the end, its `swap_remove(i)` the last
+    one in place of row i (with `group` 1 the same move of a row of `codes` and one of `scales`)."""
 
     __slots__ = ("_codes", "_scales", "_group", "_scale_type")
 
@@ -157,8 +160,8 @@ def matmul(a, b, *, dtype=torch.float32, out=None):
 
 
 def rescore(queries, rows, slots, k):
-    """The `k` best of each query's own candidate `slots` (int64 [queries, candidates], as a search returns them), scored against
-    their 8-bit rows (tv_fp8_rescore_dev): (scores float32, slots int64), sorted (score desc, slot asc).  Slots outside the
+    """The `k` best of each query's own candidate `slots` (int64 [queries, candidates] on their device: `torch.from_numpy` of
+    those that `TurboQuantIndex.search` returns, or what tv_search_dev wrote there), scored against their 8-bit rows (tv_fp8_rescore_dev): (scores float32, slots int64), sorted (score desc, slot asc).  Slots outside the
     rows count as absent; a query with fewer than `k` present ends in (-inf, -1)."""
     if not isinstance(rows, Fp8Rows):
         raise TypeError(f"rows must be Fp8Rows, got {type(rows).__name__}")

@@ -29,8 +29,9 @@ def _a_row(name, value, rows, dtype, device):
 def sample(scores, u, *, temperature=None, top_k=None, top_p=None, min_p=None, mask=None):
     """One slot from each row of `scores` (float32, float16 or bfloat16 [rows, n]; tv_sample_dev): (slots int64, probabilities
     float32).  `u` (float32 [rows], in [0, 1)) are the random numbers.  Each parameter is a number or a tensor of a value a row
-    (float32, `top_k` int32); None: temperature 1, no limit.  `mask`: int64 words of 64 slots, as `pack_mask` makes
-    them, [ceil(n / 64)] for all rows or [rows, ceil(n / 64)].  Slots are limited by top-k, then top-p, then min-p, and drawn in
+    (float32, `top_k` int32); None: temperature 1, no limit.  `mask`: int64 words of 64 slots, slot i in bit
+    i % 64 of word i // 64 (`torch.from_numpy(_lib.pack_mask(allowed)[0].view(numpy.int64))`, moved to the scores' device), [ceil(n / 64)] for all rows or
+    [rows, ceil(n / 64)].  Slots are limited by top-k, then top-p, then min-p, and drawn in
     the order of slots; a row that allows nothing gives (-1, 0).  A slot whose weight is less than 2^-(63 - ceil(log2 n)) of the best one's
     is never drawn (less than 2e-5 of a draw in all at ten million slots, a third at most at 2^31 - 1)."""
     _gpu("scores", scores, _VALUES)
