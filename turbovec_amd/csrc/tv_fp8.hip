@@ -195,7 +195,7 @@ hipError_t launch_fp8_quantize(const QuantizeArgs &a, int x_type, int scale_type
 // multiply-add a result, and one more multiplication where both sides have a scale of each row.  The product of two scales may lie outside 32 bits
 // where the result is a number (rows of 1e-20 on both sides, or of 1e23 whose products are 0), so it is not taken: the sum is multiplied
 // by a's scale, then by b's.  Where 128 rows of b share theirs, its power of two goes into their operand and what is left, 1 to 2, into a's scale.
-// (Taking the products costs nothing less, but for 4096 by 4096 of 4096 with shared scales: 67 us, and 69 so.  Powers of two into the operands for each row
+// (As fast as taking that product, except 4096 by 4096 of 4096 with shared scales: 69 us for 67.  Powers of two into the operands for each row
 // of both sides: 1024 by 20000 of 1536 into floats 90 us where this takes 82.)
 //
 // A lane of a matrix operand holds 32 codes of one row in a block.  Which 32 of the 128 does not matter as long as both operands
@@ -411,8 +411,9 @@ static hipError_t direct(const MatmulArgs &a, hipStream_t s) {
 // run that belongs there.
 //
 // Bound by the matrix unit and what feeds it: 4096 rows by 4096 of 4096 coordinates into bfloat16 56 us with e8m0 scales (2.4 PFLOP/s) and
-// 66 to 73 with floats (1.9 to 2.1; their multiply-adds), where the library's 8-bit product of that size, one scale for all of it, takes 49.  1024 by 100000
-// of 1536 into floats 320 to 336 us, 0.94 to 0.98 PFLOP/s; the library's bfloat16 product of a large size reaches 1.16.
+// 69 to 76 with floats (1.8 to 2.0, the matrix units busy for 48 %: the multiply-adds of a row step follow all its products), where the library's 8-bit product
+// of that size, one scale for all of it, takes 49.  1024 by 100000 of 1536 into floats 316 to 336 us, 0.94 to 1.0 PFLOP/s; the library's bfloat16 product of a
+// large size reaches 1.16.
 enum { kScaleBytes = 0, kScaleRows = 1, kScaleTiles = 2 };      // e8m0; floats of each row of b; floats of 128 rows of b
 
 __device__ __forceinline__ void load16_to_lds(uint32_t lds, const uint8_t *base, uint32_t offset) {

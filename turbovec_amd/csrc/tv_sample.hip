@@ -11,7 +11,7 @@
 // few, they are gathered, and everything else happens among them.  Top-k's slots are gathered without it where the best scores of the threads tell
 // which (list_top), top-p's where min-p does (list_kept).  Bound by the passes over the row, two to six, and the exponentials (20 64-bit
 // instructions each); a single row by what a pass takes at least, and by the fetching of its own instructions (one loop serves every
-// search for that).  256 rows of 100000 bfloat16 scores, top-p 0.95 and min-p 0.001: 92 us, top-k 50 and top-p 0.9: 43; one row of 100000, top-k 50 and top-p 0.9: 30 to
+// search for that).  256 rows of 100000 bfloat16 scores, top-p 0.95 and min-p 0.001: 89 to 92 us, top-k 50 and top-p 0.9: 43; one row of 100000, top-k 50 and top-p 0.9: 29 to
 // 34; ten million, half of them masked, top-p 0.5: 103.
 #include <algorithm>
 
