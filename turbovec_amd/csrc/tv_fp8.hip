@@ -190,7 +190,7 @@ hipError_t launch_fp8_quantize(const QuantizeArgs &a, int x_type, int scale_type
 //    large products.  In bfloat16 operands these results would be 24 bits good and take 2.3 times as long.  4.2 PFLOP/s measured on registers alone.
 //  * 32-bit results: the same codes as bfloat16, which holds them exactly, and the 16 x 16 x 32 instructions for those, whose sums
 //    round as 32-bit ones do (1e-8).  1.8 PFLOP/s.  A power-of-two scale goes in with the conversion (one instruction for two
-//    codes, scale included), exactly as long as code * scale is a normal number.
+//    codes, scale included), exactly as long as code * scale is one of bfloat16's: below 2^128, a multiple of 2^-133.
 // Power-of-two scales cost no instruction in either form.  Scales that are floats multiply each block's sum: a
 // multiply-add a result, and one more multiplication where both sides have a scale of each row.  The product of two scales may lie outside 32 bits
 // where the result is a number (rows of 1e-20 on both sides, or of 1e23 whose products are 0), so it is not taken: the sum is multiplied
@@ -640,7 +640,7 @@ static hipError_t matmul(const MatmulArgs &a, hipStream_t s) {
     if constexpr (EXACT) {
         if (a.a.rows <= 32) return tile<EXACT, SC, 32, 128, 1, 4>(a, s);
     }
-    // A CU's time: the tiles it gets, which come in rounds of as many as it holds at a time, times what one takes.  The rates come from 24 sizes of 65 to 6000 rows
+    // A CU's time: the tiles it gets, which come in rounds of as many as it holds at a time, times what one takes.  The rates come from 26 sizes of 65 to 6000 rows
     // by 1500 to 200000, of 384 to 4096, each scale kind: at three rounds and more 128 x 128 has 0.88 of the rate of 256 x 256 into floats on the mean
     // (0.79 to 1.10), 0.86 into 16 bits (0.58 to 1.00), 64 x 128 0.75 and 0.76, 64 x 64 0.70 and 0.61; those taken lose least over all sizes, 1.5 and
     // 2.3 % of the best tile's time.  6000 by 6000 of 4096 into floats: 321 us in tiles of 256, 282 of 128, 346 of 64 x 128; 1024 by 100000 of 1536 333, 366 and 444
