@@ -203,8 +203,9 @@ size_t tv_noalloc_scratch_bytes(void);
 
 /* ---- operators beside the search ------------------------------------------
  *
- * Rows in 8 bits, their products, re-scoring of what a search returned, and
- * drawing a slot from scores.  No counterpart in the reference.  They hold no
+ * Rows in 8 and 4 bits, their products, re-scoring of what a search returned,
+ * a norm that ends in such rows, drawing a slot from scores, and log probabilities
+ * of slots with their gradient.  No counterpart in the reference.  They hold no
  * state and take no index: every pointer but `stream` is a device pointer of
  * `device`, and the call puts its kernels on `stream` (a hipStream_t of that
  * device; NULL: its default stream) and returns without waiting.  Inputs must
@@ -275,6 +276,59 @@ int tv_sample_dev(int device, void *stream, const void *d_scores, int score_type
                   const uint64_t *d_mask_words, size_t mask_stride, const float *d_u, const float *d_temperature, const int32_t *d_top_k,
                   const float *d_top_p, const float *d_min_p, int64_t *d_out_slots, float *d_out_probs, void *d_workspace, size_t workspace_bytes);
 size_t tv_sample_workspace(size_t rows, size_t n);
+
+/* 4-bit rows hold e2m1 codes (1 sign, 2 exponent bits, 1 of mantissa: 0, 0.5, 1, 1.5, 2, 3, 4, 6; the sign is the highest
+ * bit) of dim coordinates, 1 to 16384, two a byte, coordinate 2i in the low half of byte i, and an e8m0 scale for every
+ * block of 32 coordinates (the last may be shorter) of a row.  A coordinate is code * scale.  The high half of the last byte of an
+ * odd dim is written as 0 and not looked at.  Strides of codes and scales count bytes. */
+
+/* Makes 4-bit rows of values.  With `amax` the largest magnitude of a block, its scale is the smallest power of two 2^e,
+ * e >= -126, with amax < 7 * 2^e (so that the largest value is off by half a step at most, as all others are); codes are x / scale
+ * rounded to the nearest, ties to even, at most 6.  There is no code for them: an infinity or a NaN makes its block's scale NaN (255). */
+int tv_fp4_quantize_dev(int device, void *stream, const void *d_x, int x_type, size_t x_stride, size_t rows, size_t dim,
+                        uint8_t *d_codes, size_t code_stride, uint8_t *d_scales, size_t scale_stride);
+/* The coordinates that 4-bit rows stand for: code * scale rounded once to out_type (32 bits hold it as long as it is below 2^128, bfloat16 too). */
+int tv_fp4_values_dev(int device, void *stream, const uint8_t *d_codes, size_t code_stride, const uint8_t *d_scales, size_t scale_stride,
+                      size_t rows, size_t dim, void *d_out, int out_type, size_t out_stride);
+/* out[i][j] = the inner product of row i of a (m rows) with row j of b (n rows): products of codes within a block times both scales, added in
+ * 32 bits and rounded once to out_type.  A block's sum is exact; a sum of blocks loses what 32-bit sums do, and is infinite where it, or
+ * a block's part of it, passes 2^128.  Rows that start at multiples of 16 bytes (codes and stride) are read fastest.  A result of more tiles than one
+ * launch has (2^24 of 64 x 64) fails before anything is written. */
+int tv_fp4_matmul_dev(int device, void *stream, const uint8_t *d_a, size_t a_stride, const uint8_t *d_a_scales, size_t a_scale_stride, size_t m,
+                      const uint8_t *d_b, size_t b_stride, const uint8_t *d_b_scales, size_t b_scale_stride, size_t n,
+                      size_t dim, void *d_out, int out_type, size_t out_stride);
+
+/* Kinds of rows that a norm ends in. */
+typedef enum { TV_ROWS_FP8 = 0, TV_ROWS_FP4 = 1 } tv_row_kind;
+
+/* h = x + residual (d_residual NULL: x), y = h / sqrt(mean of h^2 over the row + eps) * weight (d_weight NULL: 1), taken in 32 bits
+ * and made into rows of 8 bits, as tv_fp8_quantize_dev with a group of 1, or of 4 (scale_type TV_SCALE_E8M0), as tv_fp4_quantize_dev.  The norm is of h before
+ * it is rounded; d_sum, unless NULL, receives h rounded to x_type.  x, residual and sum have x_type; the sum may take the place of
+ * x or of the residual (same address and stride) and overlaps neither in any other way.  eps: finite, not below 0.  A row of zeros with eps 0 has
+ * no norm, nor has one with a NaN or an infinity: its values are NaN.  (Squares are added in 32 bits: an |h| from 2^63 on counts as infinite, and where a row is
+ * below 2^-63 throughout, eps is what remains.) */
+int tv_rms_norm_dev(int device, void *stream, const void *d_x, int x_type, size_t x_stride, const void *d_residual, size_t residual_stride,
+                    void *d_sum, size_t sum_stride, const void *d_weight, int weight_type, float eps, size_t rows, size_t dim,
+                    int row_kind, int scale_type, uint8_t *d_codes, size_t code_stride, void *d_scales, size_t scale_stride);
+
+/* Log probabilities under a softmax of rows of n scores, divided by a temperature a row (NULL: 1; one that is not above 0 is the limit
+ * from above, the best slots share the mass).  Slots whose mask bit is not set (d_mask_words NULL: all are; mask_stride 0: one mask for all rows) and slots of score
+ * -infinity have probability 0, whatever else stands there.  For each row: out_log_probs, of the `given` slots in d_slots (-infinity for a slot of
+ * probability 0 or outside 0 .. n - 1; the same slot may stand there twice); out_entropy, -sum p log p; the `top` slots of the highest scores,
+ * ties to the lower slot, with their log probabilities (slot -1, -infinity where fewer have a probability; a NaN is not among them).  given and top are at
+ * most 128; either may be 0.  A row with nothing allowed has entropy 0; one where an allowed score is NaN or +infinity has NaN for
+ * the entropy and every log probability that is not -infinity.  d_out_stats, unless NULL, receives four floats a row for the gradient.  All sums are taken in 32 bits. */
+int tv_log_probs_dev(int device, void *stream, const void *d_scores, int score_type, size_t score_stride, size_t rows, size_t n,
+                     const uint64_t *d_mask_words, size_t mask_stride, const float *d_temperature, const int64_t *d_slots, size_t slot_stride, size_t given,
+                     size_t top, float *d_out_log_probs, float *d_out_entropy, int64_t *d_out_top_slots, float *d_out_top_log_probs, float *d_out_stats,
+                     void *d_workspace, size_t workspace_bytes);
+size_t tv_log_probs_workspace(size_t rows, size_t n, size_t top);
+/* The gradient of the scores, in their type, from those of the log probabilities and of the entropy (either may be NULL), with the call's own inputs and the stats
+ * that it left: (sum over given of g [slot] - G p - g_entropy p (log p + entropy)) / temperature, G the sum of g over given slots that have a
+ * probability; a slot of probability 0 has gradient 0, and so has a row whose temperature is not above 0.  The same given slot twice adds up. */
+int tv_log_probs_grad_dev(int device, void *stream, const void *d_scores, int score_type, size_t score_stride, size_t rows, size_t n,
+                          const uint64_t *d_mask_words, size_t mask_stride, const float *d_temperature, const int64_t *d_slots, size_t slot_stride, size_t given,
+                          const float *d_stats, const float *d_grad_log_probs, const float *d_grad_entropy, void *d_grad_scores, size_t grad_stride);
 
 /* ---- host-only derivations (no GPU touched) ------------------------------- */
 

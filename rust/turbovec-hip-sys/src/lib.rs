@@ -47,6 +47,10 @@ pub const TV_BF16: c_int = 2;
 pub const TV_SCALE_E8M0: c_int = 0;
 pub const TV_SCALE_F32: c_int = 1;
 
+// tv_row_kind
+pub const TV_ROWS_FP8: c_int = 0;
+pub const TV_ROWS_FP4: c_int = 1;
+
 extern "C" {
     pub fn tv_status_string(status: c_int) -> *const c_char;
     pub fn tv_last_error() -> *const c_char;
@@ -87,6 +91,13 @@ extern "C" {
     pub fn tv_fp8_rescore_workspace(nq: usize, m: usize, dim: usize) -> usize;
     pub fn tv_sample_dev(device: c_int, stream: *mut c_void, d_scores: *const c_void, score_type: c_int, score_stride: usize, rows: usize, n: usize, d_mask_words: *const u64, mask_stride: usize, d_u: *const c_float, d_temperature: *const c_float, d_top_k: *const i32, d_top_p: *const c_float, d_min_p: *const c_float, d_out_slots: *mut i64, d_out_probs: *mut c_float, d_workspace: *mut c_void, workspace_bytes: usize) -> c_int;
     pub fn tv_sample_workspace(rows: usize, n: usize) -> usize;
+    pub fn tv_fp4_quantize_dev(device: c_int, stream: *mut c_void, d_x: *const c_void, x_type: c_int, x_stride: usize, rows: usize, dim: usize, d_codes: *mut u8, code_stride: usize, d_scales: *mut u8, scale_stride: usize) -> c_int;
+    pub fn tv_fp4_values_dev(device: c_int, stream: *mut c_void, d_codes: *const u8, code_stride: usize, d_scales: *const u8, scale_stride: usize, rows: usize, dim: usize, d_out: *mut c_void, out_type: c_int, out_stride: usize) -> c_int;
+    pub fn tv_fp4_matmul_dev(device: c_int, stream: *mut c_void, d_a: *const u8, a_stride: usize, d_a_scales: *const u8, a_scale_stride: usize, m: usize, d_b: *const u8, b_stride: usize, d_b_scales: *const u8, b_scale_stride: usize, n: usize, dim: usize, d_out: *mut c_void, out_type: c_int, out_stride: usize) -> c_int;
+    pub fn tv_rms_norm_dev(device: c_int, stream: *mut c_void, d_x: *const c_void, x_type: c_int, x_stride: usize, d_residual: *const c_void, residual_stride: usize, d_sum: *mut c_void, sum_stride: usize, d_weight: *const c_void, weight_type: c_int, eps: c_float, rows: usize, dim: usize, row_kind: c_int, scale_type: c_int, d_codes: *mut u8, code_stride: usize, d_scales: *mut c_void, scale_stride: usize) -> c_int;
+    pub fn tv_log_probs_dev(device: c_int, stream: *mut c_void, d_scores: *const c_void, score_type: c_int, score_stride: usize, rows: usize, n: usize, d_mask_words: *const u64, mask_stride: usize, d_temperature: *const c_float, d_slots: *const i64, slot_stride: usize, given: usize, top: usize, d_out_log_probs: *mut c_float, d_out_entropy: *mut c_float, d_out_top_slots: *mut i64, d_out_top_log_probs: *mut c_float, d_out_stats: *mut c_float, d_workspace: *mut c_void, workspace_bytes: usize) -> c_int;
+    pub fn tv_log_probs_workspace(rows: usize, n: usize, top: usize) -> usize;
+    pub fn tv_log_probs_grad_dev(device: c_int, stream: *mut c_void, d_scores: *const c_void, score_type: c_int, score_stride: usize, rows: usize, n: usize, d_mask_words: *const u64, mask_stride: usize, d_temperature: *const c_float, d_slots: *const i64, slot_stride: usize, given: usize, d_stats: *const c_float, d_grad_log_probs: *const c_float, d_grad_entropy: *const c_float, d_grad_scores: *mut c_void, grad_stride: usize) -> c_int;
 
     // ---- host-only derivations ----
     pub fn tv_host_rotation_tables(dim: c_int, signs: *mut c_float, perms: *mut u32, block: *mut c_int, inv_sqrt_block: *mut c_float) -> c_int;

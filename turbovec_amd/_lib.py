@@ -25,6 +25,7 @@ SCORE_AUTO, SCORE_L_SCALAR, SCORE_L_CLASSIC, SCORE_L_U32, SCORE_P = 0, 1, 2, 3, 
 
 F32, F16, BF16 = 0, 1, 2                       # tv_value_type
 SCALE_E8M0, SCALE_F32 = 0, 1                   # tv_scale_type
+ROWS_FP8, ROWS_FP4 = 0, 1                      # tv_row_kind
 
 # every symbol include/turbovec_hip.h declares
 EXPORTS = [
@@ -39,6 +40,7 @@ EXPORTS = [
     "tv_debug_exact_redos", "tv_debug_sampling_plan", "tv_debug_merged_calls", "tv_debug_level_repeats", "tv_debug_workspace_bytes",
     "tv_debug_gathered_searches",
     "tv_fp8_quantize_dev", "tv_fp8_matmul_dev", "tv_fp8_rescore_dev", "tv_fp8_rescore_workspace", "tv_sample_dev", "tv_sample_workspace",
+    "tv_fp4_quantize_dev", "tv_fp4_values_dev", "tv_fp4_matmul_dev", "tv_rms_norm_dev", "tv_log_probs_dev", "tv_log_probs_workspace", "tv_log_probs_grad_dev",
 ]
 
 _lib = None
@@ -124,6 +126,14 @@ def lib():
     L.tv_sample_dev.argtypes = [i32, vp, vp, i32, sz, sz, sz, vp, sz, vp, vp, vp, vp, vp, vp, vp, vp, sz]
     L.tv_sample_workspace.restype = sz
     L.tv_sample_workspace.argtypes = [sz, sz]
+    L.tv_fp4_quantize_dev.argtypes = [i32, vp, vp, i32, sz, sz, sz, vp, sz, vp, sz]
+    L.tv_fp4_values_dev.argtypes = [i32, vp, vp, sz, vp, sz, sz, sz, vp, i32, sz]
+    L.tv_fp4_matmul_dev.argtypes = [i32, vp, vp, sz, vp, sz, sz, vp, sz, vp, sz, sz, sz, vp, i32, sz]
+    L.tv_rms_norm_dev.argtypes = [i32, vp, vp, i32, sz, vp, sz, vp, sz, vp, i32, C.c_float, sz, sz, i32, i32, vp, sz, vp, sz]
+    L.tv_log_probs_dev.argtypes = [i32, vp, vp, i32, sz, sz, sz, vp, sz, vp, vp, sz, sz, sz, vp, vp, vp, vp, vp, vp, sz]
+    L.tv_log_probs_workspace.restype = sz
+    L.tv_log_probs_workspace.argtypes = [sz, sz, sz]
+    L.tv_log_probs_grad_dev.argtypes = [i32, vp, vp, i32, sz, sz, sz, vp, sz, vp, vp, sz, sz, vp, vp, vp, vp, sz]
     _lib = L
     return L
 

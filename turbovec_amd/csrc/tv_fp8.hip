@@ -6,93 +6,19 @@
 #include <cmath>
 
 #include "tv_device.h"
-#include "tv_ops.h"
+#include "tv_rows.h"
 
 namespace tv {
-
-typedef int v8i __attribute__((ext_vector_type(8)));
-typedef float v4f __attribute__((ext_vector_type(4)));
 
 // ---------------------------------------------------------------------------
 // Making 8-bit rows.  Scale of a block: amax / 448 over its finite values, or the smallest power of two not below that; codes
 // are x / scale rounded to the nearest, ties to even.
 // ---------------------------------------------------------------------------
 
-// Four values from p, those of them past `left` zero.
-template <typename T>
-__device__ __forceinline__ void load4(float (&v)[4], const T *p, int left) {
-    typedef T T4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-    if (left >= 4) {
-        const T4 x = *reinterpret_cast<const T4 *>(p);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = float(x[i]);
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < left ? float(p[i]) : 0.0f;
-}
-__device__ __forceinline__ float finite_abs(float x) {
-    const float a = fabsf(x);
-    return a < __int_as_float(0x7f800000) ? a : 0.0f;      // (a comparison with NaN is false)
-}
-// Largest over the half wave.
-template <int CTRL>
-__device__ __forceinline__ float max_moved(float v) {
-    return fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true)));
-}
-__device__ __forceinline__ float half_wave_max(float v) {
-    v = max_moved<0xb1>(v);       // quad_perm: the neighbour, the pair beside
-    v = max_moved<0x4e>(v);
-    v = max_moved<0x141>(v);      // row_half_mirror, row_mirror: the other half of 8 and of 16
-    v = max_moved<0x140>(v);
-    return fmaxf(v, __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(v), 0x401f)));      // lane ^ 16
-}
-// The scale of a block whose largest finite magnitude is `most`; `stored` is what goes to memory.
-template <bool E8>
-__device__ __forceinline__ float scale_of(float most, uint32_t &stored) {
-    if (!E8) {
-        const float s = fmaxf(most / 448.0f, 0x1p-126f);
-        stored = __float_as_uint(s);
-        return s;
-    }
-    // most = f * 2^e with 1 <= f < 2, 448 = 1.75 * 2^8: the power is e - 8, one more where f > 1.75
-    const uint32_t b = __float_as_uint(most);
-    const int e = int(b >> 23) - 127 - 8 + int((b & 0x7fffffu) > 0x600000u);
-    const int power = e < -126 ? -126 : e;                 // (denormal maxima, zero among them, end here)
-    stored = uint32_t(power + 127);
-    return __uint_as_float(stored << 23);
-}
-template <bool E8>
-__device__ __forceinline__ uint32_t codes_of(const float (&v)[4], float s) {
-    // (the inverse of a power of two from 2^-126 to 2^120 is one, so that the product is the quotient)
-    const float inverse = E8 ? __uint_as_float((254u << 23) - __float_as_uint(s)) : 0.0f;
-    float q[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = fabsf(v[i]) < __int_as_float(0x7f800000) ? (E8 ? v[i] * inverse : v[i] / s) : __int_as_float(0x7fc00000);
-    int r = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
-    return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], r, true));
-}
-__device__ __forceinline__ void store4(uint8_t *p, uint32_t c, int left) {
-    typedef uint32_t Four __attribute__((aligned(1)));
-    if (left >= 4) {
-        *reinterpret_cast<Four *>(p) = c;
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (i < left) p[i] = uint8_t(c >> (8 * i));
-}
-template <bool E8>
-__device__ __forceinline__ void store_scale(void *scales, size_t at, uint32_t stored) {
-    if (E8) static_cast<uint8_t *>(scales)[at] = uint8_t(stored);
-    else static_cast<uint32_t *>(scales)[at] = stored;
-}
-
 // A scale for each row: half a wave to a block, four blocks at a time, 16 bytes of floats a lane wherever a row starts (100K of 1535: 145 us, 207 an
 // element at a time).  Bound by memory: 400K rows of 1536 floats take 549 us, 5.6 TB/s read and
 // written (a copy reaches 4.9, half of it writes).
 constexpr int kQuantThreads = 256, kQuantUnits = 4;
-constexpr uint64_t kMostGroups = 1 << 20;    // workgroups of a launch: a grid of 2^32 threads is not allowed
 template <typename T, bool E8>
 __global__ __launch_bounds__(kQuantThreads) void k_fp8_quantize_rows(QuantizeArgs a) {
     const uint32_t blocks = (a.dim + kScaleBlock - 1) / kScaleBlock;
@@ -232,10 +158,6 @@ __device__ __forceinline__ v4f block_product(const Operand<true> &x, const Opera
 #pragma unroll
     for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v[i], y.v[i], c, 0, 0, 0);
     return c;
-}
-// An e8m0 byte as a float; 255 is NaN, and 0 the denormal 2^-127.
-__device__ __forceinline__ float e8_value(uint32_t e) {
-    return __uint_as_float(e == 255u ? 0x7fc00000u : e == 0u ? 0x00400000u : e << 23);
 }
 // The power of two (an e8m0 byte) that the operand takes of a scale that rows of b share, and what is left.  From 2^-100 to 2^103: codes times that
 // are normal numbers, and sums of their products less than 2^128.

@@ -1,4 +1,5 @@
-// The operators beside the search: 8-bit rows, their products, re-scoring of candidates, drawing from scores.
+// The operators beside the search: 8- and 4-bit rows, their products, norms that end in them, re-scoring of candidates, drawing from scores and
+// log probabilities.
 // What the entry points (tv_ops.hip) hand to the kernels; every size has been checked there.
 #pragma once
 #include <hip/hip_runtime.h>
@@ -69,6 +70,83 @@ struct SampleArgs {
 };
 size_t sample_workspace(size_t rows, size_t n);
 hipError_t launch_sample(const SampleArgs &a, int score_type, hipStream_t s);
+
+constexpr int kScaleBlock4 = 32;      // coordinates that share a scale in 4-bit rows
+// Rows in 4 bits: two e2m1 codes a byte and an e8m0 scale for each block of 32 coordinates.  Strides in bytes.
+struct Rows4 {
+    const uint8_t *codes, *scales;
+    size_t stride, scale_stride;
+    uint32_t rows;
+};
+
+struct Quantize4Args {
+    const void *x;
+    uint8_t *codes, *scales;
+    size_t x_stride, code_stride, scale_stride;
+    uint32_t rows, dim;
+};
+hipError_t launch_fp4_quantize(const Quantize4Args &a, int x_type, hipStream_t s);
+
+struct Values4Args {
+    Rows4 rows;
+    uint32_t dim;
+    void *out;
+    size_t out_stride;
+};
+hipError_t launch_fp4_values(const Values4Args &a, int out_type, hipStream_t s);
+
+struct Matmul4Args {
+    Rows4 a, b;
+    uint32_t dim;
+    void *out;
+    size_t out_stride;
+    int out_type;
+};
+hipError_t launch_fp4_matmul(const Matmul4Args &a, hipStream_t s);
+
+enum { kRowsFp8 = 0, kRowsFp4 = 1 };
+struct NormArgs {
+    const void *x, *residual;         // residual: may be null
+    void *sum;                        // may be null, x or residual
+    const void *weight;               // may be null
+    uint8_t *codes;
+    void *scales;
+    size_t x_stride, residual_stride, sum_stride, code_stride, scale_stride;
+    uint32_t rows, dim;
+    int weight_type;
+    float eps;
+};
+hipError_t launch_rms_norm(const NormArgs &a, int x_type, int row_kind, int scale_type, hipStream_t s);
+
+constexpr uint32_t kMostGiven = 128, kMostTop = 128;
+struct LogProbArgs {
+    const void *scores;
+    const uint64_t *mask;             // null: every slot is allowed
+    const float *temperature;         // a value a row, or null
+    const int64_t *slots;
+    size_t stride, mask_stride, slot_stride;
+    uint32_t rows, n, given, top;
+    float *out_log_probs, *out_entropy;
+    int64_t *out_top_slots;
+    float *out_top_log_probs;
+    float *stats;                     // may be null
+    uint8_t *ws;
+};
+size_t log_probs_workspace(size_t rows, size_t n, size_t top);
+hipError_t launch_log_probs(const LogProbArgs &a, int score_type, hipStream_t s);
+
+struct LogProbGradArgs {
+    const void *scores;
+    const uint64_t *mask;
+    const float *temperature;
+    const int64_t *slots;
+    size_t stride, mask_stride, slot_stride;
+    uint32_t rows, n, given;
+    const float *stats, *grad_log_probs, *grad_entropy;      // the last two may be null
+    void *grad;
+    size_t grad_stride;
+};
+hipError_t launch_log_probs_grad(const LogProbGradArgs &a, int score_type, hipStream_t s);
 
 // For tv_last_error (tv_api.hip).
 int op_refused(const char *why);      // TV_ERR_BAD_ARGUMENT
