@@ -81,51 +81,379 @@ hipError_t launch_fp4_values(const Values4Args &a, int out_type, hipStream_t s) 
 // A lane holds 32 codes of one row, one block: lane group g the g-th block of 128 coordinates.
 // ---------------------------------------------------------------------------
 
-// The 32 codes from coordinate 2 * k on, those past the row's end zero.
-__device__ __forceinline__ v4i codes32(const uint8_t *row, uint32_t k, uint32_t dim) {
-    const uint32_t bytes = (dim + 1u) / 2u;
-    if (k >= bytes) return v4i{0, 0, 0, 0};
-    v4i v = codes16(row, k, bytes);
-    if ((dim & 1u) && bytes - k <= 16u) {
-        const uint32_t last = bytes - 1u - k;
+// Sixteen bytes of a row's codes from byte k on without the half byte behind an odd dimension.
+__device__ __forceinline__ v4i without_half(v4i v, uint32_t k, uint32_t dim) {
+    if (dim & 1u) {
+        const uint32_t last = (dim + 1u) / 2u - 1u - k;          // (of no word where the row ends elsewhere)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (last / 4u == uint32_t(i)) v[i] &= int(~(0xf0u << (last % 4u * 8u)));
     }
     return v;
 }
+// The 32 codes from byte k of a row on, those past the row's end zero.
+__device__ __forceinline__ v4i codes32(const uint8_t *row, uint32_t k, uint32_t dim) {
+    const uint32_t bytes = (dim + 1u) / 2u;
+    return k >= bytes ? v4i{0, 0, 0, 0} : without_half(codes16(row, k, bytes), k, dim);
+}
+// Four scale bytes of a row from block k on; those past the end are 2^0 (their codes are 0, and a NaN would show).
+__device__ __forceinline__ uint32_t scales4(const uint8_t *row, uint32_t k, uint32_t blocks) {
+    uint32_t s = 0x7f7f7f7fu;
+    if (k + 4u <= blocks) __builtin_memcpy(&s, row + k, 4);
+    else
+#pragma unroll
+        for (uint32_t i = 0; i < 3; ++i)
+            if (k + i < blocks) s = (s & ~(255u << (8 * i))) | uint32_t(row[k + i]) << (8 * i);
+    return s;
+}
 __device__ __forceinline__ v8i operand4(v4i v) { return v8i{v[0], v[1], v[2], v[3], 0, 0, 0, 0}; }
 
-template <typename T>
-__global__ __launch_bounds__(64) void k_fp4_small(Matmul4Args p, uint32_t n_tiles) {
-    const int lane = threadIdx.x, col = lane & 15, g = lane >> 4;
-    const uint32_t blocks = (p.dim + 31u) / 32u;
-    const uint32_t m0 = blockIdx.x / n_tiles * 16u, n0 = blockIdx.x % n_tiles * 16u;
-    const uint32_t ra = min(m0 + col, p.a.rows - 1), rb = min(n0 + col, p.b.rows - 1);
-    const uint8_t *const a = p.a.codes + size_t(ra) * p.a.stride, *const b = p.b.codes + size_t(rb) * p.b.stride;
-    const uint8_t *const as = p.a.scales + size_t(ra) * p.a.scale_stride, *const bs = p.b.scales + size_t(rb) * p.b.scale_stride;
-    v4f acc{0, 0, 0, 0};
-    for (uint32_t k = 0; k < blocks; k += 4) {
-        const uint32_t block = k + uint32_t(g);
-        const v4i x = codes32(a, block * 16u, p.dim), y = codes32(b, block * 16u, p.dim);
-        const int xs = block < blocks ? as[block] : 127, ys = block < blocks ? bs[block] : 127;
-        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand4(x), operand4(y), acc, 4, 4, 0, xs, 0, ys);
+__device__ __forceinline__ void store_out4(void *out, size_t at, float v, int type) {
+    if (type == kF32) static_cast<float *>(out)[at] = v;
+    else if (type == kF16) static_cast<f16 *>(out)[at] = f16(v);
+    else static_cast<bf16 *>(out)[at] = bf16(v);
+}
+
+// Up to sixteen rows of a: bound by reading b once.  A wave streams 16 rows of b from memory into registers, four steps of 128 coordinates while the four
+// before are multiplied, and goes on to its next 16 rows without a pause; a lies in LDS.  Where there are few rows of b (SPLIT), the four waves of
+// a workgroup share 16 rows, each taking every fourth step, and their sums are added in the waves' order.
+constexpr int kDirect4Threads = 256, kDirect4Waves = kDirect4Threads / 64, kDirect4Steps = 4;
+constexpr uint32_t kDirect4Groups = 4;        // workgroups of a compute unit at a time
+constexpr size_t kDirect4Lds = 64 << 10, kMostLds4 = 160 << 10;
+
+__host__ __device__ inline uint32_t direct4_row(uint32_t dim) { return (dim + 127u) / 128u * 64u + 16u; }     // (rows of a a few banks apart)
+inline size_t direct4_lds(uint32_t rows, uint32_t dim) { return size_t(rows) * direct4_row(dim) + (dim + 127) / 128 * 64 + kDirect4Waves * 64 * 16; }
+
+template <bool SPLIT>
+__global__ __launch_bounds__(kDirect4Threads, kDirect4Groups) void k_fp4_direct(Matmul4Args p) {
+    extern __shared__ uint8_t smem[];
+    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
+    const uint32_t blocks = (p.dim + 31u) / 32u, steps = (p.dim + 127u) / 128u, whole = p.dim / 128u, bytes = (p.dim + 1u) / 2u, row_bytes = direct4_row(p.dim), m = p.a.rows;
+    uint32_t *const a_scales = reinterpret_cast<uint32_t *>(smem + m * row_bytes);       // [step][16]: a byte for each block of the step
+    v4f *const sums = reinterpret_cast<v4f *>(a_scales + steps * 16);                    // SPLIT: [wave][lane]
+    for (uint32_t i = threadIdx.x; i < m * steps * 4u; i += kDirect4Threads) {
+        const uint32_t r = i / (steps * 4u), c = i % (steps * 4u) * 16u;
+        *reinterpret_cast<v4i *>(smem + r * row_bytes + c) = codes32(p.a.codes + size_t(r) * p.a.stride, c, p.dim);
     }
+    for (uint32_t i = threadIdx.x; i < steps * 16u; i += kDirect4Threads)
+        a_scales[i] = scales4(p.a.scales + size_t(min(i & 15u, m - 1)) * p.a.scale_stride, (i >> 4) * 4u, blocks);
+    __syncthreads();
+    // (rows past the end are the last one: their results are not stored)
+    const uint8_t *const a = smem + min(uint32_t(col), m - 1) * row_bytes + g * 16;
+
+    const uint32_t tiles = (p.b.rows + 15) / 16, turns = (steps + kDirect4Steps - 1) / kDirect4Steps;
+    const uint32_t tile_stride = SPLIT ? gridDim.x : gridDim.x * kDirect4Waves, turn_stride = SPLIT ? kDirect4Waves : 1, first_turn = SPLIT ? wave : 0;
+    struct Place {
+        uint32_t tile, turn;
+        const uint8_t *codes, *scales;
+    };
+    auto go_to = [&](Place &at, uint32_t tile) {
+        const uint32_t row = min(tile * 16u + uint32_t(col), p.b.rows - 1);
+        at = Place{tile, first_turn, p.b.codes + size_t(row) * p.b.stride, p.b.scales + size_t(row) * p.b.scale_stride};
+    };
+    struct Turn {
+        v4i codes[kDirect4Steps];
+        uint32_t scales[kDirect4Steps];
+    };
+    auto load = [&](Turn &s, const Place &at) {
+        if (at.tile >= tiles || at.turn >= turns) return;
+        const uint32_t first = at.turn * kDirect4Steps;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const uint32_t m = m0 + 4u * g + r, n = n0 + col;
-        if (m < p.a.rows && n < p.b.rows) static_cast<T *>(p.out)[size_t(m) * p.out_stride + n] = T(acc[r]);
+        for (int i = 0; i < kDirect4Steps; ++i) s.codes[i] = *reinterpret_cast<const v4i_any *>(at.codes + min((first + i) * 64u + uint32_t(g) * 16u, bytes - 16u));
+        if (first * 4u + 16u <= blocks) {
+            __builtin_memcpy(s.scales, at.scales + first * 4u, 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kDirect4Steps; ++i) s.scales[i] = scales4(at.scales, (first + i) * 4u, blocks);
+        }
+    };
+    v4f acc = v4f{0, 0, 0, 0};
+    auto step = [&](uint32_t k, const v4i &y, uint32_t ys) {
+        const v4i x = *reinterpret_cast<const v4i *>(a + k * 64u);
+        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand4(x), operand4(y), acc, 4, 4, 0, int(a_scales[k * 16 + col] >> (8 * g)), 0, int(ys >> (8 * g)));
+    };
+    auto multiply = [&](const Turn &s, const Place &at) {
+#pragma unroll
+        for (int i = 0; i < kDirect4Steps; ++i) {
+            const uint32_t k = at.turn * kDirect4Steps + i, from = k * 64u + uint32_t(g) * 16u;
+            if (k < whole) step(k, s.codes[i], s.scales[i]);
+            else if (k < steps)               // (the row ends in this step: what was loaded are its last 16 bytes)
+                step(k, without_half(bytes_down(s.codes[i], from - min(from, bytes - 16u)), from, p.dim), s.scales[i]);
+        }
+    };
+    auto finish = [&](const Place &at) {
+        if (SPLIT) {
+            sums[threadIdx.x] = acc;
+            __syncthreads();
+            if (wave != 0) return;
+#pragma unroll
+            for (int w = 1; w < kDirect4Waves; ++w) acc += sums[w * 64 + lane];
+        }
+        const uint32_t n = at.tile * 16u + uint32_t(col);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (uint32_t(4 * g + r) < m && n < p.b.rows) store_out4(p.out, size_t(4 * g + r) * p.out_stride + n, acc[r], p.out_type);
+        acc = v4f{0, 0, 0, 0};
+    };
+    Place here, next;
+    Turn even, odd;
+    go_to(here, SPLIT ? blockIdx.x : blockIdx.x * kDirect4Waves + wave);
+    load(even, here);
+    auto turn = [&](const Turn &now, Turn &then) {
+        next = here;
+        next.turn += turn_stride;
+        if (next.turn >= turns) go_to(next, SPLIT ? tiles : here.tile + tile_stride);
+        load(then, next);
+        multiply(now, here);
+        if (next.tile != here.tile) finish(here);
+        here = next;
+    };
+    while (here.tile < tiles) {
+        turn(even, odd);
+        if (here.tile >= tiles) break;
+        turn(odd, even);
     }
 }
-template <typename T>
-static hipError_t matmul4(const Matmul4Args &a, hipStream_t s) {
-    const uint64_t mt = (a.a.rows + 15u) / 16u, nt = (a.b.rows + 15u) / 16u;
-    if (mt * nt * 64u >> 32) return hipErrorInvalidConfiguration;
-    return launch(k_fp4_small<T>, uint32_t(mt * nt), 64, 0, s, a, uint32_t(nt));
+template <bool SPLIT>
+static hipError_t direct4(const Matmul4Args &a, hipStream_t s) {
+    const uint32_t tiles = (a.b.rows + 15) / 16, most = SPLIT ? tiles : 256 * kDirect4Groups;
+    const uint32_t grid = SPLIT ? tiles : (tiles + kDirect4Waves - 1) / kDirect4Waves;
+    const size_t lds = direct4_lds(a.a.rows, a.dim);
+    if (const hipError_t e = allow_lds(reinterpret_cast<const void *>(k_fp4_direct<SPLIT>), lds); e != hipSuccess) return e;
+    return launch(k_fp4_direct<SPLIT>, grid < most ? grid : most, kDirect4Threads, lds, s, a);
 }
+
+// Many rows of a: a workgroup to a tile of TM rows of a and TN of b, WM x WN waves, each with 32 x 32 x 64 products.  (Those reach 6.4 PFLOP/s on registers alone
+// where 16 x 16 x 128 ones reach 4.9.)  256 coordinates of both at a time go to LDS, 128 bytes a row, while the 256 before are multiplied.
+//
+// A row's eight runs of 16 bytes are swapped about by the row's number: eight neighbouring lanes, which read the same run of eight rows, find
+// it in different banks.  Loads that go past the registers write lane l at 16 l, so each lane asks for the run that belongs there.  A row's eight scale
+// bytes of a stage lie in LDS in the order even blocks, odd blocks: a lane's four steps find theirs in the bytes of one word, which the instruction picks.
+//
+// A stage has four steps of 64 coordinates.  Operands of a step are read from LDS while the step before is multiplied; the barrier between two stages
+// stands before the last step of the first, whose operands are in registers by then, so that the matrix units have work across it.
+__device__ __forceinline__ void load16_to_lds4(uint32_t lds, const uint8_t *base, uint32_t offset) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void wait_loads4() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+constexpr uint32_t kStage4 = 256, kStageBytes4 = kStage4 / 2;
+template <int TM, int TN> constexpr size_t tile4_lds() { return 2 * size_t(TM + TN) * (kStageBytes4 + 8); }
+template <typename T, int COLS> constexpr int kStrip4 = 32 * (COLS * int(sizeof(T)) + 16);
+
+// A wave's results, whose lane l holds, of row l % 32 of each tile, columns 8 q + 4 (l / 32) .. + 3, to rows from m on and columns from n on: 32 rows at a time
+// through LDS, so that they leave in runs of whole cache lines.
+template <typename T, int COLS, int MT, int NT>
+__device__ __forceinline__ void store_strips4(const Matmul4Args &p, const v16f (&acc)[MT][NT], uint8_t *strip, uint32_t m, uint32_t n, int lane) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    constexpr int kEach = 16 / int(sizeof(T)), kLanes = COLS / kEach, kRowsAtOnce = 64 / kLanes, kRow = COLS * int(sizeof(T)) + 16;
+    const int row32 = lane & 31, half = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const v4f x = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                *reinterpret_cast<T4 *>(strip + row32 * kRow + (j * 32 + q * 8 + half * 4) * int(sizeof(T))) = __builtin_convertvector(x, T4);
+            }
+#pragma unroll
+        for (int r = 0; r < 32; r += kRowsAtOnce) {
+            const int row = r + lane / kLanes, at = lane % kLanes * kEach;
+            const v4i x = *reinterpret_cast<const v4i *>(strip + row * kRow + at * int(sizeof(T)));
+            const uint32_t om = m + uint32_t(i * 32 + row), on = n + uint32_t(at);
+            if (om >= p.a.rows || on >= p.b.rows) continue;
+            T *const to = static_cast<T *>(p.out) + size_t(om) * p.out_stride + on;
+            if (on + kEach <= p.b.rows) {
+                *reinterpret_cast<v4i_any *>(to) = x;
+            } else {
+                T e[kEach];
+                __builtin_memcpy(e, &x, 16);
+#pragma unroll
+                for (int l = 0; l < kEach; ++l)
+                    if (on + l < p.b.rows) to[l] = e[l];
+            }
+        }
+    }
+}
+
+template <int TM, int TN, int WM, int WN, int HELD>
+__global__ __launch_bounds__(64 * WM * WN, HELD) void k_fp4_tile(Matmul4Args p, uint32_t m_tiles, uint32_t n_tiles, bool by_n, bool direct16) {
+    extern __shared__ uint8_t smem[];
+    constexpr int kWaves = WM * WN, kThreads = 64 * kWaves, kRows = TM + TN, kGroups = kRows / 8 / kWaves, MT = TM / WM / 32, NT = TN / WN / 32;
+    constexpr uint32_t kBuffer = kRows * kStageBytes4;
+    static_assert(kRows % (8 * kWaves) == 0, "whole groups of eight rows to a wave");
+    static_assert(size_t(kWaves) * kStrip4<float, TN / WN> <= tile4_lds<TM, TN>(), "strips of all waves at once");
+    // Tiles of one strip follow each other on one XCD (workgroups go to the eight in turn), so that they find it in that one's L2.
+    uint32_t tm, tn;
+    {
+        const uint32_t xcd = blockIdx.x & 7u, i = blockIdx.x >> 3;
+        if (by_n) { tn = i / m_tiles * 8u + xcd; tm = i % m_tiles; }
+        else { tm = i / n_tiles * 8u + xcd; tn = i % n_tiles; }
+        if (tm >= m_tiles || tn >= n_tiles) return;
+    }
+    const uint32_t m0 = tm * TM, n0 = tn * TN;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)), row32 = lane & 31, half = lane >> 5;
+    const uint32_t blocks = (p.dim + 31u) / 32u, stages = (p.dim + kStage4 - 1) / kStage4;
+    const uint32_t lds0 = uint32_t(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) uint8_t *)smem));
+    uint8_t *const scales = smem + 2 * kBuffer;                  // [buffer][row][8]
+
+    // Of the rows of a and, after them, of b, wave w loads groups w, w + kWaves, ...: lane l row l / 8 of the group, run (l % 8) ^ (l / 8).
+    // (Rows past the end are the last one: their results are not stored.)
+    const uint8_t *const a0 = p.a.codes + size_t(m0) * p.a.stride, *const b0 = p.b.codes + size_t(n0) * p.b.stride;
+    const uint32_t run16 = uint32_t((lane & 7) ^ (lane >> 3)) * 16u;
+    uint32_t offset[kGroups];
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+        const uint32_t row = uint32_t((i * kWaves + wave) * 8 + (lane >> 3));
+        const bool of_a = row < uint32_t(TM);
+        const uint32_t r = of_a ? min(row, p.a.rows - 1 - m0) : min(row - TM, p.b.rows - 1 - n0);
+        offset[i] = r * uint32_t(of_a ? p.a.stride : p.b.stride) + run16;
+    }
+    const uint32_t whole = direct16 ? p.dim / kStage4 : 0u;      // stages that go to LDS past the registers: the first ones
+    auto load_group = [&](uint32_t k, uint32_t buffer, int i) {
+        const uint32_t group = uint32_t(i * kWaves + wave);
+        load16_to_lds4(lds0 + buffer * kBuffer + group * 1024u, (group * 8 < TM ? a0 : b0) + size_t(k) * kStageBytes4, offset[i]);
+    };
+    auto copy_groups = [&](uint32_t k, uint32_t buffer) {
+#pragma unroll 1
+        for (int i = 0; i < kGroups; ++i) {
+            const uint32_t group = uint32_t(i * kWaves + wave), row = group * 8 + uint32_t(lane >> 3);
+            const uint8_t *at = row < uint32_t(TM) ? a0 + size_t(min(row, p.a.rows - 1 - m0)) * p.a.stride : b0 + size_t(min(row - TM, p.b.rows - 1 - n0)) * p.b.stride;
+            *reinterpret_cast<v4i *>(smem + buffer * kBuffer + group * 1024u + lane * 16) = codes32(at, k * kStageBytes4 + run16, p.dim);
+        }
+    };
+    // A thread to the scales of every kThreads-th row.
+    constexpr int kScaleRounds = (kRows + kThreads - 1) / kThreads;
+    const uint8_t *scale_row[kScaleRounds];
+#pragma unroll
+    for (int i = 0; i < kScaleRounds; ++i) {
+        const uint32_t row = min(uint32_t(i * kThreads) + threadIdx.x, uint32_t(kRows - 1));
+        scale_row[i] = row < uint32_t(TM) ? p.a.scales + size_t(min(m0 + row, p.a.rows - 1)) * p.a.scale_stride : p.b.scales + size_t(min(n0 + row - TM, p.b.rows - 1)) * p.b.scale_stride;
+    }
+    struct Eight { uint32_t lo, hi; };
+    auto load_scales = [&](uint32_t k, Eight (&x)[kScaleRounds]) {
+#pragma unroll
+        for (int i = 0; i < kScaleRounds; ++i) {
+            if (k * 8u + 8u <= blocks) __builtin_memcpy(&x[i], scale_row[i] + k * 8u, 8);
+            else x[i] = Eight{scales4(scale_row[i], k * 8u, blocks), scales4(scale_row[i], k * 8u + 4u, blocks)};
+        }
+    };
+    auto put_scales = [&](const Eight (&x)[kScaleRounds], uint32_t buffer) {
+#pragma unroll
+        for (int i = 0; i < kScaleRounds; ++i) {
+            const uint32_t row = uint32_t(i * kThreads) + threadIdx.x;
+            if (kRows % kThreads != 0 && row >= uint32_t(kRows)) continue;
+            const Eight sorted{__builtin_amdgcn_perm(x[i].hi, x[i].lo, 0x06040200u), __builtin_amdgcn_perm(x[i].hi, x[i].lo, 0x07050301u)};
+            *reinterpret_cast<Eight *>(scales + (buffer * kRows + row) * 8u) = sorted;
+        }
+    };
+
+    const int wm = wave % WM * (TM / WM), wn = wave / WM * (TN / WN);
+    v16f acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+
+    struct Operands {
+        v4i a[MT], b[NT];
+    };
+    struct Scales {
+        int a[MT], b[NT];
+    };
+    const uint8_t *const my_a = smem + (wm + row32) * kStageBytes4, *const my_b = smem + (TM + wn + row32) * kStageBytes4;
+    auto read = [&](Operands &o, uint32_t buffer, int t) {
+        const uint32_t at = buffer * kBuffer + uint32_t((2 * t + half) ^ (row32 & 7)) * 16u;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) o.a[i] = *reinterpret_cast<const v4i *>(my_a + at + i * 32 * kStageBytes4);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) o.b[j] = *reinterpret_cast<const v4i *>(my_b + at + j * 32 * kStageBytes4);
+    };
+    auto read_scales = [&](Scales &s, uint32_t buffer) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) s.a[i] = *reinterpret_cast<const int *>(scales + (buffer * kRows + wm + i * 32 + row32) * 8u + half * 4);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) s.b[j] = *reinterpret_cast<const int *>(scales + (buffer * kRows + TM + wn + j * 32 + row32) * 8u + half * 4);
+    };
+    auto multiply = [&](const Operands &o, const Scales &s, auto t) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand4(o.b[j]), operand4(o.a[i]), acc[i][j], 4, 4, decltype(t)::value, s.b[j], decltype(t)::value, s.a[i]);
+    };
+    Eight next[kScaleRounds];
+    auto start = [&](uint32_t k) {                 // a stage's codes and scales on their way
+        if (k < whole) {
+#pragma unroll
+            for (int i = 0; i < kGroups; ++i) load_group(k, k & 1u, i);
+        } else {
+            copy_groups(k, k & 1u);
+        }
+        load_scales(k, next);
+    };
+    Operands even, odd;
+    Scales sc, sc_next;
+    start(0);
+    put_scales(next, 0);
+    wait_loads4();
+    __syncthreads();
+    read(even, 0, 0);
+    read_scales(sc, 0);
+    for (uint32_t k = 0; k < stages; ++k) {
+        const uint32_t buffer = k & 1u;
+        const bool more = k + 1 < stages;
+        if (more) start(k + 1);
+        read(odd, buffer, 1);
+        multiply(even, sc, IntC<0>{});
+        read(even, buffer, 2);
+        multiply(odd, sc, IntC<1>{});
+        read(odd, buffer, 3);
+        multiply(even, sc, IntC<2>{});
+        if (more) {
+            put_scales(next, buffer ^ 1u);
+            wait_loads4();
+            __syncthreads();
+            read(even, buffer ^ 1u, 0);
+            read_scales(sc_next, buffer ^ 1u);
+        }
+        multiply(odd, sc, IntC<3>{});
+        sc = sc_next;
+    }
+    __syncthreads();
+    uint8_t *const strip = smem + wave * kStrip4<float, TN / WN>;
+    if (p.out_type == kF32) store_strips4<float, TN / WN, MT, NT>(p, acc, strip, m0 + wm, n0 + wn, lane);
+    else if (p.out_type == kF16) store_strips4<f16, TN / WN, MT, NT>(p, acc, strip, m0 + wm, n0 + wn, lane);
+    else store_strips4<bf16, TN / WN, MT, NT>(p, acc, strip, m0 + wm, n0 + wn, lane);
+}
+
+template <int TM, int TN, int WM, int WN, int HELD>
+static hipError_t tile4(const Matmul4Args &a, hipStream_t s) {
+    const uint32_t mt = (a.a.rows + TM - 1) / TM, nt = (a.b.rows + TN - 1) / TN;
+    const bool by_n = nt >= mt;
+    const uint64_t grid = by_n ? (uint64_t(nt) + 7) / 8 * 8 * mt : (uint64_t(mt) + 7) / 8 * 8 * nt;
+    // 16 bytes at a time past the registers: rows at multiples of 16 bytes, and a tile's offsets in 32 bits
+    const bool direct16 = ((uintptr_t(a.a.codes) | uintptr_t(a.b.codes) | a.a.stride | a.b.stride) & 15) == 0 && a.a.stride < (1u << 23) && a.b.stride < (1u << 23);
+    if ((grid * (64 * WM * WN)) >> 32) return hipErrorInvalidConfiguration;      // (a result of hundreds of GB, or a narrow one of a billion columns)
+    const auto kernel = k_fp4_tile<TM, TN, WM, WN, HELD>;
+    if (const hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), tile4_lds<TM, TN>()); e != hipSuccess) return e;
+    return launch(kernel, uint32_t(grid), 64 * WM * WN, tile4_lds<TM, TN>(), s, a, mt, nt, by_n, direct16);
+}
+
 hipError_t launch_fp4_matmul(const Matmul4Args &a, hipStream_t s) {
-    if (a.out_type == kF32) return matmul4<float>(a, s);
-    return a.out_type == kF16 ? matmul4<f16>(a, s) : matmul4<bf16>(a, s);
+    if (a.a.rows <= 16 && a.dim >= 31) {
+        const bool few = a.b.rows < 256 * 4 * 16;
+        if (size_t(a.a.rows) * direct4_row(a.dim) <= kDirect4Lds) return few ? direct4<true>(a, s) : direct4<false>(a, s);
+        const size_t lds = direct4_lds(a.a.rows, a.dim);
+        if (lds <= kMostLds4 && (a.b.rows + 15) / 16 <= 256 * (kMostLds4 / lds)) return direct4<true>(a, s);
+    }
+    auto tiles = [&](uint32_t tm, uint32_t tn) { return uint64_t((a.a.rows + tm - 1) / tm) * ((a.b.rows + tn - 1) / tn); };
+    if (tiles(256, 256) >= 200) return tile4<256, 256, 2, 2, 1>(a, s);
+    if (tiles(128, 128) >= 256) return tile4<128, 128, 2, 2, 2>(a, s);
+    return tile4<64, 64, 2, 2, 4>(a, s);
 }
 
 }  // namespace tv
