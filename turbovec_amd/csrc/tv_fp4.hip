@@ -96,14 +96,15 @@ __device__ __forceinline__ v4i codes32(const uint8_t *row, uint32_t k, uint32_t 
     const uint32_t bytes = (dim + 1u) / 2u;
     return k >= bytes ? v4i{0, 0, 0, 0} : without_half(codes16(row, k, bytes), k, dim);
 }
-// Four scale bytes of a row from block k on; those past the end are 2^0 (their codes are 0, and a NaN would show).
+// Four scale bytes of a row from block k on, k < blocks; those past the end are 0 (2^-127, of codes that are 0).
 __device__ __forceinline__ uint32_t scales4(const uint8_t *row, uint32_t k, uint32_t blocks) {
-    uint32_t s = 0x7f7f7f7fu;
-    if (k + 4u <= blocks) __builtin_memcpy(&s, row + k, 4);
-    else
-#pragma unroll
-        for (uint32_t i = 0; i < 3; ++i)
-            if (k + i < blocks) s = (s & ~(255u << (8 * i))) | uint32_t(row[k + i]) << (8 * i);
+    uint32_t s = 0;
+    if (blocks >= 4u) {
+        const uint32_t at = min(k, blocks - 4u);
+        __builtin_memcpy(&s, row + at, 4);
+        return s >> (8u * (k - at));
+    }
+    for (uint32_t i = 0; k + i < blocks; ++i) s |= uint32_t(row[k + i]) << (8 * i);
     return s;
 }
 __device__ __forceinline__ v8i operand4(v4i v) { return v8i{v[0], v[1], v[2], v[3], 0, 0, 0, 0}; }
@@ -164,7 +165,7 @@ __global__ __launch_bounds__(kDirect4Threads, kDirect4Groups) void k_fp4_direct(
             __builtin_memcpy(s.scales, at.scales + first * 4u, 16);
         } else {
 #pragma unroll
-            for (int i = 0; i < kDirect4Steps; ++i) s.scales[i] = scales4(at.scales, (first + i) * 4u, blocks);
+            for (int i = 0; i < kDirect4Steps; ++i) s.scales[i] = (first + i) * 4u < blocks ? scales4(at.scales, (first + i) * 4u, blocks) : 0u;
         }
     };
     v4f acc = v4f{0, 0, 0, 0};
@@ -223,21 +224,18 @@ static hipError_t direct4(const Matmul4Args &a, hipStream_t s) {
     return launch(k_fp4_direct<SPLIT>, grid < most ? grid : most, kDirect4Threads, lds, s, a);
 }
 
-// Many rows of a: a workgroup to a tile of TM rows of a and TN of b, WM x WN waves, each with 32 x 32 x 64 products.  (Those reach 6.4 PFLOP/s on registers alone
-// where 16 x 16 x 128 ones reach 4.9.)  256 coordinates of both at a time go to LDS, 128 bytes a row, while the 256 before are multiplied.
+// Many rows of a: a workgroup to a tile of TM rows of a and TN of b, WM x WN waves, each with 32 x 32 x 64 products.  (Those reach 6.2 to 6.6 PFLOP/s on registers
+// alone, where the chip's power ends it, 16 x 16 x 128 ones 4.6 to 5.5.)  Stages of 256 coordinates of both, a cache line of 128 bytes a row, come into registers a stage
+// ahead, go from there to one half of LDS while the other is multiplied, and so reach the matrix units two stages later.  (Loads past the registers, into a ring
+// of stages of 64 bytes a row, take whole lines for half of them: 29 bytes a clock and compute unit where these take 58.)
 //
-// A row's eight runs of 16 bytes are swapped about by the row's number: eight neighbouring lanes, which read the same run of eight rows, find
-// it in different banks.  Loads that go past the registers write lane l at 16 l, so each lane asks for the run that belongs there.  A row's eight scale
-// bytes of a stage lie in LDS in the order even blocks, odd blocks: a lane's four steps find theirs in the bytes of one word, which the instruction picks.
+// A row's eight runs of 16 bytes are swapped about by the row's number: lanes that read the same run of neighbouring rows find it in different banks.  A row's eight scale
+// bytes lie in LDS as two words, of even and of odd blocks: a lane's four steps find theirs in the bytes of one word, which the instruction picks.
 //
 // A stage has four steps of 64 coordinates.  Operands of a step are read from LDS while the step before is multiplied; the barrier between two stages
 // stands before the last step of the first, whose operands are in registers by then, so that the matrix units have work across it.
-__device__ __forceinline__ void load16_to_lds4(uint32_t lds, const uint8_t *base, uint32_t offset) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
-}
-__device__ __forceinline__ void wait_loads4() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
 constexpr uint32_t kStage4 = 256, kStageBytes4 = kStage4 / 2;
+constexpr size_t kMostTileStride4 = size_t(1) << 23;      // a tile's offsets have 32 bits
 template <int TM, int TN> constexpr size_t tile4_lds() { return 2 * size_t(TM + TN) * (kStageBytes4 + 8); }
 template <typename T, int COLS> constexpr int kStrip4 = 32 * (COLS * int(sizeof(T)) + 16);
 
@@ -257,95 +255,104 @@ __device__ __forceinline__ void store_strips4(const Matmul4Args &p, const v16f (
                 const v4f x = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
                 *reinterpret_cast<T4 *>(strip + row32 * kRow + (j * 32 + q * 8 + half * 4) * int(sizeof(T))) = __builtin_convertvector(x, T4);
             }
-#pragma unroll
+        const uint32_t at = uint32_t(lane % kLanes * kEach), on = n + at;
+#pragma unroll 4
         for (int r = 0; r < 32; r += kRowsAtOnce) {
-            const int row = r + lane / kLanes, at = lane % kLanes * kEach;
-            const v4i x = *reinterpret_cast<const v4i *>(strip + row * kRow + at * int(sizeof(T)));
-            const uint32_t om = m + uint32_t(i * 32 + row), on = n + uint32_t(at);
-            if (om >= p.a.rows || on >= p.b.rows) continue;
+            const int row = r + lane / kLanes;
+            const uint32_t om = m + uint32_t(i * 32 + row);
+            const T *const from = reinterpret_cast<const T *>(strip + row * kRow) + at;
             T *const to = static_cast<T *>(p.out) + size_t(om) * p.out_stride + on;
+            if (om >= p.a.rows || on >= p.b.rows) continue;
             if (on + kEach <= p.b.rows) {
-                *reinterpret_cast<v4i_any *>(to) = x;
+                *reinterpret_cast<v4i_any *>(to) = *reinterpret_cast<const v4i *>(from);
             } else {
-                T e[kEach];
-                __builtin_memcpy(e, &x, 16);
-#pragma unroll
-                for (int l = 0; l < kEach; ++l)
-                    if (on + l < p.b.rows) to[l] = e[l];
+#pragma unroll 1
+                for (uint32_t l = 0; on + l < p.b.rows; ++l) to[l] = from[l];
             }
         }
     }
 }
 
-template <int TM, int TN, int WM, int WN, int HELD>
-__global__ __launch_bounds__(64 * WM * WN, HELD) void k_fp4_tile(Matmul4Args p, uint32_t m_tiles, uint32_t n_tiles, bool by_n, bool direct16) {
+template <typename T, int TM, int TN, int WM, int WN, int HELD>
+__global__ __launch_bounds__(64 * WM * WN, HELD) void k_fp4_tile(Matmul4Args p, uint32_t m_tiles, uint32_t n_tiles, uint32_t each_xcd) {
     extern __shared__ uint8_t smem[];
     constexpr int kWaves = WM * WN, kThreads = 64 * kWaves, kRows = TM + TN, kGroups = kRows / 8 / kWaves, MT = TM / WM / 32, NT = TN / WN / 32;
     constexpr uint32_t kBuffer = kRows * kStageBytes4;
-    static_assert(kRows % (8 * kWaves) == 0, "whole groups of eight rows to a wave");
-    static_assert(size_t(kWaves) * kStrip4<float, TN / WN> <= tile4_lds<TM, TN>(), "strips of all waves at once");
-    // Tiles of one strip follow each other on one XCD (workgroups go to the eight in turn), so that they find it in that one's L2.
+    static_assert(TM % (8 * kWaves) == 0 && TN % (8 * kWaves) == 0, "whole groups of eight rows of either side to a wave");
+    static_assert(size_t(kWaves) * kStrip4<T, TN / WN> <= tile4_lds<TM, TN>(), "strips of all waves at once");
+    // An XCD (workgroups go to the eight in turn) has tiles that follow each other: eight rows of tiles by as many columns as there are, column by column, so that its
+    // thirty-two compute units find most of what they read in its L2.
     uint32_t tm, tn;
     {
-        const uint32_t xcd = blockIdx.x & 7u, i = blockIdx.x >> 3;
-        if (by_n) { tn = i / m_tiles * 8u + xcd; tm = i % m_tiles; }
-        else { tm = i / n_tiles * 8u + xcd; tn = i % n_tiles; }
-        if (tm >= m_tiles || tn >= n_tiles) return;
+        const uint32_t id = (blockIdx.x & 7u) * each_xcd + (blockIdx.x >> 3);
+        if (id >= m_tiles * n_tiles) return;
+        const uint32_t band = id / (8u * n_tiles), in = id % (8u * n_tiles), high = min(8u, m_tiles - band * 8u);
+        tm = band * 8u + in % high;
+        tn = in / high;
     }
     const uint32_t m0 = tm * TM, n0 = tn * TN;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)), row32 = lane & 31, half = lane >> 5;
-    const uint32_t blocks = (p.dim + 31u) / 32u, stages = (p.dim + kStage4 - 1) / kStage4;
-    const uint32_t lds0 = uint32_t(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) uint8_t *)smem));
-    uint8_t *const scales = smem + 2 * kBuffer;                  // [buffer][row][8]
+    const uint32_t blocks = (p.dim + 31u) / 32u, stages = (p.dim + kStage4 - 1) / kStage4, whole = p.dim / kStage4, bytes = (p.dim + 1u) / 2u;
+    uint32_t *const scales = reinterpret_cast<uint32_t *>(smem + 2 * kBuffer);                  // [buffer][even or odd blocks][row]
 
-    // Of the rows of a and, after them, of b, wave w loads groups w, w + kWaves, ...: lane l row l / 8 of the group, run (l % 8) ^ (l / 8).
+    // Of the rows of a and, after them, of b, wave w has groups of eight w, w + kWaves, ...: lane l row l / 8 of the group, run l % 8.
     // (Rows past the end are the last one: their results are not stored.)
     const uint8_t *const a0 = p.a.codes + size_t(m0) * p.a.stride, *const b0 = p.b.codes + size_t(n0) * p.b.stride;
-    const uint32_t run16 = uint32_t((lane & 7) ^ (lane >> 3)) * 16u;
+    const uint32_t run16 = uint32_t(lane & 7) * 16u;
     uint32_t offset[kGroups];
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
         const uint32_t row = uint32_t((i * kWaves + wave) * 8 + (lane >> 3));
-        const bool of_a = row < uint32_t(TM);
-        const uint32_t r = of_a ? min(row, p.a.rows - 1 - m0) : min(row - TM, p.b.rows - 1 - n0);
-        offset[i] = r * uint32_t(of_a ? p.a.stride : p.b.stride) + run16;
+        offset[i] = i * kWaves * 8 < TM ? min(row, p.a.rows - 1 - m0) * uint32_t(p.a.stride) : min(row - TM, p.b.rows - 1 - n0) * uint32_t(p.b.stride);
     }
-    const uint32_t whole = direct16 ? p.dim / kStage4 : 0u;      // stages that go to LDS past the registers: the first ones
-    auto load_group = [&](uint32_t k, uint32_t buffer, int i) {
-        const uint32_t group = uint32_t(i * kWaves + wave);
-        load16_to_lds4(lds0 + buffer * kBuffer + group * 1024u, (group * 8 < TM ? a0 : b0) + size_t(k) * kStageBytes4, offset[i]);
+    v4i held[kGroups];
+    // (A run that the row ends in or before is the row's last 16 bytes, for ending() to put right; behind the last stage nobody looks.)
+    auto load_group = [&](uint32_t k, auto i) {
+        constexpr int I = decltype(i)::value;
+        held[I] = *reinterpret_cast<const v4i_any *>((I * kWaves * 8 < TM ? a0 : b0) + (offset[I] + min(k * kStageBytes4 + run16, bytes - 16u)));
     };
-    auto copy_groups = [&](uint32_t k, uint32_t buffer) {
-#pragma unroll 1
-        for (int i = 0; i < kGroups; ++i) {
-            const uint32_t group = uint32_t(i * kWaves + wave), row = group * 8 + uint32_t(lane >> 3);
-            const uint8_t *at = row < uint32_t(TM) ? a0 + size_t(min(row, p.a.rows - 1 - m0)) * p.a.stride : b0 + size_t(min(row - TM, p.b.rows - 1 - n0)) * p.b.stride;
-            *reinterpret_cast<v4i *>(smem + buffer * kBuffer + group * 1024u + lane * 16) = codes32(at, k * kStageBytes4 + run16, p.dim);
-        }
+    uint8_t *const my_run = smem + uint32_t(wave) * 1024u + uint32_t(lane >> 3) * kStageBytes4 + uint32_t((lane & 7) ^ (lane >> 3)) * 16u;
+    auto put_group = [&](uint32_t k, auto i) {
+        constexpr int I = decltype(i)::value;
+        *reinterpret_cast<v4i *>(my_run + (k & 1u) * kBuffer + I * kWaves * 1024) = held[I];
     };
     // A thread to the scales of every kThreads-th row.
     constexpr int kScaleRounds = (kRows + kThreads - 1) / kThreads;
+    uint64_t held_scales[kScaleRounds];
     const uint8_t *scale_row[kScaleRounds];
+    const uint32_t last_eight = blocks >= 8u ? blocks - 8u : 0u;
 #pragma unroll
     for (int i = 0; i < kScaleRounds; ++i) {
         const uint32_t row = min(uint32_t(i * kThreads) + threadIdx.x, uint32_t(kRows - 1));
         scale_row[i] = row < uint32_t(TM) ? p.a.scales + size_t(min(m0 + row, p.a.rows - 1)) * p.a.scale_stride : p.b.scales + size_t(min(n0 + row - TM, p.b.rows - 1)) * p.b.scale_stride;
+        // (rows of fewer than eight blocks have one stage)
+        held_scales[i] = 0;
+        if (blocks < 8u)
+            for (uint32_t l = 0; l < blocks; ++l) held_scales[i] |= uint64_t(scale_row[i][l]) << (8 * l);
+        if (blocks < 8u) scale_row[i] = a0;
     }
-    struct Eight { uint32_t lo, hi; };
-    auto load_scales = [&](uint32_t k, Eight (&x)[kScaleRounds]) {
+    auto load_scales = [&](uint32_t k) {
+#pragma unroll
+        for (int i = 0; i < kScaleRounds; ++i) __builtin_memcpy(&held_scales[i], scale_row[i] + min(k * 8u, last_eight), 8);
+    };
+    auto put_scales = [&](uint32_t k) {
 #pragma unroll
         for (int i = 0; i < kScaleRounds; ++i) {
-            if (k * 8u + 8u <= blocks) __builtin_memcpy(&x[i], scale_row[i] + k * 8u, 8);
-            else x[i] = Eight{scales4(scale_row[i], k * 8u, blocks), scales4(scale_row[i], k * 8u + 4u, blocks)};
+            const uint32_t row = uint32_t(i * kThreads) + threadIdx.x, lo = uint32_t(held_scales[i]), hi = uint32_t(held_scales[i] >> 32);
+            if (kRows % kThreads != 0 && row >= uint32_t(kRows)) continue;
+            uint32_t *const to = scales + (k & 1u) * 2 * kRows + row;
+            to[0] = __builtin_amdgcn_perm(hi, lo, 0x06040200u);
+            to[kRows] = __builtin_amdgcn_perm(hi, lo, 0x07050301u);
         }
     };
-    auto put_scales = [&](const Eight (&x)[kScaleRounds], uint32_t buffer) {
+    // The stage that rows end in, as it stands in registers: runs moved down to where they belong, zeros behind the end, scales too (2^-127, of codes that are 0).
+    auto ending = [&] {
+        const uint32_t from = whole * kStageBytes4 + run16;
 #pragma unroll
-        for (int i = 0; i < kScaleRounds; ++i) {
-            const uint32_t row = uint32_t(i * kThreads) + threadIdx.x;
-            if (kRows % kThreads != 0 && row >= uint32_t(kRows)) continue;
-            const Eight sorted{__builtin_amdgcn_perm(x[i].hi, x[i].lo, 0x06040200u), __builtin_amdgcn_perm(x[i].hi, x[i].lo, 0x07050301u)};
-            *reinterpret_cast<Eight *>(scales + (buffer * kRows + row) * 8u) = sorted;
+        for (int i = 0; i < kGroups; ++i) held[i] = without_half(bytes_down(held[i], from - min(from, bytes - 16u)), from, p.dim);
+        if (blocks >= 8u) {
+#pragma unroll
+            for (int i = 0; i < kScaleRounds; ++i) held_scales[i] >>= 8u * (whole * 8u - min(whole * 8u, last_eight));
         }
     };
 
@@ -365,95 +372,152 @@ __global__ __launch_bounds__(64 * WM * WN, HELD) void k_fp4_tile(Matmul4Args p, 
         int a[MT], b[NT];
     };
     const uint8_t *const my_a = smem + (wm + row32) * kStageBytes4, *const my_b = smem + (TM + wn + row32) * kStageBytes4;
-    auto read = [&](Operands &o, uint32_t buffer, int t) {
-        const uint32_t at = buffer * kBuffer + uint32_t((2 * t + half) ^ (row32 & 7)) * 16u;
+    // What goes on between a step's products, in front of each a part: reads of the next step's operands, in the order that it wants them, of the next stage's scales, stores
+    // into LDS and loads.  (A wave has its SIMD alone in the largest tiles: between two products it can give a handful of instructions; more of them in one place
+    // leave the matrix unit idle.)
+    constexpr int kSlots = MT * NT, kReads = MT + NT;
+    auto read = [&](Operands &o, uint32_t k, int t, int slot) {
+        const uint32_t at = (k & 1u) * kBuffer + uint32_t((2 * t + half) ^ (row32 & 7)) * 16u;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) o.a[i] = *reinterpret_cast<const v4i *>(my_a + at + i * 32 * kStageBytes4);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) o.b[j] = *reinterpret_cast<const v4i *>(my_b + at + j * 32 * kStageBytes4);
+        for (int l = 0; l < kReads; ++l) {
+            if (l * kSlots / kReads != slot) continue;
+            if (l == 0) o.a[0] = *reinterpret_cast<const v4i *>(my_a + at);
+            else if (l <= NT) o.b[l - 1] = *reinterpret_cast<const v4i *>(my_b + at + (l - 1) * 32 * kStageBytes4);
+            else o.a[l - NT] = *reinterpret_cast<const v4i *>(my_a + at + (l - NT) * 32 * kStageBytes4);
+        }
     };
-    auto read_scales = [&](Scales &s, uint32_t buffer) {
+    auto read_scales = [&](Scales &s, uint32_t k, int slot) {
+        const int *const from = reinterpret_cast<const int *>(scales) + ((k & 1u) * 2u + uint32_t(half)) * kRows + row32;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) s.a[i] = *reinterpret_cast<const int *>(scales + (buffer * kRows + wm + i * 32 + row32) * 8u + half * 4);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) s.b[j] = *reinterpret_cast<const int *>(scales + (buffer * kRows + TM + wn + j * 32 + row32) * 8u + half * 4);
+        for (int l = 0; l < kReads; ++l) {
+            if ((l * kSlots + kSlots / 2) / kReads != slot) continue;
+            if (l < MT) s.a[l] = from[wm + l * 32];
+            else s.b[l - MT] = from[TM + wn + (l - MT) * 32];
+        }
     };
-    auto multiply = [&](const Operands &o, const Scales &s, auto t) {
+    // In three steps' slots, group by group: what is held goes to LDS, and the next stage's takes its place.
+    auto pass_on = [&](uint32_t k, int slot) {
+        static_for<kGroups>([&](auto l) {
+            if ((decltype(l)::value * 3 * kSlots + kSlots / 2) / kGroups != slot) return;
+            put_group(k + 1, l);
+            load_group(k + 2, l);
+        });
+        if (slot == 3 * kSlots - 1) {
+            put_scales(k + 1);
+            load_scales(k + 2);
+        }
+    };
+    auto multiply = [&](const Operands &o, const Scales &s, auto t, auto &&before) {
+        constexpr int kByte = decltype(t)::value;
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand4(o.b[j]), operand4(o.a[i]), acc[i][j], 4, 4, decltype(t)::value, s.b[j], decltype(t)::value, s.a[i]);
-    };
-    Eight next[kScaleRounds];
-    auto start = [&](uint32_t k) {                 // a stage's codes and scales on their way
-        if (k < whole) {
-#pragma unroll
-            for (int i = 0; i < kGroups; ++i) load_group(k, k & 1u, i);
-        } else {
-            copy_groups(k, k & 1u);
-        }
-        load_scales(k, next);
+            for (int j = 0; j < NT; ++j) {
+                before(i * NT + j);
+                __builtin_amdgcn_sched_barrier(0);
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand4(o.b[j]), operand4(o.a[i]), acc[i][j], 4, 4, kByte, s.b[j], kByte, s.a[i]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
     };
     Operands even, odd;
     Scales sc, sc_next;
-    start(0);
-    put_scales(next, 0);
-    wait_loads4();
+    static_for<kGroups>([&](auto i) { load_group(0, i); });
+    if (blocks >= 8u) load_scales(0);
+    if (whole == 0) ending();
+    static_for<kGroups>([&](auto i) {
+        put_group(0, i);
+        load_group(1, i);
+    });
+    put_scales(0);
+    load_scales(1);
     __syncthreads();
-    read(even, 0, 0);
-    read_scales(sc, 0);
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) {
+        read(even, 0, 0, i);
+        read_scales(sc, 0, i);
+    }
+#pragma unroll 1
     for (uint32_t k = 0; k < stages; ++k) {
-        const uint32_t buffer = k & 1u;
-        const bool more = k + 1 < stages;
-        if (more) start(k + 1);
-        read(odd, buffer, 1);
-        multiply(even, sc, IntC<0>{});
-        read(even, buffer, 2);
-        multiply(odd, sc, IntC<1>{});
-        read(odd, buffer, 3);
-        multiply(even, sc, IntC<2>{});
-        if (more) {
-            put_scales(next, buffer ^ 1u);
-            wait_loads4();
-            __syncthreads();
-            read(even, buffer ^ 1u, 0);
-            read_scales(sc_next, buffer ^ 1u);
-        }
-        multiply(odd, sc, IntC<3>{});
+        if (k + 1 == whole) ending();      // (where rows end with a stage, nobody looks at the next)
+        // (The same for every stage, without a branch: across one the compiler moves products about.  Behind the last stage what is loaded and read is not used.)
+        multiply(even, sc, IntC<0>{}, [&](int slot) {
+            read(odd, k, 1, slot);
+            pass_on(k, slot);
+        });
+        multiply(odd, sc, IntC<1>{}, [&](int slot) {
+            read(even, k, 2, slot);
+            pass_on(k, kSlots + slot);
+        });
+        multiply(even, sc, IntC<2>{}, [&](int slot) {
+            read(odd, k, 3, slot);
+            pass_on(k, 2 * kSlots + slot);
+        });
+        __syncthreads();
+        multiply(odd, sc, IntC<3>{}, [&](int slot) {
+            read(even, k + 1, 0, slot);
+            read_scales(sc_next, k + 1, slot);
+        });
         sc = sc_next;
     }
     __syncthreads();
-    uint8_t *const strip = smem + wave * kStrip4<float, TN / WN>;
-    if (p.out_type == kF32) store_strips4<float, TN / WN, MT, NT>(p, acc, strip, m0 + wm, n0 + wn, lane);
-    else if (p.out_type == kF16) store_strips4<f16, TN / WN, MT, NT>(p, acc, strip, m0 + wm, n0 + wn, lane);
-    else store_strips4<bf16, TN / WN, MT, NT>(p, acc, strip, m0 + wm, n0 + wn, lane);
+    store_strips4<T, TN / WN, MT, NT>(p, acc, smem + wave * kStrip4<T, TN / WN>, m0 + wm, n0 + wn, lane);
 }
 
-template <int TM, int TN, int WM, int WN, int HELD>
+template <typename T, int TM, int TN, int WM, int WN, int HELD>
 static hipError_t tile4(const Matmul4Args &a, hipStream_t s) {
-    const uint32_t mt = (a.a.rows + TM - 1) / TM, nt = (a.b.rows + TN - 1) / TN;
-    const bool by_n = nt >= mt;
-    const uint64_t grid = by_n ? (uint64_t(nt) + 7) / 8 * 8 * mt : (uint64_t(mt) + 7) / 8 * 8 * nt;
-    // 16 bytes at a time past the registers: rows at multiples of 16 bytes, and a tile's offsets in 32 bits
-    const bool direct16 = ((uintptr_t(a.a.codes) | uintptr_t(a.b.codes) | a.a.stride | a.b.stride) & 15) == 0 && a.a.stride < (1u << 23) && a.b.stride < (1u << 23);
-    if ((grid * (64 * WM * WN)) >> 32) return hipErrorInvalidConfiguration;      // (a result of hundreds of GB, or a narrow one of a billion columns)
-    const auto kernel = k_fp4_tile<TM, TN, WM, WN, HELD>;
+    const uint64_t mt = (a.a.rows + TM - 1) / TM, nt = (a.b.rows + TN - 1) / TN, each_xcd = (mt * nt + 7) / 8;
+    if ((each_xcd * 8 * (64 * WM * WN)) >> 32) return hipErrorInvalidConfiguration;      // (a result of hundreds of GB, or a narrow one of a billion columns)
+    const auto kernel = k_fp4_tile<T, TM, TN, WM, WN, HELD>;
     if (const hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), tile4_lds<TM, TN>()); e != hipSuccess) return e;
-    return launch(kernel, uint32_t(grid), 64 * WM * WN, tile4_lds<TM, TN>(), s, a, mt, nt, by_n, direct16);
+    return launch(kernel, uint32_t(each_xcd * 8), 64 * WM * WN, tile4_lds<TM, TN>(), s, a, uint32_t(mt), uint32_t(nt), uint32_t(each_xcd));
 }
 
-hipError_t launch_fp4_matmul(const Matmul4Args &a, hipStream_t s) {
+// Rows of fewer than 16 bytes, or 8 MB and more apart: a wave to a tile of 16 by 16, its operands read where they lie.
+template <typename T>
+__global__ __launch_bounds__(64) void k_fp4_small(Matmul4Args p, uint32_t n_tiles) {
+    const int lane = threadIdx.x, col = lane & 15, g = lane >> 4;
+    const uint32_t blocks = (p.dim + 31u) / 32u;
+    const uint32_t m0 = blockIdx.x / n_tiles * 16u, n0 = blockIdx.x % n_tiles * 16u;
+    const uint32_t ra = min(m0 + col, p.a.rows - 1), rb = min(n0 + col, p.b.rows - 1);
+    const uint8_t *const a = p.a.codes + size_t(ra) * p.a.stride, *const b = p.b.codes + size_t(rb) * p.b.stride;
+    const uint8_t *const as = p.a.scales + size_t(ra) * p.a.scale_stride, *const bs = p.b.scales + size_t(rb) * p.b.scale_stride;
+    v4f acc{0, 0, 0, 0};
+    for (uint32_t k = 0; k < blocks; k += 4) {
+        const uint32_t block = k + uint32_t(g);
+        const v4i x = codes32(a, block * 16u, p.dim), y = codes32(b, block * 16u, p.dim);
+        const int xs = block < blocks ? as[block] : 0, ys = block < blocks ? bs[block] : 0;
+        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand4(x), operand4(y), acc, 4, 4, 0, xs, 0, ys);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const uint32_t m = m0 + 4u * g + r, n = n0 + col;
+        if (m < p.a.rows && n < p.b.rows) static_cast<T *>(p.out)[size_t(m) * p.out_stride + n] = T(acc[r]);
+    }
+}
+template <typename T>
+static hipError_t small4(const Matmul4Args &a, hipStream_t s) {
+    const uint64_t mt = (a.a.rows + 15u) / 16u, nt = (a.b.rows + 15u) / 16u;
+    if (mt * nt * 64u >> 32) return hipErrorInvalidConfiguration;
+    return launch(k_fp4_small<T>, uint32_t(mt * nt), 64, 0, s, a, uint32_t(nt));
+}
+
+template <typename T>
+static hipError_t matmul4(const Matmul4Args &a, hipStream_t s) {
     if (a.a.rows <= 16 && a.dim >= 31) {
         const bool few = a.b.rows < 256 * 4 * 16;
         if (size_t(a.a.rows) * direct4_row(a.dim) <= kDirect4Lds) return few ? direct4<true>(a, s) : direct4<false>(a, s);
         const size_t lds = direct4_lds(a.a.rows, a.dim);
         if (lds <= kMostLds4 && (a.b.rows + 15) / 16 <= 256 * (kMostLds4 / lds)) return direct4<true>(a, s);
     }
+    if (a.dim < 31 || a.a.stride >= kMostTileStride4 || a.b.stride >= kMostTileStride4) return small4<T>(a, s);
     auto tiles = [&](uint32_t tm, uint32_t tn) { return uint64_t((a.a.rows + tm - 1) / tm) * ((a.b.rows + tn - 1) / tn); };
-    if (tiles(256, 256) >= 200) return tile4<256, 256, 2, 2, 1>(a, s);
-    if (tiles(128, 128) >= 256) return tile4<128, 128, 2, 2, 2>(a, s);
-    return tile4<64, 64, 2, 2, 4>(a, s);
+    if (tiles(256, 256) >= 200) return tile4<T, 256, 256, 2, 2, 1>(a, s);
+    if (tiles(128, 128) >= 256) return tile4<T, 128, 128, 2, 2, 2>(a, s);
+    return tile4<T, 64, 64, 2, 2, 4>(a, s);
+}
+hipError_t launch_fp4_matmul(const Matmul4Args &a, hipStream_t s) {
+    if (a.out_type == kF32) return matmul4<float>(a, s);
+    return a.out_type == kF16 ? matmul4<f16>(a, s) : matmul4<bf16>(a, s);
 }
 
 }  // namespace tv
