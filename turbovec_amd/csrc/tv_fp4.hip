@@ -241,11 +241,12 @@ template <typename T, int COLS> constexpr int kStrip4 = 32 * (COLS * int(sizeof(
 
 // A wave's results, whose lane l holds, of row l % 32 of each tile, columns 8 q + 4 (l / 32) .. + 3, to rows from m on and columns from n on: 32 rows at a time
 // through LDS, so that they leave in runs of whole cache lines.
-template <typename T, int COLS, int MT, int NT>
+template <typename T, bool STREAM, int COLS, int MT, int NT>
 __device__ __forceinline__ void store_strips4(const Matmul4Args &p, const v16f (&acc)[MT][NT], uint8_t *strip, uint32_t m, uint32_t n, int lane) {
     typedef T T4 __attribute__((ext_vector_type(4)));
     constexpr int kEach = 16 / int(sizeof(T)), kLanes = COLS / kEach, kRowsAtOnce = 64 / kLanes, kRow = COLS * int(sizeof(T)) + 16;
     const int row32 = lane & 31, half = lane >> 5;
+    const bool inside = m + MT * 32 <= p.a.rows && n + COLS <= p.b.rows;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
 #pragma unroll
@@ -256,25 +257,42 @@ __device__ __forceinline__ void store_strips4(const Matmul4Args &p, const v16f (
                 *reinterpret_cast<T4 *>(strip + row32 * kRow + (j * 32 + q * 8 + half * 4) * int(sizeof(T))) = __builtin_convertvector(x, T4);
             }
         const uint32_t at = uint32_t(lane % kLanes * kEach), on = n + at;
-#pragma unroll 4
+        const T *const from = reinterpret_cast<const T *>(strip + lane / kLanes * kRow) + at;
+        constexpr int kRounds = 32 / kRowsAtOnce, kTogether = kRounds < 8 ? kRounds : 8;
+        if (inside) {          // (a wave waits for eight reads once, not for each of them)
+            T *to = static_cast<T *>(p.out) + size_t(m + uint32_t(i * 32 + lane / kLanes)) * p.out_stride + on;
+#pragma unroll
+            for (int r = 0; r < kRounds; r += kTogether) {
+                v4i x[kTogether];
+#pragma unroll
+                for (int l = 0; l < kTogether; ++l) x[l] = *reinterpret_cast<const v4i *>(reinterpret_cast<const uint8_t *>(from) + (r + l) * kRowsAtOnce * kRow);
+#pragma unroll
+                for (int l = 0; l < kTogether; ++l) {
+                    if constexpr (STREAM) __builtin_nontemporal_store(x[l], reinterpret_cast<v4i_any *>(to));
+                    else *reinterpret_cast<v4i_any *>(to) = x[l];
+                    to += kRowsAtOnce * p.out_stride;
+                }
+            }
+            continue;
+        }
+#pragma unroll 1
         for (int r = 0; r < 32; r += kRowsAtOnce) {
-            const int row = r + lane / kLanes;
-            const uint32_t om = m + uint32_t(i * 32 + row);
-            const T *const from = reinterpret_cast<const T *>(strip + row * kRow) + at;
-            T *const to = static_cast<T *>(p.out) + size_t(om) * p.out_stride + on;
+            const uint32_t om = m + uint32_t(i * 32 + r + lane / kLanes);
             if (om >= p.a.rows || on >= p.b.rows) continue;
+            const T *const x = reinterpret_cast<const T *>(reinterpret_cast<const uint8_t *>(from) + r * kRow);
+            T *const to = static_cast<T *>(p.out) + size_t(om) * p.out_stride + on;
             if (on + kEach <= p.b.rows) {
-                *reinterpret_cast<v4i_any *>(to) = *reinterpret_cast<const v4i *>(from);
+                *reinterpret_cast<v4i_any *>(to) = *reinterpret_cast<const v4i *>(x);
             } else {
 #pragma unroll 1
-                for (uint32_t l = 0; on + l < p.b.rows; ++l) to[l] = from[l];
+                for (uint32_t l = 0; on + l < p.b.rows; ++l) to[l] = x[l];
             }
         }
     }
 }
 
 template <typename T, int TM, int TN, int WM, int WN, int HELD>
-__global__ __launch_bounds__(64 * WM * WN, HELD) void k_fp4_tile(Matmul4Args p, uint32_t m_tiles, uint32_t n_tiles, uint32_t each_xcd) {
+__global__ __launch_bounds__(64 * WM * WN, HELD) void k_fp4_tile(Matmul4Args p, uint32_t m_tiles, uint32_t n_tiles, uint32_t each_xcd, bool stream) {
     extern __shared__ uint8_t smem[];
     constexpr int kWaves = WM * WN, kThreads = 64 * kWaves, kRows = TM + TN, kGroups = kRows / 8 / kWaves, MT = TM / WM / 32, NT = TN / WN / 32;
     constexpr uint32_t kBuffer = kRows * kStageBytes4;
@@ -460,16 +478,21 @@ __global__ __launch_bounds__(64 * WM * WN, HELD) void k_fp4_tile(Matmul4Args p, 
         sc = sc_next;
     }
     __syncthreads();
-    store_strips4<T, TN / WN, MT, NT>(p, acc, smem + wave * kStrip4<T, TN / WN>, m0 + wm, n0 + wn, lane);
+    uint8_t *const strip = smem + wave * kStrip4<T, TN / WN>;
+    if (stream) store_strips4<T, true, TN / WN, MT, NT>(p, acc, strip, m0 + wm, n0 + wn, lane);
+    else store_strips4<T, false, TN / WN, MT, NT>(p, acc, strip, m0 + wm, n0 + wn, lane);
 }
 
+// Results of rows below this leave past the L2: they would push out what other tiles read there.  (1024 by 100000 of 1536 into floats 148 us so and 170 to 185 otherwise;
+// 4096 by 16384 of 4096 175 and 170.)
+constexpr uint32_t kStreamDim4 = 2048;
 template <typename T, int TM, int TN, int WM, int WN, int HELD>
 static hipError_t tile4(const Matmul4Args &a, hipStream_t s) {
     const uint64_t mt = (a.a.rows + TM - 1) / TM, nt = (a.b.rows + TN - 1) / TN, each_xcd = (mt * nt + 7) / 8;
     if ((each_xcd * 8 * (64 * WM * WN)) >> 32) return hipErrorInvalidConfiguration;      // (a result of hundreds of GB, or a narrow one of a billion columns)
     const auto kernel = k_fp4_tile<T, TM, TN, WM, WN, HELD>;
     if (const hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), tile4_lds<TM, TN>()); e != hipSuccess) return e;
-    return launch(kernel, uint32_t(each_xcd * 8), 64 * WM * WN, tile4_lds<TM, TN>(), s, a, uint32_t(mt), uint32_t(nt), uint32_t(each_xcd));
+    return launch(kernel, uint32_t(each_xcd * 8), 64 * WM * WN, tile4_lds<TM, TN>(), s, a, uint32_t(mt), uint32_t(nt), uint32_t(each_xcd), a.dim < kStreamDim4);
 }
 
 // Rows of fewer than 16 bytes, or 8 MB and more apart: a wave to a tile of 16 by 16, its operands read where they lie.
@@ -501,19 +524,70 @@ static hipError_t small4(const Matmul4Args &a, hipStream_t s) {
     return launch(k_fp4_small<T>, uint32_t(mt * nt), 64, 0, s, a, uint32_t(nt));
 }
 
+// The tiles, and what one takes a compute unit that holds so many of them, in microseconds: for a stage, in front and behind, and for a byte of the result's type.  Fitted to 56 sizes of 17 to
+// 8192 rows by 100 to 1M, of 74 to 8192, into floats and bfloat16: the tile taken is the fastest there or within 6 % of it but for five, 24 % at worst (2669 by 15974 of 1024), 1.3 %
+// on the mean.  A compute unit's tiles come in rounds of as many as it holds, and a started round costs a whole one.
+struct TileTime {
+    uint32_t tm, tn, held;
+    double stage, once, byte;
+};
+constexpr TileTime kTiles4[] = {{256, 256, 1, 1.4, 4.5, 1.3}, {128, 128, 2, 0.55, 0.42, 0.39}, {64, 64, 4, 0.22, 0.29, 0.11}, {64, 128, 3, 0.37, 0.21, 0.27}, {32, 128, 3, 0.25, 0.32, 0.18}};
+static double tile_time4(const TileTime &t, uint32_t m, uint32_t n, uint32_t dim, size_t size) {
+    const uint64_t tiles = uint64_t((m + t.tm - 1) / t.tm) * ((n + t.tn - 1) / t.tn), one = 256 * t.held;
+    const double each = double(tiles <= one ? (tiles + 255) / 256 : (tiles + one - 1) / one * t.held);
+    return each * ((dim + kStage4 - 1) / kStage4 * t.stage + t.once + t.byte * double(size));
+}
+static int best_tile4(uint32_t m, uint32_t n, uint32_t dim, size_t size, double &time) {
+    int best = 0;
+    for (int i = 0; i < (m <= 32 ? 5 : 4); ++i)
+        if (const double t = tile_time4(kTiles4[i], m, n, dim, size); i == 0 || t < time) {
+            best = i;
+            time = t;
+        }
+    return best;
+}
+template <typename T>
+static hipError_t tiled4(const Matmul4Args &a, int tile, hipStream_t s) {
+    if (tile == 0) return tile4<T, 256, 256, 2, 2, 1>(a, s);
+    if (tile == 1) return tile4<T, 128, 128, 2, 2, 2>(a, s);
+    if (tile == 2) return tile4<T, 64, 64, 2, 2, 4>(a, s);
+    return tile == 3 ? tile4<T, 64, 128, 2, 2, 3>(a, s) : tile4<T, 32, 128, 1, 4, 3>(a, s);
+}
+
 template <typename T>
 static hipError_t matmul4(const Matmul4Args &a, hipStream_t s) {
     if (a.a.rows <= 16 && a.dim >= 31) {
+        // Sixteen rows to a wave leave waves without any; shared out, one row against 4096 to 16384 of 1536 takes 4 us.  (One row against 1M of 1536 147 us, in tiles of 64 165;
+        // sixteen against 100000 19 and 20.)
         const bool few = a.b.rows < 256 * 4 * 16;
         if (size_t(a.a.rows) * direct4_row(a.dim) <= kDirect4Lds) return few ? direct4<true>(a, s) : direct4<false>(a, s);
+        // More of a than that leaves a compute unit one workgroup or two: as long as none waits for its turn.
         const size_t lds = direct4_lds(a.a.rows, a.dim);
         if (lds <= kMostLds4 && (a.b.rows + 15) / 16 <= 256 * (kMostLds4 / lds)) return direct4<true>(a, s);
     }
     if (a.dim < 31 || a.a.stride >= kMostTileStride4 || a.b.stride >= kMostTileStride4) return small4<T>(a, s);
-    auto tiles = [&](uint32_t tm, uint32_t tn) { return uint64_t((a.a.rows + tm - 1) / tm) * ((a.b.rows + tn - 1) / tn); };
-    if (tiles(256, 256) >= 200) return tile4<T, 256, 256, 2, 2, 1>(a, s);
-    if (tiles(128, 128) >= 256) return tile4<T, 128, 128, 2, 2, 2>(a, s);
-    return tile4<T, 64, 64, 2, 2, 4>(a, s);
+    double whole = 0;
+    const int tile = best_tile4(a.a.rows, a.b.rows, a.dim, sizeof(T), whole);
+    const uint32_t mt = (a.a.rows + 255) / 256, nt = (a.b.rows + 255) / 256;
+    const uint64_t tiles = uint64_t(mt) * nt;
+    if (tile == 0 && tiles > 256 && nt >= mt) {
+        // The tiles of 256 that start a last round and do not fill it: their columns in a launch of their own, of smaller tiles, where that is less than the round.  (1024 by 100000
+        // of 1536 into floats: FIGURE.)
+        const uint32_t columns = uint32_t(tiles / 256 * 256 / mt) * 256;
+        if (columns < a.b.rows) {
+            Matmul4Args first = a, rest = a;
+            first.b.rows = columns;
+            rest.b = Rows4{a.b.codes + size_t(columns) * a.b.stride, a.b.scales + size_t(columns) * a.b.scale_stride, a.b.stride, a.b.scale_stride, a.b.rows - columns};
+            rest.out = static_cast<T *>(a.out) + columns;
+            double more = 0;
+            const int rest_tile = best_tile4(rest.a.rows, rest.b.rows, a.dim, sizeof(T), more);
+            if (tile_time4(kTiles4[0], a.a.rows, columns, a.dim, sizeof(T)) + more + 3.0 < whole) {
+                const hipError_t e = tiled4<T>(first, 0, s);
+                return e == hipSuccess ? tiled4<T>(rest, rest_tile, s) : e;
+            }
+        }
+    }
+    return tiled4<T>(a, tile, s);
 }
 hipError_t launch_fp4_matmul(const Matmul4Args &a, hipStream_t s) {
     if (a.out_type == kF32) return matmul4<float>(a, s);
