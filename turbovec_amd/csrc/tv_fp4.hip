@@ -115,10 +115,10 @@ __device__ __forceinline__ void store_out4(void *out, size_t at, float v, int ty
     else static_cast<bf16 *>(out)[at] = bf16(v);
 }
 
-// Up to sixteen rows of a: bound by reading b once.  A wave streams 16 rows of b from memory into registers, four steps of 128 coordinates while the four
+// Up to sixteen rows of a: bound by reading b once.  A wave streams 16 rows of b from memory into registers, two steps of 128 coordinates while the two
 // before are multiplied, and goes on to its next 16 rows without a pause; a lies in LDS.  Where there are few rows of b (SPLIT), the four waves of
 // a workgroup share 16 rows, each taking every fourth step, and their sums are added in the waves' order.
-constexpr int kDirect4Threads = 256, kDirect4Waves = kDirect4Threads / 64, kDirect4Steps = 4;
+constexpr int kDirect4Threads = 256, kDirect4Waves = kDirect4Threads / 64, kDirect4Steps = 2;
 constexpr uint32_t kDirect4Groups = 4;        // workgroups of a compute unit at a time
 constexpr size_t kDirect4Lds = 64 << 10, kMostLds4 = 160 << 10;
 
@@ -161,8 +161,8 @@ __global__ __launch_bounds__(kDirect4Threads, kDirect4Groups) void k_fp4_direct(
         const uint32_t first = at.turn * kDirect4Steps;
 #pragma unroll
         for (int i = 0; i < kDirect4Steps; ++i) s.codes[i] = *reinterpret_cast<const v4i_any *>(at.codes + min((first + i) * 64u + uint32_t(g) * 16u, bytes - 16u));
-        if (first * 4u + 16u <= blocks) {
-            __builtin_memcpy(s.scales, at.scales + first * 4u, 16);
+        if (first * 4u + sizeof(s.scales) <= blocks) {
+            __builtin_memcpy(s.scales, at.scales + first * 4u, sizeof(s.scales));
         } else {
 #pragma unroll
             for (int i = 0; i < kDirect4Steps; ++i) s.scales[i] = (first + i) * 4u < blocks ? scales4(at.scales, (first + i) * 4u, blocks) : 0u;
@@ -525,13 +525,13 @@ static hipError_t small4(const Matmul4Args &a, hipStream_t s) {
 }
 
 // The tiles, and what one takes a compute unit that holds so many of them, in microseconds: for a stage, in front and behind, and for a byte of the result's type.  Fitted to 56 sizes of 17 to
-// 8192 rows by 100 to 1M, of 74 to 8192, into floats and bfloat16: the tile taken is the fastest there or within 6 % of it but for five, 24 % at worst (2669 by 15974 of 1024), 1.3 %
+// 8192 rows by 100 to 1M, of 74 to 8192, into floats and bfloat16: the tile taken is the fastest there or within 6 % of it but for three, 25 % at worst (2669 by 15974 of 1024), 1.1 %
 // on the mean.  A compute unit's tiles come in rounds of as many as it holds, and a started round costs a whole one.
 struct TileTime {
     uint32_t tm, tn, held;
     double stage, once, byte;
 };
-constexpr TileTime kTiles4[] = {{256, 256, 1, 1.4, 4.5, 1.3}, {128, 128, 2, 0.55, 0.42, 0.39}, {64, 64, 4, 0.22, 0.29, 0.11}, {64, 128, 3, 0.37, 0.21, 0.27}, {32, 128, 3, 0.25, 0.32, 0.18}};
+constexpr TileTime kTiles4[] = {{256, 256, 1, 1.44, 4.3, 1.4}, {128, 128, 2, 0.59, 0.34, 0.42}, {64, 64, 4, 0.23, 0.24, 0.14}, {64, 128, 3, 0.39, 0.18, 0.3}, {32, 128, 3, 0.27, 0.33, 0.19}};
 static double tile_time4(const TileTime &t, uint32_t m, uint32_t n, uint32_t dim, size_t size) {
     const uint64_t tiles = uint64_t((m + t.tm - 1) / t.tm) * ((n + t.tn - 1) / t.tn), one = 256 * t.held;
     const double each = double(tiles <= one ? (tiles + 255) / 256 : (tiles + one - 1) / one * t.held);
