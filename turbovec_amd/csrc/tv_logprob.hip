@@ -2,6 +2,7 @@
 //
 // With m the largest score that counts, d = (score - m) / T, S = sum of exp(d) and U = sum of exp(d) d: log p = d - log S, and the entropy is
 // log S - U / S, two terms that are not below 0.  Exponentials are of base 2, with log2(e) / T as the factor.
+#include <algorithm>
 #include <cfloat>
 
 #include "tv_device.h"
@@ -29,136 +30,481 @@ struct Heat {
 __device__ __forceinline__ bool counts(const uint64_t *mask, uint32_t i, float s) {
     return (mask == nullptr || ((mask[i >> 6] >> (i & 63u)) & 1u)) && !(s == -kInf);
 }
-// The order of alternatives, 0 for what is none.
-__device__ __forceinline__ uint64_t slot_key(const uint64_t *mask, uint32_t i, float s) { return counts(mask, i, s) && s == s ? sort_key(s, i) : 0ull; }
-
-// Sums of exp(d) and exp(d) log2(exp(d)) in d's own base.
+// What a set of scores adds up to: its largest score (kNone or less: it has none), and the sums of 2^t and 2^t t over it, t = (score - largest) * factor2 <= 0.
+constexpr float kNone = -FLT_MAX;
 struct Sums {
-    float s = 0.0f, u = 0.0f;
-    __device__ __forceinline__ void add(float t) {
-        const float e = __builtin_amdgcn_exp2f(t);
-        s += e;
-        u = fmaf(e, fmaxf(t, -200.0f), u);       // (2^-200 is 0 here, an infinity times that is not)
+    float m = kNone, s = 0.0f, u = 0.0f;
+    // The same, seen from a largest score that is not below its own.  (2^-10000 is 0 here; an infinity times 0 is not.)
+    __device__ __forceinline__ void rise(float to, float factor2) {
+        const float d = fmaxf((m - to) * factor2, -10000.0f), f = __builtin_amdgcn_exp2f(d);
+        u = f * fmaf(s, d, u);
+        s *= f;
+        m = to;
     }
+    __device__ __forceinline__ void add(float score, float factor2) {
+        const float t = (score - m) * factor2, e = __builtin_amdgcn_exp2f(t);
+        s += e;
+        u = fmaf(e, fmaxf(t, -200.0f), u);
+    }
+    __device__ __forceinline__ float entropy(float log_sum) const { return s == 0.0f ? 0.0f : log_sum - kLn2 * (u / s); }
 };
 
-constexpr int kLogThreads = 256;
-template <typename F>
-__device__ __forceinline__ float over_group(float v, float *part, F &&f) {
+constexpr int kLogThreads = 256, kLogWaves = kLogThreads / 64;
+// Sums over the workgroup, in every thread; `best` has room for a float a thread and is left holding the threads' largest scores.
+struct Reduce {
+    __attribute__((aligned(16))) float best[kLogThreads];
+    float part[2 * kLogWaves];
+};
+__device__ __forceinline__ Sums group_sums(Sums v, float factor2, Reduce &r) {
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    r.best[threadIdx.x] = v.m;
+    __syncthreads();
+    float m = fmaxf(fmaxf(r.best[lane], r.best[64 + lane]), fmaxf(r.best[128 + lane], r.best[192 + lane]));
 #pragma unroll
-    for (int i = 32; i > 0; i >>= 1) v = f(v, __shfl_xor(v, i));
+    for (int i = 32; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
+    v.rise(m, factor2);
+#pragma unroll
+    for (int i = 32; i > 0; i >>= 1) {
+        v.s += __shfl_xor(v.s, i);
+        v.u += __shfl_xor(v.u, i);
+    }
+    if (lane == 0) {
+        r.part[wave] = v.s;
+        r.part[kLogWaves + wave] = v.u;
+    }
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = part[0];
-    for (int i = 1; i < kLogThreads / 64; ++i) v = f(v, part[i]);
+    v.s = (r.part[0] + r.part[1]) + (r.part[2] + r.part[3]);
+    v.u = (r.part[4] + r.part[5]) + (r.part[6] + r.part[7]);
     return v;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kLogThreads) void k_log_probs(LogProbArgs a) {
-    __shared__ float part[kLogThreads / 64];
-    __shared__ uint64_t best[kLogThreads / 64];
-    for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const T *const scores = static_cast<const T *>(a.scores) + size_t(row) * a.stride;
-        const uint64_t *const mask = a.mask == nullptr ? nullptr : a.mask + size_t(row) * a.mask_stride;
-        const Heat heat(a.temperature, row);
-        float m = -kInf;
-        for (uint32_t i = threadIdx.x; i < a.n; i += kLogThreads) {
-            const float s = float(scores[i]);
-            if (counts(mask, i, s)) m = fmaxf(m, s);
-        }
-        m = over_group(m, part, [](float x, float y) { return fmaxf(x, y); });
-        if (m == -kInf) m = 0.0f;
-        Sums sums;
-        for (uint32_t i = threadIdx.x; i < a.n; i += kLogThreads) {
-            const float s = float(scores[i]);
-            if (counts(mask, i, s)) sums.add((s - m) * heat.factor2);
-        }
-        const float s = over_group(sums.s, part, [](float x, float y) { return x + y; }), u = over_group(sums.u, part, [](float x, float y) { return x + y; });
-        const float log_sum = logf(s), entropy = s == 0.0f ? 0.0f : log_sum - kLn2 * (u / s);
-        if (threadIdx.x == 0) {
-            a.out_entropy[row] = entropy;
-            if (a.stats != nullptr) {
-                float *const to = a.stats + size_t(row) * 4;
-                to[0] = m; to[1] = log2f(s); to[2] = entropy; to[3] = 0.0f;
-            }
-        }
-        for (uint32_t i = threadIdx.x; i < a.given; i += kLogThreads) {
-            const int64_t slot = a.slots[size_t(row) * a.slot_stride + i];
-            float lp = -kInf;
-            if (slot >= 0 && slot < int64_t(a.n)) {
-                const float v = float(scores[slot]);
-                if (counts(mask, uint32_t(slot), v)) lp = heat.log_p(v - m, log_sum);
-            }
-            a.out_log_probs[size_t(row) * a.given + i] = lp;
-        }
-        uint64_t below = ~0ull;
-        for (uint32_t k = 0; k < a.top; ++k) {
-            uint64_t mine = 0;
-            if (below != 0)
-                for (uint32_t i = threadIdx.x; i < a.n; i += kLogThreads) {
-                    const uint64_t key = slot_key(mask, i, float(scores[i]));
-                    if (key < below && key > mine) mine = key;
-                }
+// The best keys of those that a workgroup has met: gathered in LDS, cut to the k best whenever the next 8 a thread might not fit.
+constexpr uint32_t kKeep = 256, kGather = kKeep + 8 * kLogThreads;
+struct Gathered {
+    uint64_t keys[kGather];
+    uint32_t count, part[2][kLogWaves];
+};
+// Of the `count` keys, kKeep < count <= kGather: the k-th largest, bit by bit from the highest on; it and those above stay.
+__device__ __forceinline__ uint64_t cut(Gathered &g, uint32_t k) {
+    constexpr int kEach = (kGather + kLogThreads - 1) / kLogThreads;
+    const uint32_t count = g.count, wave = threadIdx.x >> 6;
+    uint64_t mine[kEach];
 #pragma unroll
-            for (int i = 32; i > 0; i >>= 1) mine = max(mine, uint64_t(__shfl_xor((unsigned long long)(mine), i)));
-            __syncthreads();
-            if ((threadIdx.x & 63) == 0) best[threadIdx.x >> 6] = mine;
-            __syncthreads();
-            for (int i = 0; i < kLogThreads / 64; ++i) mine = max(mine, best[i]);
-            below = mine;
-            if (threadIdx.x == 0) {
-                float v = 0.0f;
-                uint32_t slot = 0;
-                sort_unkey(mine, v, slot);
-                a.out_top_slots[size_t(row) * a.top + k] = mine == 0 ? -1 : int64_t(slot);
-                a.out_top_log_probs[size_t(row) * a.top + k] = mine == 0 ? -kInf : heat.log_p(v - m, log_sum);
-            }
-        }
+    for (int i = 0; i < kEach; ++i) mine[i] = uint32_t(i * kLogThreads) + threadIdx.x < count ? g.keys[i * kLogThreads + threadIdx.x] : 0ull;
+    uint64_t found = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+        const uint64_t trial = found | 1ull << bit;
+        uint32_t n = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) n += uint32_t(__popcll(__ballot(mine[i] >= trial)));
+        uint32_t *const part = g.part[bit & 1];
+        if ((threadIdx.x & 63u) == 0) part[wave] = n;
+        __syncthreads();
+        if (part[0] + part[1] + part[2] + part[3] >= k) found = trial;
     }
+    if (threadIdx.x == 0) g.count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+        if (mine[i] >= found) g.keys[atomicAdd(&g.count, 1u)] = mine[i];
+    __syncthreads();
+    return found;
 }
-size_t log_probs_workspace(size_t, size_t, size_t) { return 0; }
-template <typename T>
-static hipError_t log_probs(const LogProbArgs &a, hipStream_t s) {
-    return launch(k_log_probs<T>, uint32_t(a.rows < kMostGroups ? a.rows : kMostGroups), kLogThreads, 0, s, a);
-}
-hipError_t launch_log_probs(const LogProbArgs &a, int score_type, hipStream_t s) {
-    if (score_type == kF32) return log_probs<float>(a, s);
-    return score_type == kF16 ? log_probs<f16>(a, s) : log_probs<bf16>(a, s);
+// The k best in order to `out`, zeros where there are fewer.  (A thread finds its keys' places by counting.)
+template <typename F>
+__device__ __forceinline__ void in_order(Gathered &g, uint32_t k, F &&out) {
+    uint32_t count = g.count;
+    if (count > 2 * kLogThreads) {
+        cut(g, k);
+        count = g.count;
+    }
+    if (threadIdx.x < count) {
+        const uint64_t mine = g.keys[threadIdx.x], other = threadIdx.x + kLogThreads < count ? g.keys[threadIdx.x + kLogThreads] : 0ull;
+        uint32_t place = 0, other_place = 0;
+#pragma unroll 4
+        for (uint32_t i = 0; i < count; ++i) {
+            const uint64_t x = g.keys[i];
+            place += x > mine;
+            other_place += x > other;
+        }
+        if (place < k) out(place, mine);
+        if (other != 0 && other_place < k) out(other_place, other);
+    }
+    for (uint32_t i = threadIdx.x; i < k; i += kLogThreads)
+        if (i >= count) out(i, 0ull);
 }
 
-// The gradient of a score that counts: (picked - G p - g p (log p + H)) / T, picked the sum of the gradients of the given slots that are this one.
+// A row's results from its sums and best keys.
 template <typename T>
-__global__ __launch_bounds__(kLogThreads) void k_log_probs_grad(LogProbGradArgs a) {
+__device__ __forceinline__ void finish(const LogProbArgs &a, uint32_t row, const T *scores, const uint64_t *mask, const Heat &heat, const Sums &sums, Gathered &g) {
+    const float log_sum = logf(sums.s);
+    if (threadIdx.x == 0) {
+        const float entropy = sums.entropy(log_sum);
+        a.out_entropy[row] = entropy;
+        if (a.stats != nullptr) *reinterpret_cast<float4 *>(a.stats + size_t(row) * 4) = make_float4(sums.m, log2f(sums.s), entropy, 0.0f);
+    }
+    for (uint32_t i = threadIdx.x; i < a.given; i += kLogThreads) {
+        const int64_t slot = a.slots[size_t(row) * a.slot_stride + i];
+        float lp = -kInf;
+        if (slot >= 0 && slot < int64_t(a.n)) {
+            const float v = float(scores[slot]);
+            if (counts(mask, uint32_t(slot), v)) lp = heat.log_p(v - sums.m, log_sum);
+        }
+        a.out_log_probs[size_t(row) * a.given + i] = lp;
+    }
+    if (a.top != 0)
+        in_order(g, a.top, [&](uint32_t place, uint64_t key) {
+            float v = 0.0f;
+            uint32_t slot = 0;
+            sort_unkey(key, v, slot);
+            a.out_top_slots[size_t(row) * a.top + place] = key == 0 ? -1 : int64_t(slot);
+            a.out_top_log_probs[size_t(row) * a.top + place] = key == 0 ? -kInf : heat.log_p(v - sums.m, log_sum);
+        });
+}
+
+// Scores i .. i + kEach - 1 as floats, i a multiple of kEach; what is masked and what lies behind the end is -infinity.
+template <typename T>
+struct Scores {
+    static constexpr int kEach = 16 / int(sizeof(T));
+    T v[kEach];
+    uint32_t bits;
+    __device__ __forceinline__ void load(const T *scores, const uint64_t *mask, uint32_t i) {
+        __builtin_memcpy(v, scores + i, 16);
+        bits = mask == nullptr ? ~0u : uint32_t(mask[i >> 6] >> (i & 63u));
+    }
+    __device__ __forceinline__ void load_end(const T *scores, const uint64_t *mask, uint32_t i, uint32_t n) {
+        bits = mask == nullptr ? ~0u : uint32_t(mask[i >> 6] >> (i & 63u));
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) v[j] = i + j < n ? scores[i + j] : T(-kInf);
+    }
+    template <bool MASK>
+    __device__ __forceinline__ float at(int j) const { return !MASK || ((bits >> j) & 1u) ? float(v[j]) : -kInf; }
+};
+
+// A part of a row to a workgroup, all of it where there are rows enough.  One pass takes the sums, a thread each its own from its own largest score, which it raises once for
+// four loads.  The alternatives come from the threads' largest scores: the k-th of those is one that k scores reach, and so is what its first bits say; only where a thread
+// reaches that itself, a thread's part in four for itself, is the row read again.
+struct LogPart {
+    float m, s, u, none;
+};
+constexpr int kLogLoads = 4, kLogSegments = 4;
+// Where thread t's scores lie: load l is at lo + (l * kLogThreads + t) * kEach, the first `segment` loads are its first segment.
+struct Loads {
+    uint32_t lo, hi, all, segment;
+    __device__ __forceinline__ Loads(uint32_t from, uint32_t to, uint32_t step) : lo(from), hi(to) {
+        all = (to - from + step - 1) / step;
+        constexpr uint32_t kRounds = kLogSegments * kLogLoads;
+        segment = all < 2 * kRounds ? all : (all + kRounds - 1) / kRounds * kLogLoads;
+    }
+};
+template <typename T, bool MASK>
+__device__ __forceinline__ void scan_part(const T *scores, const uint64_t *mask, const Heat &heat, const Loads &at, Sums &sums, float (&segments)[kLogSegments]) {
+    constexpr int kEach = Scores<T>::kEach;
+    constexpr uint32_t kStep = kLogThreads * kEach;
+    float segment = kNone;
+    auto take = [&](const Scores<T> *l, auto count) {
+        constexpr int kCount = decltype(count)::value;
+        float m = l[0].template at<MASK>(0);
+#pragma unroll
+        for (int i = 0; i < kCount; ++i)
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) m = fmaxf(m, l[i].template at<MASK>(j));
+        segment = fmaxf(segment, m);
+        sums.rise(fmaxf(sums.m, m), heat.factor2);
+#pragma unroll
+        for (int i = 0; i < kCount; ++i)
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) sums.add(l[i].template at<MASK>(j), heat.factor2);
+    };
+#pragma unroll
+    for (int part = 0; part < kLogSegments; ++part) {
+        const uint32_t first = at.lo + uint32_t(part) * at.segment * kStep, end = part + 1 == kLogSegments ? at.hi : min(at.lo + uint32_t(part + 1) * at.segment * kStep, at.hi);
+        segment = kNone;
+        if (uint32_t(part) * at.segment < at.all) {
+            uint32_t i = first + threadIdx.x * kEach;
+            for (; i + (kLogLoads - 1) * kStep + kEach <= end; i += kLogLoads * kStep) {
+                Scores<T> l[kLogLoads];
+#pragma unroll
+                for (int j = 0; j < kLogLoads; ++j) l[j].load(scores, mask, i + j * kStep);
+                take(l, IntC<kLogLoads>{});
+            }
+            for (; i < end; i += kStep) {
+                Scores<T> l;
+                if (i + kEach <= end) l.load(scores, mask, i);
+                else l.load_end(scores, mask, i, end);
+                take(&l, IntC<1>{});
+            }
+        }
+        segments[part] = segment;
+    }
+}
+// One that at least k of the 256 scores in `best` reach, and not far below the k-th: its first 16 bits in the scores' order.  The same in every thread.
+__device__ __forceinline__ float reached(const float *best, uint32_t k) {
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t key[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) key[i] = uint32_t(order_key(best[i * 64 + lane] + 0.0f)) ^ 0x80000000u;
+    uint32_t found = 0;
+    if (k <= 24) {          // (the largest of four threads each: 64 of those do)
+        const uint32_t one = max(max(key[0], key[1]), max(key[2], key[3]));
+#pragma unroll
+        for (int bit = 31; bit >= 16; --bit)
+            if (uint32_t(__popcll(__ballot(one >= (found | 1u << bit)))) >= k) found |= 1u << bit;
+    } else {
+#pragma unroll
+        for (int bit = 31; bit >= 16; --bit) {
+            uint32_t n = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) n += uint32_t(__popcll(__ballot(key[i] >= (found | 1u << bit))));
+            if (n >= k) found |= 1u << bit;
+        }
+    }
+    return fmaxf(order_unkey(int(found ^ 0x80000000u)), kNone);      // (nothing counts below that; a key of 0 is no number)
+}
+template <typename T, bool MASK>
+__device__ __forceinline__ void gather_part(const LogProbArgs &a, const T *scores, const uint64_t *mask, const Loads &at, const float (&segments)[kLogSegments], Gathered &g, const float *best,
+                                            uint16_t *who, uint32_t *who_count) {
+    constexpr int kEach = Scores<T>::kEach;
+    constexpr uint32_t kStep = kLogThreads * kEach;
+    const float least = reached(best, a.top);
+    if (threadIdx.x == 0) g.count = *who_count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kLogSegments; ++i)
+        if (segments[i] >= least && uint32_t(i) * at.segment < at.all) who[atomicAdd(who_count, 1u)] = uint16_t(i * kLogThreads + threadIdx.x);
+    __syncthreads();
+    const uint32_t items = *who_count * at.segment;
+    auto place = [&](uint32_t item) {      // hi where there is nothing
+        if (item >= items) return at.hi;
+        const uint32_t it = who[item / at.segment], l = it / kLogThreads * at.segment + item % at.segment;
+        const uint64_t i = at.lo + uint64_t(l) * kStep + it % kLogThreads * kEach;
+        return l < at.all && i < at.hi ? uint32_t(i) : at.hi;
+    };
+    auto load = [&](Scores<T> &l, uint32_t i) {
+        if (i >= at.hi) return;
+        if (i + kEach <= at.hi) l.load(scores, mask, i);
+        else l.load_end(scores, mask, i, at.hi);
+    };
+    auto put = [&](const Scores<T> &l, uint32_t i, uint64_t above) {
+        if (i >= at.hi) return;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            const float v = l.template at<MASK>(j);
+            if (!(v >= least)) continue;
+            const uint64_t key = sort_key(v, i + j);
+            if (key <= above) continue;
+            const uint32_t to = atomicAdd(&g.count, 1u);
+            if (to < kGather) g.keys[to] = key;
+        }
+    };
+    // As a rule all that is met fits.
+    for (uint32_t first = threadIdx.x; first < items; first += 2 * kLogThreads) {
+        Scores<T> l[2];
+        const uint32_t i[2] = {place(first), place(first + kLogThreads)};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) load(l[j], i[j]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) put(l[j], i[j], 0);
+    }
+    __syncthreads();
+    if (g.count <= kGather) return;
+    // Crowded scores: once more, cut to the best whenever the next load of all threads might not fit.
+    __syncthreads();
+    if (threadIdx.x == 0) g.count = 0;
+    __syncthreads();
+    uint64_t above = 0;
+    for (uint32_t first = 0; first < items; first += kLogThreads) {
+        Scores<T> l;
+        const uint32_t i = place(first + threadIdx.x);
+        load(l, i);
+        put(l, i, above);
+        __syncthreads();
+        const uint32_t count = g.count;
+        __syncthreads();
+        if (count > kKeep) above = cut(g, a.top);
+    }
+}
+template <typename T, bool MASK>
+__global__ __launch_bounds__(kLogThreads) void k_log_probs(LogProbArgs a, uint32_t parts, uint32_t part_size) {
+    __shared__ Reduce reduce;
+    __shared__ Gathered g;
+    __shared__ uint16_t who[kLogSegments * kLogThreads];
+    __shared__ uint32_t who_count;
+    LogPart *const out = reinterpret_cast<LogPart *>(a.ws);
+    uint64_t *const out_keys = reinterpret_cast<uint64_t *>(a.ws + size_t(a.rows) * parts * sizeof(LogPart));
+    for (uint64_t unit = blockIdx.x; unit < uint64_t(a.rows) * parts; unit += gridDim.x) {
+        const uint32_t row = uint32_t(unit / parts), lo = uint32_t(unit % parts) * part_size;
+        const Loads at(lo, min(part_size, a.n - lo) + lo, kLogThreads * Scores<T>::kEach);
+        const T *const scores = static_cast<const T *>(a.scores) + size_t(row) * a.stride;
+        const uint64_t *const mask = MASK ? a.mask + size_t(row) * a.mask_stride : nullptr;
+        const Heat heat(a.temperature, row);
+        Sums sums;
+        float segments[kLogSegments];
+        scan_part<T, MASK>(scores, mask, heat, at, sums, segments);
+        sums = group_sums(sums, heat.factor2, reduce);
+        if (a.top != 0) gather_part<T, MASK>(a, scores, mask, at, segments, g, reduce.best, who, &who_count);
+        if (parts == 1) {
+            finish(a, row, scores, mask, heat, sums, g);
+        } else {
+            if (threadIdx.x == 0) out[unit] = LogPart{sums.m, sums.s, sums.u, 0.0f};
+            if (a.top != 0) in_order(g, a.top, [&](uint32_t place, uint64_t key) { out_keys[unit * a.top + place] = key; });
+        }
+        __syncthreads();
+    }
+}
+// The parts of a row, joined.
+template <typename T>
+__global__ __launch_bounds__(kLogThreads) void k_log_probs_join(LogProbArgs a, uint32_t parts) {
+    __shared__ Reduce reduce;
+    __shared__ Gathered g;
+    __shared__ uint64_t least[kLogWaves];
+    const LogPart *const in = reinterpret_cast<const LogPart *>(a.ws);
+    const uint64_t *const in_keys = reinterpret_cast<const uint64_t *>(a.ws + size_t(a.rows) * parts * sizeof(LogPart));
     for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T *const scores = static_cast<const T *>(a.scores) + size_t(row) * a.stride;
-        const uint64_t *const mask = a.mask == nullptr ? nullptr : a.mask + size_t(row) * a.mask_stride;
+        const uint64_t *const mask = a.mask == nullptr ? nullptr : a.mask + size_t(row) * a.mask_stride, *const mine = reinterpret_cast<const uint64_t *>(in_keys) + size_t(row) * parts * a.top;
+        const Heat heat(a.temperature, row);
+        if (threadIdx.x == 0) g.count = 0;
+        Sums sums;
+        uint64_t kth = 0;          // a part's last key is one that a.top keys reach
+        for (uint32_t i = threadIdx.x; i < parts; i += kLogThreads) {
+            const LogPart p = in[size_t(row) * parts + i];
+            if (a.top != 0) kth = max(kth, mine[size_t(i) * a.top + a.top - 1]);
+            Sums more;
+            more.m = p.m; more.s = p.s; more.u = p.u;
+            const float m = fmaxf(sums.m, p.m);
+            sums.rise(m, heat.factor2);
+            more.rise(m, heat.factor2);
+            sums.s += more.s;
+            sums.u += more.u;
+        }
+        if (a.top != 0) {
+#pragma unroll
+            for (int i = 32; i > 0; i >>= 1) kth = max(kth, uint64_t(__shfl_xor((unsigned long long)(kth), i)));
+            if ((threadIdx.x & 63) == 0) least[threadIdx.x >> 6] = kth;
+        }
+        sums = group_sums(sums, heat.factor2, reduce);
+        if (a.top != 0) {
+            kth = max(max(least[0], least[1]), max(least[2], least[3]));
+            const uint32_t keys = parts * a.top;
+            for (uint32_t first = 0; first < keys; first += kLogThreads) {
+                const uint64_t key = first + threadIdx.x < keys ? mine[first + threadIdx.x] : 0ull;
+                if (key != 0 && key >= kth) g.keys[atomicAdd(&g.count, 1u)] = key;
+                __syncthreads();
+                const uint32_t count = g.count;
+                __syncthreads();
+                if (count > kGather - kLogThreads) kth = cut(g, a.top);
+            }
+        }
+        finish(a, row, scores, mask, heat, sums, g);
+        __syncthreads();
+    }
+}
+// Rows in parts where there are too few of them for the card: parts of a multiple of what a workgroup loads at once.
+static uint32_t log_parts(size_t rows, size_t n, uint32_t &part_size) {
+    constexpr size_t kOnce = 8192, kMost = 1024;      // scores; workgroups: four to a compute unit
+    const size_t at_once = (n + kOnce - 1) / kOnce, wanted = rows >= kMost ? 1 : kMost / rows;
+    const size_t each = (at_once + std::min(wanted, at_once) - 1) / std::min(wanted, at_once);
+    part_size = uint32_t(std::min(each * kOnce, n));
+    return uint32_t((n + part_size - 1) / part_size);
+}
+size_t log_probs_workspace(size_t rows, size_t n, size_t top) {
+    if (rows == 0 || n == 0) return 0;
+    uint32_t part_size;
+    const size_t parts = log_parts(rows, n, part_size);
+    return parts == 1 ? 0 : rows * parts * (sizeof(LogPart) + top * sizeof(uint64_t));
+}
+template <typename T, bool MASK>
+static hipError_t log_probs(const LogProbArgs &a, hipStream_t s) {
+    uint32_t part_size;
+    const uint32_t parts = log_parts(a.rows, a.n, part_size);
+    const uint64_t units = uint64_t(a.rows) * parts;
+    const hipError_t e = launch(k_log_probs<T, MASK>, uint32_t(units < kMostGroups ? units : kMostGroups), kLogThreads, 0, s, a, parts, part_size);
+    return e != hipSuccess || parts == 1 ? e : launch(k_log_probs_join<T>, uint32_t(a.rows < kMostGroups ? a.rows : kMostGroups), kLogThreads, 0, s, a, parts);
+}
+template <typename T>
+static hipError_t log_probs_as(const LogProbArgs &a, hipStream_t s) {
+    return a.mask == nullptr ? log_probs<T, false>(a, s) : log_probs<T, true>(a, s);
+}
+hipError_t launch_log_probs(const LogProbArgs &a, int score_type, hipStream_t s) {
+    if (score_type == kF32) return log_probs_as<float>(a, s);
+    return score_type == kF16 ? log_probs_as<f16>(a, s) : log_probs_as<bf16>(a, s);
+}
+
+// The gradient of a score that counts: (picked - p (G + g (log p + H))) / T, picked the sum of the gradients of the given slots that are this one.  With l = log2 p that is
+// (picked + p (A + B l)) / T, A = -(G + g H) and B = -g ln 2.  Bound by memory, a reading and a writing.  What is picked is added by the thread that wrote the
+// slot's own gradient, behind that.
+template <typename T, bool MASK>
+__global__ __launch_bounds__(kLogThreads) void k_log_probs_grad(LogProbGradArgs a, uint32_t parts, uint32_t part_size) {
+    constexpr int kEach = Scores<T>::kEach;
+    constexpr uint32_t kStep = kLogThreads * kEach;
+    typedef T Run __attribute__((ext_vector_type(kEach), aligned(sizeof(T))));
+    for (uint64_t unit = blockIdx.x; unit < uint64_t(a.rows) * parts; unit += gridDim.x) {
+        const uint32_t row = uint32_t(unit / parts), lo = uint32_t(unit % parts) * part_size, hi = lo + min(part_size, a.n - lo);
+        const T *const scores = static_cast<const T *>(a.scores) + size_t(row) * a.stride;
+        const uint64_t *const mask = MASK ? a.mask + size_t(row) * a.mask_stride : nullptr;
         T *const grad = static_cast<T *>(a.grad) + size_t(row) * a.grad_stride;
         const Heat heat(a.temperature, row);
-        const float m = a.stats[size_t(row) * 4], log2_sum = a.stats[size_t(row) * 4 + 1], entropy = a.stats[size_t(row) * 4 + 2];
+        const float4 stats = *reinterpret_cast<const float4 *>(a.stats + size_t(row) * 4);      // largest, log2 of the sum, entropy
         const float *const g = a.grad_log_probs + size_t(row) * a.given;
         const int64_t *const slots = a.slots + size_t(row) * a.slot_stride;
-        float all = 0.0f;
-        for (uint32_t k = 0; k < a.given; ++k)
-            if (slots[k] >= 0 && slots[k] < int64_t(a.n) && counts(mask, uint32_t(slots[k]), float(scores[slots[k]]))) all += g[k];
+        float all = 0.0f;                // (a lane to a given slot, every wave the same)
+        for (uint32_t k = threadIdx.x & 63u; k < a.given; k += 64u) {
+            const int64_t slot = slots[k];
+            if (slot >= 0 && slot < int64_t(a.n) && counts(mask, uint32_t(slot), float(scores[slot]))) all += g[k];
+        }
+#pragma unroll
+        for (int k = 32; k > 0; k >>= 1) all += __shfl_xor(all, k);
         const float g_entropy = a.grad_entropy == nullptr ? 0.0f : a.grad_entropy[row];
-        for (uint32_t i = threadIdx.x; i < a.n; i += kLogThreads) {
-            const float s = float(scores[i]);
-            float d = 0.0f;
-            if (counts(mask, i, s) && !heat.limit) {
-                const float l = fmaf(s - m, heat.factor2, -log2_sum), p = __builtin_amdgcn_exp2f(l);
-                for (uint32_t k = 0; k < a.given; ++k)
-                    if (slots[k] == int64_t(i)) d += g[k];
-                d = (d - p * (all + g_entropy * fmaf(kLn2, fmaxf(l, -200.0f), entropy))) / heat.t;
+        const float factor_a = -(all + g_entropy * stats.z), factor_b = -g_entropy * kLn2, inverse = heat.limit ? 0.0f : fminf(1.0f / heat.t, FLT_MAX);
+        auto at = [&](float s) {
+            const float l = fmaf(s - stats.x, heat.factor2, -stats.y), d = __builtin_amdgcn_exp2f(l) * fmaf(factor_b, fmaxf(l, -200.0f), factor_a);
+            return s == -kInf ? 0.0f : d;
+        };
+        auto whole = [&](const Scores<T> &l, uint32_t i) {
+            Run r;
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) r[j] = T(at(l.template at<MASK>(j)) * inverse);
+            __builtin_nontemporal_store(r, reinterpret_cast<Run *>(grad + i));
+        };
+        uint32_t i = lo + threadIdx.x * kEach;
+        for (; i + (kLogLoads - 1) * kStep + kEach <= hi; i += kLogLoads * kStep) {
+            Scores<T> l[kLogLoads];
+#pragma unroll
+            for (int j = 0; j < kLogLoads; ++j) l[j].load(scores, mask, i + j * kStep);
+#pragma unroll
+            for (int j = 0; j < kLogLoads; ++j) whole(l[j], i + j * kStep);
+        }
+        for (; i < hi; i += kStep) {
+            Scores<T> l;
+            if (i + kEach <= hi) {
+                l.load(scores, mask, i);
+                whole(l, i);
+            } else {
+                l.load_end(scores, mask, i, hi);
+#pragma unroll
+                for (int j = 0; j < kEach; ++j)
+                    if (i + j < hi) grad[i + j] = T(at(l.template at<MASK>(j)) * inverse);
             }
-            grad[i] = T(d);
+        }
+        for (uint32_t k = 0; k < (heat.limit ? 0u : a.given); ++k) {
+            const int64_t slot = slots[k];
+            if (slot < int64_t(lo) || slot >= int64_t(hi) || (uint32_t(slot) - lo) / kEach % kLogThreads != threadIdx.x) continue;
+            const float s = float(scores[slot]);
+            if (!counts(mask, uint32_t(slot), s)) continue;
+            float picked = 0.0f;               // (where the same slot stands there again, the last sum is the whole one)
+            for (uint32_t l = 0; l <= k; ++l) picked += slots[l] == slot ? g[l] : 0.0f;
+            grad[slot] = T((at(s) + picked) * inverse);
         }
     }
 }
 template <typename T>
 static hipError_t log_probs_grad(const LogProbGradArgs &a, hipStream_t s) {
-    return launch(k_log_probs_grad<T>, uint32_t(a.rows < kMostGroups ? a.rows : kMostGroups), kLogThreads, 0, s, a);
+    uint32_t part_size;
+    const uint32_t parts = log_parts(a.rows, a.n, part_size);
+    const uint64_t units = uint64_t(a.rows) * parts;
+    const uint32_t grid = uint32_t(units < kMostGroups ? units : kMostGroups);
+    return a.mask == nullptr ? launch(k_log_probs_grad<T, false>, grid, kLogThreads, 0, s, a, parts, part_size) : launch(k_log_probs_grad<T, true>, grid, kLogThreads, 0, s, a, parts, part_size);
 }
 hipError_t launch_log_probs_grad(const LogProbGradArgs &a, int score_type, hipStream_t s) {
     if (score_type == kF32) return log_probs_grad<float>(a, s);
