@@ -49,6 +49,9 @@ struct Sums {
     __device__ __forceinline__ float entropy(float log_sum) const { return s == 0.0f ? 0.0f : log_sum - kLn2 * (u / s); }
 };
 
+__device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint64_t smaller(uint64_t a, uint64_t b) { return a < b ? a : b; }
+
 constexpr int kLogThreads = 256, kLogWaves = kLogThreads / 64;
 // Sums over the workgroup, in every thread; `best` has room for a float a thread and is left holding the threads' largest scores.
 struct Reduce {
@@ -134,24 +137,30 @@ __device__ __forceinline__ void in_order(Gathered &g, uint32_t k, F &&out) {
         if (i >= count) out(i, 0ull);
 }
 
+// A thread's given slot and its score: asked for before the sums are known.
+struct Given {
+    float score;
+    bool there;
+    template <typename T>
+    __device__ __forceinline__ void load(const LogProbArgs &a, uint32_t row, const T *scores, const uint64_t *mask) {
+        there = false;
+        if (threadIdx.x >= a.given) return;
+        const int64_t slot = a.slots[size_t(row) * a.slot_stride + threadIdx.x];
+        if (slot < 0 || slot >= int64_t(a.n)) return;
+        score = float(scores[slot]);
+        there = counts(mask, uint32_t(slot), score);
+    }
+};
+static_assert(kMostGiven <= uint32_t(kLogThreads), "a thread to a given slot");
 // A row's results from its sums and best keys.
-template <typename T>
-__device__ __forceinline__ void finish(const LogProbArgs &a, uint32_t row, const T *scores, const uint64_t *mask, const Heat &heat, const Sums &sums, Gathered &g) {
+__device__ __forceinline__ void finish(const LogProbArgs &a, uint32_t row, const Given &given, const Heat &heat, const Sums &sums, Gathered &g) {
     const float log_sum = logf(sums.s);
     if (threadIdx.x == 0) {
         const float entropy = sums.entropy(log_sum);
         a.out_entropy[row] = entropy;
         if (a.stats != nullptr) *reinterpret_cast<float4 *>(a.stats + size_t(row) * 4) = make_float4(sums.m, log2f(sums.s), entropy, 0.0f);
     }
-    for (uint32_t i = threadIdx.x; i < a.given; i += kLogThreads) {
-        const int64_t slot = a.slots[size_t(row) * a.slot_stride + i];
-        float lp = -kInf;
-        if (slot >= 0 && slot < int64_t(a.n)) {
-            const float v = float(scores[slot]);
-            if (counts(mask, uint32_t(slot), v)) lp = heat.log_p(v - sums.m, log_sum);
-        }
-        a.out_log_probs[size_t(row) * a.given + i] = lp;
-    }
+    if (threadIdx.x < a.given) a.out_log_probs[size_t(row) * a.given + threadIdx.x] = given.there ? heat.log_p(given.score - sums.m, log_sum) : -kInf;
     if (a.top != 0)
         in_order(g, a.top, [&](uint32_t place, uint64_t key) {
             float v = 0.0f;
@@ -338,13 +347,15 @@ __global__ __launch_bounds__(kLogThreads) void k_log_probs(LogProbArgs a, uint32
         const T *const scores = static_cast<const T *>(a.scores) + size_t(row) * a.stride;
         const uint64_t *const mask = MASK ? a.mask + size_t(row) * a.mask_stride : nullptr;
         const Heat heat(a.temperature, row);
+        Given given;
+        if (parts == 1) given.load(a, row, scores, mask);
         Sums sums;
         float segments[kLogSegments];
         scan_part<T, MASK>(scores, mask, heat, at, sums, segments);
         sums = group_sums(sums, heat.factor2, reduce);
         if (a.top != 0) gather_part<T, MASK>(a, scores, mask, at, segments, g, reduce.best, who, &who_count);
         if (parts == 1) {
-            finish(a, row, scores, mask, heat, sums, g);
+            finish(a, row, given, heat, sums, g);
         } else {
             if (threadIdx.x == 0) out[unit] = LogPart{sums.m, sums.s, sums.u, 0.0f};
             if (a.top != 0) in_order(g, a.top, [&](uint32_t place, uint64_t key) { out_keys[unit * a.top + place] = key; });
@@ -352,57 +363,96 @@ __global__ __launch_bounds__(kLogThreads) void k_log_probs(LogProbArgs a, uint32
         __syncthreads();
     }
 }
-// The parts of a row, joined.
+// The parts of a row, joined.  Keys that cannot be among the best are told from a few of each part: its last one is one that k keys reach, and so is the lowest of all parts'
+// j-th where j keys of each are k, and the k-th of all parts' first.  Only parts whose first passes are read.
+constexpr uint32_t kMostParts = 1024;
 template <typename T>
 __global__ __launch_bounds__(kLogThreads) void k_log_probs_join(LogProbArgs a, uint32_t parts) {
     __shared__ Reduce reduce;
     __shared__ Gathered g;
-    __shared__ uint64_t least[kLogWaves];
-    const LogPart *const in = reinterpret_cast<const LogPart *>(a.ws);
-    const uint64_t *const in_keys = reinterpret_cast<const uint64_t *>(a.ws + size_t(a.rows) * parts * sizeof(LogPart));
+    __shared__ uint64_t least[2][kLogWaves];
+    __shared__ uint16_t who[kMostParts];
+    __shared__ uint32_t who_count;
+    constexpr int kEach = kMostParts / kLogThreads;
+    const uint32_t top = a.top, share = top == 0 ? 0 : (top + parts - 1) / parts;
     for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T *const scores = static_cast<const T *>(a.scores) + size_t(row) * a.stride;
-        const uint64_t *const mask = a.mask == nullptr ? nullptr : a.mask + size_t(row) * a.mask_stride, *const mine = reinterpret_cast<const uint64_t *>(in_keys) + size_t(row) * parts * a.top;
+        const uint64_t *const mask = a.mask == nullptr ? nullptr : a.mask + size_t(row) * a.mask_stride;
+        const LogPart *const in = reinterpret_cast<const LogPart *>(a.ws) + size_t(row) * parts;
+        const uint64_t *const in_keys = reinterpret_cast<const uint64_t *>(a.ws + size_t(a.rows) * parts * sizeof(LogPart)) + size_t(row) * parts * top;
         const Heat heat(a.temperature, row);
-        if (threadIdx.x == 0) g.count = 0;
+        Given given;
+        given.load(a, row, scores, mask);
+        LogPart p[kEach];
+        uint64_t first[kEach], last = 0, low = ~0ull;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const uint32_t part = uint32_t(i * kLogThreads) + threadIdx.x;
+            first[i] = 0;
+            p[i] = LogPart{kNone, 0.0f, 0.0f, 0.0f};
+            if (part >= parts) continue;
+            p[i] = in[part];
+            if (top == 0) continue;
+            const uint64_t *const keys = in_keys + size_t(part) * top;
+            first[i] = keys[0];
+            last = larger(last, keys[top - 1]);
+            low = smaller(low, keys[share - 1]);
+        }
         Sums sums;
-        uint64_t kth = 0;          // a part's last key is one that a.top keys reach
-        for (uint32_t i = threadIdx.x; i < parts; i += kLogThreads) {
-            const LogPart p = in[size_t(row) * parts + i];
-            if (a.top != 0) kth = max(kth, mine[size_t(i) * a.top + a.top - 1]);
+        float best = kNone;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) sums.m = fmaxf(sums.m, p[i].m);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
             Sums more;
-            more.m = p.m; more.s = p.s; more.u = p.u;
-            const float m = fmaxf(sums.m, p.m);
-            sums.rise(m, heat.factor2);
-            more.rise(m, heat.factor2);
+            more.m = p[i].m; more.s = p[i].s; more.u = p[i].u;
+            more.rise(sums.m, heat.factor2);
             sums.s += more.s;
             sums.u += more.u;
+            best = fmaxf(best, first[i] == 0 ? kNone : order_unkey(int(uint32_t(first[i] >> 32) ^ 0x80000000u)));
         }
-        if (a.top != 0) {
+        if (top != 0) {
 #pragma unroll
-            for (int i = 32; i > 0; i >>= 1) kth = max(kth, uint64_t(__shfl_xor((unsigned long long)(kth), i)));
-            if ((threadIdx.x & 63) == 0) least[threadIdx.x >> 6] = kth;
+            for (int i = 32; i > 0; i >>= 1) {
+                last = larger(last, uint64_t(__shfl_xor((unsigned long long)(last), i)));
+                low = smaller(low, uint64_t(__shfl_xor((unsigned long long)(low), i)));
+            }
+            if ((threadIdx.x & 63) == 0) {
+                least[0][threadIdx.x >> 6] = last;
+                least[1][threadIdx.x >> 6] = low;
+            }
+            if (threadIdx.x == 0) g.count = who_count = 0;
         }
         sums = group_sums(sums, heat.factor2, reduce);
-        if (a.top != 0) {
-            kth = max(max(least[0], least[1]), max(least[2], least[3]));
-            const uint32_t keys = parts * a.top;
-            for (uint32_t first = 0; first < keys; first += kLogThreads) {
-                const uint64_t key = first + threadIdx.x < keys ? mine[first + threadIdx.x] : 0ull;
-                if (key != 0 && key >= kth) g.keys[atomicAdd(&g.count, 1u)] = key;
+        if (top != 0) {
+            uint64_t from = larger(larger(larger(least[0][0], least[0][1]), larger(least[0][2], least[0][3])), smaller(smaller(least[1][0], least[1][1]), smaller(least[1][2], least[1][3])));
+            __syncthreads();
+            reduce.best[threadIdx.x] = best;
+            __syncthreads();
+            const float reach = reached(reduce.best, top);
+            from = larger(from, reach > kNone ? sort_key(reach, 0x7fffffffu) & ~1ull : 0ull);      // (the lowest key of that score)
+#pragma unroll
+            for (int i = 0; i < kEach; ++i)
+                if (first[i] != 0 && first[i] >= from) who[atomicAdd(&who_count, 1u)] = uint16_t(i * kLogThreads + threadIdx.x);
+            __syncthreads();
+            const uint32_t keys = who_count * top;
+            for (uint32_t at = 0; at < keys; at += kLogThreads) {
+                const uint32_t item = at + threadIdx.x;
+                const uint64_t key = item < keys ? in_keys[size_t(who[item / top]) * top + item % top] : 0ull;
+                if (key != 0 && key >= from) g.keys[atomicAdd(&g.count, 1u)] = key;
                 __syncthreads();
                 const uint32_t count = g.count;
                 __syncthreads();
-                if (count > kGather - kLogThreads) kth = cut(g, a.top);
+                if (count > kGather - kLogThreads) from = cut(g, top);
             }
         }
-        finish(a, row, scores, mask, heat, sums, g);
+        finish(a, row, given, heat, sums, g);
         __syncthreads();
     }
 }
 // Rows in parts where there are too few of them for the card: parts of a multiple of what a workgroup loads at once.
 static uint32_t log_parts(size_t rows, size_t n, uint32_t &part_size) {
-    constexpr size_t kOnce = 8192, kMost = 1024;      // scores; workgroups: four to a compute unit
+    constexpr size_t kOnce = 8192, kMost = kMostParts;      // scores; workgroups: four to a compute unit
     const size_t at_once = (n + kOnce - 1) / kOnce, wanted = rows >= kMost ? 1 : kMost / rows;
     const size_t each = (at_once + std::min(wanted, at_once) - 1) / std::min(wanted, at_once);
     part_size = uint32_t(std::min(each * kOnce, n));
