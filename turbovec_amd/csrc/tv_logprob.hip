@@ -4,6 +4,7 @@
 // log S - U / S, two terms that are not below 0.  Exponentials are of base 2, with log2(e) / T as the factor.
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 #include "tv_device.h"
 #include "tv_ops.h"
@@ -187,8 +188,21 @@ struct Scores {
         for (int j = 0; j < kEach; ++j) v[j] = i + j < n ? scores[i + j] : T(-kInf);
     }
     template <bool MASK>
-    __device__ __forceinline__ float at(int j) const { return !MASK || ((bits >> j) & 1u) ? float(v[j]) : -kInf; }
+    __device__ __forceinline__ float at(int j) const {
+        // (bfloat16 by its bits: the compiler takes largest ones in the narrow type, five instructions each)
+        float x;
+        if constexpr (sizeof(T) == 2 && !std::is_same_v<T, f16>) x = __uint_as_float(uint32_t(__builtin_bit_cast(uint16_t, v[j])) << 16);
+        else x = float(v[j]);
+        return !MASK || ((bits >> j) & 1u) ? x : -kInf;
+    }
 };
+
+// The largest of three, none of a NaN.  (Written as two maxima the compiler makes each operand canonical first.)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 
 // A part of a row to a workgroup, all of it where there are rows enough.  One pass takes the sums, a thread each its own from its own largest score, which it raises once for
 // four loads.  The alternatives come from the threads' largest scores: the k-th of those is one that k scores reach, and so is what its first bits say; only where a thread
@@ -212,18 +226,15 @@ __device__ __forceinline__ void scan_part(const T *scores, const uint64_t *mask,
     constexpr uint32_t kStep = kLogThreads * kEach;
     float segment = kNone;
     auto take = [&](const Scores<T> *l, auto count) {
-        constexpr int kCount = decltype(count)::value;
-        float m = l[0].template at<MASK>(0);
+        constexpr int kCount = decltype(count)::value * kEach;
+        float x[kCount];
 #pragma unroll
-        for (int i = 0; i < kCount; ++i)
+        for (int i = 0; i < kCount; ++i) x[i] = l[i / kEach].template at<MASK>(i % kEach);
 #pragma unroll
-            for (int j = 0; j < kEach; ++j) m = fmaxf(m, l[i].template at<MASK>(j));
-        segment = fmaxf(segment, m);
-        sums.rise(fmaxf(sums.m, m), heat.factor2);
+        for (int i = 0; i < kCount; i += 2) segment = max3(segment, x[i], x[i + 1]);
+        sums.rise(fmaxf(sums.m, segment), heat.factor2);
 #pragma unroll
-        for (int i = 0; i < kCount; ++i)
-#pragma unroll
-            for (int j = 0; j < kEach; ++j) sums.add(l[i].template at<MASK>(j), heat.factor2);
+        for (int i = 0; i < kCount; ++i) sums.add(x[i], heat.factor2);
     };
 #pragma unroll
     for (int part = 0; part < kLogSegments; ++part) {
