@@ -3,7 +3,7 @@
 
 namespace tv {
 
-// h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight; then the scales and codes of y's blocks.  A thread holds runs of eight
+// h = x + residual, y = h / sqrt(mean(h^2) + eps) * weight; then the scales and codes of y's blocks.  A lane holds runs of eight
 // neighbouring coordinates in registers from the first reading to the codes; sixteen lanes hold a block of 8-bit rows, four one of 4-bit rows.
 __device__ __forceinline__ float row16_max(float v) {
     v = max_moved<0xb1>(v);
@@ -11,9 +11,10 @@ __device__ __forceinline__ float row16_max(float v) {
     v = max_moved<0x141>(v);
     return max_moved<0x140>(v);
 }
-__device__ __forceinline__ float wave_sum(float v) {
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
-    for (int i = 32; i > 0; i >>= 1) v += __shfl_xor(v, i);
+    for (int i = LANES / 2; i > 0; i >>= 1) v += __shfl_xor(v, i);
     return v;
 }
 template <typename T>
@@ -38,41 +39,60 @@ __device__ __forceinline__ void load_weight(float (&w)[8], const void *p, int ty
 
 enum { kToFp8E8 = 0, kToFp8F32 = 1, kToFp4 = 2 };
 
-// A workgroup to a row, a thread to RUNS runs.
-constexpr int kNormThreads = 256;
-template <typename T, int TO, int RUNS>
-__global__ __launch_bounds__(kNormThreads) void k_rms_norm(NormArgs a) {
-    __shared__ float part[kNormThreads / 64];
-    for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+// LANES lanes to a row, each with RUNS runs: sixteen to sixty-four, or all of a workgroup, whose sums then go through LDS.  Bound by memory: 16384 rows of 4096 bfloat16 with a
+// residual take 88 us, 5.4 TB/s, a third of it written (a copy reaches 4.6 to 4.9).  As many lanes as a row fills, one run or two each: with 256 threads to every
+// row 100000 rows of 512 take 155 us where these take 66, 100000 of 130 floats 117 and 21; with eight runs to a lane 4096 rows of 16384 take 156 and 110, 16384 of 4096 153 and 88.
+template <typename T, int TO, int LANES, int RUNS, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_rms_norm(NormArgs a) {
+    constexpr uint32_t kTogether = THREADS / LANES;
+    constexpr bool kAll = LANES > 64;
+    __shared__ float part[kAll ? THREADS / 64 : 1];
+    const uint32_t lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
+    for (uint64_t first = uint64_t(blockIdx.x) * kTogether; first < a.rows; first += uint64_t(gridDim.x) * kTogether) {
+        const bool there = first + sub < a.rows;
+        const uint32_t row = there ? uint32_t(first) + sub : a.rows - 1;
         const T *const x = static_cast<const T *>(a.x) + size_t(row) * a.x_stride, *const r = static_cast<const T *>(a.residual) + size_t(row) * a.residual_stride;
         T *const sum = static_cast<T *>(a.sum) + size_t(row) * a.sum_stride;
         float h[RUNS][8], squares = 0.0f;
 #pragma unroll
         for (int i = 0; i < RUNS; ++i) {
-            const uint32_t at = (uint32_t(i) * kNormThreads + threadIdx.x) * 8u;
-            const int left = int(a.dim) - int(at);
-            load8<T>(h[i], x + at, left);
-            if (a.residual != nullptr) {
-                float more[8];
-                load8<T>(more, r + at, left);
+            const uint32_t at = (uint32_t(i) * LANES + lane) * 8u;
+            load8<T>(h[i], x + at, there ? int(a.dim) - int(at) : 0);
+        }
+        if (a.residual != nullptr) {
+            float more[RUNS][8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) h[i][j] += more[j];
+            for (int i = 0; i < RUNS; ++i) {
+                const uint32_t at = (uint32_t(i) * LANES + lane) * 8u;
+                load8<T>(more[i], r + at, there ? int(a.dim) - int(at) : 0);
             }
-            if (a.sum != nullptr) store8<T>(sum + at, h[i], left);
+#pragma unroll
+            for (int i = 0; i < RUNS; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) h[i][j] += more[i][j];
+        }
+#pragma unroll
+        for (int i = 0; i < RUNS; ++i) {
+            const uint32_t at = (uint32_t(i) * LANES + lane) * 8u;
+            if (a.sum != nullptr) store8<T>(sum + at, h[i], there ? int(a.dim) - int(at) : 0);
 #pragma unroll
             for (int j = 0; j < 8; ++j) squares = fmaf(h[i][j], h[i][j], squares);
         }
-        squares = wave_sum(squares);
-        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = squares;
-        __syncthreads();
-        squares = part[0] + part[1] + part[2] + part[3];
-        __syncthreads();
+        squares = lanes_sum<kAll ? 64 : LANES>(squares);
+        if constexpr (kAll) {
+            if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = squares;
+            __syncthreads();
+            squares = part[0];
+#pragma unroll
+            for (int i = 1; i < THREADS / 64; ++i) squares += part[i];
+            __syncthreads();
+        }
         const float mean = squares / float(a.dim) + a.eps;
         const float inverse = mean < __int_as_float(0x7f800000) ? 1.0f / sqrtf(mean) : __int_as_float(0x7fc00000);
 #pragma unroll
         for (int i = 0; i < RUNS; ++i) {
-            const uint32_t at = (uint32_t(i) * kNormThreads + threadIdx.x) * 8u;
-            const int left = int(a.dim) - int(at);
+            const uint32_t at = (uint32_t(i) * LANES + lane) * 8u;
+            const int left = there ? int(a.dim) - int(at) : 0;
             float y[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[j] = j < left ? h[i][j] * inverse : 0.0f;
@@ -98,19 +118,33 @@ __global__ __launch_bounds__(kNormThreads) void k_rms_norm(NormArgs a) {
                 const float lo[4] = {y[0], y[1], y[2], y[3]}, hi[4] = {y[4], y[5], y[6], y[7]};
                 uint8_t *const to = a.codes + size_t(row) * a.code_stride + at;
                 const uint32_t c0 = codes_of<TO == kToFp8E8>(lo, s), c1 = codes_of<TO == kToFp8E8>(hi, s);
-                store4(to, c0, left);
-                store4(to + 4, c1, left - 4);
+                if (left >= 8) {
+                    typedef uint32_t Two __attribute__((ext_vector_type(2), aligned(1)));
+                    *reinterpret_cast<Two *>(to) = Two{c0, c1};
+                } else {
+                    store4(to, c0, left);
+                    store4(to + 4, c1, left - 4);
+                }
                 if ((threadIdx.x & 15) == 0) store_scale<TO == kToFp8E8>(a.scales, size_t(row) * a.scale_stride + at / kScaleBlock, stored);
             }
         }
     }
 }
+template <typename T, int TO, int LANES, int RUNS, int THREADS>
+static hipError_t norm_form(const NormArgs &a, hipStream_t s) {
+    const uint64_t groups = (uint64_t(a.rows) + THREADS / LANES - 1) / (THREADS / LANES);
+    return launch(k_rms_norm<T, TO, LANES, RUNS, THREADS>, uint32_t(groups < kMostGroups ? groups : kMostGroups), THREADS, 0, s, a);
+}
+// (By a row's length alone: the order of its sums is the same whatever rows stand beside it.)
 template <typename T, int TO>
 static hipError_t norm(const NormArgs &a, hipStream_t s) {
-    const uint32_t grid = uint32_t(a.rows < kMostGroups ? a.rows : kMostGroups), runs = (a.dim + 8 * kNormThreads - 1) / (8 * kNormThreads);
-    if (runs <= 1) return launch(k_rms_norm<T, TO, 1>, grid, kNormThreads, 0, s, a);
-    if (runs <= 2) return launch(k_rms_norm<T, TO, 2>, grid, kNormThreads, 0, s, a);
-    return runs <= 4 ? launch(k_rms_norm<T, TO, 4>, grid, kNormThreads, 0, s, a) : launch(k_rms_norm<T, TO, 8>, grid, kNormThreads, 0, s, a);
+    if (a.dim <= 128) return norm_form<T, TO, 16, 1, 256>(a, s);
+    if (a.dim <= 256) return norm_form<T, TO, 32, 1, 256>(a, s);
+    if (a.dim <= 512) return norm_form<T, TO, 64, 1, 256>(a, s);
+    if (a.dim <= 1024) return norm_form<T, TO, 128, 1, 128>(a, s);
+    if (a.dim <= 2048) return norm_form<T, TO, 256, 1, 256>(a, s);
+    if (a.dim <= 4096) return norm_form<T, TO, 256, 2, 256>(a, s);
+    return a.dim <= 8192 ? norm_form<T, TO, 512, 2, 512>(a, s) : norm_form<T, TO, 1024, 2, 1024>(a, s);
 }
 template <typename T>
 static hipError_t norm_as(const NormArgs &a, int row_kind, int scale_type, hipStream_t s) {
