@@ -82,15 +82,19 @@ class LogProbs(NamedTuple):
 
 def _forward(scores, slots, temperature, mask, top, stats):
     rows, n = scores.shape
-    device = scores.device
-    given = slots.shape[1] if slots.dim() == 2 else 1
-    found = LogProbs(torch.empty(slots.shape, dtype=torch.float32, device=device), torch.empty(rows, dtype=torch.float32, device=device),
-                     torch.empty((rows, top), dtype=torch.int64, device=device), torch.empty((rows, top), dtype=torch.float32, device=device))
-    ws = _workspace(T.lib().tv_log_probs_workspace(rows, n, top), device)
-    _call(T.lib().tv_log_probs_dev, device, scores.data_ptr(), _VALUES[scores.dtype], scores.stride(0), rows, n, *_mask(mask, rows, n, device),
-          None if temperature is None else temperature.data_ptr(), slots.data_ptr(), slots.stride(0), given, top, found.log_probs.data_ptr(), found.entropy.data_ptr(),
-          found.top_slots.data_ptr(), found.top_log_probs.data_ptr(), None if stats is None else stats.data_ptr(), *ws[1:])
-    return found
+    device, new = scores.device, torch.empty_strided
+    shape = slots.shape
+    given = shape[1] if len(shape) == 2 else 1
+    log_p = new(shape, (given, 1)[-len(shape):], dtype=torch.float32, device=device)
+    entropy = new((rows,), (1,), dtype=torch.float32, device=device)
+    top_slots = new((rows, top), (top, 1), dtype=torch.int64, device=device)
+    top_log_p = new((rows, top), (top, 1), dtype=torch.float32, device=device)
+    L = T.lib()
+    ws, ws_ptr, ws_bytes = _workspace(L.tv_log_probs_workspace(rows, n, top), device)
+    _call(L.tv_log_probs_dev, device, scores.data_ptr(), _VALUES[scores.dtype], scores.stride(0), rows, n, *_mask(mask, rows, n, device),
+          None if temperature is None else temperature.data_ptr(), slots.data_ptr(), slots.stride(0), given, top, log_p.data_ptr(), entropy.data_ptr(),
+          top_slots.data_ptr(), top_log_p.data_ptr(), None if stats is None else stats.data_ptr(), ws_ptr, ws_bytes)
+    return LogProbs(log_p, entropy, top_slots, top_log_p)
 
 
 class _WithGradient(torch.autograd.Function):
