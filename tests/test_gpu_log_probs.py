@@ -450,3 +450,68 @@ def test_a_draw_and_its_log_probability_agree(log_probs):
     found = check(log_probs, scores, slots, temperature=t, allowed=allowed, top=1)
     assert int(slots[7]) == -1 and float(found.log_probs[7]) == -INF
     assert torch.allclose(found.log_probs.exp(), p, rtol=1e-4, atol=0)
+
+
+# ---- rows with a workgroup each, a large one, two large ones to a compute unit, and rows in parts ---------------
+
+FORMS = [(1, 8192), (1, 8193), (3, 20_001), (160, 16_400), (256, 9001), (257, 9001), (512, 8200), (513, 8200), (1, 100_600), (1, 100_601), (1, 8_388_608), (3, 2_800_007), (1, 9_000_001)]
+
+
+@pytest.mark.parametrize("rows,n", FORMS)
+@pytest.mark.parametrize("dtype,top", [(torch.float32, 24), (torch.bfloat16, 128), (torch.float16, 25), (torch.float32, 0)])
+def test_forms(log_probs, rows, n, dtype, top):
+    t = 0.5 + torch.rand(rows, generator=gen(40), device="cuda")
+    scores, slots = scores_of(rows, n, dtype, 41), slots_of(rows, n, 3)
+    scores[:, n - 1] = 40.0
+    check(log_probs, scores, slots, temperature=t, top=top)
+    allowed = torch.rand(rows, n, generator=gen(42), device="cuda") < 0.2
+    allowed[rows // 2] = False
+    check(log_probs, scores, slots, temperature=t, allowed=allowed, top=top)
+
+
+@pytest.mark.parametrize("rows,n", [(1, 20_000), (200, 9000), (300, 9000), (1, 8_388_608), (2, 3_000_001)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_forms_of_crowded_scores(log_probs, rows, n, dtype):
+    slots = slots_of(rows, n, 1)
+    ramp = torch.arange(n, device="cuda").float()
+    for scores in (torch.zeros(n), torch.randint(0, 5, (n,), generator=gen(43), device="cuda"), ramp % 2048 == 5, ramp % 64 < 8, ramp / n * 20, -ramp / n * 20, ramp > n - 200, (ramp > n // 3) & (ramp < n // 3 + 9000)):
+        for top in (1, 128):
+            check(log_probs, scores.to("cuda").to(dtype).expand(rows, n).contiguous(), slots, top=top)
+
+
+@pytest.mark.parametrize("rows,n", [(4, 30_000), (200, 9000), (300, 9000), (4, 300_000)])
+def test_forms_of_rows_that_show_or_have_nothing(log_probs, rows, n):
+    scores = scores_of(rows, n, torch.float32, 44)
+    scores[0, n // 2], scores[1, 1], scores[2] = float("nan"), INF, -INF
+    slots = slots_of(rows, n, 2)
+    found = log_probs(scores, slots, top=4)
+    bad = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    bad[:2] = True
+    assert torch.equal(torch.isnan(found.entropy), bad) and torch.equal(torch.isnan(found.log_probs).all(1), bad)
+    assert bool((found.log_probs[2] == -INF).all()) and float(found.entropy[2]) == 0 and bool((found.top_slots[2] == -1).all())
+    fine = log_probs(scores[3:], slots[3:], top=4)
+    check(log_probs, scores[3:], slots[3:], top=4)
+    assert all(torch.equal(x[3:], y) for x, y in zip(found, fine))          # (rows of the same form do not depend on what stands beside them)
+    cold = log_probs(scores[3:], slots[3:], temperature=0.0, top=2)
+    assert torch.equal(cold.top_slots, fine.top_slots[:, :2]) and bool((cold.log_probs[slots[3:] == cold.top_slots[:, :1]] == 0).all()) and bool((cold.entropy == 0).all())
+
+
+def test_two_graphs_at_once(log_probs):
+    """Rows in parts have a workspace: two captured calls, replayed on two streams at once, have one each."""
+    scores, slots = [scores_of(2, 400_000, torch.float32, 45 + i) for i in range(2)], slots_of(2, 400_000, 2)
+    want, graphs, got = [log_probs(s, slots, top=64) for s in scores], [], []
+    for s in scores:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got.append(log_probs(s, slots, top=64))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for stream in streams:
+        stream.wait_stream(torch.cuda.current_stream())
+    for _ in range(50):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(g, w))

@@ -53,17 +53,23 @@ struct Sums {
 __device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
 __device__ __forceinline__ uint64_t smaller(uint64_t a, uint64_t b) { return a < b ? a : b; }
 
-constexpr int kLogThreads = 256, kLogWaves = kLogThreads / 64;
+// Workgroups of kLogThreads, or of kWideThreads where a row has one to itself and would need several of the others.
+constexpr int kLogThreads = 256, kLogWaves = kLogThreads / 64, kWideThreads = 1024;
 // Sums over the workgroup, in every thread; `best` has room for a float a thread and is left holding the threads' largest scores.
+template <int THREADS>
 struct Reduce {
-    __attribute__((aligned(16))) float best[kLogThreads];
-    float part[2 * kLogWaves];
+    __attribute__((aligned(16))) float best[THREADS];
+    float part[2][THREADS / 64];
 };
-__device__ __forceinline__ Sums group_sums(Sums v, float factor2, Reduce &r) {
+template <int THREADS>
+__device__ __forceinline__ Sums group_sums(Sums v, float factor2, Reduce<THREADS> &r) {
+    constexpr int kWaves = THREADS / 64;
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     r.best[threadIdx.x] = v.m;
     __syncthreads();
-    float m = fmaxf(fmaxf(r.best[lane], r.best[64 + lane]), fmaxf(r.best[128 + lane], r.best[192 + lane]));
+    float m = r.best[lane];
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) m = fmaxf(m, r.best[i * 64 + lane]);
 #pragma unroll
     for (int i = 32; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
     v.rise(m, factor2);
@@ -73,29 +79,38 @@ __device__ __forceinline__ Sums group_sums(Sums v, float factor2, Reduce &r) {
         v.u += __shfl_xor(v.u, i);
     }
     if (lane == 0) {
-        r.part[wave] = v.s;
-        r.part[kLogWaves + wave] = v.u;
+        r.part[0][wave] = v.s;
+        r.part[1][wave] = v.u;
     }
     __syncthreads();
-    v.s = (r.part[0] + r.part[1]) + (r.part[2] + r.part[3]);
-    v.u = (r.part[4] + r.part[5]) + (r.part[6] + r.part[7]);
+    v.s = v.u = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        v.s += r.part[0][i];
+        v.u += r.part[1][i];
+    }
     return v;
 }
 
-// The best keys of those that a workgroup has met: gathered in LDS, cut to the k best whenever the next 8 a thread might not fit.
-constexpr uint32_t kKeep = 256, kGather = kKeep + 8 * kLogThreads;
+// The best keys of those that a workgroup has met: gathered in LDS, cut to the k best whenever the next 8 of each thread (of kMostMeet at most) might not fit.
+constexpr uint32_t kKeep = 256, kInOrder = 512;
+constexpr int kMostMeet = 512;
+template <int THREADS>
 struct Gathered {
+    static constexpr uint32_t kMeet = THREADS < kMostMeet ? THREADS : kMostMeet, kGather = kKeep + 8 * kMeet;
     uint64_t keys[kGather];
-    uint32_t count, part[2][kLogWaves];
+    uint32_t count, part[2][THREADS / 64];
 };
 // Of the `count` keys, kKeep < count <= kGather: the k-th largest, bit by bit from the highest on; it and those above stay.
-__device__ __forceinline__ uint64_t cut(Gathered &g, uint32_t k) {
-    constexpr int kEach = (kGather + kLogThreads - 1) / kLogThreads;
+template <int THREADS>
+__device__ __forceinline__ uint64_t cut(Gathered<THREADS> &g, uint32_t k) {
+    constexpr int kEach = int(Gathered<THREADS>::kGather + THREADS - 1) / THREADS;
     const uint32_t count = g.count, wave = threadIdx.x >> 6;
     uint64_t mine[kEach];
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) mine[i] = uint32_t(i * kLogThreads) + threadIdx.x < count ? g.keys[i * kLogThreads + threadIdx.x] : 0ull;
+    for (int i = 0; i < kEach; ++i) mine[i] = uint32_t(i * THREADS) + threadIdx.x < count ? g.keys[i * THREADS + threadIdx.x] : 0ull;
     uint64_t found = 0;
+#pragma unroll 1
     for (int bit = 63; bit >= 0; --bit) {
         const uint64_t trial = found | 1ull << bit;
         uint32_t n = 0;
@@ -104,7 +119,10 @@ __device__ __forceinline__ uint64_t cut(Gathered &g, uint32_t k) {
         uint32_t *const part = g.part[bit & 1];
         if ((threadIdx.x & 63u) == 0) part[wave] = n;
         __syncthreads();
-        if (part[0] + part[1] + part[2] + part[3] >= k) found = trial;
+        uint32_t all = 0;
+#pragma unroll
+        for (int w = 0; w < THREADS / 64; ++w) all += part[w];
+        if (all >= k) found = trial;
     }
     if (threadIdx.x == 0) g.count = 0;
     __syncthreads();
@@ -115,15 +133,16 @@ __device__ __forceinline__ uint64_t cut(Gathered &g, uint32_t k) {
     return found;
 }
 // The k best in order to `out`, zeros where there are fewer.  (A thread finds its keys' places by counting.)
-template <typename F>
-__device__ __forceinline__ void in_order(Gathered &g, uint32_t k, F &&out) {
+template <int THREADS, typename F>
+__device__ __forceinline__ void in_order(Gathered<THREADS> &g, uint32_t k, F &&out) {
+    static_assert(kInOrder <= 2 * THREADS, "two to a thread");
     uint32_t count = g.count;
-    if (count > 2 * kLogThreads) {
+    if (count > kInOrder) {
         cut(g, k);
         count = g.count;
     }
     if (threadIdx.x < count) {
-        const uint64_t mine = g.keys[threadIdx.x], other = threadIdx.x + kLogThreads < count ? g.keys[threadIdx.x + kLogThreads] : 0ull;
+        const uint64_t mine = g.keys[threadIdx.x], other = threadIdx.x + THREADS < count ? g.keys[threadIdx.x + THREADS] : 0ull;
         uint32_t place = 0, other_place = 0;
 #pragma unroll 4
         for (uint32_t i = 0; i < count; ++i) {
@@ -134,7 +153,7 @@ __device__ __forceinline__ void in_order(Gathered &g, uint32_t k, F &&out) {
         if (place < k) out(place, mine);
         if (other != 0 && other_place < k) out(other_place, other);
     }
-    for (uint32_t i = threadIdx.x; i < k; i += kLogThreads)
+    for (uint32_t i = threadIdx.x; i < k; i += THREADS)
         if (i >= count) out(i, 0ull);
 }
 
@@ -154,7 +173,8 @@ struct Given {
 };
 static_assert(kMostGiven <= uint32_t(kLogThreads), "a thread to a given slot");
 // A row's results from its sums and best keys.
-__device__ __forceinline__ void finish(const LogProbArgs &a, uint32_t row, const Given &given, const Heat &heat, const Sums &sums, Gathered &g) {
+template <int THREADS>
+__device__ __forceinline__ void finish(const LogProbArgs &a, uint32_t row, const Given &given, const Heat &heat, const Sums &sums, Gathered<THREADS> &g) {
     const float log_sum = logf(sums.s);
     if (threadIdx.x == 0) {
         const float entropy = sums.entropy(log_sum);
@@ -211,7 +231,7 @@ struct LogPart {
     float m, s, u, none;
 };
 constexpr int kLogLoads = 4, kLogSegments = 4;
-// Where thread t's scores lie: load l is at lo + (l * kLogThreads + t) * kEach, the first `segment` loads are its first segment.
+// Where thread t's scores lie: load l is at lo + (l * THREADS + t) * kEach, the first `segment` loads are its first segment.
 struct Loads {
     uint32_t lo, hi, all, segment;
     __device__ __forceinline__ Loads(uint32_t from, uint32_t to, uint32_t step) : lo(from), hi(to) {
@@ -220,10 +240,10 @@ struct Loads {
         segment = all < 2 * kRounds ? all : (all + kRounds - 1) / kRounds * kLogLoads;
     }
 };
-template <typename T, bool MASK>
+template <int THREADS, int LOADS, typename T, bool MASK>
 __device__ __forceinline__ void scan_part(const T *scores, const uint64_t *mask, const Heat &heat, const Loads &at, Sums &sums, float (&segments)[kLogSegments]) {
     constexpr int kEach = Scores<T>::kEach;
-    constexpr uint32_t kStep = kLogThreads * kEach;
+    constexpr uint32_t kStep = THREADS * kEach;
     float segment = kNone;
     auto take = [&](const Scores<T> *l, auto count) {
         constexpr int kCount = decltype(count)::value * kEach;
@@ -242,11 +262,11 @@ __device__ __forceinline__ void scan_part(const T *scores, const uint64_t *mask,
         segment = kNone;
         if (uint32_t(part) * at.segment < at.all) {
             uint32_t i = first + threadIdx.x * kEach;
-            for (; i + (kLogLoads - 1) * kStep + kEach <= end; i += kLogLoads * kStep) {
-                Scores<T> l[kLogLoads];
+            for (; i + (LOADS - 1) * kStep + kEach <= end; i += LOADS * kStep) {
+                Scores<T> l[LOADS];
 #pragma unroll
-                for (int j = 0; j < kLogLoads; ++j) l[j].load(scores, mask, i + j * kStep);
-                take(l, IntC<kLogLoads>{});
+                for (int j = 0; j < LOADS; ++j) l[j].load(scores, mask, i + j * kStep);
+                take(l, IntC<LOADS>{});
             }
             for (; i < end; i += kStep) {
                 Scores<T> l;
@@ -258,15 +278,19 @@ __device__ __forceinline__ void scan_part(const T *scores, const uint64_t *mask,
         segments[part] = segment;
     }
 }
-// One that at least k of the 256 scores in `best` reach, and not far below the k-th: its first 16 bits in the scores' order.  The same in every thread.
+// One that at least k of a score a thread in `best` reach, and not far below the k-th: its first 16 bits in the scores' order.  The same in every thread.
+template <int THREADS>
 __device__ __forceinline__ float reached(const float *best, uint32_t k) {
+    constexpr int kEach = THREADS / 64;
     const uint32_t lane = threadIdx.x & 63u;
-    uint32_t key[4];
+    uint32_t key[kEach];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) key[i] = uint32_t(order_key(best[i * 64 + lane] + 0.0f)) ^ 0x80000000u;
+    for (int i = 0; i < kEach; ++i) key[i] = uint32_t(order_key(best[i * 64 + lane] + 0.0f)) ^ 0x80000000u;
     uint32_t found = 0;
-    if (k <= 24) {          // (the largest of four threads each: 64 of those do)
-        const uint32_t one = max(max(key[0], key[1]), max(key[2], key[3]));
+    if (k <= 24) {          // (the largest of every sixty-fourth thread: 64 of those do)
+        uint32_t one = key[0];
+#pragma unroll
+        for (int i = 1; i < kEach; ++i) one = max(one, key[i]);
 #pragma unroll
         for (int bit = 31; bit >= 16; --bit)
             if (uint32_t(__popcll(__ballot(one >= (found | 1u << bit)))) >= k) found |= 1u << bit;
@@ -275,29 +299,29 @@ __device__ __forceinline__ float reached(const float *best, uint32_t k) {
         for (int bit = 31; bit >= 16; --bit) {
             uint32_t n = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) n += uint32_t(__popcll(__ballot(key[i] >= (found | 1u << bit))));
+            for (int i = 0; i < kEach; ++i) n += uint32_t(__popcll(__ballot(key[i] >= (found | 1u << bit))));
             if (n >= k) found |= 1u << bit;
         }
     }
     return fmaxf(order_unkey(int(found ^ 0x80000000u)), kNone);      // (nothing counts below that; a key of 0 is no number)
 }
-template <typename T, bool MASK>
-__device__ __forceinline__ void gather_part(const LogProbArgs &a, const T *scores, const uint64_t *mask, const Loads &at, const float (&segments)[kLogSegments], Gathered &g, const float *best,
+template <int THREADS, typename T, bool MASK>
+__device__ __forceinline__ void gather_part(const LogProbArgs &a, const T *scores, const uint64_t *mask, const Loads &at, const float (&segments)[kLogSegments], Gathered<THREADS> &g, const float *best,
                                             uint16_t *who, uint32_t *who_count) {
     constexpr int kEach = Scores<T>::kEach;
-    constexpr uint32_t kStep = kLogThreads * kEach;
-    const float least = reached(best, a.top);
+    constexpr uint32_t kStep = THREADS * kEach;
+    const float least = reached<THREADS>(best, a.top);
     if (threadIdx.x == 0) g.count = *who_count = 0;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kLogSegments; ++i)
-        if (segments[i] >= least && uint32_t(i) * at.segment < at.all) who[atomicAdd(who_count, 1u)] = uint16_t(i * kLogThreads + threadIdx.x);
+        if (segments[i] >= least && uint32_t(i) * at.segment < at.all) who[atomicAdd(who_count, 1u)] = uint16_t(i * THREADS + threadIdx.x);
     __syncthreads();
     const uint32_t items = *who_count * at.segment;
     auto place = [&](uint32_t item) {      // hi where there is nothing
         if (item >= items) return at.hi;
-        const uint32_t it = who[item / at.segment], l = it / kLogThreads * at.segment + item % at.segment;
-        const uint64_t i = at.lo + uint64_t(l) * kStep + it % kLogThreads * kEach;
+        const uint32_t it = who[item / at.segment], l = it / THREADS * at.segment + item % at.segment;
+        const uint64_t i = at.lo + uint64_t(l) * kStep + it % THREADS * kEach;
         return l < at.all && i < at.hi ? uint32_t(i) : at.hi;
     };
     auto load = [&](Scores<T> &l, uint32_t i) {
@@ -314,28 +338,28 @@ __device__ __forceinline__ void gather_part(const LogProbArgs &a, const T *score
             const uint64_t key = sort_key(v, i + j);
             if (key <= above) continue;
             const uint32_t to = atomicAdd(&g.count, 1u);
-            if (to < kGather) g.keys[to] = key;
+            if (to < Gathered<THREADS>::kGather) g.keys[to] = key;
         }
     };
     // As a rule all that is met fits.
-    for (uint32_t first = threadIdx.x; first < items; first += 2 * kLogThreads) {
+    for (uint32_t first = threadIdx.x; first < items; first += 2 * THREADS) {
         Scores<T> l[2];
-        const uint32_t i[2] = {place(first), place(first + kLogThreads)};
+        const uint32_t i[2] = {place(first), place(first + THREADS)};
 #pragma unroll
         for (int j = 0; j < 2; ++j) load(l[j], i[j]);
 #pragma unroll
         for (int j = 0; j < 2; ++j) put(l[j], i[j], 0);
     }
     __syncthreads();
-    if (g.count <= kGather) return;
-    // Crowded scores: once more, cut to the best whenever the next load of all threads might not fit.
+    if (g.count <= Gathered<THREADS>::kGather) return;
+    // Crowded scores: once more, cut to the best whenever the next loads might not fit.
     __syncthreads();
     if (threadIdx.x == 0) g.count = 0;
     __syncthreads();
     uint64_t above = 0;
-    for (uint32_t first = 0; first < items; first += kLogThreads) {
+    for (uint32_t first = 0; first < items; first += Gathered<THREADS>::kMeet) {
         Scores<T> l;
-        const uint32_t i = place(first + threadIdx.x);
+        const uint32_t i = threadIdx.x < Gathered<THREADS>::kMeet ? place(first + threadIdx.x) : at.hi;
         load(l, i);
         put(l, i, above);
         __syncthreads();
@@ -344,17 +368,18 @@ __device__ __forceinline__ void gather_part(const LogProbArgs &a, const T *score
         if (count > kKeep) above = cut(g, a.top);
     }
 }
-template <typename T, bool MASK>
-__global__ __launch_bounds__(kLogThreads) void k_log_probs(LogProbArgs a, uint32_t parts, uint32_t part_size) {
-    __shared__ Reduce reduce;
-    __shared__ Gathered g;
-    __shared__ uint16_t who[kLogSegments * kLogThreads];
+// (LOADS at once: two where a compute unit is to hold two of the wide workgroups, 64 registers a thread.)
+template <int THREADS, int LOADS, typename T, bool MASK>
+__global__ __launch_bounds__(THREADS, LOADS < kLogLoads ? 8 : 1) void k_log_probs(LogProbArgs a, uint32_t parts, uint32_t part_size) {
+    __shared__ Reduce<THREADS> reduce;
+    __shared__ Gathered<THREADS> g;
+    __shared__ uint16_t who[kLogSegments * THREADS];
     __shared__ uint32_t who_count;
     LogPart *const out = reinterpret_cast<LogPart *>(a.ws);
     uint64_t *const out_keys = reinterpret_cast<uint64_t *>(a.ws + size_t(a.rows) * parts * sizeof(LogPart));
-    for (uint64_t unit = blockIdx.x; unit < uint64_t(a.rows) * parts; unit += gridDim.x) {
+    auto one = [&](uint64_t unit) {
         const uint32_t row = uint32_t(unit / parts), lo = uint32_t(unit % parts) * part_size;
-        const Loads at(lo, min(part_size, a.n - lo) + lo, kLogThreads * Scores<T>::kEach);
+        const Loads at(lo, min(part_size, a.n - lo) + lo, THREADS * Scores<T>::kEach);
         const T *const scores = static_cast<const T *>(a.scores) + size_t(row) * a.stride;
         const uint64_t *const mask = MASK ? a.mask + size_t(row) * a.mask_stride : nullptr;
         const Heat heat(a.temperature, row);
@@ -362,16 +387,23 @@ __global__ __launch_bounds__(kLogThreads) void k_log_probs(LogProbArgs a, uint32
         if (parts == 1) given.load(a, row, scores, mask);
         Sums sums;
         float segments[kLogSegments];
-        scan_part<T, MASK>(scores, mask, heat, at, sums, segments);
+        scan_part<THREADS, LOADS, T, MASK>(scores, mask, heat, at, sums, segments);
         sums = group_sums(sums, heat.factor2, reduce);
-        if (a.top != 0) gather_part<T, MASK>(a, scores, mask, at, segments, g, reduce.best, who, &who_count);
+        if (a.top != 0) gather_part<THREADS, T, MASK>(a, scores, mask, at, segments, g, reduce.best, who, &who_count);
         if (parts == 1) {
             finish(a, row, given, heat, sums, g);
         } else {
             if (threadIdx.x == 0) out[unit] = LogPart{sums.m, sums.s, sums.u, 0.0f};
             if (a.top != 0) in_order(g, a.top, [&](uint32_t place, uint64_t key) { out_keys[unit * a.top + place] = key; });
         }
-        __syncthreads();
+    };
+    if constexpr (THREADS == kWideThreads) {
+        one(blockIdx.x);
+    } else {
+        for (uint64_t unit = blockIdx.x; unit < uint64_t(a.rows) * parts; unit += gridDim.x) {
+            one(unit);
+            __syncthreads();
+        }
     }
 }
 // The parts of a row, joined.  Keys that cannot be among the best are told from a few of each part: its last one is one that k keys reach, and so is the lowest of all parts'
@@ -379,8 +411,8 @@ __global__ __launch_bounds__(kLogThreads) void k_log_probs(LogProbArgs a, uint32
 constexpr uint32_t kMostParts = 1024;
 template <typename T>
 __global__ __launch_bounds__(kLogThreads) void k_log_probs_join(LogProbArgs a, uint32_t parts) {
-    __shared__ Reduce reduce;
-    __shared__ Gathered g;
+    __shared__ Reduce<kLogThreads> reduce;
+    __shared__ Gathered<kLogThreads> g;
     __shared__ uint64_t least[2][kLogWaves];
     __shared__ uint16_t who[kMostParts];
     __shared__ uint32_t who_count;
@@ -440,7 +472,7 @@ __global__ __launch_bounds__(kLogThreads) void k_log_probs_join(LogProbArgs a, u
             __syncthreads();
             reduce.best[threadIdx.x] = best;
             __syncthreads();
-            const float reach = reached(reduce.best, top);
+            const float reach = reached<kLogThreads>(reduce.best, top);
             from = larger(from, reach > kNone ? sort_key(reach, 0x7fffffffu) & ~1ull : 0ull);      // (the lowest key of that score)
 #pragma unroll
             for (int i = 0; i < kEach; ++i)
@@ -454,7 +486,7 @@ __global__ __launch_bounds__(kLogThreads) void k_log_probs_join(LogProbArgs a, u
                 __syncthreads();
                 const uint32_t count = g.count;
                 __syncthreads();
-                if (count > kGather - kLogThreads) from = cut(g, top);
+                if (count > Gathered<kLogThreads>::kGather - kLogThreads) from = cut(g, top);
             }
         }
         finish(a, row, given, heat, sums, g);
@@ -469,18 +501,26 @@ static uint32_t log_parts(size_t rows, size_t n, uint32_t &part_size) {
     part_size = uint32_t(std::min(each * kOnce, n));
     return uint32_t((n + part_size - 1) / part_size);
 }
+// Rows in parts that have a wide workgroup each all the same: rows enough for half of the card, and those that are not much longer than what two launches take.  (100000 bfloat16
+// scores a row, 20 alternatives: 1 row 13.7 us so and 14.4 in parts, 64 rows 14.5 and 18.6, 256 rows 17.7 and 26.5, 512 rows, two to a compute unit, 28.5 and 36.3; of 150000
+// 1 row 17.2 and 14.8, of 1000000 128 rows 81 and 63, 192 rows 84 and 96.  Without alternatives 1 row of 32000 6.6 and 7.3, of 100000 10.2 and 6.9, but a launch less.)
+static bool log_wide(size_t rows, size_t n) { return rows >= 160 || n <= 100000 + 600 * rows; }
 size_t log_probs_workspace(size_t rows, size_t n, size_t top) {
     if (rows == 0 || n == 0) return 0;
     uint32_t part_size;
     const size_t parts = log_parts(rows, n, part_size);
-    return parts == 1 ? 0 : rows * parts * (sizeof(LogPart) + top * sizeof(uint64_t));
+    return parts == 1 || log_wide(rows, n) ? 0 : rows * parts * (sizeof(LogPart) + top * sizeof(uint64_t));
 }
 template <typename T, bool MASK>
 static hipError_t log_probs(const LogProbArgs &a, hipStream_t s) {
     uint32_t part_size;
     const uint32_t parts = log_parts(a.rows, a.n, part_size);
+    if (parts > 1 && log_wide(a.rows, a.n)) {
+        const auto kernel = a.rows <= 256 ? k_log_probs<kWideThreads, kLogLoads, T, MASK> : k_log_probs<kWideThreads, kLogLoads / 2, T, MASK>;
+        return launch(kernel, a.rows, kWideThreads, 0, s, a, 1u, a.n);
+    }
     const uint64_t units = uint64_t(a.rows) * parts;
-    const hipError_t e = launch(k_log_probs<T, MASK>, uint32_t(units < kMostGroups ? units : kMostGroups), kLogThreads, 0, s, a, parts, part_size);
+    const hipError_t e = launch(k_log_probs<kLogThreads, kLogLoads, T, MASK>, uint32_t(units < kMostGroups ? units : kMostGroups), kLogThreads, 0, s, a, parts, part_size);
     return e != hipSuccess || parts == 1 ? e : launch(k_log_probs_join<T>, uint32_t(a.rows < kMostGroups ? a.rows : kMostGroups), kLogThreads, 0, s, a, parts);
 }
 template <typename T>
