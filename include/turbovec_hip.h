@@ -293,7 +293,7 @@ int tv_fp4_values_dev(int device, void *stream, const uint8_t *d_codes, size_t c
 /* out[i][j] = the inner product of row i of a (m rows) with row j of b (n rows): products of codes within a block times both scales, added in
  * 32 bits and rounded once to out_type.  A block's sum is exact; a sum of blocks loses what 32-bit sums do, and is infinite where it, or
  * a block's part of it, passes 2^128.  Rows that start at multiples of 16 bytes (codes and stride) are read fastest.  A result of more tiles than one
- * launch has (2^24 of 64 x 64) fails before anything is written. */
+ * launch has (2^24 of 64 x 64; 2^26 of 16 x 16 where rows are below 16 bytes, or 8 MB and more apart) fails before anything is written. */
 int tv_fp4_matmul_dev(int device, void *stream, const uint8_t *d_a, size_t a_stride, const uint8_t *d_a_scales, size_t a_scale_stride, size_t m,
                       const uint8_t *d_b, size_t b_stride, const uint8_t *d_b_scales, size_t b_scale_stride, size_t n,
                       size_t dim, void *d_out, int out_type, size_t out_stride);

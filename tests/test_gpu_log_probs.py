@@ -515,3 +515,28 @@ def test_two_graphs_at_once(log_probs):
     torch.cuda.synchronize()
     for g, w in zip(got, want):
         assert all(torch.equal(x, y) for x, y in zip(g, w))
+
+
+def test_what_a_call_may_also_be_given(log_probs):
+    """Rows that are one and the same, slots out of a wider table, gradients of no rows; and a temperature that wants a gradient is refused."""
+    one = scores_of(1, 3000, torch.float32, 50)
+    table = slots_of(6, 3000, 5)
+    t = torch.rand(6, generator=gen(51), device="cuda") + 0.5
+    check(log_probs, one.expand(6, 3000), table[:, 1:4], temperature=t, top=3)
+    check(log_probs, one.expand(6, 3000), table[:, 2].contiguous(), temperature=t)
+    leaf = one.clone().requires_grad_(True)
+    rows = leaf.expand(6, 3000)
+    found = log_probs(rows, table[:, 1:4], temperature=t)
+    got, = torch.autograd.grad((found.log_probs.sum(), found.entropy.sum()), leaf)
+    plain = Plain(one.expand(6, 3000), t)
+    want, off = plain.gradient(table[:, 1:4], torch.ones(6, 3, device="cuda"), torch.ones(6, device="cuda"))
+    assert bool(((got.double() - want.sum(0)).abs() <= off.sum(0) + 2.0 ** -23 * want.abs().sum(0) * 6).all())
+    none = torch.zeros(0, 100, device="cuda", requires_grad=True)
+    found = log_probs(none, torch.zeros(0, 2, dtype=torch.int64, device="cuda"), top=2)
+    grad, = torch.autograd.grad((found.log_probs.sum(), found.entropy.sum()), none)
+    assert grad.shape == (0, 100)
+    for scores in (one, leaf):
+        with pytest.raises(ValueError, match="temperature has no gradient"):
+            log_probs(scores, table[:1, 0], temperature=t[:1].clone().requires_grad_(True))
+    with torch.no_grad():
+        log_probs(one, table[:1, 0], temperature=t[:1].clone().requires_grad_(True))

@@ -226,3 +226,15 @@ def test_norm_then_scores_then_a_draw_and_its_log_probability(norm, to):
     assert torch.allclose(found.log_probs.double(), z.gather(1, slots[:, None])[:, 0], atol=1e-4)
     assert torch.allclose(found.log_probs.exp(), p, rtol=1e-4, atol=0)
     assert torch.equal(found.top_slots, torch.sort(scores, dim=1, descending=True, stable=True).indices[:, :5])
+
+
+def test_rows_that_are_one_and_the_same(norm):
+    """An input may be one row many times, the sum may not."""
+    one, other = torch.randn(1, 400, device="cuda"), torch.randn(7, 400, device="cuda")
+    made, summed = norm.add_rms_norm(one.expand(7, 400), other)
+    want, want_sum = norm.add_rms_norm(one.repeat(7, 1), other)
+    assert torch.equal(made.codes.view(torch.uint8), want.codes.view(torch.uint8)) and torch.equal(summed, want_sum)
+    made, summed = norm.add_rms_norm(other, one.expand(7, 400), out=other)
+    assert summed is other and torch.equal(other, want_sum) and torch.equal(made.codes.view(torch.uint8), want.codes.view(torch.uint8))
+    with pytest.raises(RuntimeError, match="overlap"):
+        norm.add_rms_norm(other, other, out=torch.zeros(1, 400, device="cuda").expand(7, 400))

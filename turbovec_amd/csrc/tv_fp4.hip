@@ -572,7 +572,7 @@ static hipError_t matmul4(const Matmul4Args &a, hipStream_t s) {
     const uint64_t tiles = uint64_t(mt) * nt;
     if (tile == 0 && tiles > 256 && nt >= mt) {
         // The tiles of 256 that start a last round and do not fill it: their columns in a launch of their own, of smaller tiles, where that is less than the round.  (1024 by 100000
-        // of 1536 into floats: FIGURE.)
+        // of 1536 into floats: 160 us with it and 167 to 176 without, inputs and results from memory.)
         const uint32_t columns = uint32_t(tiles / 256 * 256 / mt) * 256;
         if (columns < a.b.rows) {
             Matmul4Args first = a, rest = a;

@@ -133,7 +133,7 @@ def log_probs(scores, slots, *, temperature=None, mask=None, top=0):
     An allowed NaN or +infinity makes its row NaN.  A temperature that is not above 0 is the limit: the best slots share the mass, and the row has no gradient.
 
     `log_probs` and `entropy` carry a gradient to the scores (tv_log_probs_grad_dev; in the scores' type, rounded once, once differentiable); the alternatives carry none: give
-    them as `slots` for that."""
+    them as `slots` for that.  A temperature that requires a gradient is refused."""
     _gpu("scores", scores, _VALUES)
     rows, n = scores.shape
     if n == 0:
@@ -149,6 +149,8 @@ def log_probs(scores, slots, *, temperature=None, mask=None, top=0):
     if not 0 <= top <= _MOST_TOP:
         raise ValueError(f"top must be 0 to {_MOST_TOP}, got {top}")
     temperature = _a_row("temperature", temperature, rows, torch.float32, device)
+    if torch.is_grad_enabled() and temperature is not None and temperature.requires_grad:
+        raise ValueError("a temperature has no gradient here: detach it, or divide the scores by it")
     if scores.requires_grad and torch.is_grad_enabled():
         return LogProbs(*_WithGradient.apply(scores, slots, temperature, mask, top))
     return _forward(scores, slots, temperature, mask, top, None)
