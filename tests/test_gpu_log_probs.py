@@ -540,3 +540,36 @@ def test_what_a_call_may_also_be_given(log_probs):
             log_probs(scores, table[:1, 0], temperature=t[:1].clone().requires_grad_(True))
     with torch.no_grad():
         log_probs(one, table[:1, 0], temperature=t[:1].clone().requires_grad_(True))
+
+
+@pytest.mark.parametrize("rows,n", [(1023, 700), (1024, 700), (1024, 1), (1500, 2048), (1500, 2049), (1100, 4096), (1100, 4097), (2000, 65), (1 << 16, 33)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_short_rows(log_probs, rows, n, dtype):
+    """A wave to a row, and what is a little more than that."""
+    t = 0.5 + torch.rand(rows, generator=gen(60), device="cuda")
+    scores, slots = scores_of(rows, n, dtype, 61), slots_of(rows, n, 128)
+    allowed = torch.rand(rows, n, generator=gen(62), device="cuda") < 0.5
+    allowed[3] = False
+    scores[5] = 1.0
+    scores[6] = -INF
+    scores[7, n // 2:] = 9.0
+    for given, top in ((128, 24), (70, 25), (1, 1), (3, 0)):
+        check(log_probs, scores, slots[:, :given], temperature=t, top=top)
+        check(log_probs, scores, slots[:, :given], temperature=t, allowed=allowed, top=top)
+    check_gradient(log_probs, scores, slots[:, :66], temperature=t)
+    check_gradient(log_probs, scores, slots[:, :2], temperature=t, allowed=allowed)
+    scores[8, n // 2], scores[9, 0] = float("nan"), INF
+    found = log_probs(scores, slots, temperature=t, top=2)
+    bad = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    bad[8:10] = True
+    assert torch.equal(torch.isnan(found.entropy), bad) and torch.equal(torch.isnan(found.log_probs).all(1), bad)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_short_rows_of_crowded_scores(log_probs, dtype):
+    for n in (300, 2000):
+        slots = slots_of(1024, n, 1)
+        ramp = torch.arange(n, device="cuda").float()
+        for scores in (torch.zeros(n), torch.randint(0, 5, (n,), generator=gen(63), device="cuda"), ramp % 512 == 5, ramp % 64 < 8, ramp / n * 20, -ramp / n * 20, ramp > n - 200):
+            for top in (1, 24):
+                check(log_probs, scores.to("cuda").to(dtype).expand(1024, n).contiguous(), slots, top=top)

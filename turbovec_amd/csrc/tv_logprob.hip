@@ -53,8 +53,8 @@ struct Sums {
 __device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
 __device__ __forceinline__ uint64_t smaller(uint64_t a, uint64_t b) { return a < b ? a : b; }
 
-// Workgroups of kLogThreads, or of kWideThreads where a row has one to itself and would need several of the others.
-constexpr int kLogThreads = 256, kLogWaves = kLogThreads / 64, kWideThreads = 1024;
+// Workgroups of kLogThreads; of kWideThreads where a row has one to itself and would need several of the others, of kShortThreads for many short rows.
+constexpr int kLogThreads = 256, kLogWaves = kLogThreads / 64, kWideThreads = 1024, kShortThreads = 64;
 // Sums over the workgroup, in every thread; `best` has room for a float a thread and is left holding the threads' largest scores.
 template <int THREADS>
 struct Reduce {
@@ -135,14 +135,13 @@ __device__ __forceinline__ uint64_t cut(Gathered<THREADS> &g, uint32_t k) {
 // The k best in order to `out`, zeros where there are fewer.  (A thread finds its keys' places by counting.)
 template <int THREADS, typename F>
 __device__ __forceinline__ void in_order(Gathered<THREADS> &g, uint32_t k, F &&out) {
-    static_assert(kInOrder <= 2 * THREADS, "two to a thread");
     uint32_t count = g.count;
     if (count > kInOrder) {
         cut(g, k);
         count = g.count;
     }
-    if (threadIdx.x < count) {
-        const uint64_t mine = g.keys[threadIdx.x], other = threadIdx.x + THREADS < count ? g.keys[threadIdx.x + THREADS] : 0ull;
+    for (uint32_t first = threadIdx.x; first < count; first += 2 * THREADS) {
+        const uint64_t mine = g.keys[first], other = first + THREADS < count ? g.keys[first + THREADS] : 0ull;
         uint32_t place = 0, other_place = 0;
 #pragma unroll 4
         for (uint32_t i = 0; i < count; ++i) {
@@ -157,31 +156,39 @@ __device__ __forceinline__ void in_order(Gathered<THREADS> &g, uint32_t k, F &&o
         if (i >= count) out(i, 0ull);
 }
 
-// A thread's given slot and its score: asked for before the sums are known.
+// A thread's given slots and their scores: asked for before the sums are known.
+template <int THREADS>
 struct Given {
-    float score;
-    bool there;
+    static constexpr int kEach = (int(kMostGiven) + THREADS - 1) / THREADS;
+    float score[kEach];
+    bool there[kEach];
     template <typename T>
     __device__ __forceinline__ void load(const LogProbArgs &a, uint32_t row, const T *scores, const uint64_t *mask) {
-        there = false;
-        if (threadIdx.x >= a.given) return;
-        const int64_t slot = a.slots[size_t(row) * a.slot_stride + threadIdx.x];
-        if (slot < 0 || slot >= int64_t(a.n)) return;
-        score = float(scores[slot]);
-        there = counts(mask, uint32_t(slot), score);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const uint32_t k = uint32_t(i * THREADS) + threadIdx.x;
+            there[i] = false;
+            if (k >= a.given) continue;
+            const int64_t slot = a.slots[size_t(row) * a.slot_stride + k];
+            if (slot < 0 || slot >= int64_t(a.n)) continue;
+            score[i] = float(scores[slot]);
+            there[i] = counts(mask, uint32_t(slot), score[i]);
+        }
     }
 };
-static_assert(kMostGiven <= uint32_t(kLogThreads), "a thread to a given slot");
 // A row's results from its sums and best keys.
 template <int THREADS>
-__device__ __forceinline__ void finish(const LogProbArgs &a, uint32_t row, const Given &given, const Heat &heat, const Sums &sums, Gathered<THREADS> &g) {
+__device__ __forceinline__ void finish(const LogProbArgs &a, uint32_t row, const Given<THREADS> &given, const Heat &heat, const Sums &sums, Gathered<THREADS> &g) {
     const float log_sum = logf(sums.s);
     if (threadIdx.x == 0) {
         const float entropy = sums.entropy(log_sum);
         a.out_entropy[row] = entropy;
         if (a.stats != nullptr) *reinterpret_cast<float4 *>(a.stats + size_t(row) * 4) = make_float4(sums.m, log2f(sums.s), entropy, 0.0f);
     }
-    if (threadIdx.x < a.given) a.out_log_probs[size_t(row) * a.given + threadIdx.x] = given.there ? heat.log_p(given.score - sums.m, log_sum) : -kInf;
+#pragma unroll
+    for (int i = 0; i < given.kEach; ++i)
+        if (const uint32_t k = uint32_t(i * THREADS) + threadIdx.x; k < a.given)
+            a.out_log_probs[size_t(row) * a.given + k] = given.there[i] ? heat.log_p(given.score[i] - sums.m, log_sum) : -kInf;
     if (a.top != 0)
         in_order(g, a.top, [&](uint32_t place, uint64_t key) {
             float v = 0.0f;
@@ -278,6 +285,7 @@ __device__ __forceinline__ void scan_part(const T *scores, const uint64_t *mask,
         segments[part] = segment;
     }
 }
+constexpr uint32_t kFewAlternatives = 24;
 // One that at least k of a score a thread in `best` reach, and not far below the k-th: its first 16 bits in the scores' order.  The same in every thread.
 template <int THREADS>
 __device__ __forceinline__ float reached(const float *best, uint32_t k) {
@@ -287,7 +295,7 @@ __device__ __forceinline__ float reached(const float *best, uint32_t k) {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) key[i] = uint32_t(order_key(best[i * 64 + lane] + 0.0f)) ^ 0x80000000u;
     uint32_t found = 0;
-    if (k <= 24) {          // (the largest of every sixty-fourth thread: 64 of those do)
+    if (k <= kFewAlternatives) {          // (the largest of every sixty-fourth thread: 64 of those do)
         uint32_t one = key[0];
 #pragma unroll
         for (int i = 1; i < kEach; ++i) one = max(one, key[i]);
@@ -370,7 +378,7 @@ __device__ __forceinline__ void gather_part(const LogProbArgs &a, const T *score
 }
 // (LOADS at once: two where a compute unit is to hold two of the wide workgroups, 64 registers a thread.)
 template <int THREADS, int LOADS, typename T, bool MASK>
-__global__ __launch_bounds__(THREADS, LOADS < kLogLoads ? 8 : 1) void k_log_probs(LogProbArgs a, uint32_t parts, uint32_t part_size) {
+__global__ __launch_bounds__(THREADS, THREADS == kWideThreads && LOADS < kLogLoads ? 8 : 1) void k_log_probs(LogProbArgs a, uint32_t parts, uint32_t part_size) {
     __shared__ Reduce<THREADS> reduce;
     __shared__ Gathered<THREADS> g;
     __shared__ uint16_t who[kLogSegments * THREADS];
@@ -383,7 +391,7 @@ __global__ __launch_bounds__(THREADS, LOADS < kLogLoads ? 8 : 1) void k_log_prob
         const T *const scores = static_cast<const T *>(a.scores) + size_t(row) * a.stride;
         const uint64_t *const mask = MASK ? a.mask + size_t(row) * a.mask_stride : nullptr;
         const Heat heat(a.temperature, row);
-        Given given;
+        Given<THREADS> given;
         if (parts == 1) given.load(a, row, scores, mask);
         Sums sums;
         float segments[kLogSegments];
@@ -424,7 +432,7 @@ __global__ __launch_bounds__(kLogThreads) void k_log_probs_join(LogProbArgs a, u
         const LogPart *const in = reinterpret_cast<const LogPart *>(a.ws) + size_t(row) * parts;
         const uint64_t *const in_keys = reinterpret_cast<const uint64_t *>(a.ws + size_t(a.rows) * parts * sizeof(LogPart)) + size_t(row) * parts * top;
         const Heat heat(a.temperature, row);
-        Given given;
+        Given<kLogThreads> given;
         given.load(a, row, scores, mask);
         LogPart p[kEach];
         uint64_t first[kEach], last = 0, low = ~0ull;
@@ -505,6 +513,9 @@ static uint32_t log_parts(size_t rows, size_t n, uint32_t &part_size) {
 // scores a row, 20 alternatives: 1 row 13.7 us so and 14.4 in parts, 64 rows 14.5 and 18.6, 256 rows 17.7 and 26.5, 512 rows, two to a compute unit, 28.5 and 36.3; of 150000
 // 1 row 17.2 and 14.8, of 1000000 128 rows 81 and 63, 192 rows 84 and 96.  Without alternatives 1 row of 32000 6.6 and 7.3, of 100000 10.2 and 6.9, but a launch less.)
 static bool log_wide(size_t rows, size_t n) { return rows >= 160 || n <= 100000 + 600 * rows; }
+// Many rows of a few loads have a wave each, as long as its 64 largest scores tell the alternatives apart.  (Rows of 1000 bfloat16 scores with 5 alternatives: 1024 rows 7.9 us so and 8.5
+// with workgroups of 256, 4096 rows 10.2 and 21.9, 65536 rows 88 and 275; their gradients 4096 rows 8.2 and 11.4, 65536 rows 73 and 152.)
+static bool log_short(size_t rows, size_t n, size_t size, size_t top) { return rows >= 1024 && n * size <= 8192 && top <= kFewAlternatives; }
 size_t log_probs_workspace(size_t rows, size_t n, size_t top) {
     if (rows == 0 || n == 0) return 0;
     uint32_t part_size;
@@ -520,6 +531,8 @@ static hipError_t log_probs(const LogProbArgs &a, hipStream_t s) {
         return launch(kernel, a.rows, kWideThreads, 0, s, a, 1u, a.n);
     }
     const uint64_t units = uint64_t(a.rows) * parts;
+    if (log_short(a.rows, a.n, sizeof(T), a.top))
+        return launch(k_log_probs<kShortThreads, kLogLoads / 2, T, MASK>, uint32_t(units < kMostGroups ? units : kMostGroups), kShortThreads, 0, s, a, 1u, a.n);
     const hipError_t e = launch(k_log_probs<kLogThreads, kLogLoads, T, MASK>, uint32_t(units < kMostGroups ? units : kMostGroups), kLogThreads, 0, s, a, parts, part_size);
     return e != hipSuccess || parts == 1 ? e : launch(k_log_probs_join<T>, uint32_t(a.rows < kMostGroups ? a.rows : kMostGroups), kLogThreads, 0, s, a, parts);
 }
@@ -535,10 +548,10 @@ hipError_t launch_log_probs(const LogProbArgs &a, int score_type, hipStream_t s)
 // The gradient of a score that counts: (picked - p (G + g (log p + H))) / T, picked the sum of the gradients of the given slots that are this one.  With l = log2 p that is
 // (picked + p (A + B l)) / T, A = -(G + g H) and B = -g ln 2.  Bound by memory, a reading and a writing.  What is picked is added by the thread that wrote the
 // slot's own gradient, behind that.
-template <typename T, bool MASK>
-__global__ __launch_bounds__(kLogThreads) void k_log_probs_grad(LogProbGradArgs a, uint32_t parts, uint32_t part_size) {
+template <int THREADS, typename T, bool MASK>
+__global__ __launch_bounds__(THREADS) void k_log_probs_grad(LogProbGradArgs a, uint32_t parts, uint32_t part_size) {
     constexpr int kEach = Scores<T>::kEach;
-    constexpr uint32_t kStep = kLogThreads * kEach;
+    constexpr uint32_t kStep = THREADS * kEach;
     typedef T Run __attribute__((ext_vector_type(kEach), aligned(sizeof(T))));
     for (uint64_t unit = blockIdx.x; unit < uint64_t(a.rows) * parts; unit += gridDim.x) {
         const uint32_t row = uint32_t(unit / parts), lo = uint32_t(unit % parts) * part_size, hi = lo + min(part_size, a.n - lo);
@@ -590,7 +603,7 @@ __global__ __launch_bounds__(kLogThreads) void k_log_probs_grad(LogProbGradArgs 
         }
         for (uint32_t k = 0; k < (heat.limit ? 0u : a.given); ++k) {
             const int64_t slot = slots[k];
-            if (slot < int64_t(lo) || slot >= int64_t(hi) || (uint32_t(slot) - lo) / kEach % kLogThreads != threadIdx.x) continue;
+            if (slot < int64_t(lo) || slot >= int64_t(hi) || (uint32_t(slot) - lo) / kEach % THREADS != threadIdx.x) continue;
             const float s = float(scores[slot]);
             if (!counts(mask, uint32_t(slot), s)) continue;
             float picked = 0.0f;               // (where the same slot stands there again, the last sum is the whole one)
@@ -599,17 +612,22 @@ __global__ __launch_bounds__(kLogThreads) void k_log_probs_grad(LogProbGradArgs 
         }
     }
 }
-template <typename T>
+template <int THREADS, typename T>
 static hipError_t log_probs_grad(const LogProbGradArgs &a, hipStream_t s) {
     uint32_t part_size;
     const uint32_t parts = log_parts(a.rows, a.n, part_size);
     const uint64_t units = uint64_t(a.rows) * parts;
     const uint32_t grid = uint32_t(units < kMostGroups ? units : kMostGroups);
-    return a.mask == nullptr ? launch(k_log_probs_grad<T, false>, grid, kLogThreads, 0, s, a, parts, part_size) : launch(k_log_probs_grad<T, true>, grid, kLogThreads, 0, s, a, parts, part_size);
+    const auto kernel = a.mask == nullptr ? k_log_probs_grad<THREADS, T, false> : k_log_probs_grad<THREADS, T, true>;
+    return launch(kernel, grid, THREADS, 0, s, a, parts, part_size);
+}
+template <typename T>
+static hipError_t log_probs_grad_as(const LogProbGradArgs &a, hipStream_t s) {
+    return log_short(a.rows, a.n, sizeof(T), 0) ? log_probs_grad<kShortThreads, T>(a, s) : log_probs_grad<kLogThreads, T>(a, s);
 }
 hipError_t launch_log_probs_grad(const LogProbGradArgs &a, int score_type, hipStream_t s) {
-    if (score_type == kF32) return log_probs_grad<float>(a, s);
-    return score_type == kF16 ? log_probs_grad<f16>(a, s) : log_probs_grad<bf16>(a, s);
+    if (score_type == kF32) return log_probs_grad_as<float>(a, s);
+    return score_type == kF16 ? log_probs_grad_as<f16>(a, s) : log_probs_grad_as<bf16>(a, s);
 }
 
 }  // namespace tv
