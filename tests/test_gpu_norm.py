@@ -238,3 +238,34 @@ def test_rows_that_are_one_and_the_same(norm):
     assert summed is other and torch.equal(other, want_sum) and torch.equal(made.codes.view(torch.uint8), want.codes.view(torch.uint8))
     with pytest.raises(RuntimeError, match="overlap"):
         norm.add_rms_norm(other, other, out=torch.zeros(1, 400, device="cuda").expand(7, 400))
+
+
+@pytest.mark.parametrize("to", ["fp8", "fp4"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [100, 512, 1536, 2048, 4096, 16384])
+def test_scales_next_to_a_border(norm, dim, dtype, to):
+    """Weights that bring each block's largest value next to where its power of two changes.  Of what the kernel decides by, the mean is off by what a thread's 8 or 16 squares lose in 32 bits, over
+    many threads: by six standard deviations of sqrt(16) 2^-25 / sqrt(threads), half of which reaches the root; two products are off by 2^-24 each, but for 8-bit rows of 513 to 2048 two-byte values."""
+    block, border = (32, 7.0) if to == "fp4" else (128, 448.0)
+    threads = max(dim // 16, 6)
+    off = 6 * 4 * 2.0 ** -25 / threads ** 0.5 / 2 + (0.0 if to == "fp8" and dtype == torch.bfloat16 and 512 < dim <= 2048 else 2 * 2.0 ** -24)
+    told = 0
+    for seed in range(60):
+        g = gen(100 + seed)
+        x = torch.randn(1, dim, generator=g, device="cuda").to(dtype)
+        h = x.double()
+        unit = h / torch.sqrt((h * h).mean() + EPS)
+        weight = torch.full((dim,), 2.0 ** -9, device="cuda")
+        best = torch.nn.functional.pad(unit.abs(), (0, -dim % block)).view(-1, block)
+        at = best.argmax(1) + torch.arange(len(best), device="cuda") * block
+        near = border * 2.0 ** torch.randint(-12, -8, (len(at),), generator=g, device="cuda").double() * (1 + 8 * off * (torch.rand(len(at), generator=g, device="cuda").double() - 0.5))
+        weight[at] = (near / unit[0, at].abs()).float()
+        most = torch.nn.functional.pad((unit * weight.double()).abs(), (0, -dim % block)).view(-1, block).amax(1)
+        over = torch.log2(most / border)
+        want = torch.floor(over) + 1 if to == "fp4" else torch.ceil(over)
+        clear = ((over - torch.round(over)).abs() * 0.6931 > off) & (most > 0)
+        got = torch.log2(norm.rms_norm(x, weight, eps=EPS, to=to).scales.double())[0]
+        assert bool((got == want)[clear].all()), (seed, over[clear & (got != want)] - torch.round(over[clear & (got != want)]))
+        assert bool(((got - over).abs() < 1.01).all())
+        told += int((clear & ((over - torch.round(over)).abs() < 8 * off)).sum())
+    assert told > 10

@@ -113,6 +113,7 @@ struct NormArgs {
     void *scales;
     size_t x_stride, residual_stride, sum_stride, code_stride, scale_stride;
     uint32_t rows, dim;
+    double share;                     // 1 / dim
     int weight_type;
     float eps;
 };

@@ -242,7 +242,7 @@ int tv_rms_norm_dev(int device, void *stream, const void *d_x, int x_type, size_
     OnDevice on(device);
     if (on.rc != TV_OK) return on.rc;
     const tv::NormArgs a{d_x, d_residual, d_sum, d_weight, d_codes, d_scales, x_stride, residual_stride, sum_stride, code_stride, scale_stride,
-                         uint32_t(rows), uint32_t(dim), weight_type, eps};
+                         uint32_t(rows), uint32_t(dim), 1.0 / double(dim), weight_type, eps};
     const hipError_t e = tv::launch_rms_norm(a, x_type, row_kind, scale_type, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? TV_OK : op_failed(e, "tv_rms_norm_dev");
 }
