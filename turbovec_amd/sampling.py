@@ -99,20 +99,17 @@ def _forward(scores, slots, temperature, mask, top, stats):
 
 class _WithGradient(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, scores, slots, temperature, mask, top):
+    def forward(ctx, scores, slots, temperature, mask, top, alternatives):
         stats = torch.empty((scores.shape[0], 4), dtype=torch.float32, device=scores.device)
-        found = _forward(scores, slots, temperature, mask, top, stats)
+        log_p, entropy, *alternatives[:] = _forward(scores, slots, temperature, mask, top, stats)
         ctx.save_for_backward(scores, slots, temperature, mask, stats)
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(found.top_slots, found.top_log_probs)
-        return tuple(found)
+        return log_p, entropy
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, g_log_probs, g_entropy, _slots, _top):
+    def backward(ctx, g_log_probs, g_entropy):
         scores, slots, temperature, mask, stats = ctx.saved_tensors
-        if g_log_probs is None and g_entropy is None:
-            return None, None, None, None, None
         rows, n = scores.shape
         device = scores.device
         g_log_probs, g_entropy = (None if g is None else g.contiguous() for g in (g_log_probs, g_entropy))       # (a sum's is one number, spread)
@@ -120,7 +117,7 @@ class _WithGradient(torch.autograd.Function):
         _call(T.lib().tv_log_probs_grad_dev, device, scores.data_ptr(), _VALUES[scores.dtype], scores.stride(0), rows, n, *_mask(mask, rows, n, device),
               None if temperature is None else temperature.data_ptr(), slots.data_ptr(), slots.stride(0), slots.shape[1] if slots.dim() == 2 else 1, stats.data_ptr(),
               None if g_log_probs is None else g_log_probs.data_ptr(), None if g_entropy is None else g_entropy.data_ptr(), grad.data_ptr(), n)
-        return grad, None, None, None, None
+        return grad, None, None, None, None, None
 
 
 def log_probs(scores, slots, *, temperature=None, mask=None, top=0):
@@ -152,5 +149,6 @@ def log_probs(scores, slots, *, temperature=None, mask=None, top=0):
     if torch.is_grad_enabled() and temperature is not None and temperature.requires_grad:
         raise ValueError("a temperature has no gradient here: detach it, or divide the scores by it")
     if scores.requires_grad and torch.is_grad_enabled():
-        return LogProbs(*_WithGradient.apply(scores, slots, temperature, mask, top))
+        alternatives = []          # (they carry no gradient, and need no place in its graph)
+        return LogProbs(*_WithGradient.apply(scores, slots, temperature, mask, top, alternatives), *alternatives)
     return _forward(scores, slots, temperature, mask, top, None)
