@@ -61,7 +61,7 @@ def _made(x, residual, summed, weight, eps, to, scale):
 
 def rms_norm(x, weight=None, *, eps=1e-6, to="fp8", scale="e8m0"):
     """Rows x / sqrt(mean(x^2) + eps) * weight as `Fp8Rows` (`to` "fp8"; scales "e8m0" or "f32") or `Fp4Rows` ("fp4") (tv_rms_norm_dev).  `x`: float32,
-    float16 or bfloat16 [rows, dim]; `weight`: [dim] of any of these, or none.  All of it is taken in 32 bits and rounded once, to the codes."""
+    float16 or bfloat16 [rows, dim]; `weight`: [dim] of any of these, or none.  All of it is taken in 32 bits (long sums in 64) and rounded once, to the codes."""
     return _made(_gpu("x", x, _VALUES), None, None, weight, eps, to, scale)
 
 
