@@ -1,4 +1,4 @@
-"""Every form of the 4-bit product -- rows of b streamed past those of a, 16 of them to a wave or shared out over four; tiles of five sizes, a last round's columns in
+"""Every form of the 4-bit product -- rows of b streamed past those of a, 16 of them to a wave or shared out over four or eight; tiles of five sizes, a last round's columns in
 smaller ones; rows too short or too far apart for those -- into each type, over rows that start anywhere, last tiles that are partly empty and last blocks that
 are odd."""
 import pytest
@@ -7,9 +7,9 @@ torch = pytest.importorskip("torch")
 
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
 TILES = {(256, 256): (1, 1.44, 4.3, 1.4), (128, 128): (2, 0.59, 0.34, 0.42), (64, 64): (4, 0.23, 0.24, 0.14), (64, 128): (3, 0.39, 0.18, 0.3), (32, 128): (3, 0.27, 0.33, 0.19)}
-SIZES = [(5, 400), (16, 17_001), (17, 5000), (20, 70_003), (257, 3001), (700, 6001), (1030, 13_007), (300, 40_001), (1030, 44_001)]
+SIZES = [(5, 400), (7, 9000), (16, 17_001), (17, 5000), (20, 70_003), (257, 3001), (700, 6001), (1030, 13_007), (300, 40_001), (1030, 44_001)]
 DIMS = [201, 385, 1500]
-LONG = [(16, 700, 8199, "shared out"), (16, 9001, 8199, "tile")]          # rows of a that take most of a compute unit's LDS
+LONG = [(16, 700, 8199, "over eight"), (16, 9001, 8199, "tile")]          # rows of a that take most of a compute unit's LDS
 
 
 def form(m, n, dim, size):
@@ -26,11 +26,12 @@ def form(m, n, dim, size):
 
     if m <= 16 and dim >= 31:
         row, blocks = -(-dim // 128) * 64 + 16, -(-dim // 128)
-        lds = m * row + blocks * 64 + 4096
+        wide = -(-n // 16) <= 512
+        lds = m * row + blocks * 64 + (8192 if wide else 4096)
         if m * row <= 64 << 10:
-            return "shared out" if n < 256 * 4 * 16 else "streamed"
+            return "streamed" if n >= 256 * 4 * 16 else "over eight" if wide else "over four"
         if lds <= 160 << 10 and -(-n // 16) <= 256 * ((160 << 10) // lds):
-            return "shared out"
+            return "over eight" if wide else "over four"
     if dim < 31:
         return "small"
     tile, mt, nt = best(n), -(-m // 256), -(-n // 256)
@@ -45,7 +46,7 @@ def form(m, n, dim, size):
 
 def test_sizes_reach_every_form():
     reached = {form(m, n, dim, size) for m, n in SIZES for dim in DIMS for size in (2, 4)}
-    assert {"shared out", "streamed", *TILES} <= reached, reached
+    assert {"over eight", "over four", "streamed", *TILES} <= reached, reached
     assert any(isinstance(f[0], tuple) for f in reached), reached
     for m, n, dim, what in LONG:
         assert (form(m, n, dim, 4) if what != "tile" else "tile" if form(m, n, dim, 4) in TILES else "") == what

@@ -115,35 +115,27 @@ __device__ __forceinline__ void store_out4(void *out, size_t at, float v, int ty
     else static_cast<bf16 *>(out)[at] = bf16(v);
 }
 
-// Up to sixteen rows of a: bound by reading b once.  A wave streams 16 rows of b from memory into registers, two steps of 128 coordinates while the two
-// before are multiplied, and goes on to its next 16 rows without a pause; a lies in LDS.  Where there are few rows of b (SPLIT), the four waves of
-// a workgroup share 16 rows, each taking every fourth step, and their sums are added in the waves' order.
-constexpr int kDirect4Threads = 256, kDirect4Waves = kDirect4Threads / 64, kDirect4Steps = 2;
-constexpr uint32_t kDirect4Groups = 4;        // workgroups of a compute unit at a time
+// Up to sixteen rows of a: bound by reading b once.  A wave streams 16 rows of b from memory into registers, STEPS steps of 128 coordinates while those
+// before are multiplied, and goes on to its next 16 rows without a pause; a lies in LDS, and comes there behind the first of b.  Where there are few rows of b (SPLIT), the waves of
+// a workgroup share 16 rows, each taking every WAVES-th turn, and their sums are added in the waves' order.
 constexpr size_t kDirect4Lds = 64 << 10, kMostLds4 = 160 << 10;
 
 __host__ __device__ inline uint32_t direct4_row(uint32_t dim) { return (dim + 127u) / 128u * 64u + 16u; }     // (rows of a a few banks apart)
-inline size_t direct4_lds(uint32_t rows, uint32_t dim) { return size_t(rows) * direct4_row(dim) + (dim + 127) / 128 * 64 + kDirect4Waves * 64 * 16; }
+inline size_t direct4_lds(uint32_t rows, uint32_t dim, int waves) { return size_t(rows) * direct4_row(dim) + (dim + 127) / 128 * 64 + size_t(waves) * 64 * 16; }
 
-template <bool SPLIT>
-__global__ __launch_bounds__(kDirect4Threads, kDirect4Groups) void k_fp4_direct(Matmul4Args p) {
+template <bool SPLIT, int WAVES, int STEPS>
+__global__ __launch_bounds__(64 * WAVES, 4) void k_fp4_direct(Matmul4Args p) {
     extern __shared__ uint8_t smem[];
+    constexpr int kThreads = 64 * WAVES;
     const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
     const uint32_t blocks = (p.dim + 31u) / 32u, steps = (p.dim + 127u) / 128u, whole = p.dim / 128u, bytes = (p.dim + 1u) / 2u, row_bytes = direct4_row(p.dim), m = p.a.rows;
     uint32_t *const a_scales = reinterpret_cast<uint32_t *>(smem + m * row_bytes);       // [step][16]: a byte for each block of the step
     v4f *const sums = reinterpret_cast<v4f *>(a_scales + steps * 16);                    // SPLIT: [wave][lane]
-    for (uint32_t i = threadIdx.x; i < m * steps * 4u; i += kDirect4Threads) {
-        const uint32_t r = i / (steps * 4u), c = i % (steps * 4u) * 16u;
-        *reinterpret_cast<v4i *>(smem + r * row_bytes + c) = codes32(p.a.codes + size_t(r) * p.a.stride, c, p.dim);
-    }
-    for (uint32_t i = threadIdx.x; i < steps * 16u; i += kDirect4Threads)
-        a_scales[i] = scales4(p.a.scales + size_t(min(i & 15u, m - 1)) * p.a.scale_stride, (i >> 4) * 4u, blocks);
-    __syncthreads();
     // (rows past the end are the last one: their results are not stored)
     const uint8_t *const a = smem + min(uint32_t(col), m - 1) * row_bytes + g * 16;
 
-    const uint32_t tiles = (p.b.rows + 15) / 16, turns = (steps + kDirect4Steps - 1) / kDirect4Steps;
-    const uint32_t tile_stride = SPLIT ? gridDim.x : gridDim.x * kDirect4Waves, turn_stride = SPLIT ? kDirect4Waves : 1, first_turn = SPLIT ? wave : 0;
+    const uint32_t tiles = (p.b.rows + 15) / 16, turns = (steps + STEPS - 1) / STEPS;
+    const uint32_t tile_stride = SPLIT ? gridDim.x : gridDim.x * WAVES, turn_stride = SPLIT ? WAVES : 1, first_turn = SPLIT ? wave : 0;
     struct Place {
         uint32_t tile, turn;
         const uint8_t *codes, *scales;
@@ -153,19 +145,19 @@ __global__ __launch_bounds__(kDirect4Threads, kDirect4Groups) void k_fp4_direct(
         at = Place{tile, first_turn, p.b.codes + size_t(row) * p.b.stride, p.b.scales + size_t(row) * p.b.scale_stride};
     };
     struct Turn {
-        v4i codes[kDirect4Steps];
-        uint32_t scales[kDirect4Steps];
+        v4i codes[STEPS];
+        uint32_t scales[STEPS];
     };
     auto load = [&](Turn &s, const Place &at) {
         if (at.tile >= tiles || at.turn >= turns) return;
-        const uint32_t first = at.turn * kDirect4Steps;
+        const uint32_t first = at.turn * STEPS;
 #pragma unroll
-        for (int i = 0; i < kDirect4Steps; ++i) s.codes[i] = *reinterpret_cast<const v4i_any *>(at.codes + min((first + i) * 64u + uint32_t(g) * 16u, bytes - 16u));
+        for (int i = 0; i < STEPS; ++i) s.codes[i] = *reinterpret_cast<const v4i_any *>(at.codes + min((first + i) * 64u + uint32_t(g) * 16u, bytes - 16u));
         if (first * 4u + sizeof(s.scales) <= blocks) {
             __builtin_memcpy(s.scales, at.scales + first * 4u, sizeof(s.scales));
         } else {
 #pragma unroll
-            for (int i = 0; i < kDirect4Steps; ++i) s.scales[i] = (first + i) * 4u < blocks ? scales4(at.scales, (first + i) * 4u, blocks) : 0u;
+            for (int i = 0; i < STEPS; ++i) s.scales[i] = (first + i) * 4u < blocks ? scales4(at.scales, (first + i) * 4u, blocks) : 0u;
         }
     };
     v4f acc = v4f{0, 0, 0, 0};
@@ -175,8 +167,8 @@ __global__ __launch_bounds__(kDirect4Threads, kDirect4Groups) void k_fp4_direct(
     };
     auto multiply = [&](const Turn &s, const Place &at) {
 #pragma unroll
-        for (int i = 0; i < kDirect4Steps; ++i) {
-            const uint32_t k = at.turn * kDirect4Steps + i, from = k * 64u + uint32_t(g) * 16u;
+        for (int i = 0; i < STEPS; ++i) {
+            const uint32_t k = at.turn * STEPS + i, from = k * 64u + uint32_t(g) * 16u;
             if (k < whole) step(k, s.codes[i], s.scales[i]);
             else if (k < steps)               // (the row ends in this step: what was loaded are its last 16 bytes)
                 step(k, without_half(bytes_down(s.codes[i], from - min(from, bytes - 16u)), from, p.dim), s.scales[i]);
@@ -188,7 +180,7 @@ __global__ __launch_bounds__(kDirect4Threads, kDirect4Groups) void k_fp4_direct(
             __syncthreads();
             if (wave != 0) return;
 #pragma unroll
-            for (int w = 1; w < kDirect4Waves; ++w) acc += sums[w * 64 + lane];
+            for (int w = 1; w < WAVES; ++w) acc += sums[w * 64 + lane];
         }
         const uint32_t n = at.tile * 16u + uint32_t(col);
 #pragma unroll
@@ -198,8 +190,35 @@ __global__ __launch_bounds__(kDirect4Threads, kDirect4Groups) void k_fp4_direct(
     };
     Place here, next;
     Turn even, odd;
-    go_to(here, SPLIT ? blockIdx.x : blockIdx.x * kDirect4Waves + wave);
+    go_to(here, SPLIT ? blockIdx.x : blockIdx.x * WAVES + wave);
     load(even, here);
+    // a, eight runs to a thread on their way at a time, behind the first rows of b.
+    constexpr int kRuns = 8;
+    const uint32_t a_runs = m * steps * 4u;
+    for (uint32_t first = threadIdx.x; first < a_runs; first += kRuns * kThreads) {
+        v4i run[kRuns];
+        uint32_t r[kRuns], c[kRuns];
+#pragma unroll
+        for (int l = 0; l < kRuns; ++l) {
+            const uint32_t i = first + uint32_t(l * kThreads);
+            r[l] = i / (steps * 4u);
+            c[l] = i % (steps * 4u) * 16u;
+            if (i < a_runs) run[l] = *reinterpret_cast<const v4i_any *>(p.a.codes + size_t(r[l]) * p.a.stride + min(c[l], bytes - 16u));
+        }
+#pragma unroll
+        for (int l = 0; l < kRuns; ++l)
+            if (first + uint32_t(l * kThreads) < a_runs) *reinterpret_cast<v4i *>(smem + r[l] * row_bytes + c[l]) = without_half(bytes_down(run[l], c[l] - min(c[l], bytes - 16u)), c[l], p.dim);
+    }
+    for (uint32_t first = threadIdx.x; first < steps * 16u; first += 4 * kThreads) {
+        uint32_t four[4];
+#pragma unroll
+        for (int l = 0; l < 4; ++l)
+            if (const uint32_t i = first + uint32_t(l * kThreads); i < steps * 16u) four[l] = scales4(p.a.scales + size_t(min(i & 15u, m - 1)) * p.a.scale_stride, (i >> 4) * 4u, blocks);
+#pragma unroll
+        for (int l = 0; l < 4; ++l)
+            if (const uint32_t i = first + uint32_t(l * kThreads); i < steps * 16u) a_scales[i] = four[l];
+    }
+    __syncthreads();
     auto turn = [&](const Turn &now, Turn &then) {
         next = here;
         next.turn += turn_stride;
@@ -215,13 +234,13 @@ __global__ __launch_bounds__(kDirect4Threads, kDirect4Groups) void k_fp4_direct(
         turn(odd, even);
     }
 }
-template <bool SPLIT>
+template <bool SPLIT, int WAVES, int STEPS>
 static hipError_t direct4(const Matmul4Args &a, hipStream_t s) {
-    const uint32_t tiles = (a.b.rows + 15) / 16, most = SPLIT ? tiles : 256 * kDirect4Groups;
-    const uint32_t grid = SPLIT ? tiles : (tiles + kDirect4Waves - 1) / kDirect4Waves;
-    const size_t lds = direct4_lds(a.a.rows, a.dim);
-    if (const hipError_t e = allow_lds(reinterpret_cast<const void *>(k_fp4_direct<SPLIT>), lds); e != hipSuccess) return e;
-    return launch(k_fp4_direct<SPLIT>, grid < most ? grid : most, kDirect4Threads, lds, s, a);
+    const uint32_t tiles = (a.b.rows + 15) / 16, grid = SPLIT ? tiles : min((tiles + WAVES - 1) / WAVES, 256u * 16u / WAVES);
+    const size_t lds = direct4_lds(a.a.rows, a.dim, WAVES);
+    const auto kernel = k_fp4_direct<SPLIT, WAVES, STEPS>;
+    if (const hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), lds); e != hipSuccess) return e;
+    return launch(kernel, grid, 64 * WAVES, lds, s, a);
 }
 
 // Many rows of a: a workgroup to a tile of TM rows of a and TN of b, WM x WN waves, each with 32 x 32 x 64 products.  (Those reach 6.2 to 6.6 PFLOP/s on registers
@@ -557,13 +576,16 @@ static hipError_t tiled4(const Matmul4Args &a, int tile, hipStream_t s) {
 template <typename T>
 static hipError_t matmul4(const Matmul4Args &a, hipStream_t s) {
     if (a.a.rows <= 16 && a.dim >= 31) {
-        // Sixteen rows to a wave leave waves without any; shared out, one row against 4096 to 16384 of 1536 takes 4 us.  (One row against 1M of 1536 147 us, in tiles of 64 165;
-        // sixteen against 100000 19 and 20.)
-        const bool few = a.b.rows < 256 * 4 * 16;
-        if (size_t(a.a.rows) * direct4_row(a.dim) <= kDirect4Lds) return few ? direct4<true>(a, s) : direct4<false>(a, s);
-        // More of a than that leaves a compute unit one workgroup or two: as long as none waits for its turn.
-        const size_t lds = direct4_lds(a.a.rows, a.dim);
-        if (lds <= kMostLds4 && (a.b.rows + 15) / 16 <= 256 * (kMostLds4 / lds)) return direct4<true>(a, s);
+        // Sixteen rows to a wave leave waves without any; shared out over four, one row against 4096 to 16384 of 1536 takes 4 us.  (One row against 1M of 1536 141 us, in tiles of 64 165;
+        // sixteen against 100000 18 and 20.)  Over eight where a compute unit has two workgroups at most: sixteen rows against 8192 of 8192 13 us and 15 over four, 4096 of 16384 14 and 18;
+        // against 14000 of 4096 13 and 11.
+        const uint32_t groups = (a.b.rows + 15) / 16;
+        const bool few = a.b.rows < 256 * 4 * 16, wide = groups <= 512;
+        const size_t lds = direct4_lds(a.a.rows, a.dim, wide ? 8 : 4);
+        // (More of a than 64 KB leaves a compute unit one workgroup or two: as long as none waits for its turn.)
+        const bool fits = size_t(a.a.rows) * direct4_row(a.dim) <= kDirect4Lds;
+        if (fits && !few) return direct4<false, 4, 2>(a, s);
+        if (fits || (lds <= kMostLds4 && groups <= 256 * (kMostLds4 / lds))) return wide ? direct4<true, 8, 2>(a, s) : direct4<true, 4, 4>(a, s);
     }
     if (a.dim < 31 || a.a.stride >= kMostTileStride4 || a.b.stride >= kMostTileStride4) return small4<T>(a, s);
     double whole = 0;
