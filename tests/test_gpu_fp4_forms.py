@@ -1,5 +1,5 @@
 """Every form of the 4-bit product -- rows of b streamed past those of a, 16 of them to a wave or shared out over four or eight; tiles of five sizes, a last round's columns in
-smaller ones; rows too short or too far apart for those -- into each type, over rows that start anywhere, last tiles that are partly empty and last blocks that
+smaller ones, small tiles whose waves share the stages; rows too short or too far apart for those -- into each type, over rows that start anywhere, last tiles that are partly empty and last blocks that
 are odd."""
 import pytest
 
@@ -9,7 +9,9 @@ DTYPES = [torch.float32, torch.float16, torch.bfloat16]
 TILES = {(256, 256): (1, 1.44, 4.3, 1.4), (128, 128): (2, 0.59, 0.34, 0.42), (64, 64): (4, 0.23, 0.24, 0.14), (64, 128): (3, 0.39, 0.18, 0.3), (32, 128): (3, 0.27, 0.33, 0.19)}
 SIZES = [(5, 400), (7, 9000), (16, 17_001), (17, 5000), (20, 70_003), (257, 3001), (700, 6001), (1030, 13_007), (300, 40_001), (1030, 44_001)]
 DIMS = [201, 385, 1500]
-LONG = [(16, 700, 8199, "over eight"), (16, 9001, 8199, "tile")]          # rows of a that take most of a compute unit's LDS
+LONG = [(16, 700, 8199, "over eight"), (16, 9001, 8199, "tile"),          # rows of a that take most of a compute unit's LDS
+        (17, 1000, 1793, "shared 32"), (40, 90, 2048, "shared 32"), (300, 700, 2049, "shared 32"), (33, 64, 2303, "shared 32"), (32, 1000, 2304, "shared 32"), (17, 31, 4100, "shared 32"),
+        (64, 5001, 1281, "shared 64"), (64, 5001, 2048, "shared 64"), (130, 2500, 1537, "shared 64"), (70, 3333, 2303, "shared 64"), (128, 4000, 2305, "shared 64")]
 
 
 def form(m, n, dim, size):
@@ -34,6 +36,10 @@ def form(m, n, dim, size):
             return "over eight" if wide else "over four"
     if dim < 31:
         return "small"
+    if dim > 7 * 256 and -(-m // 32) * -(-n // 32) <= 256:
+        return "shared 32"
+    if dim > 5 * 256 and -(-m // 64) * -(-n // 32) <= 256:
+        return "shared 64"
     tile, mt, nt = best(n), -(-m // 256), -(-n // 256)
     if tile == (256, 256) and mt * nt > 256 and nt >= mt:
         columns = mt * nt // 256 * 256 // mt * 256
@@ -46,7 +52,7 @@ def form(m, n, dim, size):
 
 def test_sizes_reach_every_form():
     reached = {form(m, n, dim, size) for m, n in SIZES for dim in DIMS for size in (2, 4)}
-    assert {"over eight", "over four", "streamed", *TILES} <= reached, reached
+    assert {"over eight", "over four", "streamed", "shared 64", *TILES} <= reached, reached
     assert any(isinstance(f[0], tuple) for f in reached), reached
     for m, n, dim, what in LONG:
         assert (form(m, n, dim, 4) if what != "tile" else "tile" if form(m, n, dim, 4) in TILES else "") == what
@@ -126,3 +132,16 @@ def test_rows_eight_megabytes_apart(m, n, dim):
     for far in ((1 << 23) - 1, 1 << 23, (1 << 23) + 5):
         check(fp4, m, n, dim, (far, (dim + 1) // 2))
         check(fp4, m, n, dim, ((dim + 1) // 2, far))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,dim,what", [(17, 150, 2100, "shared 32"), (64, 4200, 1600, "shared 64"), (9, 5000, 4097, "over eight"), (12, 9000, 1000, "over four")])
+def test_nan_stays_in_its_row(m, n, dim, what):
+    """Whichever waves have the block that it stands in, and wherever a row ends."""
+    from turbovec_amd import fp4
+    assert form(m, n, dim, 4) == what
+    x, y = (torch.randn(r, dim, generator=torch.Generator(device="cuda").manual_seed(r), device="cuda") for r in (m, n))
+    x[1, dim - 1], x[3, 300], y[5, 40], y[n - 1, 0], y[20, dim - 1] = float("nan"), float("inf"), float("inf"), float("nan"), float("inf")
+    want = torch.zeros(m, n, dtype=torch.bool, device="cuda")
+    want[[1, 3]], want[:, [5, 20, n - 1]] = True, True
+    assert torch.equal(torch.isnan(fp4.matmul(fp4.quantize(x), fp4.quantize(y))), want)

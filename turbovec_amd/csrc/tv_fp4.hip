@@ -310,8 +310,8 @@ __device__ __forceinline__ void store_strips4(const Matmul4Args &p, const v16f (
     }
 }
 
-template <typename T, int TM, int TN, int WM, int WN, int HELD>
-__global__ __launch_bounds__(64 * WM * WN, HELD) void k_fp4_tile(Matmul4Args p, uint32_t m_tiles, uint32_t n_tiles, uint32_t each_xcd, bool stream) {
+template <typename T, int TM, int TN, int WM, int WN, int HELD, int KS>
+__global__ __launch_bounds__(64 * WM * WN * KS, (HELD * KS * WM * WN + 3) / 4) void k_fp4_tile(Matmul4Args p, uint32_t m_tiles, uint32_t n_tiles, uint32_t each_xcd, bool stream) {
     extern __shared__ uint8_t smem[];
     constexpr int kWaves = WM * WN, kThreads = 64 * kWaves, kRows = TM + TN, kGroups = kRows / 8 / kWaves, MT = TM / WM / 32, NT = TN / WN / 32;
     constexpr uint32_t kBuffer = kRows * kStageBytes4;
@@ -328,9 +328,13 @@ __global__ __launch_bounds__(64 * WM * WN, HELD) void k_fp4_tile(Matmul4Args p, 
         tn = in / high;
     }
     const uint32_t m0 = tm * TM, n0 = tn * TN;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)), row32 = lane & 31, half = lane >> 5;
+    const int lane = threadIdx.x & 63, all_waves = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)), wave = all_waves % kWaves, row32 = lane & 31, half = lane >> 5;
     const uint32_t blocks = (p.dim + 31u) / 32u, stages = (p.dim + kStage4 - 1) / kStage4, whole = p.dim / kStage4, bytes = (p.dim + 1u) / 2u;
-    uint32_t *const scales = reinterpret_cast<uint32_t *>(smem + 2 * kBuffer);                  // [buffer][even or odd blocks][row]
+    // KS groups of waves, with LDS of their own, take every KS-th stage; where a group has one less it multiplies zeros.
+    const uint32_t group = uint32_t(all_waves / kWaves), thread = threadIdx.x % kThreads, turns = (stages + KS - 1) / KS;
+    auto stage = [&](uint32_t k) { return KS == 1 ? k : k * KS + group; };
+    uint8_t *const mine = smem + group * uint32_t(tile4_lds<TM, TN>());
+    uint32_t *const scales = reinterpret_cast<uint32_t *>(mine + 2 * kBuffer);                  // [buffer][even or odd blocks][row]
 
     // Of the rows of a and, after them, of b, wave w has groups of eight w, w + kWaves, ...: lane l row l / 8 of the group, run l % 8.
     // (Rows past the end are the last one: their results are not stored.)
@@ -343,12 +347,12 @@ __global__ __launch_bounds__(64 * WM * WN, HELD) void k_fp4_tile(Matmul4Args p, 
         offset[i] = i * kWaves * 8 < TM ? min(row, p.a.rows - 1 - m0) * uint32_t(p.a.stride) : min(row - TM, p.b.rows - 1 - n0) * uint32_t(p.b.stride);
     }
     v4i held[kGroups];
-    // (A run that the row ends in or before is the row's last 16 bytes, for ending() to put right; behind the last stage nobody looks.)
+    // (A run that the row ends in or before is the row's last 16 bytes, for ending() to put right.)
     auto load_group = [&](uint32_t k, auto i) {
         constexpr int I = decltype(i)::value;
-        held[I] = *reinterpret_cast<const v4i_any *>((I * kWaves * 8 < TM ? a0 : b0) + (offset[I] + min(k * kStageBytes4 + run16, bytes - 16u)));
+        held[I] = *reinterpret_cast<const v4i_any *>((I * kWaves * 8 < TM ? a0 : b0) + (offset[I] + min(stage(k) * kStageBytes4 + run16, bytes - 16u)));
     };
-    uint8_t *const my_run = smem + uint32_t(wave) * 1024u + uint32_t(lane >> 3) * kStageBytes4 + uint32_t((lane & 7) ^ (lane >> 3)) * 16u;
+    uint8_t *const my_run = mine + uint32_t(wave) * 1024u + uint32_t(lane >> 3) * kStageBytes4 + uint32_t((lane & 7) ^ (lane >> 3)) * 16u;
     auto put_group = [&](uint32_t k, auto i) {
         constexpr int I = decltype(i)::value;
         *reinterpret_cast<v4i *>(my_run + (k & 1u) * kBuffer + I * kWaves * 1024) = held[I];
@@ -360,7 +364,7 @@ __global__ __launch_bounds__(64 * WM * WN, HELD) void k_fp4_tile(Matmul4Args p, 
     const uint32_t last_eight = blocks >= 8u ? blocks - 8u : 0u;
 #pragma unroll
     for (int i = 0; i < kScaleRounds; ++i) {
-        const uint32_t row = min(uint32_t(i * kThreads) + threadIdx.x, uint32_t(kRows - 1));
+        const uint32_t row = min(uint32_t(i * kThreads) + thread, uint32_t(kRows - 1));
         scale_row[i] = row < uint32_t(TM) ? p.a.scales + size_t(min(m0 + row, p.a.rows - 1)) * p.a.scale_stride : p.b.scales + size_t(min(n0 + row - TM, p.b.rows - 1)) * p.b.scale_stride;
         // (rows of fewer than eight blocks have one stage)
         held_scales[i] = 0;
@@ -370,12 +374,12 @@ __global__ __launch_bounds__(64 * WM * WN, HELD) void k_fp4_tile(Matmul4Args p, 
     }
     auto load_scales = [&](uint32_t k) {
 #pragma unroll
-        for (int i = 0; i < kScaleRounds; ++i) __builtin_memcpy(&held_scales[i], scale_row[i] + min(k * 8u, last_eight), 8);
+        for (int i = 0; i < kScaleRounds; ++i) __builtin_memcpy(&held_scales[i], scale_row[i] + min(stage(k) * 8u, last_eight), 8);
     };
     auto put_scales = [&](uint32_t k) {
 #pragma unroll
         for (int i = 0; i < kScaleRounds; ++i) {
-            const uint32_t row = uint32_t(i * kThreads) + threadIdx.x, lo = uint32_t(held_scales[i]), hi = uint32_t(held_scales[i] >> 32);
+            const uint32_t row = uint32_t(i * kThreads) + thread, lo = uint32_t(held_scales[i]), hi = uint32_t(held_scales[i] >> 32);
             if (kRows % kThreads != 0 && row >= uint32_t(kRows)) continue;
             uint32_t *const to = scales + (k & 1u) * 2 * kRows + row;
             to[0] = __builtin_amdgcn_perm(hi, lo, 0x06040200u);
@@ -383,13 +387,13 @@ __global__ __launch_bounds__(64 * WM * WN, HELD) void k_fp4_tile(Matmul4Args p, 
         }
     };
     // The stage that rows end in, as it stands in registers: runs moved down to where they belong, zeros behind the end, scales too (2^-127, of codes that are 0).
-    auto ending = [&] {
-        const uint32_t from = whole * kStageBytes4 + run16;
+    auto ending = [&](uint32_t at) {
+        const uint32_t from = at * kStageBytes4 + run16;
 #pragma unroll
         for (int i = 0; i < kGroups; ++i) held[i] = without_half(bytes_down(held[i], from - min(from, bytes - 16u)), from, p.dim);
         if (blocks >= 8u) {
 #pragma unroll
-            for (int i = 0; i < kScaleRounds; ++i) held_scales[i] >>= 8u * (whole * 8u - min(whole * 8u, last_eight));
+            for (int i = 0; i < kScaleRounds; ++i) held_scales[i] = at * 8u >= blocks ? 0u : held_scales[i] >> (8u * (at * 8u - min(at * 8u, last_eight)));
         }
     };
 
@@ -408,7 +412,7 @@ __global__ __launch_bounds__(64 * WM * WN, HELD) void k_fp4_tile(Matmul4Args p, 
     struct Scales {
         int a[MT], b[NT];
     };
-    const uint8_t *const my_a = smem + (wm + row32) * kStageBytes4, *const my_b = smem + (TM + wn + row32) * kStageBytes4;
+    const uint8_t *const my_a = mine + (wm + row32) * kStageBytes4, *const my_b = mine + (TM + wn + row32) * kStageBytes4;
     // What goes on between a step's products, in front of each a part: reads of the next step's operands, in the order that it wants them, of the next stage's scales, stores
     // into LDS and loads.  (A wave has its SIMD alone in the largest tiles: between two products it can give a handful of instructions; more of them in one place
     // leave the matrix unit idle.)
@@ -460,7 +464,7 @@ __global__ __launch_bounds__(64 * WM * WN, HELD) void k_fp4_tile(Matmul4Args p, 
     Scales sc, sc_next;
     static_for<kGroups>([&](auto i) { load_group(0, i); });
     if (blocks >= 8u) load_scales(0);
-    if (whole == 0) ending();
+    if (stage(0) >= whole) ending(stage(0));
     static_for<kGroups>([&](auto i) {
         put_group(0, i);
         load_group(1, i);
@@ -474,8 +478,8 @@ __global__ __launch_bounds__(64 * WM * WN, HELD) void k_fp4_tile(Matmul4Args p, 
         read_scales(sc, 0, i);
     }
 #pragma unroll 1
-    for (uint32_t k = 0; k < stages; ++k) {
-        if (k + 1 == whole) ending();      // (where rows end with a stage, nobody looks at the next)
+    for (uint32_t k = 0; k < turns; ++k) {
+        if (KS == 1 ? k + 1 == whole : stage(k + 1) >= whole) ending(stage(k + 1));      // (where rows end with a stage, nobody looks at the next)
         // (The same for every stage, without a branch: across one the compiler moves products about.  Behind the last stage what is loaded and read is not used.)
         multiply(even, sc, IntC<0>{}, [&](int slot) {
             read(odd, k, 1, slot);
@@ -497,6 +501,28 @@ __global__ __launch_bounds__(64 * WM * WN, HELD) void k_fp4_tile(Matmul4Args p, 
         sc = sc_next;
     }
     __syncthreads();
+    if constexpr (KS > 1) {          // (the groups' sums, added in their order)
+        float *const sums = reinterpret_cast<float *>(smem + tile4_lds<TM, TN>());
+        constexpr uint32_t kEach = MT * NT * 16;
+        if (group != 0) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sums[((group - 1) * kEach + uint32_t((i * NT + j) * 16 + r)) * kThreads + thread] = acc[i][j][r];
+        }
+        __syncthreads();
+        if (group != 0) return;
+#pragma unroll
+        for (int g = 1; g < KS; ++g)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[i][j][r] += sums[(uint32_t(g - 1) * kEach + uint32_t((i * NT + j) * 16 + r)) * kThreads + thread];
+    }
     uint8_t *const strip = smem + wave * kStrip4<T, TN / WN>;
     if (stream) store_strips4<T, true, TN / WN, MT, NT>(p, acc, strip, m0 + wm, n0 + wn, lane);
     else store_strips4<T, false, TN / WN, MT, NT>(p, acc, strip, m0 + wm, n0 + wn, lane);
@@ -505,13 +531,14 @@ __global__ __launch_bounds__(64 * WM * WN, HELD) void k_fp4_tile(Matmul4Args p, 
 // Results of rows below this leave past the L2: they would push out what other tiles read there.  (1024 by 100000 of 1536 into floats 148 us so and 170 to 185 otherwise;
 // 4096 by 16384 of 4096 175 and 170.)
 constexpr uint32_t kStreamDim4 = 2048;
-template <typename T, int TM, int TN, int WM, int WN, int HELD>
+template <typename T, int TM, int TN, int WM, int WN, int HELD, int KS = 1>
 static hipError_t tile4(const Matmul4Args &a, hipStream_t s) {
     const uint64_t mt = (a.a.rows + TM - 1) / TM, nt = (a.b.rows + TN - 1) / TN, each_xcd = (mt * nt + 7) / 8;
-    if ((each_xcd * 8 * (64 * WM * WN)) >> 32) return hipErrorInvalidConfiguration;      // (a result of hundreds of GB, or a narrow one of a billion columns)
-    const auto kernel = k_fp4_tile<T, TM, TN, WM, WN, HELD>;
-    if (const hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), tile4_lds<TM, TN>()); e != hipSuccess) return e;
-    return launch(kernel, uint32_t(each_xcd * 8), 64 * WM * WN, tile4_lds<TM, TN>(), s, a, uint32_t(mt), uint32_t(nt), uint32_t(each_xcd), a.dim < kStreamDim4);
+    if ((each_xcd * 8 * (64 * WM * WN * KS)) >> 32) return hipErrorInvalidConfiguration;      // (a result of hundreds of GB, or a narrow one of a billion columns)
+    const auto kernel = k_fp4_tile<T, TM, TN, WM, WN, HELD, KS>;
+    constexpr size_t kLds = KS * tile4_lds<TM, TN>();
+    if (const hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), kLds); e != hipSuccess) return e;
+    return launch(kernel, uint32_t(each_xcd * 8), 64 * WM * WN * KS, kLds, s, a, uint32_t(mt), uint32_t(nt), uint32_t(each_xcd), a.dim < kStreamDim4);
 }
 
 // Rows of fewer than 16 bytes, or 8 MB and more apart: a wave to a tile of 16 by 16, its operands read where they lie.
@@ -588,6 +615,12 @@ static hipError_t matmul4(const Matmul4Args &a, hipStream_t s) {
         if (fits || (lds <= kMostLds4 && groups <= 256 * (kMostLds4 / lds))) return wide ? direct4<true, 8, 2>(a, s) : direct4<true, 4, 4>(a, s);
     }
     if (a.dim < 31 || a.a.stride >= kMostTileStride4 || a.b.stride >= kMostTileStride4) return small4<T>(a, s);
+    // Few tiles leave compute units idle, and one alone takes in no more than 25 to 50 GB a second: smaller ones, whose stages groups of waves share.  (64 rows against 8192 of 8192 10.9 us so and 14.5 in tiles of
+    // 64, 32 against 4096 of 16384 11.4 and 24.6, 17 against 4096 of 4096 5.4 and 8.3, 128 against 4096 of 4096 6.9 and 8.6; two tiles to a compute unit, 64 against 16384 of 8192, 17.3 and 15.8.)
+    const uint32_t stages = (a.dim + kStage4 - 1) / kStage4;
+    const auto tiles4 = [&](uint32_t tm, uint32_t tn) { return uint64_t((a.a.rows + tm - 1) / tm) * ((a.b.rows + tn - 1) / tn); };
+    if (stages >= 8 && tiles4(32, 32) <= 256) return tile4<T, 32, 32, 1, 1, 2, 4>(a, s);
+    if (stages >= 6 && tiles4(64, 32) <= 256) return tile4<T, 64, 32, 2, 1, 2, 2>(a, s);
     double whole = 0;
     const int tile = best_tile4(a.a.rows, a.b.rows, a.dim, sizeof(T), whole);
     const uint32_t mt = (a.a.rows + 255) / 256, nt = (a.b.rows + 255) / 256;
