@@ -597,7 +597,7 @@ static hipError_t tiled4(const Matmul4Args &a, int tile, hipStream_t s) {
     if (tile == 0) return tile4<T, 256, 256, 2, 2, 1>(a, s);
     if (tile == 1) return tile4<T, 128, 128, 2, 2, 2>(a, s);
     if (tile == 2) return tile4<T, 64, 64, 2, 2, 4>(a, s);
-    return tile == 3 ? tile4<T, 64, 128, 2, 2, 3>(a, s) : tile4<T, 32, 128, 1, 4, 3>(a, s);
+    return tile == 3 ? tile4<T, 64, 128, 1, 4, 3>(a, s) : tile4<T, 32, 128, 1, 4, 3>(a, s);
 }
 
 template <typename T>
