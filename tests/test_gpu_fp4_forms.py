@@ -7,7 +7,7 @@ torch = pytest.importorskip("torch")
 
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
 TILES = {(256, 256): (1, 1.44, 4.3, 1.4), (128, 128): (2, 0.59, 0.34, 0.42), (64, 64): (4, 0.23, 0.24, 0.14), (64, 128): (3, 0.39, 0.18, 0.3), (32, 128): (3, 0.27, 0.33, 0.19)}
-SIZES = [(5, 400), (7, 9000), (16, 17_001), (17, 5000), (20, 70_003), (257, 3001), (700, 6001), (1030, 13_007), (300, 40_001), (1030, 44_001)]
+SIZES = [(5, 400), (7, 9000), (16, 17_001), (17, 5000), (20, 70_003), (257, 3001), (700, 6001), (700, 6016), (1030, 13_007), (300, 40_001), (1030, 44_001)]
 DIMS = [201, 385, 1500]
 LONG = [(16, 700, 8199, "over eight"), (16, 9001, 8199, "tile"),          # rows of a that take most of a compute unit's LDS
         (17, 1000, 1793, "shared 32"), (40, 90, 2048, "shared 32"), (300, 700, 2049, "shared 32"), (33, 64, 2303, "shared 32"), (32, 1000, 2304, "shared 32"), (17, 31, 4100, "shared 32"),

@@ -258,9 +258,11 @@ constexpr size_t kMostTileStride4 = size_t(1) << 23;      // a tile's offsets ha
 template <int TM, int TN> constexpr size_t tile4_lds() { return 2 * size_t(TM + TN) * (kStageBytes4 + 8); }
 template <typename T, int COLS> constexpr int kStrip4 = 32 * (COLS * int(sizeof(T)) + 16);
 
+// Ways of results to memory: through the L2, past it with eight of a wave's reads from LDS on their way, past it one read and one store after the other.
+enum { kThroughL2 = 0, kPastL2 = 1, kPaced = 2 };
 // A wave's results, whose lane l holds, of row l % 32 of each tile, columns 8 q + 4 (l / 32) .. + 3, to rows from m on and columns from n on: 32 rows at a time
 // through LDS, so that they leave in runs of whole cache lines.
-template <typename T, bool STREAM, int COLS, int MT, int NT>
+template <typename T, int WAY, int COLS, int MT, int NT>
 __device__ __forceinline__ void store_strips4(const Matmul4Args &p, const v16f (&acc)[MT][NT], uint8_t *strip, uint32_t m, uint32_t n, int lane) {
     typedef T T4 __attribute__((ext_vector_type(4)));
     constexpr int kEach = 16 / int(sizeof(T)), kLanes = COLS / kEach, kRowsAtOnce = 64 / kLanes, kRow = COLS * int(sizeof(T)) + 16;
@@ -278,6 +280,26 @@ __device__ __forceinline__ void store_strips4(const Matmul4Args &p, const v16f (
         const uint32_t at = uint32_t(lane % kLanes * kEach), on = n + at;
         const T *const from = reinterpret_cast<const T *>(strip + lane / kLanes * kRow) + at;
         constexpr int kRounds = 32 / kRowsAtOnce, kTogether = kRounds < 8 ? kRounds : 8;
+        if constexpr (WAY == kPaced) {
+            const uint32_t first = m + uint32_t(i * 32 + lane / kLanes);
+            const bool whole = on + kEach <= p.b.rows;
+            T *to = static_cast<T *>(p.out) + size_t(first) * p.out_stride + on;
+#pragma unroll
+            for (int r = 0; r < kRounds; ++r) {
+                if (inside || (whole && first + uint32_t(r * kRowsAtOnce) < p.a.rows))
+                    __builtin_nontemporal_store(*reinterpret_cast<const v4i *>(reinterpret_cast<const uint8_t *>(from) + r * kRowsAtOnce * kRow), reinterpret_cast<v4i_any *>(to));
+                to += kRowsAtOnce * p.out_stride;
+            }
+            if (inside || whole || on >= p.b.rows) continue;
+#pragma unroll 1
+            for (uint32_t r = 0; r < 32 && first + r < p.a.rows; r += kRowsAtOnce) {          // (the last columns, fewer than a lane stores at once)
+                const T *const x = reinterpret_cast<const T *>(reinterpret_cast<const uint8_t *>(from) + r * kRow);
+                T *const row = static_cast<T *>(p.out) + size_t(first + r) * p.out_stride + on;
+#pragma unroll 1
+                for (uint32_t l = 0; on + l < p.b.rows; ++l) row[l] = x[l];
+            }
+            continue;
+        }
         if (inside) {          // (a wave waits for eight reads once, not for each of them)
             T *to = static_cast<T *>(p.out) + size_t(m + uint32_t(i * 32 + lane / kLanes)) * p.out_stride + on;
 #pragma unroll
@@ -287,7 +309,7 @@ __device__ __forceinline__ void store_strips4(const Matmul4Args &p, const v16f (
                 for (int l = 0; l < kTogether; ++l) x[l] = *reinterpret_cast<const v4i *>(reinterpret_cast<const uint8_t *>(from) + (r + l) * kRowsAtOnce * kRow);
 #pragma unroll
                 for (int l = 0; l < kTogether; ++l) {
-                    if constexpr (STREAM) __builtin_nontemporal_store(x[l], reinterpret_cast<v4i_any *>(to));
+                    if constexpr (WAY == kPastL2) __builtin_nontemporal_store(x[l], reinterpret_cast<v4i_any *>(to));
                     else *reinterpret_cast<v4i_any *>(to) = x[l];
                     to += kRowsAtOnce * p.out_stride;
                 }
@@ -311,7 +333,7 @@ __device__ __forceinline__ void store_strips4(const Matmul4Args &p, const v16f (
 }
 
 template <typename T, int TM, int TN, int WM, int WN, int HELD, int KS>
-__global__ __launch_bounds__(64 * WM * WN * KS, (HELD * KS * WM * WN + 3) / 4) void k_fp4_tile(Matmul4Args p, uint32_t m_tiles, uint32_t n_tiles, uint32_t each_xcd, bool stream) {
+__global__ __launch_bounds__(64 * WM * WN * KS, (HELD * KS * WM * WN + 3) / 4) void k_fp4_tile(Matmul4Args p, uint32_t m_tiles, uint32_t n_tiles, uint32_t each_xcd, int way) {
     extern __shared__ uint8_t smem[];
     constexpr int kWaves = WM * WN, kThreads = 64 * kWaves, kRows = TM + TN, kGroups = kRows / 8 / kWaves, MT = TM / WM / 32, NT = TN / WN / 32;
     constexpr uint32_t kBuffer = kRows * kStageBytes4;
@@ -524,21 +546,25 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (HELD * KS * WM * WN + 3) / 4) v
                     for (int r = 0; r < 16; ++r) acc[i][j][r] += sums[(uint32_t(g - 1) * kEach + uint32_t((i * NT + j) * 16 + r)) * kThreads + thread];
     }
     uint8_t *const strip = smem + wave * kStrip4<T, TN / WN>;
-    if (stream) store_strips4<T, true, TN / WN, MT, NT>(p, acc, strip, m0 + wm, n0 + wn, lane);
-    else store_strips4<T, false, TN / WN, MT, NT>(p, acc, strip, m0 + wm, n0 + wn, lane);
+    if (way == kPaced) store_strips4<T, kPaced, TN / WN, MT, NT>(p, acc, strip, m0 + wm, n0 + wn, lane);
+    else if (way == kPastL2) store_strips4<T, kPastL2, TN / WN, MT, NT>(p, acc, strip, m0 + wm, n0 + wn, lane);
+    else store_strips4<T, kThroughL2, TN / WN, MT, NT>(p, acc, strip, m0 + wm, n0 + wn, lane);
 }
 
-// Results of rows below this leave past the L2: they would push out what other tiles read there.  (1024 by 100000 of 1536 into floats 148 us so and 170 to 185 otherwise;
-// 4096 by 16384 of 4096 175 and 170.)
-constexpr uint32_t kStreamDim4 = 2048;
+// Results of rows below kStreamDim4 leave past the L2: they would push out what other tiles read there.  (1024 by 98304 of 1536 into floats 139 us, through it 153; 4096 by 16384 of 4096 175
+// and 170.)  Where the result's rows start in the middle of a cache line and there is little to do between two tiles' results, a wave gives eight stores at a time (1000 by 50001 of 768 into floats 55 us
+// and 86, into bfloat16 46 and 63; 1024 by 100001 of 1536 191 and 182, 163 and 137; rows at whole lines, 1024 by 98304 of 1536, 155 and 139).
+constexpr uint32_t kStreamDim4 = 2048, kPacedDim4 = 1280;
 template <typename T, int TM, int TN, int WM, int WN, int HELD, int KS = 1>
 static hipError_t tile4(const Matmul4Args &a, hipStream_t s) {
     const uint64_t mt = (a.a.rows + TM - 1) / TM, nt = (a.b.rows + TN - 1) / TN, each_xcd = (mt * nt + 7) / 8;
     if ((each_xcd * 8 * (64 * WM * WN * KS)) >> 32) return hipErrorInvalidConfiguration;      // (a result of hundreds of GB, or a narrow one of a billion columns)
+    const bool lines = (a.out_stride * sizeof(T) % 64 | reinterpret_cast<uintptr_t>(a.out) % 64) == 0;
+    const int way = a.dim >= kStreamDim4 ? kThroughL2 : lines || TM < 128 || a.dim >= kPacedDim4 ? kPaced : kPastL2;
     const auto kernel = k_fp4_tile<T, TM, TN, WM, WN, HELD, KS>;
     constexpr size_t kLds = KS * tile4_lds<TM, TN>();
     if (const hipError_t e = allow_lds(reinterpret_cast<const void *>(kernel), kLds); e != hipSuccess) return e;
-    return launch(kernel, uint32_t(each_xcd * 8), 64 * WM * WN * KS, kLds, s, a, uint32_t(mt), uint32_t(nt), uint32_t(each_xcd), a.dim < kStreamDim4);
+    return launch(kernel, uint32_t(each_xcd * 8), 64 * WM * WN * KS, kLds, s, a, uint32_t(mt), uint32_t(nt), uint32_t(each_xcd), way);
 }
 
 // Rows of fewer than 16 bytes, or 8 MB and more apart: a wave to a tile of 16 by 16, its operands read where they lie.
