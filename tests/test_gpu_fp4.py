@@ -359,3 +359,13 @@ def test_more_rows_than_a_grid_has(fp4):
     near = (v - x).abs()
     assert float(near[:1000].max()) <= 1 and float(near[-1000:].max()) <= 1 and float(near.max()) <= 1
     assert bool((v[-1000:] != 0)[x[-1000:] != 0].all())
+
+
+def test_a_result_past_four_gigabytes(fp4):
+    """Rows of one block, whose sums are exact in every form: the same wherever in the result they stand."""
+    m, n = 70_001, 40_000
+    a, b = fp4.quantize(wild(m, 32, 30, 2)), fp4.quantize(wild(n, 32, 31, 2))
+    got = fp4.matmul(a, b, dtype=torch.bfloat16)
+    for i in (0, 26_843, 53_687, m - 1):
+        row = fp4.Fp4Rows(a.codes[i:i + 1], a.scales[i:i + 1])
+        assert torch.equal(got[i:i + 1], fp4.matmul(row, b, dtype=torch.bfloat16))
