@@ -11,7 +11,7 @@ namespace tv {
 // the largest code, 6, and what would be the next, 8, so that the largest value is rounded as the others are.
 // ---------------------------------------------------------------------------
 
-// A thread to eight coordinates, four neighbours to a block.
+// A thread to eight coordinates, four neighbours to a block.  Bound by memory: 400000 rows of 1536 floats 482 to 520 us, 5.3 to 5.8 TB/s, an eighth of it written; of bfloat16 286 to 327, 5.0 to 5.4.
 constexpr int kThreads4 = 256;
 template <typename T>
 __global__ __launch_bounds__(kThreads4) void k_fp4_quantize(Quantize4Args a) {
@@ -38,6 +38,7 @@ hipError_t launch_fp4_quantize(const Quantize4Args &a, int x_type, hipStream_t s
     return x_type == kF16 ? launch(k_fp4_quantize<f16>, grid, kThreads4, 0, s, a) : launch(k_fp4_quantize<bf16>, grid, kThreads4, 0, s, a);
 }
 
+// (400000 rows of 1536 into bfloat16 291 to 300 us, 5.2 TB/s, four fifths of it written.)
 template <typename T>
 __global__ __launch_bounds__(kThreads4) void k_fp4_values(Values4Args a) {
     typedef T T8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
