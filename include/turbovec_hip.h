@@ -313,7 +313,8 @@ int tv_rms_norm_dev(int device, void *stream, const void *d_x, int x_type, size_
                     int row_kind, int scale_type, uint8_t *d_codes, size_t code_stride, void *d_scales, size_t scale_stride);
 
 /* Log probabilities under a softmax of rows of n scores, divided by a temperature a row (NULL: 1; one that is not above 0 is the limit
- * from above, the best slots share the mass).  Slots whose mask bit is not set (d_mask_words NULL: all are; mask_stride 0: one mask for all rows) and slots of score
+ * from above, the best slots share the mass; an infinite one gives all slots that have a probability the same).  A score that is 2^128 or more below the row's largest
+ * has probability 0 at every temperature.  Slots whose mask bit is not set (d_mask_words NULL: all are; mask_stride 0: one mask for all rows) and slots of score
  * -infinity have probability 0, whatever else stands there.  For each row: out_log_probs, of the `given` slots in d_slots (-infinity for a slot of
  * probability 0 or outside 0 .. n - 1; the same slot may stand there twice); out_entropy, -sum p log p; the `top` slots of the highest scores,
  * ties to the lower slot, with their log probabilities (slot -1, -infinity where fewer have a probability; a NaN is not among them).  given and top are at

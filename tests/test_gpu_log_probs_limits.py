@@ -1,0 +1,54 @@
+"""Log probabilities where a parameter or a score is at its limit, in every form that a call may take."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+from test_gpu_log_probs import DTYPES, INF, U, check, check_gradient, gen, log_probs, scores_of, slots_of  # noqa: E402, F401
+
+# A wave to a row, workgroups of 256 and of 1024 threads, rows in parts; rows that end with a load of all types, and rows that do not.
+FORMS = [(5, 1), (5, 7), (3, 1003), (3, 1008), (1030, 333), (1030, 1000), (1030, 2500), (2, 20_001), (200, 9003), (300, 9003), (2, 300_001), (2, 300_032)]
+
+
+@pytest.mark.parametrize("rows,n", FORMS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_an_infinite_temperature(log_probs, rows, n, dtype):  # noqa: F811
+    """Slots that have a probability share the mass, whatever is masked, -infinity or behind the row's end; the gradient is 0.  (A sum of equal terms loses what its additions do: log S is off by no more than
+    check allows, and a hundred roundings; the logarithm by two of itself.)"""
+    scores, slots = scores_of(rows, n, dtype, 70), slots_of(rows, n, 2)
+    t = torch.full((rows,), INF, device="cuda")
+    scores[0, n // 2] = -INF
+    slots[:, 0] = n // 2
+    check(log_probs, scores, slots, temperature=t, top=3)
+    check_gradient(log_probs, scores, slots, temperature=t)
+    allowed = torch.rand(rows, n, generator=gen(71), device="cuda") < 0.5
+    allowed[rows - 1] = False
+    allowed[rows - 1, n - 1] = True
+    allowed[1] = False
+    found = check(log_probs, scores, slots, temperature=INF, allowed=allowed, top=3)
+    there = (allowed & (scores > -INF)).sum(1).double()
+    want = torch.where(there > 0, there.log(), 0.0)
+    assert bool(((found.entropy.double() - want).abs() <= (100 + 2 * want) * U).all())
+    check_gradient(log_probs, scores, slots, temperature=t, allowed=allowed)
+    if rows > 2:                                       # beside rows of other temperatures
+        t[1::2] = 0.7
+        check(log_probs, scores, slots, temperature=t, allowed=allowed, top=3)
+        check_gradient(log_probs, scores, slots, temperature=t, allowed=allowed)
+
+
+def test_the_largest_temperatures(log_probs):  # noqa: F811
+    """Scores as far apart as 32 bits hold, at temperatures whose inverse is no normal number; what lies further from the best has no probability."""
+    low, high = torch.finfo(torch.float32).min, torch.finfo(torch.float32).max
+    scores = torch.tensor([[0.0, low / 2, low, -1.0, 0.0]] * 4, device="cuda")
+    slots = torch.arange(5, device="cuda").expand(4, 5).contiguous()
+    t = torch.tensor([high, 1e38, 2.0 ** 126, INF], device="cuda")
+    check(log_probs, scores[:3], slots[:3], temperature=t[:3], top=5)
+    found = log_probs(scores, slots, temperature=t)
+    assert float((found.log_probs[3] + math.log(5)).abs().max()) <= 2.0 ** -20          # (the smallest factor times the largest distance is 2^-21)
+    scores = torch.tensor([[high, low, high]], device="cuda")
+    for temperature in (1.0, INF):
+        found = log_probs(scores, slots[:1, :3].contiguous(), temperature=temperature, top=3)
+        assert float(found.log_probs[0, 1]) == -INF and float((found.log_probs[0, ::2] + math.log(2)).abs().max()) < 1e-6 and abs(float(found.entropy[0]) - math.log(2)) < 1e-6
+        assert found.top_slots.tolist() == [[0, 2, 1]]

@@ -15,17 +15,18 @@ constexpr float kInf = __builtin_inff(), kLog2e = 1.4426950408889634f, kLn2 = 0.
 constexpr uint64_t kMostGroups = 1 << 20;    // workgroups of a launch: a grid of 2^32 threads is not allowed
 
 // A row's temperature: the factors of a distance to the best score, in natural logarithms and in those of base 2.  A temperature that is not above 0 has the
-// largest that there is: distances other than 0 are then infinite for all purposes.
+// largest that there is: distances other than 0 are then infinite for all purposes.  An infinite one has the smallest, not 0: what does not count lies at -infinity,
+// and stays there.
 struct Heat {
     float t, factor2;
     bool limit;
     __device__ __forceinline__ Heat(const float *temperature, uint32_t row) {
         t = temperature == nullptr ? 1.0f : temperature[row];
         limit = !(t > 0.0f);
-        factor2 = limit ? FLT_MAX : fminf(kLog2e / t, FLT_MAX);
+        factor2 = limit ? FLT_MAX : fminf(fmaxf(kLog2e / t, FLT_TRUE_MIN), FLT_MAX);
     }
-    // log p of a slot at distance d <= 0, of a sum whose logarithm is log_sum
-    __device__ __forceinline__ float log_p(float d, float log_sum) const { return (limit ? (d < 0.0f ? -kInf : d) : d / t) - log_sum; }
+    // log p of a slot at distance d <= 0, of a sum whose logarithm is log_sum.  (A distance that 32 bits do not hold is infinite at every temperature.)
+    __device__ __forceinline__ float log_p(float d, float log_sum) const { return (limit ? (d < 0.0f ? -kInf : d) : d == -kInf ? d : d / t) - log_sum; }
 };
 // Whether a score counts: allowed, and not -infinity.  (NaN counts: it shows.)
 __device__ __forceinline__ bool counts(const uint64_t *mask, uint32_t i, float s) {
