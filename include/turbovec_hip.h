@@ -312,8 +312,8 @@ int tv_rms_norm_dev(int device, void *stream, const void *d_x, int x_type, size_
                     void *d_sum, size_t sum_stride, const void *d_weight, int weight_type, float eps, size_t rows, size_t dim,
                     int row_kind, int scale_type, uint8_t *d_codes, size_t code_stride, void *d_scales, size_t scale_stride);
 
-/* Log probabilities under a softmax of rows of n scores, divided by a temperature a row (NULL: 1; one that is not above 0 is the limit
- * from above, the best slots share the mass; an infinite one gives all slots that have a probability the same).  A score that is 2^128 or more below the row's largest
+/* Log probabilities under a softmax of rows of n scores, divided by a temperature a row (NULL: 1; one below 2^-126 or NaN is the limit
+ * towards 0, the best slots share the mass; an infinite one gives all slots that have a probability the same).  A score that is 2^128 or more below the row's largest
  * has probability 0 at every temperature.  Slots whose mask bit is not set (d_mask_words NULL: all are; mask_stride 0: one mask for all rows) and slots of score
  * -infinity have probability 0, whatever else stands there.  For each row: out_log_probs, of the `given` slots in d_slots (-infinity for a slot of
  * probability 0 or outside 0 .. n - 1; the same slot may stand there twice); out_entropy, -sum p log p; the `top` slots of the highest scores,
@@ -327,7 +327,7 @@ int tv_log_probs_dev(int device, void *stream, const void *d_scores, int score_t
 size_t tv_log_probs_workspace(size_t rows, size_t n, size_t top);
 /* The gradient of the scores, in their type, from those of the log probabilities and of the entropy (either may be NULL), with the call's own inputs and the stats
  * that it left: (sum over given of g [slot] - G p - g_entropy p (log p + entropy)) / temperature, G the sum of g over given slots that have a
- * probability; a slot of probability 0 has gradient 0, and so has a row whose temperature is not above 0.  The same given slot twice adds up. */
+ * probability; a slot of probability 0 has gradient 0, and so has a row at the limit.  The same given slot twice adds up. */
 int tv_log_probs_grad_dev(int device, void *stream, const void *d_scores, int score_type, size_t score_stride, size_t rows, size_t n,
                           const uint64_t *d_mask_words, size_t mask_stride, const float *d_temperature, const int64_t *d_slots, size_t slot_stride, size_t given,
                           const float *d_stats, const float *d_grad_log_probs, const float *d_grad_entropy, void *d_grad_scores, size_t grad_stride);

@@ -52,3 +52,26 @@ def test_the_largest_temperatures(log_probs):  # noqa: F811
         found = log_probs(scores, slots[:1, :3].contiguous(), temperature=temperature, top=3)
         assert float(found.log_probs[0, 1]) == -INF and float((found.log_probs[0, ::2] + math.log(2)).abs().max()) < 1e-6 and abs(float(found.entropy[0]) - math.log(2)) < 1e-6
         assert found.top_slots.tolist() == [[0, 2, 1]]
+
+
+@pytest.mark.parametrize("rows,n", FORMS)
+def test_no_distance_is_too_small_for_the_limit(log_probs, rows, n):  # noqa: F811
+    """At a temperature of 0 the best slots share the mass, however little the others lie below them."""
+    if n < 7:
+        return
+    low = 2.0 ** -149
+    for dtype, step in ((torch.float32, 3 * low), (torch.float32, 1e-39), (torch.bfloat16, 2.0 ** -133), (torch.float16, 2.0 ** -24)):
+        scores = torch.zeros(rows, n, device="cuda", dtype=dtype)
+        best = [1, n // 2, n - 1]
+        scores[:, best] = step
+        slots = torch.tensor([best + [0]], device="cuda").expand(rows, 4).contiguous()
+        found = log_probs(scores, slots, temperature=0.0, top=4)
+        assert float((found.log_probs[:, :3] + math.log(3)).abs().max()) <= 4 * U and bool((found.log_probs[:, 3] == -INF).all())
+        assert float((found.entropy - math.log(3)).abs().max()) <= 4 * U
+        assert bool((found.top_slots == torch.tensor(best + [0], device="cuda")).all()) and bool((found.top_log_probs[:, 3] == -INF).all())
+        found = log_probs(-scores, slots, temperature=-1.0)                        # the best are all others
+        assert float((found.log_probs[:, 3] + math.log(n - 3)).abs().max()) <= (100 + 2 * math.log(n)) * U and bool((found.log_probs[:, :3] == -INF).all())
+    scores = torch.zeros(rows, n, device="cuda")
+    scores[:, best] = 1e-40
+    found = log_probs(scores, slots, temperature=1e-40)                            # no normal number
+    assert float((found.log_probs[:, :3] + math.log(3)).abs().max()) <= 4 * U and bool((found.log_probs[:, 3] == -INF).all())

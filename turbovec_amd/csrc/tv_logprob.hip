@@ -14,17 +14,18 @@ namespace tv {
 constexpr float kInf = __builtin_inff(), kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr uint64_t kMostGroups = 1 << 20;    // workgroups of a launch: a grid of 2^32 threads is not allowed
 
-// A row's temperature: the factors of a distance to the best score, in natural logarithms and in those of base 2.  A temperature that is not above 0 has the
-// largest that there is: distances other than 0 are then infinite for all purposes.  An infinite one has the smallest, not 0: what does not count lies at -infinity,
-// and stays there.
+// A row's temperature: the factors of a distance to the best score, in natural logarithms and in those of base 2.  One that is no normal number above 0 is the limit: every distance
+// other than 0 is infinite, whatever a product says.  An infinite one has the smallest factor, not 0: what does not count lies at -infinity, and stays there.
 struct Heat {
     float t, factor2;
     bool limit;
     __device__ __forceinline__ Heat(const float *temperature, uint32_t row) {
         t = temperature == nullptr ? 1.0f : temperature[row];
-        limit = !(t > 0.0f);
-        factor2 = limit ? FLT_MAX : fminf(fmaxf(kLog2e / t, FLT_TRUE_MIN), FLT_MAX);
+        limit = !(t >= FLT_MIN);
+        factor2 = limit ? FLT_MAX : fmaxf(kLog2e / t, FLT_TRUE_MIN);
     }
+    // The distance of a largest score from another that is not below it, for base 2.  (2^-10000 is 0 here; an infinity times 0 is not.)
+    __device__ __forceinline__ float below(float m, float to) const { return limit ? (m < to ? -10000.0f : 0.0f) : fmaxf((m - to) * factor2, -10000.0f); }
     // log p of a slot at distance d <= 0, of a sum whose logarithm is log_sum.  (A distance that 32 bits do not hold is infinite at every temperature.)
     __device__ __forceinline__ float log_p(float d, float log_sum) const { return (limit ? (d < 0.0f ? -kInf : d) : d == -kInf ? d : d / t) - log_sum; }
 };
@@ -36,9 +37,9 @@ __device__ __forceinline__ bool counts(const uint64_t *mask, uint32_t i, float s
 constexpr float kNone = -FLT_MAX;
 struct Sums {
     float m = kNone, s = 0.0f, u = 0.0f;
-    // The same, seen from a largest score that is not below its own.  (2^-10000 is 0 here; an infinity times 0 is not.)
-    __device__ __forceinline__ void rise(float to, float factor2) {
-        const float d = fmaxf((m - to) * factor2, -10000.0f), f = __builtin_amdgcn_exp2f(d);
+    // The same, seen from a largest score that is not below its own.
+    __device__ __forceinline__ void rise(float to, const Heat &heat) {
+        const float d = heat.below(m, to), f = __builtin_amdgcn_exp2f(d);
         u = f * fmaf(s, d, u);
         s *= f;
         m = to;
@@ -63,7 +64,7 @@ struct Reduce {
     float part[2][THREADS / 64];
 };
 template <int THREADS>
-__device__ __forceinline__ Sums group_sums(Sums v, float factor2, Reduce<THREADS> &r) {
+__device__ __forceinline__ Sums group_sums(Sums v, const Heat &heat, Reduce<THREADS> &r) {
     constexpr int kWaves = THREADS / 64;
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
     r.best[threadIdx.x] = v.m;
@@ -73,7 +74,7 @@ __device__ __forceinline__ Sums group_sums(Sums v, float factor2, Reduce<THREADS
     for (int i = 1; i < kWaves; ++i) m = fmaxf(m, r.best[i * 64 + lane]);
 #pragma unroll
     for (int i = 32; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
-    v.rise(m, factor2);
+    v.rise(m, heat);
 #pragma unroll
     for (int i = 32; i > 0; i >>= 1) {
         v.s += __shfl_xor(v.s, i);
@@ -261,7 +262,11 @@ __device__ __forceinline__ void scan_part(const T *scores, const uint64_t *mask,
         for (int i = 0; i < kCount; ++i) x[i] = l[i / kEach].template at<MASK>(i % kEach);
 #pragma unroll
         for (int i = 0; i < kCount; i += 2) segment = max3(segment, x[i], x[i + 1]);
-        sums.rise(fmaxf(sums.m, segment), heat.factor2);
+        sums.rise(fmaxf(sums.m, segment), heat);
+        if (heat.limit) {
+#pragma unroll
+            for (int i = 0; i < kCount; ++i) x[i] = x[i] < sums.m ? -kInf : x[i];
+        }
 #pragma unroll
         for (int i = 0; i < kCount; ++i) sums.add(x[i], heat.factor2);
     };
@@ -398,7 +403,7 @@ __global__ __launch_bounds__(THREADS, THREADS == kWideThreads && LOADS < kLogLoa
         Sums sums;
         float segments[kLogSegments];
         scan_part<THREADS, LOADS, T, MASK>(scores, mask, heat, at, sums, segments);
-        sums = group_sums(sums, heat.factor2, reduce);
+        sums = group_sums(sums, heat, reduce);
         if (a.top != 0) gather_part<THREADS, T, MASK>(a, scores, mask, at, segments, g, reduce.best, who, &who_count);
         if (parts == 1) {
             finish(a, row, given, heat, sums, g);
@@ -459,7 +464,7 @@ __global__ __launch_bounds__(kLogThreads) void k_log_probs_join(LogProbArgs a, u
         for (int i = 0; i < kEach; ++i) {
             Sums more;
             more.m = p[i].m; more.s = p[i].s; more.u = p[i].u;
-            more.rise(sums.m, heat.factor2);
+            more.rise(sums.m, heat);
             sums.s += more.s;
             sums.u += more.u;
             best = fmaxf(best, first[i] == 0 ? kNone : order_unkey(int(uint32_t(first[i] >> 32) ^ 0x80000000u)));
@@ -476,7 +481,7 @@ __global__ __launch_bounds__(kLogThreads) void k_log_probs_join(LogProbArgs a, u
             }
             if (threadIdx.x == 0) g.count = who_count = 0;
         }
-        sums = group_sums(sums, heat.factor2, reduce);
+        sums = group_sums(sums, heat, reduce);
         if (top != 0) {
             uint64_t from = larger(larger(larger(least[0][0], least[0][1]), larger(least[0][2], least[0][3])), smaller(smaller(least[1][0], least[1][1]), smaller(least[1][2], least[1][3])));
             __syncthreads();
@@ -572,7 +577,7 @@ __global__ __launch_bounds__(THREADS) void k_log_probs_grad(LogProbGradArgs a, u
 #pragma unroll
         for (int k = 32; k > 0; k >>= 1) all += __shfl_xor(all, k);
         const float g_entropy = a.grad_entropy == nullptr ? 0.0f : a.grad_entropy[row];
-        const float factor_a = -(all + g_entropy * stats.z), factor_b = -g_entropy * kLn2, inverse = heat.limit ? 0.0f : fminf(1.0f / heat.t, FLT_MAX);
+        const float factor_a = -(all + g_entropy * stats.z), factor_b = -g_entropy * kLn2, inverse = heat.limit ? 0.0f : 1.0f / heat.t;
         auto at = [&](float s) {
             const float l = fmaf(s - stats.x, heat.factor2, -stats.y), d = __builtin_amdgcn_exp2f(l) * fmaf(factor_b, fmaxf(l, -200.0f), factor_a);
             return s == -kInf ? 0.0f : d;

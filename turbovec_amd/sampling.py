@@ -127,7 +127,7 @@ def log_probs(scores, slots, *, temperature=None, mask=None, top=0):
 
     A slot that the mask leaves out, one outside the row (-1, a draw from a row that allows nothing) and one of score -infinity have log probability -infinity, and what
     stands in a masked place never counts; a row that allows nothing has entropy 0, and where fewer than `top` slots have a probability the alternatives end in (-1, -infinity).
-    An allowed NaN or +infinity makes its row NaN.  A temperature that is not above 0 is the limit: the best slots share the mass, and the row has no gradient. An infinite
+    An allowed NaN or +infinity makes its row NaN.  A temperature below 2^-126, 0 and negative ones among them, is the limit: the best slots share the mass, and the row has no gradient.  An infinite
     one gives every slot that has a probability the same, and the row's gradient is 0.
 
     `log_probs` and `entropy` carry a gradient to the scores (tv_log_probs_grad_dev; in the scores' type, rounded once, once differentiable); the alternatives carry none: give
