@@ -75,3 +75,22 @@ def test_no_distance_is_too_small_for_the_limit(log_probs, rows, n):  # noqa: F8
     scores[:, best] = 1e-40
     found = log_probs(scores, slots, temperature=1e-40)                            # no normal number
     assert float((found.log_probs[:, :3] + math.log(3)).abs().max()) <= 4 * U and bool((found.log_probs[:, 3] == -INF).all())
+
+
+@pytest.mark.parametrize("rows,n", FORMS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_signalling_nan_hides_no_score(log_probs, rows, n, dtype):  # noqa: F811
+    """A NaN of any kind shows in the row's sums and is not among its best slots; those beside it are."""
+    if n < 20:
+        return
+    bits, kind = {torch.float32: (0x7f800001, torch.int32), torch.float16: (0x7c01, torch.int16), torch.bfloat16: (0x7f81, torch.int16)}[dtype]
+    scores = scores_of(rows, n, dtype, 72)
+    for at in {0, 1, 6, n // 2, n - 2, n - 1}:
+        scores[:, max(at - 1, 0):at + 2] = 20.0 + at / n
+    order = scores.clone()
+    for at in (1, n // 2, n - 1):
+        scores.view(kind)[:, at] = bits
+        order[:, at] = -INF
+    found = log_probs(scores, slots_of(rows, n, 2), top=6)
+    assert bool(torch.isnan(found.entropy).all()) and bool(torch.isnan(found.log_probs).all())
+    assert torch.equal(found.top_slots, torch.sort(order, dim=1, descending=True, stable=True).indices[:, :6])

@@ -226,7 +226,7 @@ struct Scores {
     }
 };
 
-// The largest of three, none of a NaN.  (Written as two maxima the compiler makes each operand canonical first.)
+// The largest of three; a quiet NaN is passed over, a signalling one is not.  (Written as two maxima the compiler makes each operand canonical first.)
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
@@ -290,6 +290,11 @@ __device__ __forceinline__ void scan_part(const T *scores, const uint64_t *mask,
             }
         }
         segments[part] = segment;
+    }
+    // A signalling NaN takes the largest score before it along, so what it stands in is read again, all of it.
+    if (sums.s != sums.s) {
+#pragma unroll
+        for (int part = 0; part < kLogSegments; ++part) segments[part] = kInf;
     }
 }
 constexpr uint32_t kFewAlternatives = 24;
