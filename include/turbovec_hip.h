@@ -319,7 +319,8 @@ int tv_rms_norm_dev(int device, void *stream, const void *d_x, int x_type, size_
  * probability 0 or outside 0 .. n - 1; the same slot may stand there twice); out_entropy, -sum p log p; the `top` slots of the highest scores,
  * ties to the lower slot, with their log probabilities (slot -1, -infinity where fewer have a probability; a NaN is not among them).  given and top are at
  * most 128; either may be 0.  A row with nothing allowed has entropy 0; one where an allowed score is NaN or +infinity has NaN for
- * the entropy and every log probability that is not -infinity.  d_out_stats, unless NULL, receives four floats a row for the gradient.  All sums are taken in 32 bits. */
+ * the entropy and every log probability that is not -infinity.  d_out_stats, unless NULL, receives four floats a row for the gradient.  All sums are taken in 32 bits: a thread
+ * adds up to 32 scores for themselves and those sums, no more than n / 4096 and a dozen (n / 8192 of two-byte scores), one after the other. */
 int tv_log_probs_dev(int device, void *stream, const void *d_scores, int score_type, size_t score_stride, size_t rows, size_t n,
                      const uint64_t *d_mask_words, size_t mask_stride, const float *d_temperature, const int64_t *d_slots, size_t slot_stride, size_t given,
                      size_t top, float *d_out_log_probs, float *d_out_entropy, int64_t *d_out_top_slots, float *d_out_top_log_probs, float *d_out_stats,

@@ -49,6 +49,10 @@ struct Sums {
         s += e;
         u = fmaf(e, fmaxf(t, -200.0f), u);
     }
+    __device__ __forceinline__ void join(const Sums &other) {
+        s += other.s;
+        u += other.u;
+    }
     __device__ __forceinline__ float entropy(float log_sum) const { return s == 0.0f ? 0.0f : log_sum - kLn2 * (u / s); }
 };
 
@@ -267,8 +271,11 @@ __device__ __forceinline__ void scan_part(const T *scores, const uint64_t *mask,
 #pragma unroll
             for (int i = 0; i < kCount; ++i) x[i] = x[i] < sums.m ? -kInf : x[i];
         }
+        Sums some;                      // (what is loaded at once is added for itself: the long sum loses a rounding for each of those, not for each score)
+        some.m = sums.m;
 #pragma unroll
-        for (int i = 0; i < kCount; ++i) sums.add(x[i], heat.factor2);
+        for (int i = 0; i < kCount; ++i) some.add(x[i], heat.factor2);
+        sums.join(some);
     };
 #pragma unroll
     for (int part = 0; part < kLogSegments; ++part) {
