@@ -8,6 +8,7 @@ no gradient; log probabilities and entropies carry one to the scores.
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as T
 from .fp8 import _VALUES, _call, _gpu, _same_device, _workspace
@@ -97,6 +98,15 @@ def _forward(scores, slots, temperature, mask, top, stats):
     return LogProbs(log_p, entropy, top_slots, top_log_p)
 
 
+def _no_tangent(**tensors):
+    """There is no derivative forward: a tangent that is dropped would read as zero."""
+    if getattr(forward_ad, "_current_level", 0) < 0:          # (outside of every level, where this torch says so: no tensor has one)
+        return
+    for name, t in tensors.items():
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{name}: log_probs has no forward-mode derivative")
+
+
 class _WithGradient(torch.autograd.Function):
     @staticmethod
     def forward(ctx, scores, slots, temperature, mask, top, alternatives):
@@ -131,7 +141,8 @@ def log_probs(scores, slots, *, temperature=None, mask=None, top=0):
     one gives every slot that has a probability the same, and the row's gradient is 0.
 
     `log_probs` and `entropy` carry a gradient to the scores (tv_log_probs_grad_dev; in the scores' type, rounded once, once differentiable); the alternatives carry none: give
-    them as `slots` for that.  A temperature that requires a gradient is refused."""
+    them as `slots` for that.  A temperature that requires a gradient is refused, and so are scores or a temperature with a forward-mode tangent."""
+    _no_tangent(scores=scores, temperature=temperature)
     _gpu("scores", scores, _VALUES)
     rows, n = scores.shape
     if n == 0:
