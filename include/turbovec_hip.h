@@ -305,8 +305,9 @@ typedef enum { TV_ROWS_FP8 = 0, TV_ROWS_FP4 = 1 } tv_row_kind;
  * and made into rows of 8 bits, as tv_fp8_quantize_dev with a group of 1, or of 4 (scale_type TV_SCALE_E8M0), as tv_fp4_quantize_dev.  The norm is of h before
  * it is rounded; d_sum, unless NULL, receives h rounded to x_type.  x, residual and sum have x_type; the sum may take the place of
  * x or of the residual (same address and stride) and overlaps neither in any other way.  eps: finite, not below 0.  A row of zeros with eps 0 has
- * no norm, nor has one with a NaN or an infinity: its values are NaN.  (Squares are taken in 32 bits, up to 32 of them added there and
- * those sums in 64: an |h| from 2^64 on counts as infinite, one from 2^61 on may, and where a row is below 2^-63 throughout, eps is what remains.)  A power of two as a scale is the one that h in 32 bits
+ * no norm, nor has one with a NaN or an infinity: its values are NaN.  (Squares are taken in 32 bits, up to 16 of them added there and
+ * those sums in 64: an |h| from 2^64 on counts as infinite, one from 2^62 on may; of a row that is below 2^-63 throughout the squares lose bits, below 2^-75 all of them, and eps is what
+ * remains.)  A power of two as a scale is the one that h in 32 bits
  * and all that follows in 64 would have, but for a few in 10^8 blocks. */
 int tv_rms_norm_dev(int device, void *stream, const void *d_x, int x_type, size_t x_stride, const void *d_residual, size_t residual_stride,
                     void *d_sum, size_t sum_stride, const void *d_weight, int weight_type, float eps, size_t rows, size_t dim,

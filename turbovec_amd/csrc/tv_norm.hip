@@ -95,6 +95,7 @@ template <typename T> constexpr int norm_waves(int lanes, int runs, int most) { 
 // LANES lanes to a row, each with RUNS runs: sixteen to sixty-four, or (0) all of a workgroup, as many waves as the row fills, whose sums then go through LDS.
 template <typename T, int TO, int LANES, int RUNS, int MOST>
 __global__ __launch_bounds__(MOST, norm_waves<T>(LANES, RUNS, MOST)) void k_rms_norm(NormArgs a) {
+    static_assert(RUNS * 8 <= 16, "squares of a thread that are added in 32 bits: 16 of up to 2^124 are below 2^128");
     constexpr bool kAll = LANES == 0;
     constexpr int kLanes = kAll ? 64 : LANES;
     __shared__ double part[kAll ? MOST / 64 : 1];
