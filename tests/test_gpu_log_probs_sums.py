@@ -102,3 +102,20 @@ def test_the_gradient_sums_to_nothing(log_probs, rows, n, dtype):  # noqa: F811
     off = (3 * plain.mean + JOINED + 16 + 80) * U * (2 + plain.mean + plain.log_sum)
     assert bool((grad.double().sum(1).abs() <= size * half + (2 + plain.entropy) * (off + 8 * U) * 4 + n * (2.0 ** -25 if dtype == torch.float16 else 0)).all())
     check_gradient(log_probs, scores, slots)
+
+
+@pytest.mark.parametrize("rows,n,top", [(1, 80_500, 0), (1, 80_501, 0), (64, 112_000, 0), (64, 112_001, 0), (1, 101_780, 1), (1, 101_781, 1), (1, 126_100, 20), (1, 126_101, 20), (3, 285_820, 128), (3, 285_821, 128),
+                                        (159, 159_500, 0), (159, 159_501, 0), (160, 159_501, 0)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_in_one_and_in_parts(log_probs, rows, n, top, dtype):  # noqa: F811
+    """Both sides of where a row's scores go to one workgroup or to several."""
+    at_once = min(rows, 8)
+    scores = scores_of(at_once, n, dtype, 97).repeat(-(-rows // at_once), 1)[:rows]
+    slots = slots_of(at_once, n, 3).repeat(-(-rows // at_once), 1)[:rows]
+    found = log_probs(scores, slots, top=top)
+    plain = Plain(scores[:at_once])
+    near(found._replace(log_probs=found.log_probs[:at_once], entropy=found.entropy[:at_once]), plain, slots[:at_once], 24, 24)
+    if top:
+        assert torch.equal(found.top_slots[:at_once], plain.ranked(top))
+    for x in found[:2]:
+        assert torch.equal(x[:at_once].repeat(-(-rows // at_once), *[1] * (x.dim() - 1))[:rows], x)

@@ -528,10 +528,14 @@ static uint32_t log_parts(size_t rows, size_t n, uint32_t &part_size) {
     part_size = uint32_t(std::min(each * kOnce, n));
     return uint32_t((n + part_size - 1) / part_size);
 }
-// Rows in parts that have a wide workgroup each all the same: rows enough for half of the card, and those that are not much longer than what two launches take.  (100000 bfloat16
-// scores a row, 20 alternatives: 1 row 13.7 us so and 14.4 in parts, 64 rows 14.5 and 18.6, 256 rows 17.7 and 26.5, 512 rows, two to a compute unit, 28.5 and 36.3; of 150000
-// 1 row 17.2 and 14.8, of 1000000 128 rows 81 and 63, 192 rows 84 and 96.  Without alternatives 1 row of 32000 6.6 and 7.3, of 100000 10.2 and 6.9, but a launch less.)
-static bool log_wide(size_t rows, size_t n) { return rows >= 160 || n <= 100000 + 600 * rows; }
+// Rows in parts that have a wide workgroup each all the same: rows enough for half of the card, and those that are not much longer than what a second launch takes, and the parts'
+// ranking of their best where alternatives are asked for.  A second launch costs a call among others 3.7 us on the host, one that is waited for and one in a graph less: the border lies between what these
+// two have.  (us so and in parts, bfloat16, in a graph / waited for.  1 row without alternatives: 64000 scores 8.2 and 7.3 / 26.9 and 28.6, 80000 9.2 and 8.3 / 27.8 and 28.6, 100000 9.9 and 7.1 / 28.6 and
+// 28.4; with 1 100000 12.3 and 10.9 / 31.2 and 32.4, 128256 14.8 and 11.0 / 33.8 and 32.4; with 20 100000 13.6 and 14.7 / 32.7 and 35.9, 128256 16.5 and 14.5 / 35.3 and 35.7, 151936 17.5 and 15.7 / 36.6 and 36.5; with
+// 128 200000 32.7 and 33.0 / 52 and 57, 300000 36 and 37 / 55 and 57.  64 rows: without 100000 10.8 and 11.1 / 30.1 and 31.4, 128256 13.8 and 11.1 / 32.9 and 31.6, with 20 200000 21.8 and 22.7 / 41 and 44,
+// 300000 28.1 and 26.6 / 47.7 and 47.4, with 128 400000 - / 67 and 85.  128 rows without: 151936 15.5 and 15.6 / 34.7 and 36.1, 300000 26.6 and 22.0 / 45 and 42; 192 rows without: 200000 20.9 and 22.0,
+// 500000 44 and 49.)
+static bool log_wide(size_t rows, size_t n, size_t top) { return rows >= 160 || n <= 80000 + (top != 0 ? 20000 : 0) + 1200 * top + rows * (500 + 80 * top); }
 // Many rows of a few loads have a wave each, as long as its 64 largest scores tell the alternatives apart.  (Rows of 1000 bfloat16 scores with 5 alternatives: 1024 rows 7.9 us so and 8.5
 // with workgroups of 256, 4096 rows 10.2 and 21.9, 65536 rows 88 and 275; their gradients 4096 rows 8.2 and 11.4, 65536 rows 73 and 152.)
 static bool log_short(size_t rows, size_t n, size_t size, size_t top) { return rows >= 1024 && n * size <= 8192 && top <= kFewAlternatives; }
@@ -539,13 +543,13 @@ size_t log_probs_workspace(size_t rows, size_t n, size_t top) {
     if (rows == 0 || n == 0) return 0;
     uint32_t part_size;
     const size_t parts = log_parts(rows, n, part_size);
-    return parts == 1 || log_wide(rows, n) ? 0 : rows * parts * (sizeof(LogPart) + top * sizeof(uint64_t));
+    return parts == 1 || log_wide(rows, n, top) ? 0 : rows * parts * (sizeof(LogPart) + top * sizeof(uint64_t));
 }
 template <typename T, bool MASK>
 static hipError_t log_probs(const LogProbArgs &a, hipStream_t s) {
     uint32_t part_size;
     const uint32_t parts = log_parts(a.rows, a.n, part_size);
-    if (parts > 1 && log_wide(a.rows, a.n)) {
+    if (parts > 1 && log_wide(a.rows, a.n, a.top)) {
         const auto kernel = a.rows <= 256 ? k_log_probs<kWideThreads, kLogLoads, T, MASK> : k_log_probs<kWideThreads, kLogLoads / 2, T, MASK>;
         return launch(kernel, a.rows, kWideThreads, 0, s, a, 1u, a.n);
     }
