@@ -24,8 +24,6 @@ struct Heat {
         limit = !(t >= FLT_MIN);
         factor2 = limit ? FLT_MAX : fmaxf(kLog2e / t, FLT_TRUE_MIN);
     }
-    // The distance of a largest score from another that is not below it, for base 2.  (2^-10000 is 0 here; an infinity times 0 is not.)
-    __device__ __forceinline__ float below(float m, float to) const { return limit ? (m < to ? -10000.0f : 0.0f) : fmaxf((m - to) * factor2, -10000.0f); }
     // log p of a slot at distance d <= 0, of a sum whose logarithm is log_sum.  (A distance that 32 bits do not hold is infinite at every temperature.)
     __device__ __forceinline__ float log_p(float d, float log_sum) const { return (limit ? (d < 0.0f ? -kInf : d) : d == -kInf ? d : d / t) - log_sum; }
 };
@@ -37,12 +35,17 @@ __device__ __forceinline__ bool counts(const uint64_t *mask, uint32_t i, float s
 constexpr float kNone = -FLT_MAX;
 struct Sums {
     float m = kNone, s = 0.0f, u = 0.0f;
-    // The same, seen from a largest score that is not below its own.
-    __device__ __forceinline__ void rise(float to, const Heat &heat) {
-        const float d = heat.below(m, to), f = __builtin_amdgcn_exp2f(d);
+    // The same, seen from a largest score that is not below its own.  (2^-10000 is 0 here; an infinity times 0 is not.)
+    __device__ __forceinline__ void rise(float to, float factor2) {
+        const float d = fmaxf((m - to) * factor2, -10000.0f), f = __builtin_amdgcn_exp2f(d);
         u = f * fmaf(s, d, u);
         s *= f;
         m = to;
+    }
+    // At the limit nothing of it is left then where its own is below.  (A NaN stays.)
+    __device__ __forceinline__ void outdo(float to) {
+        s = m < to ? s * 0.0f : s;
+        u = m < to ? u * 0.0f : u;
     }
     __device__ __forceinline__ void add(float score, float factor2) {
         const float t = (score - m) * factor2, e = __builtin_amdgcn_exp2f(t);
@@ -78,7 +81,8 @@ __device__ __forceinline__ Sums group_sums(Sums v, const Heat &heat, Reduce<THRE
     for (int i = 1; i < kWaves; ++i) m = fmaxf(m, r.best[i * 64 + lane]);
 #pragma unroll
     for (int i = 32; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
-    v.rise(m, heat);
+    if (heat.limit) v.outdo(m);
+    v.rise(m, heat.factor2);
 #pragma unroll
     for (int i = 32; i > 0; i >>= 1) {
         v.s += __shfl_xor(v.s, i);
@@ -266,11 +270,13 @@ __device__ __forceinline__ void scan_part(const T *scores, const uint64_t *mask,
         for (int i = 0; i < kCount; ++i) x[i] = l[i / kEach].template at<MASK>(i % kEach);
 #pragma unroll
         for (int i = 0; i < kCount; i += 2) segment = max3(segment, x[i], x[i + 1]);
-        sums.rise(fmaxf(sums.m, segment), heat);
+        const float largest = fmaxf(sums.m, segment);
         if (heat.limit) {
+            sums.outdo(largest);
 #pragma unroll
-            for (int i = 0; i < kCount; ++i) x[i] = x[i] < sums.m ? -kInf : x[i];
+            for (int i = 0; i < kCount; ++i) x[i] = x[i] < largest ? -kInf : x[i];
         }
+        sums.rise(largest, heat.factor2);
         Sums some;                      // (what is loaded at once is added for itself: the long sum loses a rounding for each of those, not for each score)
         some.m = sums.m;
 #pragma unroll
@@ -476,7 +482,8 @@ __global__ __launch_bounds__(kLogThreads) void k_log_probs_join(LogProbArgs a, u
         for (int i = 0; i < kEach; ++i) {
             Sums more;
             more.m = p[i].m; more.s = p[i].s; more.u = p[i].u;
-            more.rise(sums.m, heat);
+            if (heat.limit) more.outdo(sums.m);
+            more.rise(sums.m, heat.factor2);
             sums.s += more.s;
             sums.u += more.u;
             best = fmaxf(best, first[i] == 0 ? kNone : order_unkey(int(uint32_t(first[i] >> 32) ^ 0x80000000u)));
