@@ -11,7 +11,7 @@ namespace tv {
 // the largest code, 6, and what would be the next, 8, so that the largest value is rounded as the others are.
 // ---------------------------------------------------------------------------
 
-// A thread to eight coordinates, four neighbours to a block.  Bound by memory: 400000 rows of 1536 floats 482 to 520 us, 5.3 to 5.8 TB/s, an eighth of it written; of bfloat16 286 to 327, 5.0 to 5.4.
+// A thread to eight coordinates, four neighbours to a block.  Bound by memory: 400000 rows of 1536 floats 482 to 520 us, 5.3 to 5.8 TB/s, an eighth of it written; of bfloat16 286 to 327, 4.8 to 5.4.
 constexpr int kThreads4 = 256;
 template <typename T>
 __global__ __launch_bounds__(kThreads4) void k_fp4_quantize(Quantize4Args a) {

@@ -401,7 +401,7 @@ __device__ __forceinline__ void gather_part(const LogProbArgs &a, const T *score
         if (count > kKeep) above = cut(g, a.top);
     }
 }
-// (LOADS at once: two where a compute unit is to hold two of the wide workgroups, 64 registers a thread.)
+// (LOADS at once: two where a compute unit is to hold two of the wide workgroups, 64 registers a thread, nine more spilled.)
 template <int THREADS, int LOADS, typename T, bool MASK>
 __global__ __launch_bounds__(THREADS, THREADS == kWideThreads && LOADS < kLogLoads ? 8 : 1) void k_log_probs(LogProbArgs a, uint32_t parts, uint32_t part_size) {
     __shared__ Reduce<THREADS> reduce;

@@ -90,7 +90,9 @@ struct Run8 {
 // Whether a workgroup that goes on to a next row asks for it, and keeps the weights, while it has the row before in hand.  Floats have twice the bytes on their way and no registers left, but for
 // the longest rows, where few workgroups are held (4096 of 16384 84 us so and 97).
 template <typename T> constexpr bool norm_ahead(int runs, int most) { return sizeof(T) == 2 || (runs == 2 && most == 1024); }
-// Waves of a SIMD at once: what they hold fits in 64, 72, 80 or 128 registers.
+// Waves of a SIMD at once, which leave 64, 72, 80 or 128 registers to each.  Two runs a lane spill 2 to 7 of 80, but for floats into float scales, and one run of floats 2 of 64 where a workgroup's row goes
+// into 8 bits with power-of-two scales.  More registers hold all, for fewer rows on their way (us so and with those: bfloat16 without a residual, 96 registers, 16384 of 5120 64 and 78, 8192 of 8192 50
+// and 54, but 16384 of 4096 48 and 44; floats with a residual, 72, 8192 of 8192 165 and 175, but 40000 of 1536 150 and 139).
 template <typename T> constexpr int norm_waves(int lanes, int runs, int most) { return runs == 1 ? (sizeof(T) == 2 || lanes == 0 ? 8 : 7) : runs == 2 && most < 1024 ? 6 : 4; }
 // LANES lanes to a row, each with RUNS runs: sixteen to sixty-four, or (0) all of a workgroup, as many waves as the row fills, whose sums then go through LDS.
 template <typename T, int TO, int LANES, int RUNS, int MOST>
@@ -222,7 +224,7 @@ static hipError_t norm_form(const NormArgs &a, hipStream_t s) {
     const uint64_t held = stays ? 256u * (4u * norm_waves<T>(LANES, RUNS, MOST) * 64u / threads) : kMostGroups;
     return launch(k_rms_norm<T, TO, LANES, RUNS, MOST>, uint32_t(groups < held ? groups : held), threads, 0, s, a);
 }
-// Bound by memory: 16384 rows of 4096 bfloat16 with a residual take 82 us, 5.7 TB/s, a third of it written (a copy reaches 4.6 to 4.9), 8192 of 8192 85, 16384 of 5120 113.  With a residual most is on its
+// Bound by memory: 16384 rows of 4096 bfloat16 with a residual take 82 us, 5.7 TB/s, 43 % of it written (a copy reaches 4.6 to 4.9), 8192 of 8192 85, 16384 of 5120 113.  With a residual most is on its
 // way at a time with a run to a lane and a workgroup to a row (with two runs and workgroups that stay 90, 90 and 112); without one, with two runs and workgroups that stay and ask for their
 // next row in time (16384 of 4096 made 8-bit 43 us so, a workgroup to each row 48 to 59; 16384 of 5120 made 4-bit 54, and 81 with a power of two of lanes).  The longest rows have
 // two runs and workgroups that stay either way (4096 of 16384 bfloat16 with a residual 88 us, a workgroup to each row 109).
