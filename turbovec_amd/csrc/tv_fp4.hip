@@ -552,15 +552,17 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (HELD * KS * WM * WN + 3) / 4) v
     else store_strips4<T, kThroughL2, TN / WN, MT, NT>(p, acc, strip, m0 + wm, n0 + wn, lane);
 }
 
-// Results of rows below kStreamDim4 leave past the L2: they would push out what other tiles read there.  (1024 by 98304 of 1536 into floats 139 us, through it 153; 4096 by 16384 of 4096 175
-// and 170.)  Where the result's rows start in the middle of a cache line and there is little to do between two tiles' results, a wave gives eight stores at a time (1000 by 50001 of 768 into floats 55 us
-// and 86, into bfloat16 46 and 63; 1024 by 100001 of 1536 191 and 182, 163 and 137; rows at whole lines, 1024 by 98304 of 1536, 155 and 139).
+// Results of rows below kStreamDim4 leave past the L2: they would push out what other tiles read there.  (1024 by 98304 of 1536 into floats 134 to 139 us, through it 154; of 2048 177 and 171, 4096 by
+// 16384 of 4096 172 and 172, into bfloat16 157 and 148.)  Where the result's rows start in the middle of a cache line and there is little to do between two tiles' results, a wave gives eight stores at a
+// time (1000 by 50001 of 768 into floats 55 us and 87, into bfloat16 45 and 64; 1000 by 50000, every other row in the middle of a line, 48 and 53; 1024 by 100001 of 1536 191 and 166, 156 and 136; rows
+// at whole lines, 1024 by 98304 of 1536, 152 and 137).
+constexpr size_t kLine = 128;
 constexpr uint32_t kStreamDim4 = 2048, kPacedDim4 = 1280;
 template <typename T, int TM, int TN, int WM, int WN, int HELD, int KS = 1>
 static hipError_t tile4(const Matmul4Args &a, hipStream_t s) {
     const uint64_t mt = (a.a.rows + TM - 1) / TM, nt = (a.b.rows + TN - 1) / TN, each_xcd = (mt * nt + 7) / 8;
     if ((each_xcd * 8 * (64 * WM * WN * KS)) >> 32) return hipErrorInvalidConfiguration;      // (a result of hundreds of GB, or a narrow one of a billion columns)
-    const bool lines = (a.out_stride * sizeof(T) % 64 | reinterpret_cast<uintptr_t>(a.out) % 64) == 0;
+    const bool lines = (a.out_stride * sizeof(T) % kLine | reinterpret_cast<uintptr_t>(a.out) % kLine) == 0;
     const int way = a.dim >= kStreamDim4 ? kThroughL2 : lines || TM < 128 || a.dim >= kPacedDim4 ? kPaced : kPastL2;
     const auto kernel = k_fp4_tile<T, TM, TN, WM, WN, HELD, KS>;
     constexpr size_t kLds = KS * tile4_lds<TM, TN>();
