@@ -570,7 +570,8 @@ static hipError_t tile4(const Matmul4Args &a, hipStream_t s) {
     return launch(kernel, uint32_t(each_xcd * 8), 64 * WM * WN * KS, kLds, s, a, uint32_t(mt), uint32_t(nt), uint32_t(each_xcd), way);
 }
 
-// Rows of fewer than 16 bytes, or 8 MB and more apart: a wave to a tile of 16 by 16, its operands read where they lie.
+// Rows of fewer than 16 bytes, or 8 MB and more apart: a wave to a tile of 16 by 16, its operands read where they lie.  (Bound by its waves, which wait once for what they read and store a
+// value a lane: 1024 by 100000 of 16 into floats 275 us, 1.5 TB/s, one by 1M of 24 64; 64 by 200 of 1536, rows 8 MB apart, 8.2, close together 5.5 in tiles.)
 template <typename T>
 __global__ __launch_bounds__(64) void k_fp4_small(Matmul4Args p, uint32_t n_tiles) {
     const int lane = threadIdx.x, col = lane & 15, g = lane >> 4;
@@ -600,8 +601,9 @@ static hipError_t small4(const Matmul4Args &a, hipStream_t s) {
 }
 
 // The tiles, and what one takes a compute unit that holds so many of them, in microseconds: for a stage, in front and behind, and for a byte of the result's type.  Fitted to 56 sizes of 17 to
-// 8192 rows by 100 to 1M, of 74 to 8192, into floats and bfloat16: the tile taken is the fastest there or within 6 % of it but for three, 25 % at worst (2669 by 15974 of 1024), 1.1 %
-// on the mean.  A compute unit's tiles come in rounds of as many as it holds, and a started round costs a whole one.
+// 8192 rows by 100 to 1M, of 74 to 8192, into floats and bfloat16.  Of these and 44 others, timed with the tiles as they are now, the tile taken is the fastest or within 6 % of it but for twelve, 28 % at worst (6262
+// by 7351 of 768: results whose rows start anywhere cost tiles of 256 more than this knows), 2.0 % on the mean; constants fitted anew to all of them do as well, 1.9 %.  A compute unit's tiles come in rounds of as
+// many as it holds, and a started round costs a whole one.
 struct TileTime {
     uint32_t tm, tn, held;
     double stage, once, byte;
@@ -656,7 +658,7 @@ static hipError_t matmul4(const Matmul4Args &a, hipStream_t s) {
     const uint64_t tiles = uint64_t(mt) * nt;
     if (tile == 0 && tiles > 256 && nt >= mt) {
         // The tiles of 256 that start a last round and do not fill it: their columns in a launch of their own, of smaller tiles, where that is less than the round.  (1024 by 100000
-        // of 1536 into floats: 160 us with it and 167 to 176 without, inputs and results from memory.)
+        // of 1536 into floats 145 us with it and 151 without, into bfloat16 120 and 126, inputs and results from memory.)
         const uint32_t columns = uint32_t(tiles / 256 * 256 / mt) * 256;
         if (columns < a.b.rows) {
             Matmul4Args first = a, rest = a;
