@@ -283,7 +283,9 @@ size_t tv_sample_workspace(size_t rows, size_t n);
  * odd dim is written as 0 and not looked at.  Strides of codes and scales count bytes. */
 
 /* Makes 4-bit rows of values.  With `amax` the largest magnitude of a block, its scale is the smallest power of two 2^e,
- * e >= -126, with amax < 7 * 2^e (so that the largest value is off by half a step at most, as all others are); codes are x / scale
+ * e >= -126, with amax < 7 * 2^e (so that the largest value is off by half a step at most, as all others are; a conversion that takes
+ * 2^(floor(log2 amax) - 2), as is usual for the format, has half that scale where amax is 1.75 times a power of two or more, and cuts what is above 6 of it: rows made so are
+ * rows here too, of other bytes); codes are x / scale
  * rounded to the nearest, ties to even, at most 6.  There is no code for them: an infinity or a NaN makes its block's scale NaN (255). */
 int tv_fp4_quantize_dev(int device, void *stream, const void *d_x, int x_type, size_t x_stride, size_t rows, size_t dim,
                         uint8_t *d_codes, size_t code_stride, uint8_t *d_scales, size_t scale_stride);

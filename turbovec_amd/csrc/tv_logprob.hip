@@ -12,7 +12,6 @@
 namespace tv {
 
 constexpr float kInf = __builtin_inff(), kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr uint64_t kMostGroups = 1 << 20;    // workgroups of a launch: a grid of 2^32 threads is not allowed
 
 // A row's temperature: the factors of a distance to the best score, in natural logarithms and in those of base 2.  One that is no normal number above 0 is the limit: every distance
 // other than 0 is infinite, whatever a product says.  An infinite one has the smallest factor, not 0: what does not count lies at -infinity, and stays there.

@@ -157,6 +157,7 @@ int op_failed(hipError_t e, const char *what);
 inline hipError_t allow_lds(const void *kernel, size_t bytes) {
     return bytes <= 65536 ? hipSuccess : hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
 }
+constexpr uint64_t kMostGroups = 1 << 20;    // workgroups of a launch: a grid of 2^32 threads is not allowed
 // A launch that reports its own error, and none that an earlier call of the process left behind.
 template <typename... P, typename... A>
 hipError_t launch(void (*kernel)(P...), dim3 grid, dim3 threads, size_t lds, hipStream_t s, const A &...a) {

@@ -8,8 +8,6 @@ typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 
-constexpr uint64_t kMostGroups = 1 << 20;    // workgroups of a launch: a grid of 2^32 threads is not allowed
-
 // Four values from p, those of them past `left` zero.
 template <typename T>
 __device__ __forceinline__ void load4(float (&v)[4], const T *p, int left) {

@@ -74,7 +74,10 @@ class Fp4Rows:
 
 
 def quantize(x):
-    """4-bit rows of `x` (float32, float16 or bfloat16 [rows, dim]; tv_fp4_quantize_dev).  A block with an infinity or a NaN is NaN."""
+    """4-bit rows of `x` (float32, float16 or bfloat16 [rows, dim]; tv_fp4_quantize_dev).  A block with an infinity or a NaN is NaN.
+
+    A block's scale is the smallest power of two that its largest magnitude is below 7 times of, which rounds that one as all others.  The format's usual conversion takes
+    half of it where the largest is 1.75 times a power of two or more, and cuts at 6: rows made so can be given to `Fp4Rows`, but have other bytes."""
     _gpu("x", x, _VALUES)
     rows, dim = x.shape
     if not 1 <= dim <= _MAX_DIM:
