@@ -570,8 +570,8 @@ static hipError_t tile4(const Matmul4Args &a, hipStream_t s) {
     return launch(kernel, uint32_t(each_xcd * 8), 64 * WM * WN * KS, kLds, s, a, uint32_t(mt), uint32_t(nt), uint32_t(each_xcd), way);
 }
 
-// Rows of fewer than 16 bytes, or 8 MB and more apart: a wave to a tile of 16 by 16, its operands read where they lie.  (Bound by its waves, which wait once for what they read and store a
-// value a lane: 1024 by 100000 of 16 into floats 275 us, 1.5 TB/s, one by 1M of 24 64; 64 by 200 of 1536, rows 8 MB apart, 8.2, close together 5.5 in tiles.)
+// Rows of fewer than 16 bytes, or 8 MB and more apart: a wave to a tile of 16 by 16, its operands read where they lie.  (Bound by its waves, 390 vector instructions for
+// 256 results, and half of the time they wait: 1024 by 100000 of 16 into floats 275 us, 1.5 TB/s, one by 1M of 24 64; 64 by 200 of 1536, rows 8 MB apart, 8.2, close together 5.5 in tiles.)
 template <typename T>
 __global__ __launch_bounds__(64) void k_fp4_small(Matmul4Args p, uint32_t n_tiles) {
     const int lane = threadIdx.x, col = lane & 15, g = lane >> 4;
@@ -658,7 +658,7 @@ static hipError_t matmul4(const Matmul4Args &a, hipStream_t s) {
     const uint64_t tiles = uint64_t(mt) * nt;
     if (tile == 0 && tiles > 256 && nt >= mt) {
         // The tiles of 256 that start a last round and do not fill it: their columns in a launch of their own, of smaller tiles, where that is less than the round.  (1024 by 100000
-        // of 1536 into floats 145 us with it and 151 without, into bfloat16 120 and 126, inputs and results from memory.)
+        // of 1536 into floats 145 us with it and 151 without, into bfloat16 120 and 126.)
         const uint32_t columns = uint32_t(tiles / 256 * 256 / mt) * 256;
         if (columns < a.b.rows) {
             Matmul4Args first = a, rest = a;
