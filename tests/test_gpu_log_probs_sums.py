@@ -104,8 +104,8 @@ def test_the_gradient_sums_to_nothing(log_probs, rows, n, dtype):  # noqa: F811
     check_gradient(log_probs, scores, slots)
 
 
-@pytest.mark.parametrize("rows,n,top", [(1, 80_500, 0), (1, 80_501, 0), (64, 112_000, 0), (64, 112_001, 0), (1, 101_780, 1), (1, 101_781, 1), (1, 126_100, 20), (1, 126_101, 20), (3, 285_820, 128), (3, 285_821, 128),
-                                        (159, 159_500, 0), (159, 159_501, 0), (160, 159_501, 0)])
+@pytest.mark.parametrize("rows,n,top", [(1, 80_600, 0), (1, 80_601, 0), (64, 118_400, 0), (64, 118_401, 0), (1, 101_100, 1), (1, 101_101, 1), (1, 110_600, 20), (1, 110_601, 20), (3, 165_800, 128), (3, 165_801, 128),
+                                        (159, 175_400, 0), (159, 175_401, 0), (160, 175_401, 0)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_rows_in_one_and_in_parts(log_probs, rows, n, top, dtype):  # noqa: F811
     """Both sides of where a row's scores go to one workgroup or to several."""

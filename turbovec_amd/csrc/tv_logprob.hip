@@ -537,11 +537,11 @@ static uint32_t log_parts(size_t rows, size_t n, uint32_t &part_size) {
 // Rows in parts that have a wide workgroup each all the same: rows enough for half of the card, and those that are not much longer than what a second launch takes, and the parts'
 // ranking of their best where alternatives are asked for.  A second launch costs a call among others 3.7 us on the host, one that is waited for and one in a graph less: the border lies between what these
 // two have.  (us so and in parts, bfloat16, in a graph / waited for.  1 row without alternatives: 64000 scores 8.2 and 7.3 / 26.9 and 28.6, 80000 9.2 and 8.3 / 27.8 and 28.6, 100000 9.9 and 7.1 / 28.6 and
-// 28.4; with 1 100000 12.3 and 10.9 / 31.2 and 32.4, 128256 14.8 and 11.0 / 33.8 and 32.4; with 20 100000 13.6 and 14.7 / 32.7 and 35.9, 128256 16.5 and 14.5 / 35.3 and 35.7, 151936 17.5 and 15.7 / 36.6 and 36.5; with
-// 128 200000 32.7 and 33.0 / 52 and 57, 300000 36 and 37 / 55 and 57.  64 rows: without 100000 10.8 and 11.1 / 30.1 and 31.4, 128256 13.8 and 11.1 / 32.9 and 31.6, with 20 200000 21.8 and 22.7 / 41 and 44,
-// 300000 28.1 and 26.6 / 47.7 and 47.4, with 128 400000 - / 67 and 85.  128 rows without: 151936 15.5 and 15.6 / 34.7 and 36.1, 300000 26.6 and 22.0 / 45 and 42; 192 rows without: 200000 20.9 and 22.0,
-// 500000 44 and 49.)
-static bool log_wide(size_t rows, size_t n, size_t top) { return rows >= 160 || n <= 80000 + (top != 0 ? 20000 : 0) + 1200 * top + rows * (500 + 80 * top); }
+// 28.4; with 1 100000 12.3 and 10.9 / 31.2 and 32.4, 128256 14.8 and 11.0 / 33.8 and 32.4; with 20 100000 13.6 and 14.7 / 32.7 and 35.9, 128256 16.5 and 14.5 / 35.3 and 35.7; with 128 151936 28 and 31 / 48 and
+// 50.  64 rows: without 100000 10.8 and 11.1 / 30.1 and 31.4, 128256 13.8 and 11.1 / 32.9 and 31.6; with 20 128256 18.0 and 19.7 / 37 and 40; with 128 151936 30 and 47 / 50 and 68.  128 rows without:
+// 151936 15.5 and 15.6 / 34.7 and 36.1, 200000 18.0 and 17.7 / 37 and 38; 192 rows without: 200000 20.9 and 22.0, 500000 44 and 49.  Scores of which thousands tie with the best are gathered in turns, of
+// which parts have fewer each: 64 equal rows of 128256 with 20 227 and 111.  That is why many alternatives do not raise the border to where random scores have theirs, 300000 and more with 128.)
+static bool log_wide(size_t rows, size_t n, size_t top) { return rows >= 160 || n <= 80000 + (top != 0 ? 20000 : 0) + 500 * top + 600 * rows; }
 // Many rows of a few loads have a wave each, as long as its 64 largest scores tell the alternatives apart.  (Rows of 1000 bfloat16 scores with 5 alternatives: 1024 rows 7.9 us so and 8.5
 // with workgroups of 256, 4096 rows 10.2 and 21.9, 65536 rows 88 and 275; their gradients 4096 rows 8.2 and 11.4, 65536 rows 73 and 152.)
 static bool log_short(size_t rows, size_t n, size_t size, size_t top) { return rows >= 1024 && n * size <= 8192 && top <= kFewAlternatives; }
